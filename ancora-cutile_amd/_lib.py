@@ -137,6 +137,17 @@ _PROTOS = {
     "anc_adamw_rows": (None, [u64, i64, u64, u64, u64, u64, u64, u64, i64, i64, u64, i32,
                               C.POINTER(AdamWHyper), f32, u32, u64, u64]),
     "anc_embed_dw_scatter": (None, [u64, u64, u64, u64, u64, u64, u64, i64, i64, i64, u64]),
+    "anc_embed_lookup": (None, [u64, i32, i64, u64, C.c_int, i64, i64, f32, u64, C.c_int, u64]),
+    "anc_id_groups_device_workspace_bytes": (i64, [i64, i64]),
+    "anc_id_groups_device": (None, [u64, i32, i64, i64, i64, u64, u64, u64, u64, u64, u64, u64, u64, i64, u64]),
+    "anc_embed_dw_workspace_bytes": (i64, [i64, i64]),
+    "anc_embed_dw": (None, [u64, u64, u64, u64, u64, i64, u64, C.c_int, i64, f32, u64, u64, i64, u64, i64, u64]),
+    "anc_route_capacity": (i64, [i64, i64, i64]),
+    "anc_route_workspace_bytes": (i64, [i64, i64]),
+    "anc_route": (None, [u64, i32, i64, i64, i64, u64, u64, u64, u64, i64, u64, i64, u64]),
+    "anc_dispatch": (None, [u64, u64, u64, i64, i64, i64, i64, u64, u64, C.c_int, i64, u64]),
+    "anc_combine": (None, [u64, u64, i64, i64, u64, C.c_int, u64, C.c_int, i64, u64]),
+    "anc_combine_grad": (None, [u64, u64, u64, u64, i64, i64, i64, i64, u64, C.c_int, u64, u64, C.c_int, u64, i64, u64]),
     "anc_cast_bf16": (None, [u64, u64, i64, C.c_int, u32, u64]),
     "anc_muon_momentum": (None, [u64, u64, u64, i64, i64, f32, C.c_int, C.c_int, C.c_int,
                                  C.c_int, u64, u64]),

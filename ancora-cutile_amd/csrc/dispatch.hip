@@ -1,0 +1,212 @@
+// Rows of tokens to the experts' segments and back, over the slots that anc_route (group.hip) assigned: slot[t * k + j] is
+// the place of token t's choice j, -1 where the choice names no expert (a masked token).
+//     dispatch:      xs[slot] = x[t]; the rows that fill up a segment become zero
+//     combine:       y[t] = sum over j of w[t, j] * ys[slot]          (w = 1: the gradient of dispatch)
+//     combine_grad:  dys[slot] = w[t, j] * dy[t];  dw[t, j] = <dy[t], ys[slot]>
+// All are bound by memory. They go by token, not by slot: a token's own row is read or written once for its k choices.
+#include "rows.h"
+
+namespace {
+
+using namespace anc_rows;
+
+constexpr int kLanes = 256;
+constexpr int kPadRows = 8;                 // rows that one workgroup clears
+
+// Rows between an expert's last token and the end of its segment: workgroup `b` of those that clear them.
+template <int T, int VEC>
+__device__ __forceinline__ void clear_padding(int b, int align, const int32_t *counts, const int32_t *offsets, int64_t H, elem_t<T> *out) {
+  const int per = (align - 1 + kPadRows - 1) / kPadRows, e = b / per;
+  const int64_t from = (int64_t)offsets[e] + counts[e] + (int64_t)(b - e * per) * kPadRows, end = offsets[e + 1];
+  const int64_t to = from + kPadRows < end ? from + kPadRows : end;
+  if (from >= to) return;
+  float zero[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) zero[k] = 0.0f;
+  for (int64_t i = threadIdx.x; i < (to - from) * (H / VEC); i += kLanes) store<T, VEC>(out + from * H + i * VEC, zero);
+}
+
+template <int T, int VEC>
+__global__ void __launch_bounds__(kLanes)
+k_dispatch(const int32_t *__restrict__ slot, const int32_t *__restrict__ counts, const int32_t *__restrict__ offsets, int64_t tokens,
+           int k, int align, int64_t main_blocks, uint32_t pieces, int64_t H, const elem_t<T> *__restrict__ x,
+           elem_t<T> *__restrict__ xs) {
+  if ((int64_t)blockIdx.x >= main_blocks) {
+    clear_padding<T, VEC>((int)((int64_t)blockIdx.x - main_blocks), align, counts, offsets, H, xs);
+    return;
+  }
+  const int64_t i = (int64_t)blockIdx.x * kLanes + threadIdx.x, t = i / pieces;
+  if (t >= tokens) return;
+  const int64_t col = (i - t * pieces) * VEC;
+  const Raw<T, VEC> v = load<T, VEC>(x + t * H + col);
+  for (int j = 0; j < k; ++j) {
+    const int64_t s = slot[t * k + j];
+    if (s >= 0) store<T, VEC>(xs + s * H + col, v);
+  }
+}
+
+template <int TI, int TO, int VEC, bool WEIGHTS>
+__global__ void __launch_bounds__(kLanes)
+k_combine(const int32_t *__restrict__ slot, const float *__restrict__ w, int64_t tokens, int k, uint32_t pieces, int64_t H,
+          const elem_t<TI> *__restrict__ ys, elem_t<TO> *__restrict__ y) {
+  const int64_t i = (int64_t)blockIdx.x * kLanes + threadIdx.x, t = i / pieces;
+  if (t >= tokens) return;
+  const int64_t col = (i - t * pieces) * VEC;
+  float acc[VEC];
+#pragma unroll
+  for (int q = 0; q < VEC; ++q) acc[q] = 0.0f;
+  constexpr int D = 4;
+  for (int j0 = 0; j0 < k; j0 += D) {
+    Raw<TI, VEC> v[D];
+    int64_t s[D];
+    float f[D];
+#pragma unroll
+    for (int j = 0; j < D; ++j) {
+      s[j] = j0 + j < k ? slot[t * k + j0 + j] : -1;
+      f[j] = WEIGHTS && j0 + j < k ? w[t * k + j0 + j] : 1.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < D; ++j)
+      if (s[j] >= 0) v[j] = load<TI, VEC>(ys + s[j] * H + col);
+#pragma unroll
+    for (int j = 0; j < D; ++j) {
+      if (s[j] < 0) continue;
+      float a[VEC];
+      widen<TI, VEC>(v[j], a);
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) acc[q] = WEIGHTS ? fmaf(f[j], a[q], acc[q]) : acc[q] + a[q];
+    }
+  }
+  store<TO, VEC>(y + t * H + col, acc);
+}
+
+// One wavefront per token: its row of dy stays in registers over the k choices, the products are summed over the lanes.
+template <int TY, int TS, int VEC>
+__global__ void __launch_bounds__(kLanes)
+k_combine_grad(const int32_t *__restrict__ slot, const float *__restrict__ w, const int32_t *__restrict__ counts,
+               const int32_t *__restrict__ offsets, int64_t tokens, int k, int align, int64_t main_blocks, int64_t H,
+               const elem_t<TY> *__restrict__ dy, const elem_t<TS> *__restrict__ ys, elem_t<TS> *__restrict__ dys,
+               float *__restrict__ dw) {
+  if ((int64_t)blockIdx.x >= main_blocks) {
+    clear_padding<TS, VEC>((int)((int64_t)blockIdx.x - main_blocks), align, counts, offsets, H, dys);
+    return;
+  }
+  const int lane = (int)(threadIdx.x & 63);
+  const int64_t t = (int64_t)blockIdx.x * (kLanes / 64) + (threadIdx.x >> 6);
+  if (t >= tokens) return;
+  for (int j = 0; j < k; ++j) {
+    const int64_t s = slot[t * k + j];
+    const float f = w[t * k + j];
+    float dot = 0.0f;
+    if (s >= 0)
+      for (int64_t col = (int64_t)lane * VEC; col < H; col += 64 * VEC) {
+        float g[VEC], a[VEC], o[VEC];
+        widen<TY, VEC>(load<TY, VEC>(dy + t * H + col), g);
+        widen<TS, VEC>(load<TS, VEC>(ys + s * H + col), a);
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) {
+          dot = fmaf(g[q], a[q], dot);
+          o[q] = f * g[q];
+        }
+        store<TS, VEC>(dys + s * H + col, o);
+      }
+    dot = anc_wave_sum_f32(dot);
+    if (lane == 0) dw[t * k + j] = dot;
+  }
+}
+
+int check_rows(const char *who, uint64_t slot, int64_t tokens, int64_t k, int64_t H) {
+  ANC_REQUIRE(tokens >= 0 && tokens < (1ll << 31) && k > 0 && k <= 512 && H > 0 && H <= (1ll << 20) && tokens * H < (1ll << 38),
+              "%s: %lld tokens of width %lld with %lld choices", who, (long long)tokens, (long long)H, (long long)k);
+  ANC_REQUIRE(slot != 0 && (slot & 3) == 0, "%s: null or misaligned slots", who);
+  return ANC_OK;
+}
+int check_segments(const char *who, uint64_t counts, uint64_t offsets, int64_t experts, int64_t align) {
+  ANC_REQUIRE(counts && offsets && ((counts | offsets) & 3) == 0 && experts > 0 && experts <= 512 && align > 0 && align <= 256,
+              "%s: bad segments (%lld experts, align %lld)", who, (long long)experts, (long long)align);
+  return ANC_OK;
+}
+int64_t pad_blocks(int64_t experts, int64_t align) { return experts * ((align - 1 + kPadRows - 1) / kPadRows); }
+
+}  // namespace
+
+extern "C" int anc_dispatch(uint64_t slot, uint64_t counts, uint64_t offsets, int64_t tokens, int64_t k, int64_t experts, int64_t align,
+                            uint64_t x, uint64_t xs, int type, int64_t H, uint64_t stream) {
+  if (int rc = check_rows("anc_dispatch", slot, tokens, k, H)) return rc;
+  if (int rc = check_segments("anc_dispatch", counts, offsets, experts, align)) return rc;
+  ANC_REQUIRE(type_ok(type), "anc_dispatch: type %d", type);
+  ANC_REQUIRE(x && xs && (x | xs) % (uint64_t)elem_size(type) == 0, "anc_dispatch: null or misaligned pointers");
+  const Ptr ps[2] = {{x, type}, {xs, type}};
+  const int vec = piece(H, ps);
+  const int64_t blocks = (tokens * (H / vec) + kLanes - 1) / kLanes, all = blocks + pad_blocks(experts, align);
+  ANC_REQUIRE(all < (1ll << 31), "anc_dispatch: too large for one call");
+  if (tokens == 0) return ANC_OK;
+  hipStream_t s = anc_stream(stream);
+  AncProfScope prof(ANC_PROF_MISC, s);
+  with_type(type, [&](auto t) {
+    with_piece(vec, [&](auto v) {
+      constexpr int T = decltype(t)::value, VEC = decltype(v)::value;
+      hipLaunchKernelGGL((k_dispatch<T, VEC>), dim3((unsigned)all), dim3(kLanes), 0, s, (const int32_t *)slot, (const int32_t *)counts,
+                         (const int32_t *)offsets, tokens, (int)k, (int)align, blocks, (uint32_t)(H / VEC), H, (const elem_t<T> *)x,
+                         (elem_t<T> *)xs);
+    });
+  });
+  ANC_LAUNCH_CHECK();
+  return ANC_OK;
+}
+
+extern "C" int anc_combine(uint64_t slot, uint64_t weights, int64_t tokens, int64_t k, uint64_t ys, int ys_type, uint64_t y, int y_type,
+                           int64_t H, uint64_t stream) {
+  if (int rc = check_rows("anc_combine", slot, tokens, k, H)) return rc;
+  ANC_REQUIRE(type_ok(ys_type) && type_ok(y_type), "anc_combine: types %d and %d", ys_type, y_type);
+  ANC_REQUIRE(ys && y && ys % (uint64_t)elem_size(ys_type) == 0 && y % (uint64_t)elem_size(y_type) == 0 && (weights & 3) == 0,
+              "anc_combine: null or misaligned pointers");
+  const Ptr ps[2] = {{ys, ys_type}, {y, y_type}};
+  const int vec = piece(H, ps);
+  const int64_t blocks = (tokens * (H / vec) + kLanes - 1) / kLanes;
+  ANC_REQUIRE(blocks < (1ll << 31), "anc_combine: too large for one call");
+  if (tokens == 0) return ANC_OK;
+  hipStream_t s = anc_stream(stream);
+  AncProfScope prof(ANC_PROF_MISC, s);
+  with_type(ys_type, [&](auto ti) {
+    with_type(y_type, [&](auto to) {
+      with_piece(vec, [&](auto v) {
+        constexpr int TI = decltype(ti)::value, TO = decltype(to)::value, VEC = decltype(v)::value;
+        auto kernel = weights != 0 ? k_combine<TI, TO, VEC, true> : k_combine<TI, TO, VEC, false>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kLanes), 0, s, (const int32_t *)slot, (const float *)weights, tokens,
+                           (int)k, (uint32_t)(H / VEC), H, (const elem_t<TI> *)ys, (elem_t<TO> *)y);
+      });
+    });
+  });
+  ANC_LAUNCH_CHECK();
+  return ANC_OK;
+}
+
+extern "C" int anc_combine_grad(uint64_t slot, uint64_t weights, uint64_t counts, uint64_t offsets, int64_t tokens, int64_t k,
+                                int64_t experts, int64_t align, uint64_t dy, int dy_type, uint64_t ys, uint64_t dys, int ys_type,
+                                uint64_t dw, int64_t H, uint64_t stream) {
+  if (int rc = check_rows("anc_combine_grad", slot, tokens, k, H)) return rc;
+  if (int rc = check_segments("anc_combine_grad", counts, offsets, experts, align)) return rc;
+  ANC_REQUIRE(type_ok(dy_type) && type_ok(ys_type), "anc_combine_grad: types %d and %d", dy_type, ys_type);
+  ANC_REQUIRE(weights && dy && ys && dys && dw && ((weights | dw) & 3) == 0 && dy % (uint64_t)elem_size(dy_type) == 0 &&
+                  (ys | dys) % (uint64_t)elem_size(ys_type) == 0,
+              "anc_combine_grad: null or misaligned pointers");
+  const Ptr ps[3] = {{dy, dy_type}, {ys, ys_type}, {dys, ys_type}};
+  const int vec = piece(H, ps);
+  const int64_t blocks = (tokens + kLanes / 64 - 1) / (kLanes / 64), all = blocks + pad_blocks(experts, align);
+  if (tokens == 0) return ANC_OK;
+  hipStream_t s = anc_stream(stream);
+  AncProfScope prof(ANC_PROF_MISC, s);
+  with_type(dy_type, [&](auto ty) {
+    with_type(ys_type, [&](auto ts) {
+      with_piece(vec, [&](auto v) {
+        constexpr int TY = decltype(ty)::value, TS = decltype(ts)::value, VEC = decltype(v)::value;
+        hipLaunchKernelGGL((k_combine_grad<TY, TS, VEC>), dim3((unsigned)all), dim3(kLanes), 0, s, (const int32_t *)slot,
+                           (const float *)weights, (const int32_t *)counts, (const int32_t *)offsets, tokens, (int)k, (int)align, blocks, H,
+                           (const elem_t<TY> *)dy, (const elem_t<TS> *)ys, (elem_t<TS> *)dys, (float *)dw);
+      });
+    });
+  });
+  ANC_LAUNCH_CHECK();
+  return ANC_OK;
+}

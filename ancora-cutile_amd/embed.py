@@ -5,6 +5,9 @@ used at ancora/model/resident_moe_model.py:262-271, 333-334). `RowSparseAdamW` h
 in the reference, whose AdamW sweeps the whole embedding every step (ancora/optim/adamw.py:92-97):
 it updates only the rows a step's tokens touch and replays the steps a row missed when the row is
 next needed, so that every row it hands out is bit-identical to the dense optimizer's.
+
+For ids that lie on the device: `embed_lookup` (rows times a scale), `DeviceIdGroups` (the group arrays, made there) and
+`embed_dw` (the gradient over them, whatever the ids' frequencies).
 """
 import ctypes
 import threading
@@ -175,6 +178,130 @@ def embed_dw_scatter(groups, dy, si, out=None, compact=None, V=None):
     api.anc_embed_dw_scatter(base + 2 * step, base + step, base + 3 * step, base, dy.ptr,
                              0 if out is None else out.ptr, 0 if compact is None else compact.ptr,
                              M, 0 if V is None else V, H, int(si))
+
+
+def _ids(buf, who, most=None):
+    """(bytes per id, number of ids) of a device array of ids."""
+    if buf.dtype not in (np.int32, np.int64):
+        raise ValueError(f"{who}: ids are int32 or int64, got {buf.dtype}")
+    if most is not None and buf.size > most:
+        raise ValueError(f"{who}: {buf.size} ids, room for {most}")
+    return buf.dtype.itemsize, buf.size
+
+
+def _type(buf, who):
+    if buf.dtype == np.uint16:
+        return _lib.BF16
+    if buf.dtype == np.float32:
+        return _lib.F32
+    raise ValueError(f"{who}: rows are float32 or bf16 bits (uint16), got {buf.dtype}")
+
+
+def _rows_of(buf, rows, H, who, name):
+    """`buf` holds at least `rows` rows of H elements."""
+    if len(buf.shape) != 2 or buf.shape[1] != H or buf.shape[0] < rows:
+        raise ValueError(f"{who}: {name} is {buf.shape}, ({rows}, {H}) expected")
+
+
+def embed_lookup(ids, table, si, out, scale=1.0, n=None):
+    """out[i] = scale * table[ids[i]] for the first n ids (default: all), asynchronous on stream `si`. ids: int32 or int64
+    DevBuf; table (V, H) and out (>= n, H): float32 or bf16 bits, each of its own type. An id outside [0, V) gives a zero row;
+    rows of `out` behind n are left as they were. The product is fp32, rounded once."""
+    nbytes, have = _ids(ids, "embed_lookup")
+    n = have if n is None else int(n)
+    if not 0 <= n <= have:
+        raise ValueError(f"embed_lookup: {n} of {have} ids")
+    if len(table.shape) != 2:
+        raise ValueError(f"embed_lookup: table is {table.shape}, (V, H) expected")
+    V, H = table.shape
+    _rows_of(out, n, H, "embed_lookup", "out")
+    api.anc_embed_lookup(ids.ptr, nbytes, n, table.ptr, _type(table, "embed_lookup"), V, H, float(scale), out.ptr,
+                         _type(out, "embed_lookup"), int(si))
+
+
+class DeviceIdGroups:
+    """The arrays of `IdGroups` made on the device from ids that lie there: no copy to the host, and `group` may be captured
+    into a graph. Room for M ids of a table of V rows; `srt`, `start`, `cnt`, `gid` are (M, 1) int32 as in `IdGroups`, with
+    gid -1 behind the last group, and `count` (1,) int32 holds the number of groups. Ids outside [0, V) are left out.
+
+        groups = DeviceIdGroups(M, V)
+        groups.group(ids, si)                              # every step
+        embed_dw(groups, dy, si, compact=rows)             # or out=dE
+        opt.step(groups.gid, groups.M, rows, si)           # RowSparseAdamW: M rows, those behind the last group left out
+
+    The arrays and the gradient's partial rows are one set of buffers: calls on different streams (or replays of graphs)
+    that use one object are put in order by the caller; work that overlaps takes an object each."""
+
+    def __init__(self, M, V):
+        _lib.init()
+        self.M, self.V = int(M), int(V)
+        nbytes = api.anc_id_groups_device_workspace_bytes(self.M, self.V)
+        if nbytes < 0:
+            raise ValueError(f"DeviceIdGroups: room for {M} ids (1 .. 2^20) of a table of {V} rows (1 .. 2^31 - 1)")
+        self._block = DevBuf.empty((6 * self.M + 1,), np.int32)
+        self._ws = DevBuf.empty((nbytes,), np.uint8)
+        self._parts = []                       # partial rows of `embed_dw`, by width; kept: a graph may hold an address
+        arrays = [DevBuf(shape=(self.M, 1), dtype=np.int32, ptr=self._block.ptr + 4 * i * self.M) for i in range(6)]
+        self.srt, self.start, self.cnt, self.gid, self._key, self._grp = arrays
+        self.count = DevBuf(shape=(1,), dtype=np.int32, ptr=self._block.ptr + 24 * self.M)
+        self._at = tuple(a.ptr for a in arrays) + (self.count.ptr, self._ws.ptr, nbytes)
+        self.n = None                          # ids of the last `group`
+
+    def base_on(self, si):
+        """Device address of srt, start, cnt, gid, one after the other (what `embed_dw_scatter` takes)."""
+        self._used("embed_dw_scatter")
+        return self._block.ptr
+
+    def _used(self, who):
+        if self._block is None:
+            raise _lib.AncoraError("DeviceIdGroups: freed")
+        if self.n is None and who:
+            raise _lib.AncoraError(f"{who}: no ids were grouped yet")
+
+    def group(self, ids, si, n=None):
+        """Group the first n (default: all) of `ids`, an int32 or int64 DevBuf of at most M ids. Asynchronous on `si`."""
+        self._used(None)
+        nbytes, have = _ids(ids, "DeviceIdGroups.group", self.M if n is None else None)
+        n = have if n is None else int(n)
+        if not 0 <= n <= min(have, self.M):
+            raise ValueError(f"DeviceIdGroups.group: {n} of {have} ids, room for {self.M}")
+        api.anc_id_groups_device(ids.ptr, nbytes, n, self.M, self.V, *self._at, int(si))
+        self.n = n
+
+    def _part(self, H):
+        nbytes = api.anc_embed_dw_workspace_bytes(self.M, H)
+        for b in self._parts:
+            if b.nbytes >= nbytes:
+                return b
+        self._parts.append(DevBuf.empty((nbytes,), np.uint8))
+        return self._parts[-1]
+
+    def free(self):
+        if self._block is not None:
+            for b in (self._block, self._ws, *self._parts):
+                b.free()
+            self._block, self._parts = None, []
+
+
+def embed_dw(groups, dy, si, out=None, compact=None, scale=1.0):
+    """Gradient of `embed_lookup` over the ids of `groups` (a `DeviceIdGroups`). dy: (n, H) float32 or bf16 bits.
+    out: (V, H) fp32, added onto in place, or compact: (>= n, H) fp32 that receives one summed row per group (rows
+    behind the last group are left as they were). Sums are fp32 in a fixed order: the same bits on every run."""
+    groups._used("embed_dw")
+    if (out is None) == (compact is None):
+        raise ValueError("embed_dw: one of out and compact")
+    H = dy.shape[-1]
+    _rows_of(dy, groups.n, H, "embed_dw", "dy")
+    target = out if compact is None else compact
+    if target.dtype != np.float32:
+        raise ValueError(f"embed_dw: the gradient is float32, got {target.dtype}")
+    if compact is None and tuple(out.shape) != (groups.V, H):
+        raise ValueError(f"embed_dw: out is {out.shape}, ({groups.V}, {H}) expected")
+    _rows_of(target, 0 if compact is None else groups.n, H, "embed_dw", "compact")
+    part = groups._part(H)
+    srt, start, cnt, _, key, grp = groups._at[:6]
+    api.anc_embed_dw(srt, start, cnt, key, grp, groups.n, dy.ptr, _type(dy, "embed_dw"), H, float(scale),
+                     0 if out is None else out.ptr, 0 if compact is None else compact.ptr, groups.V, part.ptr, part.nbytes, int(si))
 
 
 class RowSparseAdamW:

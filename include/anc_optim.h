@@ -319,6 +319,64 @@ int anc_id_groups(const int32_t *ids, int64_t n, int32_t *srt, int32_t *start, i
                   int64_t *n_groups);
 int anc_unique_ids(const int32_t *ids, int64_t n, int32_t *out, int64_t *n_out);
 
+/* The input embedding from ids that lie on the device. Ids are int32 or int64 (ids_bytes 4 or 8); one outside
+ * [0, V) names no row: its lookup is a zero row, its gradient is left out. Types are ANC_F32 or ANC_BF16, rows are
+ * contiguous, any H; rows that start 16-byte aligned with H % 8 == 0 move fastest.
+ *
+ * anc_embed_lookup: out[i] = scale * table[ids[i]] for i < n, product in fp32, one rounding. */
+int anc_embed_lookup(uint64_t ids, int32_t ids_bytes, int64_t n, uint64_t table, int table_type, int64_t V, int64_t H,
+                     float scale, uint64_t out, int out_type, uint64_t stream);
+
+/* anc_id_groups_device: the arrays of anc_id_groups made on the device, of n <= M ids (M <= 2^20), without a host
+ * round trip. srt, start, cnt, gid: int32[M]; the groups cover the ids that name a row (the others lie behind them in srt);
+ * groups behind the last have start = cnt = 0 and gid = -1, so that anc_embed_dw_scatter and anc_adamw_rows leave them out.
+ * key, grp: int32[M], id and group of every sorted position (V and -1 where none); count: int32, the number of groups.
+ * Entries n .. M of srt, key and grp are left as they were. workspace: anc_id_groups_device_workspace_bytes(M, V). */
+int64_t anc_id_groups_device_workspace_bytes(int64_t M, int64_t V);
+int anc_id_groups_device(uint64_t ids, int32_t ids_bytes, int64_t n, int64_t M, int64_t V, uint64_t srt, uint64_t start,
+                         uint64_t cnt, uint64_t gid, uint64_t key, uint64_t grp, uint64_t count, uint64_t workspace,
+                         int64_t workspace_bytes, uint64_t stream);
+
+/* anc_embed_dw: the table's gradient over those groups, dy (n, H).
+ *   out != 0:     out[id] += scale * sum of the id's rows, out (V, H) fp32; rows that no id names are not touched
+ *   compact != 0: compact[g] = scale * that sum, (n, H) fp32; rows behind the last group are left as they were
+ * Rows are added in fp32 in sorted order within chunks of 16, 32 or 64 positions (by n), chunks in a fixed order: the same
+ * bits on every run, a function of n, the ids and dy. One id may hold most of the batch at no loss of speed (a group of
+ * anc_embed_dw_scatter, whose bits are the sequential sum's, is one workgroup's). */
+int64_t anc_embed_dw_workspace_bytes(int64_t M, int64_t H);        /* enough for every n <= M */
+int anc_embed_dw(uint64_t srt, uint64_t start, uint64_t cnt, uint64_t key, uint64_t grp, int64_t n, uint64_t dy, int dy_type,
+                 int64_t H, float scale, uint64_t out, uint64_t compact, int64_t V, uint64_t workspace,
+                 int64_t workspace_bytes, uint64_t stream);
+
+/* ------------------------------------------------------ tokens by expert ---
+ * anc_route: n = tokens * k assignments (expert_ids[t * k + j], int32 or int64) in a stable order by expert. Expert e's
+ * segment is the slots offsets[e] .. offsets[e + 1), its tokens first (counts[e] of them, in ascending order of t * k + j),
+ * filled up to a multiple of `align` (a power of two up to 256). An assignment outside [0, experts) has no slot.
+ *   counts int32[experts], offsets int32[experts + 1], slot int32[n] (-1: none), src int32[capacity]: the assignment of a
+ *   slot (-1: filling, or behind the last segment). capacity >= anc_route_capacity(n, experts, align) slots.
+ * n <= 2^22, experts <= 512. The same expert may be named twice for one token. */
+int64_t anc_route_capacity(int64_t assignments, int64_t experts, int64_t align);
+int64_t anc_route_workspace_bytes(int64_t assignments, int64_t experts);
+int anc_route(uint64_t expert_ids, int32_t ids_bytes, int64_t n, int64_t experts, int64_t align, uint64_t counts,
+              uint64_t offsets, uint64_t slot, uint64_t src, int64_t capacity, uint64_t workspace, int64_t workspace_bytes,
+              uint64_t stream);
+
+/* Rows there and back over the slots of anc_route (slot int32[tokens * k]); types ANC_F32 or ANC_BF16, sums in fp32 with
+ * one rounding at the end, choices in ascending order.
+ *   anc_dispatch:      xs[slot[t, j]] = x[t]; the rows that fill up a segment become zero, rows behind the last segment and
+ *                      without a slot are left as they were
+ *   anc_combine:       y[t] = sum over j of weights[t, j] * ys[slot[t, j]] (weights fp32; 0: all one, which is the gradient
+ *                      of anc_dispatch); a choice without a slot adds nothing, a token without any gives a zero row
+ *   anc_combine_grad:  dys[slot[t, j]] = weights[t, j] * dy[t], filling rows zero as in anc_dispatch;
+ *                      dw[t, j] = <dy[t], ys[slot[t, j]]> fp32, 0 for a choice without a slot */
+int anc_dispatch(uint64_t slot, uint64_t counts, uint64_t offsets, int64_t tokens, int64_t k, int64_t experts, int64_t align,
+                 uint64_t x, uint64_t xs, int type, int64_t H, uint64_t stream);
+int anc_combine(uint64_t slot, uint64_t weights, int64_t tokens, int64_t k, uint64_t ys, int ys_type, uint64_t y, int y_type,
+                int64_t H, uint64_t stream);
+int anc_combine_grad(uint64_t slot, uint64_t weights, uint64_t counts, uint64_t offsets, int64_t tokens, int64_t k,
+                     int64_t experts, int64_t align, uint64_t dy, int dy_type, uint64_t ys, uint64_t dys, int ys_type,
+                     uint64_t dw, int64_t H, uint64_t stream);
+
 /* p16 = bf16(p32): replaces `_cast_bf16` (ancora/kernels/fused.py:285-290). */
 int anc_cast_bf16(uint64_t p32, uint64_t p16, int64_t n, int sr, uint32_t seed,
                   uint64_t stream);

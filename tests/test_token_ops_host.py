@@ -1,0 +1,184 @@
+"""What the operators indexed by token refuse, at the C boundary and in the host layer, without a GPU: no launch is reached."""
+import numpy as np
+import pytest
+
+P = 1 << 20          # an address that is aligned and never read
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from ancora_cutile_amd import _lib
+    return _lib.load()
+
+
+def _refused(lib, name, args, word):
+    assert getattr(lib, name)(*args) == 2, (name, args)
+    assert word in lib.anc_last_error().decode(), lib.anc_last_error()
+
+
+def _but(args, at, value):
+    return args[:at] + (value,) + args[at + 1:]
+
+
+def test_lookup_refusals(lib):
+    ok = (P, 4, 10, P, 1, 100, 64, 1.0, P, 1, 0)
+    for at, value, word in ((0, 0, "null"), (0, P + 2, "misaligned"), (1, 2, "bytes"), (2, -1, "n="), (2, 1 << 31, "n="), (3, 0, "null"),
+                            (3, P + 1, "misaligned"), (4, 2, "types"), (5, 0, "V="), (6, 0, "H="), (6, (1 << 20) + 1, "H="), (8, 0, "null"),
+                            (8, P + 1, "misaligned"), (9, -1, "types")):
+        _refused(lib, "anc_embed_lookup", _but(ok, at, value), word)
+    _refused(lib, "anc_embed_lookup", _but(_but(ok, 0, P + 4), 1, 8), "misaligned")
+    _refused(lib, "anc_embed_lookup", _but(_but(ok, 2, (1 << 31) - 1), 6, 1 << 20), "too many")
+    assert lib.anc_embed_lookup(*_but(_but(ok, 2, 0), 0, 0)) == 0                # no ids: nothing to do
+
+
+def test_group_refusals(lib):
+    ws = lib.anc_id_groups_device_workspace_bytes(100000, 5000)
+    assert ws > 0 and lib.anc_id_groups_device_workspace_bytes(100, 5000) > 0
+    for M, V in ((0, 10), ((1 << 20) + 1, 10), (10, 0), (10, 1 << 31)):
+        assert lib.anc_id_groups_device_workspace_bytes(M, V) == -1
+    ok = (P, 4, 90000, 100000, 5000, P, P, P, P, P, P, P, P, ws, 0)
+    for at, value, word in ((0, 0, "null"), (0, P + 1, "misaligned"), (1, 1, "bytes"), (2, -1, "n="), (2, 100001, "n="), (3, 1 << 21, "M="),
+                            (4, 0, "V="), (4, 1 << 31, "V="), (13, 100, "workspace holds")) + \
+            tuple((i, 0, "null") for i in range(5, 13)) + tuple((i, P + 2, "misaligned") for i in range(5, 13)):
+        _refused(lib, "anc_id_groups_device", _but(ok, at, value), word)
+
+
+def test_gradient_refusals(lib):
+    ws = lib.anc_embed_dw_workspace_bytes(1000, 64)
+    assert ws == 63 * 2 * 64 * 4
+    # one buffer serves every batch up to its size: chunks are shorter for smaller ones
+    assert lib.anc_embed_dw_workspace_bytes(20000, 8) == lib.anc_embed_dw_workspace_bytes(16384, 8)
+    for M, H in ((0, 64), ((1 << 20) + 1, 64), (10, 0), (10, (1 << 20) + 1)):
+        assert lib.anc_embed_dw_workspace_bytes(M, H) == -1
+    ok = (P, P, P, P, P, 1000, P, 1, 64, 1.0, P, 0, 500, P, ws, 0)
+    for at, value, word in ((5, -1, "n="), (5, (1 << 20) + 1, "n="), (6, 0, "null"), (6, P + 1, "misaligned"), (7, 7, "type"), (8, 0, "H="),
+                            (10, 0, "one of"), (10, P + 2, "misaligned"), (11, P, "one of"), (12, 0, "V="), (13, 0, "null"), (13, P + 8, "misaligned"),
+                            (14, ws - 1, "workspace holds")) + tuple((i, 0, "null") for i in range(5)):
+        _refused(lib, "anc_embed_dw", _but(ok, at, value), word)
+
+
+def test_route_refusals(lib):
+    assert lib.anc_route_capacity(100, 8, 16) == 100 + 8 * 15 and lib.anc_route_capacity(3, 8, 16) == 3 + 3 * 15
+    for a in ((0, 8, 1), ((1 << 22) + 1, 8, 1), (10, 0, 1), (10, 513, 1), (10, 8, 0), (10, 8, 3), (10, 8, 512)):
+        assert lib.anc_route_capacity(*a) == -1
+    A, E = 50000, 60
+    ws, cap = lib.anc_route_workspace_bytes(A, E), lib.anc_route_capacity(A, E, 32)
+    ok = (P, 4, A, E, 32, P, P, P, P, cap, P, ws, 0)
+    for at, value, word in ((0, 0, "null"), (0, P + 2, "misaligned"), (1, 3, "bytes"), (2, -1, "assignments"), (3, 0, "experts"), (3, 600, "experts"),
+                            (4, 24, "align"), (9, cap - 1, "needed"), (9, 1 << 31, "needed"), (11, ws - 1, "workspace holds")) + \
+            tuple((i, 0, "null") for i in (5, 6, 7, 8, 10)) + tuple((i, P + 1, "misaligned") for i in (5, 6, 7, 8, 10)):
+        _refused(lib, "anc_route", _but(ok, at, value), word)
+
+
+def test_row_mover_refusals(lib):
+    ok = (P, P, P, 10, 2, 4, 16, P, P, 1, 64, 0)
+    for at, value, word in ((0, 0, "slots"), (0, P + 2, "slots"), (1, 0, "segments"), (2, P + 1, "segments"), (3, -1, "tokens"), (4, 0, "choices"),
+                            (4, 513, "choices"), (5, 0, "segments"), (5, 513, "segments"), (6, 0, "segments"), (7, 0, "null"), (8, 0, "null"),
+                            (8, P + 1, "misaligned"), (9, 5, "type"), (10, 0, "width")):
+        _refused(lib, "anc_dispatch", _but(ok, at, value), word)
+    ok = (P, P, 10, 2, P, 1, P, 0, 64, 0)
+    for at, value, word in ((0, 0, "slots"), (1, P + 2, "misaligned"), (2, -1, "tokens"), (3, 0, "choices"), (4, 0, "null"), (5, 9, "types"), (6, 0, "null"),
+                            (6, P + 2, "misaligned"), (7, 9, "types"), (8, 0, "width")):
+        _refused(lib, "anc_combine", _but(ok, at, value), word)
+    ok = (P, P, P, P, 10, 2, 4, 16, P, 0, P, P, 1, P, 64, 0)
+    for at, value, word in ((0, 0, "slots"), (1, 0, "null"), (2, 0, "segments"), (3, 0, "segments"), (4, -1, "tokens"), (8, 0, "null"), (8, P + 2, "misaligned"),
+                            (9, 3, "types"), (10, 0, "null"), (11, P + 1, "misaligned"), (12, 3, "types"), (13, 0, "null"), (13, P + 2, "misaligned")):
+        _refused(lib, "anc_combine_grad", _but(ok, at, value), word)
+
+
+def _buf(shape, dtype):
+    from ancora_cutile_amd import DevBuf
+    return DevBuf(shape=shape, dtype=dtype)
+
+
+def test_embedding_calls_that_do_not_fit_launch_nothing(fake_device):
+    from ancora_cutile_amd import DeviceIdGroups, embed_dw, embed_lookup
+    from ancora_cutile_amd._lib import AncoraError
+    V, H, M = 50, 16, 30
+    ids, table, out = _buf((M,), np.int32), _buf((V, H), np.uint16), _buf((M, H), np.float32)
+    embed_lookup(ids, table, 0, out)
+    assert len(fake_device.calls("anc_embed_lookup")) == 1
+    for bad in (lambda: embed_lookup(_buf((M,), np.float32), table, 0, out), lambda: embed_lookup(ids, _buf((V, H), np.int32), 0, out),
+                lambda: embed_lookup(ids, _buf((V * H,), np.uint16), 0, out), lambda: embed_lookup(ids, table, 0, _buf((M - 1, H), np.uint16)),
+                lambda: embed_lookup(ids, table, 0, _buf((M, H + 1), np.uint16)), lambda: embed_lookup(ids, table, 0, out, n=M + 1),
+                lambda: embed_lookup(ids, table, 0, out, n=-1), lambda: embed_lookup(ids, table, 0, _buf((M, H), np.int32))):
+        with pytest.raises(ValueError):
+            bad()
+    assert len(fake_device.calls("anc_embed_lookup")) == 1
+    for M_, V_ in ((0, 5), ((1 << 20) + 1, 5), (5, 0), (5, 1 << 31)):
+        with pytest.raises(ValueError):
+            DeviceIdGroups(M_, V_)
+    g = DeviceIdGroups(M, V)
+    dy, rows, dE = _buf((M, H), np.uint16), _buf((M, H), np.float32), _buf((V, H), np.float32)
+    with pytest.raises(AncoraError):
+        embed_dw(g, dy, 0, out=dE)                                    # nothing grouped yet
+    for bad in (lambda: g.group(_buf((M + 1,), np.int32), 0), lambda: g.group(_buf((M,), np.uint32), 0), lambda: g.group(ids, 0, M + 1),
+                lambda: g.group(ids, 0, -1)):
+        with pytest.raises(ValueError):
+            bad()
+    assert not fake_device.calls("anc_id_groups_device")
+    g.group(ids, 0)
+    for bad in (lambda: embed_dw(g, dy, 0), lambda: embed_dw(g, dy, 0, out=dE, compact=rows), lambda: embed_dw(g, dy, 0, out=rows),
+                lambda: embed_dw(g, _buf((M - 1, H), np.uint16), 0, out=dE), lambda: embed_dw(g, _buf((M, H + 1), np.uint16), 0, out=dE),
+                lambda: embed_dw(g, dy, 0, compact=_buf((M - 1, H), np.float32)), lambda: embed_dw(g, dy, 0, compact=_buf((M, H), np.uint16)),
+                lambda: embed_dw(g, _buf((M, H), np.int32), 0, out=dE)):
+        with pytest.raises(ValueError):
+            bad()
+    assert not fake_device.calls("anc_embed_dw")
+    # partial rows: one buffer for a width, kept while a wider one joins it (a captured graph may hold its address)
+    embed_dw(g, dy, 0, out=dE)
+    first = fake_device.calls("anc_embed_dw")[-1][13]
+    wide = _buf((M, 4 * H), np.uint16)
+    embed_dw(g, wide, 0, compact=_buf((M, 4 * H), np.float32))
+    assert fake_device.calls("anc_embed_dw")[-1][13] != first and first in fake_device.blocks
+    embed_dw(g, dy, 0, out=dE)
+    assert fake_device.calls("anc_embed_dw")[-1][13] == first
+    g.free()
+    g.free()
+    assert first not in fake_device.blocks
+    with pytest.raises(AncoraError):
+        g.group(ids, 0)
+    with pytest.raises(AncoraError):
+        embed_dw(g, dy, 0, out=dE)
+
+
+def test_routing_calls_that_do_not_fit_launch_nothing(fake_device):
+    from ancora_cutile_amd import RoutePlan, combine, combine_grad, dispatch_grad
+    from ancora_cutile_amd._lib import AncoraError
+    from ancora_cutile_amd.dispatch import dispatch
+    T, k, E, H = 20, 2, 4, 24
+    for a in ((0, k, E), (T, 0, E), (T, 513, E), (T, k, 0), (T, k, 513), (T, k, E, 0), (T, k, E, 3), (T, k, E, 512), (1 << 22, 2, E)):
+        with pytest.raises(ValueError):
+            RoutePlan(*a)
+    p = RoutePlan(T, k, E, 8)
+    S = p.capacity
+    x, xs, w = _buf((T, H), np.uint16), _buf((S, H), np.uint16), _buf((T, k), np.float32)
+    ids = _buf((T, k), np.int64)
+    with pytest.raises(AncoraError):
+        dispatch(p, x, 0, xs)
+    for bad in (lambda: p.route(_buf((T * k,), np.int32), 0), lambda: p.route(_buf((T, k + 1), np.int32), 0), lambda: p.route(_buf((T, k), np.float32), 0),
+                lambda: p.route(_buf((T + 1, k), np.int32), 0), lambda: p.route(ids, 0, T + 1), lambda: p.route(ids, 0, -1)):
+        with pytest.raises(ValueError):
+            bad()
+    assert not fake_device.calls("anc_route")
+    p.route(ids, 0)
+    f = lambda *sh: _buf(sh, np.float32)                                            # noqa: E731
+    for bad in (lambda: dispatch(p, x, 0, f(S, H)), lambda: dispatch(p, x, 0, _buf((S - 1, H), np.uint16)), lambda: dispatch(p, _buf((T - 1, H), np.uint16), 0, xs),
+                lambda: dispatch(p, x, 0, _buf((S, H + 1), np.uint16)), lambda: dispatch(p, _buf((T, H), np.int32), 0, _buf((S, H), np.int32)),
+                lambda: combine(p, _buf((S - 1, H), np.uint16), w, 0, x), lambda: combine(p, xs, f(T, k + 1), 0, x), lambda: combine(p, xs, f(T - 1, k), 0, x),
+                lambda: combine(p, xs, _buf((T, k), np.uint16), 0, x), lambda: combine(p, xs, w, 0, f(T - 1, H)), lambda: dispatch_grad(p, xs, 0, f(T, H + 1)),
+                lambda: combine_grad(p, x, xs, w, 0, f(S, H), f(T, k)), lambda: combine_grad(p, x, xs, w, 0, xs, f(T, k + 1)),
+                lambda: combine_grad(p, x, xs, w, 0, _buf((S - 1, H), np.uint16), f(T, k)), lambda: combine_grad(p, f(T - 1, H), xs, w, 0, xs, f(T, k))):
+        with pytest.raises(ValueError):
+            bad()
+    assert not any(fake_device.calls(n) for n in ("anc_dispatch", "anc_combine", "anc_combine_grad"))
+    dispatch(p, x, 0, xs)
+    combine(p, xs, w, 0, f(T, H))
+    dispatch_grad(p, xs, 0, x)
+    combine_grad(p, x, xs, w, 0, _buf((S, H), np.uint16), f(T, k))
+    assert [len(fake_device.calls(n)) for n in ("anc_dispatch", "anc_combine", "anc_combine_grad")] == [1, 2, 1]
+    p.free()
+    p.free()
+    for bad in (lambda: p.route(ids, 0), lambda: dispatch(p, x, 0, xs)):
+        with pytest.raises(AncoraError):
+            bad()
