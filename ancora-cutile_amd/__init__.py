@@ -15,6 +15,6 @@ from .muon import (Muon, DeviceMuon, MuonScratch, ResidentMuon, BatchedProjMuon,
 from .moe import ExpertMuonScratch, ExpertOptimizer, GroupedMoEFFNOptim                          # noqa: F401
 from .hybrid import HybridOptimizer, default_is_muon, resident_is_muon       # noqa: F401
 from .quant import Mxfp8WeightCache, quant_mxfp8_w                          # noqa: F401
-from .grads import gemm_dW, transpose_acts, DwWorkspace                       # noqa: F401
+from .grads import gemm_dW, transpose_acts, DwWorkspace, expert_dW            # noqa: F401
 from .embed import embed_lookup, DeviceIdGroups, embed_dw                     # noqa: F401
 from .dispatch import RoutePlan, dispatch_grad, combine, combine_grad         # noqa: F401

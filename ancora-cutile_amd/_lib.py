@@ -87,6 +87,12 @@ class DwProblem(C.Structure):
                 ("x_row_major", i32), ("reserved", i32)]
 
 
+class ExpertDwProblem(C.Structure):
+    """anc_expert_dw_problem_t: one stacked weight of the experts' weight-gradient call."""
+    _fields_ = [("x", u64), ("dy", u64), ("dW", u64), ("g16", u64), ("K", i64), ("N", i64),
+                ("accumulate", i32), ("reserved", i32)]
+
+
 # name -> (restype, argtypes); restype None means "int status, checked".
 _PROTOS = {
     "anc_last_error": (C.c_char_p, []),
@@ -163,6 +169,7 @@ _PROTOS = {
     "anc_quant_mxfp8_w_multi": (None, [u64, i32, i64, C.c_int, u64]),
     "anc_gemm_dw_workspace_bytes": (i64, [i64, i64, i64]),
     "anc_gemm_dw_multi": (None, [C.POINTER(DwProblem), i32, u64]),
+    "anc_expert_dw_multi": (None, [C.POINTER(ExpertDwProblem), i32, u64, u64, i64, u64]),
     "anc_gemm_dw_info": (None, [i64, i64, i64, C.POINTER(C.c_double), C.POINTER(i32)]),
     "anc_ns_workspace_bytes": (i64, [i64, i64, i64, C.c_int]),
     "anc_ns_batched": (None, [u64, i64, i64, i64, C.c_int, C.POINTER(f32), f32, C.c_int, u64, i64,

@@ -1,0 +1,251 @@
+// The experts' weight gradients over tokens sorted by expert (anc_route): for every expert e
+//     dW[e] (K, N) (+)= sum over its tokens s of x[s]^T dy[s],   x (slots, K), dy (slots, N) bf16, fp32 accumulation.
+// Segments are ragged and known on the device only, so the grid covers every expert's whole weight and a workgroup reads its segment.
+//
+// One workgroup owns 128x256 outputs of one expert and runs the expert's tokens in ascending order, 32 a step, one accumulator per
+// element: no split of the tokens, an expert's bits are a function of its own rows. Both operands lie token by token, and
+// the product contracts over tokens, so tiles [32 tokens][128 or 256 columns] go straight to LDS and the fragments come from
+// transposing LDS reads. Three stages of 24 KiB, two workgroups per CU: one's stores run under the other's products.
+// Rows past the segment's end and stages past the last are never fetched: the buffer descriptor of a stage ends with the segment, and
+// loads beyond it give zeros. (Columns past K or N are the next row's: they meet outputs that are not stored.)
+#include "lds_dma.h"
+#include "ns_common.h"
+
+namespace {
+
+constexpr int TM = 128, TN = 256, TK = 32, kStages = 3;
+constexpr int kBytesA = TK * TM * 2, kBytesB = TK * TN * 2, kStage = kBytesA + kBytesB;
+constexpr int kLanes = 256, kWaves = 4;                        // a wavefront: all 128 rows x 64 columns
+constexpr int kPiecesA = kBytesA / 1024 / kWaves, kPiecesB = kBytesB / 1024 / kWaves, kPieces = kPiecesA + kPiecesB;
+constexpr int kUnit = 8;                                       // tiles that follow each other on one XCD
+constexpr int kMostProblems = 8;
+
+struct DwOne {
+  const uint16_t *x, *dy;
+  float *dW;
+  uint16_t *g16;
+  int K, N, tn, tiles;                                         // tiles of one expert, tn of them side by side
+  int accumulate;
+};
+struct DwMulti {
+  const int32_t *counts, *offsets;
+  int count, experts;
+  int unit0[kMostProblems + 1];                                // first unit of each problem
+  DwOne p[kMostProblems];
+};
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// `records` bytes from `base` on are there, the rest reads as zero.
+__device__ __forceinline__ i32x4 descriptor(const char *base, uint32_t records) {
+  const uint64_t b = (uint64_t)base;
+  return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)b), __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32) & 0xFFFF),
+               __builtin_amdgcn_readfirstlane((int)records), 0x00020000};
+}
+// 16 bytes per lane from descriptor + off (per lane) to LDS address lds_base + 16 * lane.
+__device__ __forceinline__ void dma16_bounded(i32x4 desc, uint32_t off, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds_base), "v"(off), "s"(desc)
+               : "memory", "m0");
+}
+
+// One operand's rows of a tile: where the next stage starts and how many bytes of the segment are left from there.
+struct Feed {
+  const char *at;
+  int64_t left, step;
+  __device__ __forceinline__ i32x4 desc() const {
+    return descriptor(at, left <= 0 ? 0u : left < 0xFFFFFFFFll ? (uint32_t)left : 0xFFFFFFFFu);
+  }
+  __device__ __forceinline__ void next() { at += step; left -= step; }
+};
+
+__global__ void __launch_bounds__(kLanes, 2) k_expert_dw(DwMulti m) {
+  __shared__ __attribute__((aligned(1024))) unsigned char ring[kStages * kStage];
+  // Units of kUnit tiles are dealt round the XCDs, so that a unit's tiles, which read the same rows, share an L2 and the experts' different
+  // lengths spread over all of them.
+  const int b = (int)blockIdx.x, xcd = b % kXcds, q = b / kXcds;
+  const int unit = (q / kUnit) * kXcds + xcd;
+  int pi = 0;
+  while (pi + 1 < m.count && unit >= m.unit0[pi + 1]) ++pi;
+  if (unit >= m.unit0[m.count]) return;
+  const DwOne &p = m.p[pi];
+  const int per = (p.tiles + kUnit - 1) / kUnit, u = unit - m.unit0[pi], e = u / per, tile = (u - e * per) * kUnit + q % kUnit;
+  if (tile >= p.tiles) return;
+  const int m0 = tile / p.tn * TM, n0 = (tile % p.tn) * TN;
+  const int K = p.K, N = p.N, rows = m.counts[e];
+  const int64_t first = m.offsets[e];
+  const int lane = (int)(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+
+  Feed fa{(const char *)(p.x + first * K + m0), ((int64_t)rows * K - m0) * 2, (int64_t)TK * K * 2};
+  Feed fb{(const char *)(p.dy + first * N + n0), ((int64_t)rows * N - n0) * 2, (int64_t)TK * N * 2};
+  // Piece i of an operand's tile is 1 KiB of LDS: 4 rows of 256 bytes (x) or 2 of 512 (dy). The 16-byte chunk of a row is XORed with 4 * (row & 3),
+  // so that the four rows that a transposing read touches fall into different banks.
+  uint32_t va[kPiecesA], vb[kPiecesB];
+#pragma unroll
+  for (int i = 0; i < kPiecesA; ++i) {
+    const int row = (wave * kPiecesA + i) * 4 + (lane >> 4);
+    va[i] = (uint32_t)(row * K * 2 + (((lane & 15) ^ ((row & 3) << 2)) * 16));
+  }
+#pragma unroll
+  for (int i = 0; i < kPiecesB; ++i) {
+    const int row = (wave * kPiecesB + i) * 2 + (lane >> 5);
+    vb[i] = (uint32_t)(row * N * 2 + (((lane & 31) ^ ((row & 3) << 2)) * 16));
+  }
+  auto issue = [&](int i, const i32x4 &da, const i32x4 &db, unsigned char *stage) {
+    if (i < kPiecesA) dma16_bounded(da, va[i], lds_addr(stage + (wave * kPiecesA + i) * 1024));
+    else dma16_bounded(db, vb[i - kPiecesA], lds_addr(stage + kBytesA + (wave * kPiecesB + i - kPiecesA) * 1024));
+  };
+  auto issue_all = [&](unsigned char *stage) {
+    const i32x4 da = fa.desc(), db = fb.desc();
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) issue(i, da, db, stage);
+    fa.next();
+    fb.next();
+  };
+
+  // Fragments: lane -> column lane % 32 of a 32-column block, 8 consecutive tokens (8 * (lane / 32) on) of 16.
+  int ta[4], tb[2];
+  {
+    const int s16 = lane & 15, g16 = lane >> 4, half = (s16 & 3) >> 1, row = 8 * (g16 >> 1) + (s16 >> 2), sw = (s16 >> 2) << 2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ta[i] = row * 256 + (((i * 4 + 2 * (g16 & 1) + half) ^ sw) * 16) + (s16 & 1) * 8;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      tb[i] = kBytesA + row * 512 + (((wave * 8 + i * 4 + 2 * (g16 & 1) + half) ^ sw) * 16) + (s16 & 1) * 8;
+  }
+  f32x16 acc[4][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+
+  const int steps = (rows + TK - 1) / TK;
+  if (steps > 0) {
+    bf16x8 a[2][4], c[2][2];
+    // fragment i (0 .. 5: b0 b1 a0 a1 a2 a3) of 16 tokens kk of a stage
+    auto load = [&](int set, int i, const unsigned char *stage, int kk) {
+      if (i < 2) c[set][i] = anc_lds_tr_frag(stage + tb[i] + kk * (16 * 512), stage + tb[i] + kk * (16 * 512) + 4 * 512);
+      else a[set][i - 2] = anc_lds_tr_frag(stage + ta[i - 2] + kk * (16 * 256), stage + ta[i - 2] + kk * (16 * 256) + 4 * 256);
+    };
+    auto multiply = [&](int set, int idx) {      // operands exchanged: a lane holds runs of 4 columns of one row
+      acc[idx >> 1][idx & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c[set][idx & 1], a[set][idx >> 1], acc[idx >> 1][idx & 1], 0, 0, 0);
+    };
+    for (int i = 0; i < kStages; ++i) issue_all(ring + i * kStage);
+    wait_vm<2 * kPieces>();
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < 6; ++i) load(0, i, ring, 0);
+    // One step: the first half's products over the reads of the second half; then every wavefront has read the stage and the
+    // next one has landed for all; then the second half's products over the next stage's first reads and the fetches of
+    // the stage after the next two into the place just read.
+    auto step = [&](unsigned char *here, unsigned char *next) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        multiply(0, i);
+        __builtin_amdgcn_sched_barrier(0);
+        if (i < 6) load(1, i, here, 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      wait_vm<kPieces>();
+      lds_barrier();
+      const i32x4 da = fa.desc(), db = fb.desc();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        multiply(1, i);
+        __builtin_amdgcn_sched_barrier(0);
+        if (i < 6) {
+          load(0, i, next, 0);
+          issue(i, da, db, here);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      fa.next();
+      fb.next();
+    };
+    int here = 0;
+    for (int t = 0; t < steps; ++t) {
+      const int next = here + kStage < kStages * kStage ? here + kStage : 0;
+      step(ring + here, ring + next);
+      here = next;
+    }
+  }
+  wait_vm<0>();                                  // (zeros still on their way into the stages)
+  lds_barrier();
+
+  // Out through LDS, 32 rows of 64 columns at a time, so that stores are rows of 256 bytes.
+  unsigned char *r = ring + wave * 8192;
+  const int cols = N - n0 - wave * 64;           // this wavefront's columns that exist
+  const int64_t out0 = (int64_t)e * K * N + (int64_t)m0 * N + n0 + wave * 64;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int rr = lane & 31, hh = lane >> 5;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *(anc_f32x4 *)(r + rr * 256 + (((j * 8 + 2 * g + hh) ^ (rr & 15)) * 16)) =
+            anc_f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+    lds_wave_sync();
+#pragma unroll
+    for (int z = 0; z < 8; ++z) {
+      const int idx = z * 64 + lane, row = idx >> 4, ch = idx & 15;
+      anc_f32x4 v = *(const anc_f32x4 *)(r + row * 256 + ((ch ^ (row & 15)) * 16));
+      if (m0 + i * 32 + row < K && ch * 4 < cols) {
+        const int64_t off = out0 + (int64_t)(i * 32 + row) * N + ch * 4;
+        if (p.accumulate) {
+          const anc_f32x4 o = *(const anc_f32x4 *)(p.dW + off);
+          v = anc_f32x4{o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w};
+        }
+        anc_st_stream((anc_f32x4 *)(p.dW + off), v);
+        if (p.g16 != nullptr) anc_st_stream((anc_u32x2 *)(p.g16 + off), anc_u32x2{anc_pk_bf16(v.x, v.y), anc_pk_bf16(v.z, v.w)});
+      }
+    }
+    lds_wave_sync();
+  }
+}
+
+}  // namespace
+
+extern "C" int anc_expert_dw_multi(const anc_expert_dw_problem_t *probs, int32_t n_probs, uint64_t counts, uint64_t offsets,
+                                   int64_t experts, uint64_t stream) {
+  ANC_REQUIRE(probs != nullptr && n_probs >= 1 && n_probs <= kMostProblems, "anc_expert_dw_multi: 1..%d problems", kMostProblems);
+  ANC_REQUIRE(counts && offsets && ((counts | offsets) & 3) == 0 && experts > 0 && experts <= 512,
+              "anc_expert_dw_multi: bad segments (%lld experts)", (long long)experts);
+  DwMulti m{};
+  m.counts = (const int32_t *)counts;
+  m.offsets = (const int32_t *)offsets;
+  m.count = n_probs;
+  m.experts = (int)experts;
+  int64_t units = 0;
+  for (int i = 0; i < n_probs; ++i) {
+    const anc_expert_dw_problem_t &b = probs[i];
+    ANC_REQUIRE(b.K > 0 && b.N > 0 && b.K % 8 == 0 && b.N % 8 == 0 && b.K <= (1 << 20) && b.N <= (1 << 20),
+                "anc_expert_dw_multi: needs K %% 8 == 0 and N %% 8 == 0 (K=%lld N=%lld)", (long long)b.K, (long long)b.N);
+    ANC_REQUIRE(b.x && b.dy && b.dW && ((b.x | b.dy | b.dW) & 15) == 0 && (b.g16 & 7) == 0,
+                "anc_expert_dw_multi: null or misaligned pointer");
+    DwOne &p = m.p[i];
+    p.x = (const uint16_t *)b.x;
+    p.dy = (const uint16_t *)b.dy;
+    p.dW = (float *)b.dW;
+    p.g16 = (uint16_t *)b.g16;
+    p.K = (int)b.K;
+    p.N = (int)b.N;
+    p.accumulate = b.accumulate != 0;
+    p.tn = (p.N + TN - 1) / TN;
+    const int64_t tiles = (int64_t)((p.K + TM - 1) / TM) * p.tn;
+    ANC_REQUIRE(tiles < (1 << 24), "anc_expert_dw_multi: %lld x %lld is too large", (long long)b.K, (long long)b.N);
+    p.tiles = (int)tiles;
+    m.unit0[i] = (int)units;
+    units += (tiles + kUnit - 1) / kUnit * experts;
+    ANC_REQUIRE(units < (1 << 27), "anc_expert_dw_multi: too large for one call");
+  }
+  for (int i = n_probs; i <= kMostProblems; ++i) m.unit0[i] = (int)units;
+  const int64_t grid = (units + kXcds - 1) / kXcds * kXcds * kUnit;
+  ANC_REQUIRE(grid < (1ll << 31), "anc_expert_dw_multi: too large for one call");
+  hipStream_t s = anc_stream(stream);
+  AncProfScope prof(ANC_PROF_DW_GEMM, s);
+  hipLaunchKernelGGL(k_expert_dw, dim3((unsigned)grid), dim3(kLanes), 0, s, m);
+  ANC_LAUNCH_CHECK();
+  return ANC_OK;
+}

@@ -20,12 +20,14 @@ import struct
 import numpy as np
 
 from . import _lib
-from ._lib import api, DwProblem
+from ._lib import api, DwProblem, ExpertDwProblem
 from .devbuf import DevBuf
 
 MAX_PER_CALL = 8
 _DW = struct.Struct("=5Q4q2iQ2i")          # anc_dw_problem_t
 assert _DW.size == ctypes.sizeof(DwProblem)
+_EDW = struct.Struct("=4Q2q2i")            # anc_expert_dw_problem_t
+assert _EDW.size == ctypes.sizeof(ExpertDwProblem)
 
 
 def dw_workspace_bytes(T, K, N):
@@ -113,3 +115,37 @@ def gemm_dW(problems, si=0, segments=None):
                           0 if g16 is None else g16.ptr, ws_ptr, T, K, N, ws_bytes,
                           1 if p.get("accumulate", False) else 0, S, gn, 0 if x is None else 1, 0)
         api.anc_gemm_dw_multi(arr, len(group), int(si))
+
+
+def _expert_problem(plan, p):
+    """(K, N) of one problem of `expert_dW`, its buffers checked against the plan."""
+    x, dy, dW, g16 = p["x"], p["dy"], p["dW"], p.get("g16")
+    K, N = x.shape[-1], dy.shape[-1]
+    for name, b in (("x", x), ("dy", dy)):
+        if b.dtype != np.uint16 or len(b.shape) != 2 or b.shape[0] < plan.capacity:
+            raise ValueError(f"expert_dW: {name} is {b.shape} {b.dtype}, ({plan.capacity}, ...) of bf16 bits expected")
+    for name, b, dtype in (("dW", dW, np.float32), ("g16", g16, np.uint16)):
+        if b is not None and (b.dtype != dtype or b.size != plan.E * K * N or b.shape[-1] != N):
+            raise ValueError(f"expert_dW: {name} is {b.shape} {b.dtype}, ({plan.E}, {K}, {N}) {np.dtype(dtype)} expected")
+    if K % 8 or N % 8:
+        raise ValueError(f"expert_dW: K={K} and N={N} must be multiples of 8")
+    return K, N
+
+
+def expert_dW(plan, problems, si=0):
+    """The experts' weight gradients over tokens that `plan` (a `dispatch.RoutePlan`) has sorted: problems is a list of dicts
+    {x (capacity, K), dy (capacity, N): DevBuf of bf16 bits; dW: DevBuf (E, K, N) or (E*K, N) fp32; g16: DevBuf of the same shape for
+    the bf16 copy, or None; accumulate: bool}. dW[e] (+)= x[segment e]^T dy[segment e] for each, 8 weights per launch (hand over the
+    three of a layer in one call). Experts without tokens get zeros. What `ExpertOptimizer.step` and `GroupedMoEFFNOptim.step`
+    read. Asynchronous on stream `si`."""
+    plan._used("expert_dW")
+    shapes = [_expert_problem(plan, p) for p in problems]
+    counts, offsets = plan._at[:2]
+    for i in range(0, len(problems), MAX_PER_CALL):
+        group = problems[i:i + MAX_PER_CALL]
+        arr = (ExpertDwProblem * len(group))()
+        for k, (p, (K, N)) in enumerate(zip(group, shapes[i:])):
+            g16 = p.get("g16")
+            _EDW.pack_into(arr, k * _EDW.size, p["x"].ptr, p["dy"].ptr, p["dW"].ptr, 0 if g16 is None else g16.ptr, K, N,
+                           1 if p.get("accumulate", False) else 0, 0)
+        api.anc_expert_dw_multi(arr, len(group), counts, offsets, plan.E, int(si))

@@ -486,6 +486,20 @@ int anc_gemm_dw_multi(const anc_dw_problem_t *problems, int32_t n_problems, uint
 /* FLOPs of one problem (2 T K N, all executed) and the segment count of the shape rule (segments = -1). */
 int anc_gemm_dw_info(int64_t T, int64_t K, int64_t N, double *flops, int32_t *segments);
 
+/* The experts' weight gradients over tokens sorted by expert: for every expert dW[e] (+)= x_e^T dy_e over the counts[e] rows from
+ * slot offsets[e] on (the arrays of anc_route, on the device: no host round trip), up to 8 weights per call. x (slots, K) and
+ * dy (slots, N) bf16, dW (experts, K, N) fp32 overwritten, or added onto when `accumulate` is set; an expert without tokens gets zeros
+ * (or keeps dW). g16, if not 0, receives the bf16 copy of the final dW. Rows that fill up a segment are not read, whatever they hold.
+ * An expert's tokens are added in ascending order, one accumulator per element: its bits are a function of its own rows.
+ * K, N multiples of 8; x, dy, dW 16-byte aligned. */
+typedef struct {
+  uint64_t x, dy, dW, g16;
+  int64_t  K, N;
+  int32_t  accumulate, reserved;
+} anc_expert_dw_problem_t;
+int anc_expert_dw_multi(const anc_expert_dw_problem_t *problems, int32_t n_problems, uint64_t counts, uint64_t offsets,
+                        int64_t experts, uint64_t stream);
+
 /* MXFP8 re-quantisation of bf16 weights (E, K, N) after the step: per block of 32 consecutive K
  * and per column one E8M0 scale byte = (biased fp32 exponent of the block's amax) - 7 (0 below
  * 7), elements E4M3FN(w / 2^(byte-127)) rounded to nearest even. col_major = 0 writes

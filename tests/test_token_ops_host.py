@@ -182,3 +182,42 @@ def test_routing_calls_that_do_not_fit_launch_nothing(fake_device):
     for bad in (lambda: p.route(ids, 0), lambda: dispatch(p, x, 0, xs)):
         with pytest.raises(AncoraError):
             bad()
+
+
+def test_expert_gradient_refusals(lib):
+    import ctypes
+    from ancora_cutile_amd._lib import ExpertDwProblem
+    fields = dict(x=P, dy=P, dW=P, g16=0, K=64, N=128, accumulate=0, reserved=0)
+
+    def call(n=1, counts=P, offsets=P, experts=4, **kw):
+        arr = (ExpertDwProblem * 9)(*[ExpertDwProblem(**{**fields, **kw}) for _ in range(9)])
+        return lib.anc_expert_dw_multi(arr, n, counts, offsets, experts, 0)
+
+    for kw, word in ((dict(n=0), "problems"), (dict(n=9), "problems"), (dict(counts=0), "segments"), (dict(offsets=P + 2), "segments"),
+                     (dict(experts=0), "segments"), (dict(experts=513), "segments"), (dict(K=12), "K % 8"), (dict(N=0), "K % 8"),
+                     (dict(N=(1 << 20) + 8), "K % 8"), (dict(x=0), "null"), (dict(dy=P + 8), "misaligned"), (dict(dW=P + 4), "misaligned"),
+                     (dict(g16=P + 4), "misaligned")):
+        assert call(**kw) == 2 and word in lib.anc_last_error().decode(), (kw, lib.anc_last_error())
+    assert lib.anc_expert_dw_multi(ctypes.POINTER(ExpertDwProblem)(), 1, P, P, 4, 0) == 2
+
+
+def test_expert_gradient_calls_that_do_not_fit_launch_nothing(fake_device):
+    from ancora_cutile_amd import RoutePlan, expert_dW
+    from ancora_cutile_amd._lib import AncoraError
+    E, K, N = 3, 16, 24
+    p = RoutePlan(10, 2, E, 4)
+    S = p.capacity
+    good = dict(x=_buf((S, K), np.uint16), dy=_buf((S, N), np.uint16), dW=_buf((E, K, N), np.float32))
+    with pytest.raises(AncoraError):
+        expert_dW(p, [good], 0)
+    p.route(_buf((10, 2), np.int32), 0)
+    for bad in (dict(x=_buf((S - 1, K), np.uint16)), dict(x=_buf((S, K), np.float32)), dict(dy=_buf((S * N,), np.uint16)),
+                dict(dW=_buf((E, K, N), np.uint16)), dict(dW=_buf((E, K, N + 8), np.float32)), dict(dW=_buf((E, N, K), np.float32)),
+                dict(g16=_buf((E, K, N), np.float32)), dict(x=_buf((S, 12), np.uint16), dW=_buf((E, 12, N), np.float32))):
+        with pytest.raises(ValueError):
+            expert_dW(p, [good, {**good, **bad}], 0)
+    assert not fake_device.calls("anc_expert_dw_multi")
+    expert_dW(p, [dict(good, dW=_buf((E * K, N), np.float32))] * 11, 0)
+    assert [a[1] for a in fake_device.calls("anc_expert_dw_multi")] == [8, 3]
+    expert_dW(p, [], 0)
+    assert len(fake_device.calls("anc_expert_dw_multi")) == 2
