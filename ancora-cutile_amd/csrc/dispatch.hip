@@ -28,30 +28,38 @@ __device__ __forceinline__ void clear_padding(int b, int align, const int32_t *c
 
 template <int T, int VEC>
 __global__ void __launch_bounds__(kLanes)
-k_dispatch(const int32_t *__restrict__ slot, const int32_t *__restrict__ counts, const int32_t *__restrict__ offsets, int64_t tokens,
-           int k, int align, int64_t main_blocks, uint32_t pieces, int64_t H, const elem_t<T> *__restrict__ x,
+k_dispatch(const int32_t *__restrict__ slot, const int32_t *__restrict__ counts, const int32_t *__restrict__ offsets, uint32_t total,
+           int k, int align, uint32_t main_blocks, FastDiv pieces, int64_t H, const elem_t<T> *__restrict__ x,
            elem_t<T> *__restrict__ xs) {
-  if ((int64_t)blockIdx.x >= main_blocks) {
-    clear_padding<T, VEC>((int)((int64_t)blockIdx.x - main_blocks), align, counts, offsets, H, xs);
+  if (blockIdx.x >= main_blocks) {
+    clear_padding<T, VEC>((int)(blockIdx.x - main_blocks), align, counts, offsets, H, xs);
     return;
   }
-  const int64_t i = (int64_t)blockIdx.x * kLanes + threadIdx.x, t = i / pieces;
-  if (t >= tokens) return;
-  const int64_t col = (i - t * pieces) * VEC;
-  const Raw<T, VEC> v = load<T, VEC>(x + t * H + col);
-  for (int j = 0; j < k; ++j) {
-    const int64_t s = slot[t * k + j];
-    if (s >= 0) store<T, VEC>(xs + s * H + col, v);
+  const uint32_t i = blockIdx.x * (uint32_t)kLanes + threadIdx.x;
+  if (i >= total) return;
+  const uint32_t t = pieces.div(i);
+  const int64_t col = (int64_t)(i - t * pieces.d) * VEC;
+  const Raw<T, VEC> v = load<T, VEC>(x + (int64_t)t * H + col);
+  const int32_t *to = slot + (int64_t)t * k;
+  constexpr int D = 4;
+  for (int j0 = 0; j0 < k; j0 += D) {
+    int64_t s[D];
+#pragma unroll
+    for (int j = 0; j < D; ++j) s[j] = to[j0 + j < k ? j0 + j : k - 1];
+#pragma unroll
+    for (int j = 0; j < D; ++j)
+      if (j0 + j < k && s[j] >= 0) store<T, VEC>(xs + s[j] * H + col, v);
   }
 }
 
 template <int TI, int TO, int VEC, bool WEIGHTS>
 __global__ void __launch_bounds__(kLanes)
-k_combine(const int32_t *__restrict__ slot, const float *__restrict__ w, int64_t tokens, int k, uint32_t pieces, int64_t H,
+k_combine(const int32_t *__restrict__ slot, const float *__restrict__ w, uint32_t total, int k, FastDiv pieces, int64_t H,
           const elem_t<TI> *__restrict__ ys, elem_t<TO> *__restrict__ y) {
-  const int64_t i = (int64_t)blockIdx.x * kLanes + threadIdx.x, t = i / pieces;
-  if (t >= tokens) return;
-  const int64_t col = (i - t * pieces) * VEC;
+  const uint32_t i = blockIdx.x * (uint32_t)kLanes + threadIdx.x;
+  if (i >= total) return;
+  const uint32_t row = pieces.div(i);
+  const int64_t t = row, col = (int64_t)(i - row * pieces.d) * VEC;
   float acc[VEC];
 #pragma unroll
   for (int q = 0; q < VEC; ++q) acc[q] = 0.0f;
@@ -62,8 +70,10 @@ k_combine(const int32_t *__restrict__ slot, const float *__restrict__ w, int64_t
     float f[D];
 #pragma unroll
     for (int j = 0; j < D; ++j) {
-      s[j] = j0 + j < k ? slot[t * k + j0 + j] : -1;
-      f[j] = WEIGHTS && j0 + j < k ? w[t * k + j0 + j] : 1.0f;
+      const int64_t a = t * k + (j0 + j < k ? j0 + j : k - 1);
+      const int64_t at = slot[a];
+      f[j] = WEIGHTS ? w[a] : 1.0f;
+      s[j] = j0 + j < k ? at : -1;
     }
 #pragma unroll
     for (int j = 0; j < D; ++j)
@@ -80,7 +90,9 @@ k_combine(const int32_t *__restrict__ slot, const float *__restrict__ w, int64_t
   store<TO, VEC>(y + t * H + col, acc);
 }
 
-// One wavefront per token: its row of dy stays in registers over the k choices, the products are summed over the lanes.
+// One wavefront per token, four choices at a time: their rows are in flight together, dy comes from the caches for the next
+// four. The four products' sums over the lanes are made together: at the first two steps of the butterfly a lane hands half of its sums
+// on and keeps the other half, so that four sums take 7 exchanges instead of 24.
 template <int TY, int TS, int VEC>
 __global__ void __launch_bounds__(kLanes)
 k_combine_grad(const int32_t *__restrict__ slot, const float *__restrict__ w, const int32_t *__restrict__ counts,
@@ -92,26 +104,50 @@ k_combine_grad(const int32_t *__restrict__ slot, const float *__restrict__ w, co
     return;
   }
   const int lane = (int)(threadIdx.x & 63);
-  const int64_t t = (int64_t)blockIdx.x * (kLanes / 64) + (threadIdx.x >> 6);
+  const int64_t t = (int64_t)blockIdx.x * (kLanes / 64) + __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   if (t >= tokens) return;
-  for (int j = 0; j < k; ++j) {
-    const int64_t s = slot[t * k + j];
-    const float f = w[t * k + j];
-    float dot = 0.0f;
-    if (s >= 0)
-      for (int64_t col = (int64_t)lane * VEC; col < H; col += 64 * VEC) {
-        float g[VEC], a[VEC], o[VEC];
-        widen<TY, VEC>(load<TY, VEC>(dy + t * H + col), g);
-        widen<TS, VEC>(load<TS, VEC>(ys + s * H + col), a);
+  constexpr int D = 4;
+  for (int j0 = 0; j0 < k; j0 += D) {
+    int64_t s[D];
+    float f[D], dot[D];
+#pragma unroll
+    for (int j = 0; j < D; ++j) {
+      const int64_t a = t * k + (j0 + j < k ? j0 + j : k - 1);
+      s[j] = slot[a];
+      f[j] = w[a];
+      dot[j] = 0.0f;
+      if (j0 + j >= k) s[j] = -1;
+    }
+    for (int64_t col = (int64_t)lane * VEC; col < H; col += 64 * VEC) {
+      float g[VEC];
+      Raw<TS, VEC> v[D];
+      const Raw<TY, VEC> own = load<TY, VEC>(dy + t * H + col);
+#pragma unroll
+      for (int j = 0; j < D; ++j)
+        if (s[j] >= 0) v[j] = load<TS, VEC>(ys + s[j] * H + col);
+      widen<TY, VEC>(own, g);
+#pragma unroll
+      for (int j = 0; j < D; ++j) {
+        if (s[j] < 0) continue;
+        float a[VEC], o[VEC];
+        widen<TS, VEC>(v[j], a);
 #pragma unroll
         for (int q = 0; q < VEC; ++q) {
-          dot = fmaf(g[q], a[q], dot);
-          o[q] = f * g[q];
+          dot[j] = fmaf(g[q], a[q], dot[j]);
+          o[q] = f[j] * g[q];
         }
-        store<TS, VEC>(dys + s * H + col, o);
+        store<TS, VEC>(dys + s[j] * H + col, o);
       }
-    dot = anc_wave_sum_f32(dot);
-    if (lane == 0) dw[t * k + j] = dot;
+    }
+    // lane bit 5 chooses the pair (0, 1) or (2, 3), bit 4 the one of the pair
+    const bool hi = (lane & 32) != 0, odd = (lane & 16) != 0;
+    const float a = (hi ? dot[2] : dot[0]) + __shfl_xor(hi ? dot[0] : dot[2], 32, 64);
+    const float b = (hi ? dot[3] : dot[1]) + __shfl_xor(hi ? dot[1] : dot[3], 32, 64);
+    float sum = (odd ? b : a) + __shfl_xor(odd ? a : b, 16, 64);
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    const int j = j0 + (hi ? 2 : 0) + (odd ? 1 : 0);
+    if ((lane & 15) == 0 && j < k) dw[t * k + j] = sum;
   }
 }
 
@@ -138,19 +174,21 @@ extern "C" int anc_dispatch(uint64_t slot, uint64_t counts, uint64_t offsets, in
   ANC_REQUIRE(x && xs && (x | xs) % (uint64_t)elem_size(type) == 0, "anc_dispatch: null or misaligned pointers");
   const Ptr ps[2] = {{x, type}, {xs, type}};
   const int vec = piece(H, ps);
-  const int64_t blocks = (tokens * (H / vec) + kLanes - 1) / kLanes, all = blocks + pad_blocks(experts, align);
-  ANC_REQUIRE(all < (1ll << 31), "anc_dispatch: too large for one call");
-  if (tokens == 0) return ANC_OK;
+  const int64_t per_row = H / vec, most = kMostPieces / per_row;
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_MISC, s);
-  with_type(type, [&](auto t) {
-    with_piece(vec, [&](auto v) {
-      constexpr int T = decltype(t)::value, VEC = decltype(v)::value;
-      hipLaunchKernelGGL((k_dispatch<T, VEC>), dim3((unsigned)all), dim3(kLanes), 0, s, (const int32_t *)slot, (const int32_t *)counts,
-                         (const int32_t *)offsets, tokens, (int)k, (int)align, blocks, (uint32_t)(H / VEC), H, (const elem_t<T> *)x,
-                         (elem_t<T> *)xs);
+  for (int64_t r = 0; r < tokens; r += most) {       // (the first launch clears the padding)
+    const int64_t rows = tokens - r < most ? tokens - r : most, total = rows * per_row;
+    const int64_t blocks = (total + kLanes - 1) / kLanes, all = blocks + (r == 0 ? pad_blocks(experts, align) : 0);
+    with_type(type, [&](auto t) {
+      with_piece(vec, [&](auto v) {
+        constexpr int T = decltype(t)::value, VEC = decltype(v)::value;
+        hipLaunchKernelGGL((k_dispatch<T, VEC>), dim3((unsigned)all), dim3(kLanes), 0, s, (const int32_t *)slot + r * k,
+                           (const int32_t *)counts, (const int32_t *)offsets, (uint32_t)total, (int)k, (int)align, (uint32_t)blocks,
+                           fast_div((uint32_t)per_row), H, (const elem_t<T> *)x + r * H, (elem_t<T> *)xs);
+      });
     });
-  });
+  }
   ANC_LAUNCH_CHECK();
   return ANC_OK;
 }
@@ -163,21 +201,23 @@ extern "C" int anc_combine(uint64_t slot, uint64_t weights, int64_t tokens, int6
               "anc_combine: null or misaligned pointers");
   const Ptr ps[2] = {{ys, ys_type}, {y, y_type}};
   const int vec = piece(H, ps);
-  const int64_t blocks = (tokens * (H / vec) + kLanes - 1) / kLanes;
-  ANC_REQUIRE(blocks < (1ll << 31), "anc_combine: too large for one call");
-  if (tokens == 0) return ANC_OK;
+  const int64_t per_row = H / vec, most = kMostPieces / per_row;
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_MISC, s);
-  with_type(ys_type, [&](auto ti) {
-    with_type(y_type, [&](auto to) {
-      with_piece(vec, [&](auto v) {
-        constexpr int TI = decltype(ti)::value, TO = decltype(to)::value, VEC = decltype(v)::value;
-        auto kernel = weights != 0 ? k_combine<TI, TO, VEC, true> : k_combine<TI, TO, VEC, false>;
-        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kLanes), 0, s, (const int32_t *)slot, (const float *)weights, tokens,
-                           (int)k, (uint32_t)(H / VEC), H, (const elem_t<TI> *)ys, (elem_t<TO> *)y);
+  for (int64_t r = 0; r < tokens; r += most) {
+    const int64_t rows = tokens - r < most ? tokens - r : most, total = rows * per_row;
+    with_type(ys_type, [&](auto ti) {
+      with_type(y_type, [&](auto to) {
+        with_piece(vec, [&](auto v) {
+          constexpr int TI = decltype(ti)::value, TO = decltype(to)::value, VEC = decltype(v)::value;
+          auto kernel = weights != 0 ? k_combine<TI, TO, VEC, true> : k_combine<TI, TO, VEC, false>;
+          hipLaunchKernelGGL(kernel, dim3((unsigned)((total + kLanes - 1) / kLanes)), dim3(kLanes), 0, s, (const int32_t *)slot + r * k,
+                             weights != 0 ? (const float *)weights + r * k : (const float *)nullptr, (uint32_t)total, (int)k,
+                             fast_div((uint32_t)per_row), H, (const elem_t<TI> *)ys, (elem_t<TO> *)y + r * H);
+        });
       });
     });
-  });
+  }
   ANC_LAUNCH_CHECK();
   return ANC_OK;
 }

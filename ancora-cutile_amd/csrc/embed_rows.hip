@@ -8,27 +8,35 @@ namespace {
 
 using namespace anc_rows;
 
-// One piece of VEC elements per lane, (row, piece) flattened over the grid.
+// U pieces of VEC elements per lane, (row, piece) flattened over the grid. The U ids and then the U pieces are in flight together.
 constexpr int kLookupLanes = 256;
-template <int TT, int TO, int VEC>
+template <int TT, int TO, int VEC, int U>
 __global__ void __launch_bounds__(kLookupLanes)
-k_embed_lookup(const void *__restrict__ ids, int wide, int64_t n, int64_t V, uint32_t pieces, int64_t H, float scale,
+k_embed_lookup(const void *__restrict__ ids, int wide, uint32_t total, int64_t V, FastDiv pieces, int64_t H, float scale,
                const elem_t<TT> *__restrict__ table, elem_t<TO> *__restrict__ out) {
-  const int64_t i = (int64_t)blockIdx.x * kLookupLanes + threadIdx.x;
-  const int64_t row = i / pieces;
-  if (row >= n) return;
-  const int64_t col = (i - row * pieces) * VEC;
-  const int64_t id = wide ? ((const int64_t *)ids)[row] : (int64_t)((const int32_t *)ids)[row];
-  float x[VEC];
-  if (id >= 0 && id < V) {
-    widen<TT, VEC>(load<TT, VEC>(table + id * H + col), x);
+  const uint32_t first = blockIdx.x * (uint32_t)(kLookupLanes * U) + threadIdx.x;
+  uint32_t row[U];
+  int64_t id[U], col[U];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) x[k] = x[k] * scale;
-  } else {
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) x[k] = 0.0f;
+  for (int u = 0; u < U; ++u) {
+    const uint32_t i = first + u * kLookupLanes < total ? first + u * kLookupLanes : total - 1;
+    row[u] = pieces.div(i);
+    col[u] = (int64_t)(i - row[u] * pieces.d) * VEC;
+    id[u] = wide ? ((const int64_t *)ids)[row[u]] : (int64_t)((const int32_t *)ids)[row[u]];
   }
-  store<TO, VEC>(out + row * H + col, x);
+  Raw<TT, VEC> r[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) r[u] = load<TT, VEC>(table + (id[u] >= 0 && id[u] < V ? id[u] : 0) * H + col[u]);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (first + u * kLookupLanes >= total) return;
+    float x[VEC];
+    widen<TT, VEC>(r[u], x);
+    const bool there = id[u] >= 0 && id[u] < V;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) x[k] = there ? x[k] * scale : 0.0f;
+    store<TO, VEC>(out + (int64_t)row[u] * H + col[u], x);
+  }
 }
 
 // The gradient walks the sorted positions in chunks of `chunk` (at most 64): a workgroup takes one chunk's rows of dy one after the
@@ -44,27 +52,13 @@ struct EmbedDw {
 };
 constexpr int kDwLanes = 256;
 
-template <int VEC> __device__ __forceinline__ void put_row(const EmbedDw &p, int g, int64_t key, int64_t col, const float (&acc)[VEC]) {
-  float x[VEC];
-  if (p.compact != nullptr) {
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) x[k] = p.scale * acc[k];
-    store<ANC_F32, VEC>(p.compact + (int64_t)g * p.H + col, x);
-  } else {
-    float *at = p.out + key * p.H + col;
-    widen<ANC_F32, VEC>(load<ANC_F32, VEC>(at), x);
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) x[k] = x[k] + p.scale * acc[k];
-    store<ANC_F32, VEC>(at, x);
-  }
-}
-
-template <int TD, int VEC>
+template <int TD, int VEC, bool DENSE>
 __global__ void __launch_bounds__(kDwLanes) k_embed_dw(EmbedDw p, const elem_t<TD> *__restrict__ dy) {
   const int lane = (int)(threadIdx.x & 63);
   const int64_t p0 = (int64_t)blockIdx.x * p.chunk, here = p0 + lane;
   const bool in = lane < p.chunk && here < p.n;
-  const int idx = in ? p.srt[here] : 0, grp = in ? p.grp[here] : -1, key = in ? p.key[here] : 0;
+  const int64_t at = in ? here : p.n - 1;
+  const int idx = p.srt[at], key = p.key[at], read = p.grp[at], grp = in ? read : -1;
   const int came = p0 > 0 ? p.grp[p0 - 1] : -1;                          // the group before the chunk
   const int goes = p0 + p.chunk < p.n ? p.grp[p0 + p.chunk] : -1;        // ... and behind it
   const int m = __popcll(__ballot(grp >= 0));                            // (ids that name no row lie at the end)
@@ -72,62 +66,70 @@ __global__ void __launch_bounds__(kDwLanes) k_embed_dw(EmbedDw p, const elem_t<T
   const bool live = col < p.H;
   const int64_t c0 = live ? col : 0;                                     // (every lane stays: its indices serve the others)
   float acc[VEC];
-  int cur = -1, cur_key = 0;
-  auto flush = [&]() {
-    if (cur < 0 || !live) return;
-    if (cur == came || cur == goes)
-      store<ANC_F32, VEC>(p.part + ((int64_t)blockIdx.x * 2 + (cur == came ? 0 : 1)) * p.H + c0, acc);
-    else
-      put_row<VEC>(p, cur, cur_key, c0, acc);
-  };
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
   constexpr int D = 8;
   for (int i = 0; i < m; i += D) {
     Raw<TD, VEC> v[D];
+    Raw<ANC_F32, VEC> old[DENSE ? D : 1];
+    int g[D], next[D];
 #pragma unroll
     for (int j = 0; j < D; ++j) {
-      const int r = __builtin_amdgcn_readlane(idx, i + j < m ? i + j : m - 1);
-      v[j] = load<TD, VEC>(dy + (int64_t)r * p.H + c0);
+      const int q = i + j < m ? i + j : m - 1;
+      g[j] = __builtin_amdgcn_readlane(grp, q);
+      next[j] = q + 1 < m ? __builtin_amdgcn_readlane(grp, q + 1) : -1;  // (a group that goes on behind the chunk ends here, too)
+      v[j] = load<TD, VEC>(dy + (int64_t)__builtin_amdgcn_readlane(idx, q) * p.H + c0);
+      if constexpr (DENSE)
+        if (next[j] != g[j] && g[j] != came && g[j] != goes)
+          old[j] = load<ANC_F32, VEC>(p.out + (int64_t)__builtin_amdgcn_readlane(key, q) * p.H + c0);
     }
 #pragma unroll
     for (int j = 0; j < D; ++j) {
-      if (i + j >= m) break;
-      const int g = __builtin_amdgcn_readlane(grp, i + j);
-      if (g != cur) {
-        flush();
-        cur = g;
-        cur_key = __builtin_amdgcn_readlane(key, i + j);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
-      }
+      if (i + j >= m) continue;
       float x[VEC];
       widen<TD, VEC>(v[j], x);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) acc[k] = acc[k] + x[k];
+      if (next[j] == g[j]) continue;
+      if (live) {
+        if (g[j] == came || g[j] == goes) {
+          store<ANC_F32, VEC>(p.part + ((int64_t)blockIdx.x * 2 + (g[j] == came ? 0 : 1)) * p.H + c0, acc);
+        } else {
+          if constexpr (DENSE) widen<ANC_F32, VEC>(old[j], x);
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) x[k] = DENSE ? x[k] + p.scale * acc[k] : p.scale * acc[k];
+          store<ANC_F32, VEC>(DENSE ? p.out + (int64_t)__builtin_amdgcn_readlane(key, i + j) * p.H + c0 : p.compact + (int64_t)g[j] * p.H + c0, x);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
     }
   }
-  flush();
 }
 
 // Chunk c's part 1 begins a group that goes on: the parts of it, in order. The four wavefronts take a quarter of the list each
-// (a third of 65536 positions on one id: 676 partial rows), their sums meet in LDS.
+// (a third of 65536 positions on one id: 338 partial rows of 64 positions), 16 rows in flight, and their sums meet in LDS.
 template <int VEC>
 __global__ void __launch_bounds__(kDwLanes) k_embed_dw_join(EmbedDw p) {
   constexpr int W = kDwLanes / 64;
   __shared__ float sums[W][64 * VEC];
   const int64_t c = blockIdx.x, last = (c + 1) * p.chunk - 1;
   if (last + 1 >= p.n) return;
-  const int g = p.grp[last];
-  if (g < 0 || p.grp[last + 1] != g || (c > 0 && p.grp[last - p.chunk] == g)) return;     // (uniform over the workgroup)
-  const int64_t ce = ((int64_t)p.start[g] + p.cnt[g] - 1) / p.chunk;
+  const int g = p.grp[last], behind = p.grp[last + 1], before = c > 0 ? p.grp[last - p.chunk] : -1;
+  if (g < 0 || behind != g || before == g) return;     // (uniform over the workgroup)
+  const int64_t key = p.key[last], ce = ((int64_t)p.start[g] + p.cnt[g] - 1) / p.chunk;
   const int lane = (int)(threadIdx.x & 63), wave = (int)(threadIdx.x >> 6);
   const int64_t col = ((int64_t)blockIdx.y * 64 + lane) * VEC;
   const bool live = col < p.H;
   const int64_t c0 = live ? col : 0, many = ce - c + 1, per = (many + W - 1) / W;
   const int64_t lo = wave * per < many ? wave * per : many, hi = lo + per < many ? lo + per : many;
+  float *to = p.compact != nullptr ? p.compact + (int64_t)g * p.H + c0 : p.out + key * p.H + c0;
+  Raw<ANC_F32, VEC> old;
+  if (p.compact == nullptr) old = load<ANC_F32, VEC>(to);
   float acc[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
-  constexpr int D = 8;
+  constexpr int D = 16;
   for (int64_t i = lo; i < hi; i += D) {
     Raw<ANC_F32, VEC> v[D];
 #pragma unroll
@@ -137,11 +139,12 @@ __global__ void __launch_bounds__(kDwLanes) k_embed_dw_join(EmbedDw p) {
     }
 #pragma unroll
     for (int j = 0; j < D; ++j) {
-      if (i + j >= hi) break;
       float x[VEC];
       widen<ANC_F32, VEC>(v[j], x);
+      if (i + j < hi) {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) acc[k] = acc[k] + x[k];
+        for (int k = 0; k < VEC; ++k) acc[k] = acc[k] + x[k];
+      }
     }
   }
 #pragma unroll
@@ -152,7 +155,11 @@ __global__ void __launch_bounds__(kDwLanes) k_embed_dw_join(EmbedDw p) {
   for (int w = 1; w < W; ++w)
 #pragma unroll
     for (int k = 0; k < VEC; ++k) acc[k] = acc[k] + sums[w][lane * VEC + k];
-  put_row<VEC>(p, g, p.key[last], c0, acc);
+  float x[VEC];
+  if (p.compact == nullptr) widen<ANC_F32, VEC>(old, x);
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) x[k] = p.compact == nullptr ? x[k] + p.scale * acc[k] : p.scale * acc[k];
+  store<ANC_F32, VEC>(to, x);
 }
 
 // Positions per chunk: enough chunks to fill the card, at most 64 (one index per lane).
@@ -160,6 +167,7 @@ constexpr int64_t kChunk16Most = 16384, kChunk32Most = 32768;
 int dw_chunk(int64_t n) { return n <= kChunk16Most ? 16 : n <= kChunk32Most ? 32 : 64; }
 int64_t dw_chunks(int64_t n) { return (n + dw_chunk(n) - 1) / dw_chunk(n); }
 constexpr int64_t kMostPositions = 1ll << 20;
+constexpr int64_t kFewPieces = 1 << 19;              // of a lookup: below, one piece per lane
 
 }  // namespace
 
@@ -175,19 +183,25 @@ extern "C" int anc_embed_lookup(uint64_t ids, int32_t ids_bytes, int64_t n, uint
               "anc_embed_lookup: misaligned pointers");
   const Ptr ps[2] = {{table, table_type}, {out, out_type}};
   const int vec = piece(H, ps);
-  const int64_t blocks = (n * (H / vec) + kLookupLanes - 1) / kLookupLanes;
-  ANC_REQUIRE(blocks < (1ll << 31), "anc_embed_lookup: %lld rows of %lld are too many for one call", (long long)n, (long long)H);
+  const int64_t per_row = H / vec, most = kMostPieces / per_row;
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_MISC, s);
-  with_type(table_type, [&](auto tt) {
-    with_type(out_type, [&](auto to) {
-      with_piece(vec, [&](auto v) {
-        constexpr int TT = decltype(tt)::value, TO = decltype(to)::value, VEC = decltype(v)::value;
-        hipLaunchKernelGGL((k_embed_lookup<TT, TO, VEC>), dim3((unsigned)blocks), dim3(kLookupLanes), 0, s, (const void *)ids,
-                           ids_bytes == 8, n, V, (uint32_t)(H / VEC), H, scale, (const elem_t<TT> *)table, (elem_t<TO> *)out);
+  for (int64_t r = 0; r < n; r += most) {
+    const int64_t rows = n - r < most ? n - r : most, total = rows * per_row;
+    const int u = total >= kFewPieces ? 4 : 1;
+    const dim3 grid((unsigned)((total + u * kLookupLanes - 1) / (u * kLookupLanes)));
+    with_type(table_type, [&](auto tt) {
+      with_type(out_type, [&](auto to) {
+        with_piece(vec, [&](auto v) {
+          constexpr int TT = decltype(tt)::value, TO = decltype(to)::value, VEC = decltype(v)::value;
+          auto kernel = u == 4 ? k_embed_lookup<TT, TO, VEC, 4> : k_embed_lookup<TT, TO, VEC, 1>;
+          hipLaunchKernelGGL(kernel, grid, dim3(kLookupLanes), 0, s, (const void *)(ids + (uint64_t)(r * ids_bytes)), ids_bytes == 8,
+                             (uint32_t)total, V, fast_div((uint32_t)per_row), H, scale, (const elem_t<TT> *)table,
+                             (elem_t<TO> *)out + r * H);
+        });
       });
     });
-  });
+  }
   ANC_LAUNCH_CHECK();
   return ANC_OK;
 }
@@ -228,11 +242,13 @@ extern "C" int anc_embed_dw(uint64_t srt, uint64_t start, uint64_t cnt, uint64_t
     const int64_t waves = (H + 64 * VEC - 1) / (64 * VEC), wide = waves < kDwLanes / 64 ? waves : kDwLanes / 64;
     with_type(dy_type, [&](auto t) {
       constexpr int T = decltype(t)::value;
-      hipLaunchKernelGGL((k_embed_dw<T, VEC>), dim3((unsigned)chunks, (unsigned)((waves + wide - 1) / wide)), dim3((unsigned)(64 * wide)), 0,
-                         s, p, (const elem_t<T> *)dy);
+      auto kernel = out != 0 ? k_embed_dw<T, VEC, true> : k_embed_dw<T, VEC, false>;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)chunks, (unsigned)((waves + wide - 1) / wide)), dim3((unsigned)(64 * wide)), 0, s, p,
+                         (const elem_t<T> *)dy);
     });
+    constexpr int JV = VEC == 8 ? 4 : VEC;           // narrower pieces: more wavefronts on a long list
     if (chunks > 1)
-      hipLaunchKernelGGL((k_embed_dw_join<VEC>), dim3((unsigned)(chunks - 1), (unsigned)waves), dim3(kDwLanes), 0, s, p);
+      hipLaunchKernelGGL((k_embed_dw_join<JV>), dim3((unsigned)(chunks - 1), (unsigned)((H + 64 * JV - 1) / (64 * JV))), dim3(kDwLanes), 0, s, p);
   });
   ANC_LAUNCH_CHECK();
   return ANC_OK;

@@ -2,22 +2,23 @@
 //     dW[e] (K, N) (+)= sum over its tokens s of x[s]^T dy[s],   x (slots, K), dy (slots, N) bf16, fp32 accumulation.
 // Segments are ragged and known on the device only, so the grid covers every expert's whole weight and a workgroup reads its segment.
 //
-// One workgroup owns 128x256 outputs of one expert and runs the expert's tokens in ascending order, 32 a step, one accumulator per
-// element: no split of the tokens, an expert's bits are a function of its own rows. Both operands lie token by token, and
-// the product contracts over tokens, so tiles [32 tokens][128 or 256 columns] go straight to LDS and the fragments come from
-// transposing LDS reads. Three stages of 24 KiB, two workgroups per CU: one's stores run under the other's products.
-// Rows past the segment's end and stages past the last are never fetched: the buffer descriptor of a stage ends with the segment, and
-// loads beyond it give zeros. (Columns past K or N are the next row's: they meet outputs that are not stored.)
+// One workgroup owns 256x256 (or 128x256) outputs of one expert and runs the expert's tokens in ascending order, 32 a step, one
+// accumulator per element: no split of the tokens, an expert's bits are a function of its own rows. Both operands lie token by token, and
+// the product contracts over tokens, so tiles [32 tokens][columns] go straight to LDS, three stages of them, and the fragments
+// come from transposing LDS reads. Rows past the segment's end and stages past the last are never fetched: the buffer descriptor of a
+// stage ends with the segment, and loads beyond it give zeros. (Columns past K or N are the next row's: they meet outputs that are
+// not stored.)
+//
+// What bounds it is the operands' way into LDS, some 13 bytes per clock and CU, then the outputs' bytes. One layer of 16 experts, three
+// weights of 1024x1024 with bf16 copies, 16384 rows in segments of 1:4: 177 us with 128x256 tiles and the experts in their order, 8 tiles
+// at a time to an XCD; 151 with the experts by falling length and 16 .. 32 tiles at a time, 138 with 256x256 tiles, 103 of them
+// without the stores.
 #include "lds_dma.h"
 #include "ns_common.h"
 
 namespace {
 
-constexpr int TM = 128, TN = 256, TK = 32, kStages = 3;
-constexpr int kBytesA = TK * TM * 2, kBytesB = TK * TN * 2, kStage = kBytesA + kBytesB;
-constexpr int kLanes = 256, kWaves = 4;                        // a wavefront: all 128 rows x 64 columns
-constexpr int kPiecesA = kBytesA / 1024 / kWaves, kPiecesB = kBytesB / 1024 / kWaves, kPieces = kPiecesA + kPiecesB;
-constexpr int kUnit = 8;                                       // tiles that follow each other on one XCD
+constexpr int TN = 256, TK = 32, kStages = 3, kRowB = TN * 2, kBytesB = TK * kRowB;
 constexpr int kMostProblems = 8;
 
 struct DwOne {
@@ -28,9 +29,9 @@ struct DwOne {
   int accumulate;
 };
 struct DwMulti {
-  const int32_t *counts, *offsets;
-  int count, experts;
-  int unit0[kMostProblems + 1];                                // first unit of each problem
+  const int32_t *counts, *offsets, *order;
+  int count, experts, unit;                                    // tiles that follow each other on one XCD
+  int unit0[kMostProblems + 1];                                // first unit of each problem among an expert's
   DwOne p[kMostProblems];
 };
 
@@ -58,17 +59,23 @@ struct Feed {
   __device__ __forceinline__ void next() { at += step; left -= step; }
 };
 
-__global__ void __launch_bounds__(kLanes, 2) k_expert_dw(DwMulti m) {
+// Wavefronts of 128 rows x 64 columns, two to a SIMD: TM = 256 is one workgroup of eight per CU, TM = 128 two of four.
+template <int TM>
+__global__ void __launch_bounds__(TM * 2, 2) k_expert_dw(DwMulti m) {
+  constexpr int kWaves = TM / 32, kRowA = TM * 2, kBytesA = TK * kRowA, kStage = kBytesA + kBytesB;
+  constexpr int kPiecesA = kBytesA / 1024 / kWaves, kPiecesB = kBytesB / 1024 / kWaves, kPieces = kPiecesA + kPiecesB;
+  static_assert(kWaves * 8192 <= kStages * kStage, "room for the way out");
   __shared__ __attribute__((aligned(1024))) unsigned char ring[kStages * kStage];
-  // Units of kUnit tiles are dealt round the XCDs, so that a unit's tiles, which read the same rows, share an L2 and the experts' different
-  // lengths spread over all of them.
-  const int b = (int)blockIdx.x, xcd = b % kXcds, q = b / kXcds;
-  const int unit = (q / kUnit) * kXcds + xcd;
+  // Units of some tiles of one weight go round the XCDs, back and forth: a unit's tiles read the same rows and share an L2, and with
+  // the experts by falling length every XCD gets about as much.
+  const int b = (int)blockIdx.x, xcd = b % kXcds, q = b / kXcds, round = q / m.unit;
+  const int unit = round * kXcds + ((round & 1) ? kXcds - 1 - xcd : xcd), per = m.unit0[m.count], rank = unit / per, mine = unit - rank * per;
+  if (rank >= m.experts) return;
+  const int e = m.order[rank];
   int pi = 0;
-  while (pi + 1 < m.count && unit >= m.unit0[pi + 1]) ++pi;
-  if (unit >= m.unit0[m.count]) return;
+  while (pi + 1 < m.count && mine >= m.unit0[pi + 1]) ++pi;
   const DwOne &p = m.p[pi];
-  const int per = (p.tiles + kUnit - 1) / kUnit, u = unit - m.unit0[pi], e = u / per, tile = (u - e * per) * kUnit + q % kUnit;
+  const int tile = (mine - m.unit0[pi]) * m.unit + q % m.unit;
   if (tile >= p.tiles) return;
   const int m0 = tile / p.tn * TM, n0 = (tile % p.tn) * TN;
   const int K = p.K, N = p.N, rows = m.counts[e];
@@ -77,13 +84,13 @@ __global__ void __launch_bounds__(kLanes, 2) k_expert_dw(DwMulti m) {
 
   Feed fa{(const char *)(p.x + first * K + m0), ((int64_t)rows * K - m0) * 2, (int64_t)TK * K * 2};
   Feed fb{(const char *)(p.dy + first * N + n0), ((int64_t)rows * N - n0) * 2, (int64_t)TK * N * 2};
-  // Piece i of an operand's tile is 1 KiB of LDS: 4 rows of 256 bytes (x) or 2 of 512 (dy). The 16-byte chunk of a row is XORed with 4 * (row & 3),
-  // so that the four rows that a transposing read touches fall into different banks.
+  // Piece i of an operand's tile is 1 KiB of LDS: 4 rows of 256 bytes or 2 of 512. The 16-byte chunk of a row is XORed with 4 * (row & 3), so
+  // that the four rows that a transposing read touches fall into different banks.
   uint32_t va[kPiecesA], vb[kPiecesB];
 #pragma unroll
   for (int i = 0; i < kPiecesA; ++i) {
-    const int row = (wave * kPiecesA + i) * 4 + (lane >> 4);
-    va[i] = (uint32_t)(row * K * 2 + (((lane & 15) ^ ((row & 3) << 2)) * 16));
+    const int row = (wave * kPiecesA + i) * (1024 / kRowA) + lane / (kRowA / 16);
+    va[i] = (uint32_t)(row * K * 2 + (((lane % (kRowA / 16)) ^ ((row & 3) << 2)) * 16));
   }
 #pragma unroll
   for (int i = 0; i < kPiecesB; ++i) {
@@ -107,10 +114,10 @@ __global__ void __launch_bounds__(kLanes, 2) k_expert_dw(DwMulti m) {
   {
     const int s16 = lane & 15, g16 = lane >> 4, half = (s16 & 3) >> 1, row = 8 * (g16 >> 1) + (s16 >> 2), sw = (s16 >> 2) << 2;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ta[i] = row * 256 + (((i * 4 + 2 * (g16 & 1) + half) ^ sw) * 16) + (s16 & 1) * 8;
+    for (int i = 0; i < 4; ++i) ta[i] = row * kRowA + ((((wave >> 2) * 16 + i * 4 + 2 * (g16 & 1) + half) ^ sw) * 16) + (s16 & 1) * 8;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      tb[i] = kBytesA + row * 512 + (((wave * 8 + i * 4 + 2 * (g16 & 1) + half) ^ sw) * 16) + (s16 & 1) * 8;
+      tb[i] = kBytesA + row * kRowB + ((((wave & 3) * 8 + i * 4 + 2 * (g16 & 1) + half) ^ sw) * 16) + (s16 & 1) * 8;
   }
   f32x16 acc[4][2];
 #pragma unroll
@@ -126,13 +133,13 @@ __global__ void __launch_bounds__(kLanes, 2) k_expert_dw(DwMulti m) {
     // fragment i (0 .. 5: b0 b1 a0 a1 a2 a3) of 16 tokens kk of a stage
     auto load = [&](int set, int i, const unsigned char *stage, int kk) {
       if (i < 2) c[set][i] = anc_lds_tr_frag(stage + tb[i] + kk * (16 * 512), stage + tb[i] + kk * (16 * 512) + 4 * 512);
-      else a[set][i - 2] = anc_lds_tr_frag(stage + ta[i - 2] + kk * (16 * 256), stage + ta[i - 2] + kk * (16 * 256) + 4 * 256);
+      else a[set][i - 2] = anc_lds_tr_frag(stage + ta[i - 2] + kk * (16 * kRowA), stage + ta[i - 2] + kk * (16 * kRowA) + 4 * kRowA);
     };
     auto multiply = [&](int set, int idx) {      // operands exchanged: a lane holds runs of 4 columns of one row
       acc[idx >> 1][idx & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c[set][idx & 1], a[set][idx >> 1], acc[idx >> 1][idx & 1], 0, 0, 0);
     };
     for (int i = 0; i < kStages; ++i) issue_all(ring + i * kStage);
-    wait_vm<2 * kPieces>();
+    wait_vm<(kStages - 1) * kPieces>();
     lds_barrier();
 #pragma unroll
     for (int i = 0; i < 6; ++i) load(0, i, ring, 0);
@@ -147,17 +154,15 @@ __global__ void __launch_bounds__(kLanes, 2) k_expert_dw(DwMulti m) {
         if (i < 6) load(1, i, here, 1);
         __builtin_amdgcn_sched_barrier(0);
       }
-      wait_vm<kPieces>();
+      wait_vm<(kStages - 2) * kPieces>();
       lds_barrier();
       const i32x4 da = fa.desc(), db = fb.desc();
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         multiply(1, i);
         __builtin_amdgcn_sched_barrier(0);
-        if (i < 6) {
-          load(0, i, next, 0);
-          issue(i, da, db, here);
-        }
+        if (i < 6) load(0, i, next, 0);
+        if (i < kPieces) issue(i, da, db, here);
         __builtin_amdgcn_sched_barrier(0);
       }
       fa.next();
@@ -175,8 +180,9 @@ __global__ void __launch_bounds__(kLanes, 2) k_expert_dw(DwMulti m) {
 
   // Out through LDS, 32 rows of 64 columns at a time, so that stores are rows of 256 bytes.
   unsigned char *r = ring + wave * 8192;
-  const int cols = N - n0 - wave * 64;           // this wavefront's columns that exist
-  const int64_t out0 = (int64_t)e * K * N + (int64_t)m0 * N + n0 + wave * 64;
+  const int row0 = m0 + (wave >> 2) * 128;
+  const int cols = N - n0 - (wave & 3) * 64;           // this wavefront's columns that exist
+  const int64_t out0 = (int64_t)e * K * N + (int64_t)row0 * N + n0 + (wave & 3) * 64;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int rr = lane & 31, hh = lane >> 5;
@@ -191,7 +197,7 @@ __global__ void __launch_bounds__(kLanes, 2) k_expert_dw(DwMulti m) {
     for (int z = 0; z < 8; ++z) {
       const int idx = z * 64 + lane, row = idx >> 4, ch = idx & 15;
       anc_f32x4 v = *(const anc_f32x4 *)(r + row * 256 + ((ch ^ (row & 15)) * 16));
-      if (m0 + i * 32 + row < K && ch * 4 < cols) {
+      if (row0 + i * 32 + row < K && ch * 4 < cols) {
         const int64_t off = out0 + (int64_t)(i * 32 + row) * N + ch * 4;
         if (p.accumulate) {
           const anc_f32x4 o = *(const anc_f32x4 *)(p.dW + off);
@@ -208,44 +214,42 @@ __global__ void __launch_bounds__(kLanes, 2) k_expert_dw(DwMulti m) {
 }  // namespace
 
 extern "C" int anc_expert_dw_multi(const anc_expert_dw_problem_t *probs, int32_t n_probs, uint64_t counts, uint64_t offsets,
-                                   int64_t experts, uint64_t stream) {
+                                   uint64_t order, int64_t experts, uint64_t stream) {
   ANC_REQUIRE(probs != nullptr && n_probs >= 1 && n_probs <= kMostProblems, "anc_expert_dw_multi: 1..%d problems", kMostProblems);
-  ANC_REQUIRE(counts && offsets && ((counts | offsets) & 3) == 0 && experts > 0 && experts <= 512,
+  ANC_REQUIRE(counts && offsets && order && ((counts | offsets | order) & 3) == 0 && experts > 0 && experts <= 512,
               "anc_expert_dw_multi: bad segments (%lld experts)", (long long)experts);
   DwMulti m{};
   m.counts = (const int32_t *)counts;
   m.offsets = (const int32_t *)offsets;
+  m.order = (const int32_t *)order;
   m.count = n_probs;
   m.experts = (int)experts;
-  int64_t units = 0;
+  int64_t wide = 0;                                  // tiles of 256x256
   for (int i = 0; i < n_probs; ++i) {
     const anc_expert_dw_problem_t &b = probs[i];
-    ANC_REQUIRE(b.K > 0 && b.N > 0 && b.K % 8 == 0 && b.N % 8 == 0 && b.K <= (1 << 20) && b.N <= (1 << 20),
+    ANC_REQUIRE(b.K > 0 && b.N > 0 && b.K % 8 == 0 && b.N % 8 == 0 && b.K <= (1 << 17) && b.N <= (1 << 17),
                 "anc_expert_dw_multi: needs K %% 8 == 0 and N %% 8 == 0 (K=%lld N=%lld)", (long long)b.K, (long long)b.N);
     ANC_REQUIRE(b.x && b.dy && b.dW && ((b.x | b.dy | b.dW) & 15) == 0 && (b.g16 & 7) == 0,
                 "anc_expert_dw_multi: null or misaligned pointer");
-    DwOne &p = m.p[i];
-    p.x = (const uint16_t *)b.x;
-    p.dy = (const uint16_t *)b.dy;
-    p.dW = (float *)b.dW;
-    p.g16 = (uint16_t *)b.g16;
-    p.K = (int)b.K;
-    p.N = (int)b.N;
-    p.accumulate = b.accumulate != 0;
-    p.tn = (p.N + TN - 1) / TN;
-    const int64_t tiles = (int64_t)((p.K + TM - 1) / TM) * p.tn;
-    ANC_REQUIRE(tiles < (1 << 24), "anc_expert_dw_multi: %lld x %lld is too large", (long long)b.K, (long long)b.N);
-    p.tiles = (int)tiles;
-    m.unit0[i] = (int)units;
-    units += (tiles + kUnit - 1) / kUnit * experts;
-    ANC_REQUIRE(units < (1 << 27), "anc_expert_dw_multi: too large for one call");
+    m.p[i] = DwOne{(const uint16_t *)b.x, (const uint16_t *)b.dy, (float *)b.dW, (uint16_t *)b.g16, (int)b.K, (int)b.N,
+                   (int)((b.N + TN - 1) / TN), 0, b.accumulate != 0};
+    wide += (b.K + 255) / 256 * m.p[i].tn * experts;
   }
-  for (int i = n_probs; i <= kMostProblems; ++i) m.unit0[i] = (int)units;
-  const int64_t grid = (units + kXcds - 1) / kXcds * kXcds * kUnit;
+  // 256x256 tiles where they give every CU one; fewer, and twice as many of 128x256 are at work.
+  const int TM = wide >= 256 ? 256 : 128;
+  for (int i = 0; i < n_probs; ++i) m.p[i].tiles = (m.p[i].K + TM - 1) / TM * m.p[i].tn;
+  // The tiles that stay together: a whole weight of 16 or 32 tiles, fewer where that leaves an XCD less than six units to even out.
+  for (m.unit = 32;; m.unit /= 2) {
+    m.unit0[0] = 0;
+    for (int i = 0; i < n_probs; ++i) m.unit0[i + 1] = m.unit0[i] + (m.p[i].tiles + m.unit - 1) / m.unit;
+    if (m.unit == 4 || m.unit0[n_probs] * experts >= 6 * kXcds) break;
+  }
+  const int64_t units = m.unit0[n_probs] * experts, grid = (units + kXcds - 1) / kXcds * kXcds * m.unit;
   ANC_REQUIRE(grid < (1ll << 31), "anc_expert_dw_multi: too large for one call");
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_DW_GEMM, s);
-  hipLaunchKernelGGL(k_expert_dw, dim3((unsigned)grid), dim3(kLanes), 0, s, m);
+  if (TM == 256) hipLaunchKernelGGL(k_expert_dw<256>, dim3((unsigned)grid), dim3(512), 0, s, m);
+  else           hipLaunchKernelGGL(k_expert_dw<128>, dim3((unsigned)grid), dim3(256), 0, s, m);
   ANC_LAUNCH_CHECK();
   return ANC_OK;
 }

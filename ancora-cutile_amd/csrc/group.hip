@@ -19,21 +19,27 @@ constexpr int kMostItems = 16;                       // per lane of the one-work
 constexpr int kSmallMax = 1024 * kMostItems;
 constexpr int kBlockLanes = 256, kBlockItems = 8, kBlock = kBlockLanes * kBlockItems;
 
-// Lanes of the wavefront that hold the same digit as this one (among those with `in`).
+// Lanes of the wavefront that hold the same digit as this one, among those with `in`. (Six vector instructions a bit: the digit's bit
+// as 0 or -1, its ballot, and two words of agreement.)
 __device__ __forceinline__ uint64_t same_digit(uint32_t d, int bits, bool in) {
-  uint64_t m = __ballot(in);
+  const uint64_t all = __ballot(in);
+  uint32_t lo = (uint32_t)all, hi = (uint32_t)(all >> 32);
   for (int b = 0; b < bits; ++b) {
-    const bool s = (d >> b) & 1u;
-    const uint64_t v = __ballot(s);
-    m &= s ? v : ~v;
+    const uint32_t s = (uint32_t)__builtin_amdgcn_sbfe((int)d, b, 1);
+    const uint64_t v = __ballot(s != 0);
+    lo &= ~((uint32_t)v ^ s);
+    hi &= ~((uint32_t)(v >> 32) ^ s);
   }
-  return m;
+  return (uint64_t)hi << 32 | lo;
 }
-// Rank of this lane's item among the wavefront's items of its digit so far; `count` is the wavefront's own row in LDS.
+__device__ __forceinline__ int lanes_before(uint64_t m) {
+  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+}
+// Rank of this lane's item among the wavefront's items of its digit so far; `count` is the wavefront's own row in LDS. Lanes without
+// `in` take no part.
 __device__ __forceinline__ int take_rank(volatile int *count, uint32_t d, int bits, bool in) {
   const uint64_t m = same_digit(d, bits, in);
-  const int lane = (int)(threadIdx.x & 63);
-  const int before = __popcll(m & ((1ull << lane) - 1));
+  const int before = lanes_before(m);
   int old = 0;
   if (in) old = count[d];
   __builtin_amdgcn_wave_barrier();
@@ -70,10 +76,27 @@ __device__ __forceinline__ int block_scan(int v, int *tmp, int &total) {
   return base + inc - v;
 }
 
-// A token id as a key: V for one that names no row.
-__device__ __forceinline__ uint32_t id_key(const void *ids, int wide, int64_t p, uint32_t V) {
-  const int64_t id = wide ? ((const int64_t *)ids)[p] : (int64_t)((const int32_t *)ids)[p];
-  return id >= 0 && id < (int64_t)V ? (uint32_t)id : V;
+// The ids at `first`, first + step, ..., as keys: V for one that names no row and for what lies behind the last. (Addresses are
+// clamped instead of the loads guarded, so that all of them are in flight at once; n > 0.)
+template <int ITEMS>
+__device__ __forceinline__ void load_keys(const void *ids, int wide, int64_t first, int step, int64_t n, uint32_t V, uint32_t (&key)[ITEMS]) {
+  int64_t id[ITEMS];
+  if (wide) {
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      const int64_t p = first + (int64_t)j * step;
+      id[j] = ((const int64_t *)ids)[p < n ? p : n - 1];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      const int64_t p = first + (int64_t)j * step;
+      id[j] = ((const int32_t *)ids)[p < n ? p : n - 1];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j)
+    key[j] = first + (int64_t)j * step < n && id[j] >= 0 && id[j] < (int64_t)V ? (uint32_t)id[j] : V;
 }
 
 struct Groups {
@@ -94,14 +117,17 @@ k_group_small(const void *__restrict__ ids, int wide, int n, int M, uint32_t V, 
   const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63, first = wave * (64 * ITEMS) + lane;
   int idx[ITEMS];
   uint32_t key[ITEMS];
+  if (n > 0) {
+    load_keys<ITEMS>(ids, wide, first, 64, n, V, key);       // (what lies behind the last id stays behind the ids that name no row)
+  } else {
 #pragma unroll
-  for (int j = 0; j < ITEMS; ++j) {
-    const int p = first + 64 * j;
-    idx[j] = p;
-    key[j] = p < n ? id_key(ids, wide, p, V) : V;    // (what lies behind the last id stays behind the ids that name no row)
+    for (int j = 0; j < ITEMS; ++j) key[j] = V;
   }
 #pragma unroll
-  for (int j = 0; j < ITEMS; ++j) skey[first + 64 * j] = key[j];
+  for (int j = 0; j < ITEMS; ++j) {
+    idx[j] = first + 64 * j;
+    skey[first + 64 * j] = key[j];
+  }
   for (int shift = 0; shift < bits; shift += kDigitBits) {
     const int b = bits - shift < kDigitBits ? bits - shift : kDigitBits, digits = 1 << b;
     for (int i = tid; i < W << b; i += 1024) count[i] = 0;
@@ -111,16 +137,19 @@ k_group_small(const void *__restrict__ ids, int wide, int n, int M, uint32_t V, 
     for (int j = 0; j < ITEMS; ++j)
       rank[j] = take_rank(count + (wave << b), (key[j] >> shift) & (digits - 1), b, true);
     __syncthreads();
-    int sum = 0, total;
-    if (tid < digits)
+    int c[W], sum = 0, total;
+#pragma unroll
+    for (int w = 0; w < W; ++w) c[w] = tid < digits ? count[(w << b) + tid] : 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) sum += c[w];
+    int at = block_scan<1024>(sum, tmp, total);
+    if (tid < digits) {
+#pragma unroll
       for (int w = 0; w < W; ++w) {
-        const int c = count[(w << b) + tid];
-        count[(w << b) + tid] = sum;
-        sum += c;
+        count[(w << b) + tid] = at;
+        at += c[w];
       }
-    const int base = block_scan<1024>(sum, tmp, total);
-    if (tid < digits)
-      for (int w = 0; w < W; ++w) count[(w << b) + tid] += base;
+    }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j)
@@ -182,14 +211,14 @@ k_radix_count(const void *__restrict__ ids, int wide, int64_t n, int64_t M, uint
   __shared__ int h[kDigits];
   const int tid = (int)threadIdx.x;
   const int64_t blocks = gridDim.x, b = blockIdx.x;
+  uint32_t key[kBlockItems];
+  load_keys<kBlockItems>(ids, wide, b * kBlock + tid, kBlockLanes, n, V, key);
   for (int i = tid; i < kDigits; i += kBlockLanes) h[i] = 0;
   __syncthreads();
   const uint32_t mask = bits < kDigitBits ? (1u << bits) - 1 : (uint32_t)kDigits - 1;
 #pragma unroll
-  for (int j = 0; j < kBlockItems; ++j) {
-    const int64_t p = b * kBlock + j * kBlockLanes + tid;
-    if (p < n) atomicAdd(&h[id_key(ids, wide, p, V) & mask], 1);
-  }
+  for (int j = 0; j < kBlockItems; ++j)
+    if (b * kBlock + j * kBlockLanes + tid < n) atomicAdd(&h[key[j] & mask], 1);
   __syncthreads();
   for (int i = tid; i < kDigits; i += kBlockLanes) {
     hist[b * kDigits + i] = h[i];
@@ -213,14 +242,17 @@ k_radix_scatter(const void *__restrict__ ids, int wide, const int32_t *__restric
   const uint32_t mask = (1u << nb) - 1;
   uint32_t key[kBlockItems];
   int32_t idx[kBlockItems];
+  if (key_in != nullptr) {
 #pragma unroll
-  for (int j = 0; j < kBlockItems; ++j) {
-    const int64_t p = first + 64 * j;
-    key[j] = 0; idx[j] = 0;
-    if (p < n) {
-      key[j] = key_in != nullptr ? (uint32_t)key_in[p] : id_key(ids, wide, p, V);
-      idx[j] = key_in != nullptr ? idx_in[p] : (int32_t)p;
+    for (int j = 0; j < kBlockItems; ++j) {
+      const int64_t p = first + 64 * j < n ? first + 64 * j : n - 1;
+      key[j] = (uint32_t)key_in[p];
+      idx[j] = idx_in[p];
     }
+  } else {
+    load_keys<kBlockItems>(ids, wide, first, 64, n, V, key);
+#pragma unroll
+    for (int j = 0; j < kBlockItems; ++j) idx[j] = (int32_t)(first + 64 * j);
   }
   for (int i = tid; i < W * kDigits; i += kBlockLanes) count[i] = 0;
   // counts of this lane's digits over all blocks, and over the blocks before this one
@@ -257,40 +289,67 @@ k_radix_scatter(const void *__restrict__ ids, int wide, const int32_t *__restric
     }
   }
   __syncthreads();
+  // The next pass's digit counts, by the blocks that the items move to. One atomic for the lanes that agree in both (a frequent id
+  // is thousands of items of one block and digit), one each for the few whose neighbours went to another block.
+  const int left = bits - shift - kDigitBits, next_bits = left < kDigitBits ? left : kDigitBits;
 #pragma unroll
   for (int j = 0; j < kBlockItems; ++j) {
-    if (first + 64 * j >= n) continue;
-    const int at = count[wave * kDigits + ((key[j] >> shift) & mask)] + rank[j];
-    key_out[at] = (int32_t)key[j];
-    idx_out[at] = idx[j];
+    const bool in = first + 64 * j < n;
+    const int at = in ? count[wave * kDigits + ((key[j] >> shift) & mask)] + rank[j] : 0;
+    if (in) {
+      key_out[at] = (int32_t)key[j];
+      idx_out[at] = idx[j];
+    }
     if (hist_next != nullptr) {
-      const int left = bits - shift - kDigitBits;
-      const uint32_t next = (key[j] >> (shift + kDigitBits)) & (left < kDigitBits ? (1u << left) - 1 : (uint32_t)kDigits - 1);
-      atomicAdd(&hist_next[(int64_t)(at / kBlock) * kDigits + next], 1);
+      const uint32_t next = (key[j] >> (shift + kDigitBits)) & ((1u << next_bits) - 1);
+      const int to = at / kBlock;
+      const uint64_t same = same_digit(next, next_bits, in);
+      const int leader = in ? __builtin_ctzll(same) : lane, to_leader = __shfl(to, leader, 64);
+      const uint64_t with = same & __ballot(to == to_leader);
+      if (in && (lane == leader || to != to_leader))
+        atomicAdd(&hist_next[(int64_t)to * kDigits + next], lane == leader ? __popcll(with) : 1);
     }
   }
 }
 
-__device__ __forceinline__ bool is_head(const int32_t *key, int64_t p, int64_t n, uint32_t V) {
-  if (p >= n) return false;
-  const uint32_t k = (uint32_t)key[p];
-  return k < V && (p == 0 || (uint32_t)key[p - 1] != k);
+// Bit j: item first + j * step begins a group.
+__device__ __forceinline__ int head_bits(const int32_t *key, int64_t first, int step, int64_t n, uint32_t V) {
+  uint32_t k[kBlockItems], before[kBlockItems];
+#pragma unroll
+  for (int j = 0; j < kBlockItems; ++j) {
+    const int64_t p = first + (int64_t)j * step < n ? first + (int64_t)j * step : n - 1;
+    k[j] = (uint32_t)key[p];
+    before[j] = (uint32_t)key[p > 0 ? p - 1 : 0];
+  }
+  int bits = 0;
+#pragma unroll
+  for (int j = 0; j < kBlockItems; ++j) {
+    const int64_t p = first + (int64_t)j * step;
+    bits |= p < n && k[j] < V && (p == 0 || before[j] != k[j]) ? 1 << j : 0;
+  }
+  return bits;
 }
 __global__ void __launch_bounds__(kBlockLanes)
 k_heads(const int32_t *__restrict__ key, int64_t n, uint32_t V, int *__restrict__ heads) {
   __shared__ int tmp[kBlockLanes / 64];
-  int mine = 0, total;
-#pragma unroll
-  for (int j = 0; j < kBlockItems; ++j)
-    mine += is_head(key, (int64_t)blockIdx.x * kBlock + j * kBlockLanes + threadIdx.x, n, V) ? 1 : 0;
-  block_scan<kBlockLanes>(mine, tmp, total);
+  int total;
+  block_scan<kBlockLanes>(__popc(head_bits(key, (int64_t)blockIdx.x * kBlock + threadIdx.x, kBlockLanes, n, V)), tmp, total);
   if (threadIdx.x == 0) heads[blockIdx.x] = total;
 }
 __global__ void __launch_bounds__(kBlockLanes)
 k_groups(int64_t n, int64_t M, uint32_t V, const int *__restrict__ heads, Groups o) {
   __shared__ int tmp[kBlockLanes / 64];
   const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63, blocks = (int)gridDim.x, b = (int)blockIdx.x;
-  int all = 0, below = 0, total, run;
+  const int64_t first = (int64_t)b * kBlock + wave * (64 * kBlockItems) + lane;
+  uint32_t k[kBlockItems], after[kBlockItems];
+#pragma unroll
+  for (int j = 0; j < kBlockItems; ++j) {
+    const int64_t p = first + 64 * j < n ? first + 64 * j : n - 1;
+    k[j] = (uint32_t)o.key[p];
+    after[j] = (uint32_t)o.key[p + 1 < n ? p + 1 : p];
+  }
+  const int head = head_bits(o.key, first, 64, n, V);
+  int all = 0, below = 0, total, run, in_block;
   for (int c = tid; c < blocks; c += kBlockLanes) {
     const int v = heads[c];
     all += v;
@@ -298,30 +357,23 @@ k_groups(int64_t n, int64_t M, uint32_t V, const int *__restrict__ heads, Groups
   }
   block_scan<kBlockLanes>(all, tmp, total);
   block_scan<kBlockLanes>(below, tmp, run);
-  const int64_t first = (int64_t)b * kBlock + wave * (64 * kBlockItems) + lane;
-  int mine = 0, in_block;
-  int head[kBlockItems];
-#pragma unroll
-  for (int j = 0; j < kBlockItems; ++j) {
-    head[j] = is_head(o.key, first + 64 * j, n, V) ? 1 : 0;
-    mine += head[j];
-  }
+  const int mine = __popc(head);
   run += block_scan<kBlockLanes>(mine, tmp, in_block) - (wave_scan(mine) - mine);
 #pragma unroll
   for (int j = 0; j < kBlockItems; ++j) {
     const int64_t p = first + 64 * j;
-    const uint64_t m = __ballot(head[j]);
-    const int g = run + __popcll(m & ((1ull << lane) - 1)) - (head[j] ? 0 : 1);
+    const bool is_head = (head >> j) & 1;
+    const uint64_t m = __ballot(is_head);
+    const int g = run + __popcll(m & ((1ull << lane) - 1)) - (is_head ? 0 : 1);
     run += __popcll(m);
     if (p >= n) continue;
-    const uint32_t k = (uint32_t)o.key[p];
-    o.grp[p] = k < V ? g : -1;
-    if (head[j]) {
+    o.grp[p] = k[j] < V ? g : -1;
+    if (is_head) {
       o.start[g] = (int32_t)p;
-      o.gid[g] = (int32_t)k;
+      o.gid[g] = (int32_t)k[j];
       atomicAdd(&o.cnt[g], -(int)p);                 // (a group's head and its last item meet in its count)
     }
-    if (k < V && (p + 1 == n || (uint32_t)o.key[p + 1] != k)) atomicAdd(&o.cnt[g], (int)p + 1);
+    if (k[j] < V && (p + 1 == n || after[j] != k[j])) atomicAdd(&o.cnt[g], (int)p + 1);
   }
   for (int64_t g = total + (int64_t)b * kBlockLanes + tid; g < M; g += (int64_t)blocks * kBlockLanes) {
     o.start[g] = 0;
@@ -334,11 +386,29 @@ k_groups(int64_t n, int64_t M, uint32_t V, const int *__restrict__ heads, Groups
 constexpr int kMostExperts = kDigits;
 
 struct Route {
-  int32_t *counts, *offsets, *slot, *src;
+  int32_t *counts, *offsets, *order, *slot, *src;
 };
-__device__ __forceinline__ int expert_of(const void *ids, int wide, int64_t p, int E) {
-  const int64_t e = wide ? ((const int64_t *)ids)[p] : (int64_t)((const int32_t *)ids)[p];
-  return e >= 0 && e < E ? (int)e : -1;
+// The experts by falling number of tokens, lower ones first where equal: an expert's place is the number of experts before it, found
+// by looking at all of them (LANES / E lanes share the looking). Beyond kMostOrdered that would take longer than it gives: many
+// short segments even out in any order.
+constexpr int kMostOrdered = 256;
+template <int LANES>
+__device__ __forceinline__ void order_experts(const int *scnt, int E, int32_t *order) {
+  if (E > kMostOrdered) {
+    for (int e = (int)threadIdx.x; e < E; e += LANES) order[e] = e;
+    return;
+  }
+  constexpr int L = LANES / kMostOrdered;            // lanes per expert, neighbours
+  const int e = (int)threadIdx.x / L;
+  const int mine = e < E ? scnt[e] : 0;
+  int before = 0;
+  for (int j = (int)threadIdx.x % L; j < E; j += L) {
+    const int c = scnt[j];
+    before += c > mine || (c == mine && j < e) ? 1 : 0;
+  }
+#pragma unroll
+  for (int o = 1; o < L; o <<= 1) before += __shfl_xor(before, o, 64);
+  if (e < E && (int)threadIdx.x % L == 0) order[before] = e;
 }
 __device__ __forceinline__ int filled_up(int c, int align) { return (c + align - 1) & -align; }
 
@@ -350,24 +420,32 @@ k_route_small(const void *__restrict__ ids, int wide, int n, int E, int bits, in
   __shared__ int tmp[W];
   __shared__ int soff[kMostExperts + 1], scnt[kMostExperts];
   const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63, first = wave * (64 * ITEMS) + lane;
-  int e[ITEMS], rank[ITEMS];
+  uint32_t e[ITEMS];                                 // E: no expert
+  int rank[ITEMS];
+  if (n > 0) {
+    load_keys<ITEMS>(ids, wide, first, 64, n, (uint32_t)E, e);
+  } else {
 #pragma unroll
-  for (int j = 0; j < ITEMS; ++j) e[j] = first + 64 * j < n ? expert_of(ids, wide, first + 64 * j, E) : -1;
+    for (int j = 0; j < ITEMS; ++j) e[j] = (uint32_t)E;
+  }
   for (int i = tid; i < W * E; i += 1024) count[i] = 0;
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < ITEMS; ++j) rank[j] = take_rank(count + wave * E, (uint32_t)(e[j] < 0 ? 0 : e[j]), bits, e[j] >= 0);
+  for (int j = 0; j < ITEMS; ++j) rank[j] = take_rank(count + wave * E, e[j], bits, e[j] < (uint32_t)E);
   __syncthreads();
-  int sum = 0, total;
-  if (tid < E)
-    for (int w = 0; w < W; ++w) {
-      const int c = count[w * E + tid];
-      count[w * E + tid] = sum;
-      sum += c;
-    }
+  int c[W], sum = 0, total;
+#pragma unroll
+  for (int w = 0; w < W; ++w) c[w] = tid < E ? count[w * E + tid] : 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) sum += c[w];
   const int base = block_scan<1024>(filled_up(sum, align), tmp, total);
   if (tid < E) {
-    for (int w = 0; w < W; ++w) count[w * E + tid] += base;
+    int at = base;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      count[w * E + tid] = at;
+      at += c[w];
+    }
     soff[tid] = base;
     scnt[tid] = sum;
     o.counts[tid] = sum;
@@ -375,11 +453,12 @@ k_route_small(const void *__restrict__ ids, int wide, int n, int E, int bits, in
   }
   if (tid == 0) { soff[E] = total; o.offsets[E] = total; }
   __syncthreads();
+  order_experts<1024>(scnt, E, o.order);
 #pragma unroll
   for (int j = 0; j < ITEMS; ++j) {
     const int p = first + 64 * j;
     if (p >= n) continue;
-    const int s = e[j] < 0 ? -1 : count[wave * E + e[j]] + rank[j];
+    const int s = e[j] < (uint32_t)E ? count[wave * E + e[j]] + rank[j] : -1;
     o.slot[p] = s;
     if (s >= 0) o.src[s] = p;
   }
@@ -392,14 +471,13 @@ __global__ void __launch_bounds__(kBlockLanes)
 k_route_count(const void *__restrict__ ids, int wide, int64_t n, int E, int *__restrict__ hist) {
   __shared__ int h[kMostExperts];
   const int tid = (int)threadIdx.x;
+  uint32_t e[kBlockItems];
+  load_keys<kBlockItems>(ids, wide, (int64_t)blockIdx.x * kBlock + tid, kBlockLanes, n, (uint32_t)E, e);
   for (int i = tid; i < E; i += kBlockLanes) h[i] = 0;
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < kBlockItems; ++j) {
-    const int64_t p = (int64_t)blockIdx.x * kBlock + j * kBlockLanes + tid;
-    const int e = p < n ? expert_of(ids, wide, p, E) : -1;
-    if (e >= 0) atomicAdd(&h[e], 1);
-  }
+  for (int j = 0; j < kBlockItems; ++j)
+    if (e[j] < (uint32_t)E) atomicAdd(&h[e[j]], 1);
   __syncthreads();
   for (int i = tid; i < E; i += kBlockLanes) hist[(int64_t)blockIdx.x * E + i] = h[i];
 }
@@ -412,9 +490,9 @@ k_route_place(const void *__restrict__ ids, int wide, int64_t n, int E, int bits
   __shared__ int soff[kMostExperts + 1], scnt[kMostExperts];
   const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63, blocks = (int)gridDim.x, b = (int)blockIdx.x;
   const int64_t first = (int64_t)b * kBlock + wave * (64 * kBlockItems) + lane;
-  int e[kBlockItems], rank[kBlockItems], all[PER], below[PER];
-#pragma unroll
-  for (int j = 0; j < kBlockItems; ++j) e[j] = first + 64 * j < n ? expert_of(ids, wide, first + 64 * j, E) : -1;
+  uint32_t e[kBlockItems];
+  int rank[kBlockItems], all[PER], below[PER];
+  load_keys<kBlockItems>(ids, wide, first, 64, n, (uint32_t)E, e);
   for (int i = tid; i < W * E; i += kBlockLanes) count[i] = 0;
 #pragma unroll
   for (int q = 0; q < PER; ++q) {
@@ -432,7 +510,7 @@ k_route_place(const void *__restrict__ ids, int wide, int64_t n, int E, int bits
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kBlockItems; ++j)
-    rank[j] = take_rank(count + wave * E, (uint32_t)(e[j] < 0 ? 0 : e[j]), bits, e[j] >= 0);
+    rank[j] = take_rank(count + wave * E, e[j], bits, e[j] < (uint32_t)E);
   int sum = 0, total;
 #pragma unroll
   for (int q = 0; q < PER; ++q) sum += filled_up(all[q], align);
@@ -459,11 +537,12 @@ k_route_place(const void *__restrict__ ids, int wide, int64_t n, int E, int bits
     if (b == 0) o.offsets[E] = total;
   }
   __syncthreads();
+  if (b == blocks - 1) order_experts<kBlockLanes>(scnt, E, o.order);
 #pragma unroll
   for (int j = 0; j < kBlockItems; ++j) {
     const int64_t p = first + 64 * j;
     if (p >= n) continue;
-    const int s = e[j] < 0 ? -1 : count[wave * E + e[j]] + rank[j];
+    const int s = e[j] < (uint32_t)E ? count[wave * E + e[j]] + rank[j] : -1;
     o.slot[p] = s;
     if (s >= 0) o.src[s] = (int32_t)p;
   }
@@ -563,21 +642,21 @@ extern "C" int64_t anc_route_workspace_bytes(int64_t assignments, int64_t expert
 }
 
 extern "C" int anc_route(uint64_t expert_ids, int32_t ids_bytes, int64_t n, int64_t experts, int64_t align, uint64_t counts,
-                         uint64_t offsets, uint64_t slot, uint64_t src, int64_t capacity, uint64_t workspace,
+                         uint64_t offsets, uint64_t order, uint64_t slot, uint64_t src, int64_t capacity, uint64_t workspace,
                          int64_t workspace_bytes, uint64_t stream) {
   int64_t need;
   if (int rc = check_route("anc_route", n > 0 ? n : 1, experts, align, need)) return rc;
   ANC_REQUIRE(n >= 0 && capacity >= (n > 0 ? need : 1) && capacity < (1ll << 31), "anc_route: %lld assignments, room for %lld slots, %lld needed",
               (long long)n, (long long)capacity, (long long)need);
   ANC_REQUIRE(ids_bytes == 4 || ids_bytes == 8, "anc_route: ids of %d bytes (4 or 8)", (int)ids_bytes);
-  ANC_REQUIRE((expert_ids != 0 || n == 0) && counts && offsets && slot && src && workspace, "anc_route: null pointer");
-  ANC_REQUIRE(expert_ids % (uint64_t)ids_bytes == 0 && ((counts | offsets | slot | src | workspace) & 3) == 0,
+  ANC_REQUIRE((expert_ids != 0 || n == 0) && counts && offsets && order && slot && src && workspace, "anc_route: null pointer");
+  ANC_REQUIRE(expert_ids % (uint64_t)ids_bytes == 0 && ((counts | offsets | order | slot | src | workspace) & 3) == 0,
               "anc_route: misaligned pointers");
   const int64_t ws = anc_route_workspace_bytes(n > 0 ? n : 1, experts);
   ANC_REQUIRE(workspace_bytes >= ws, "anc_route: workspace holds %lld bytes, %lld needed", (long long)workspace_bytes, (long long)ws);
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_MISC, s);
-  const Route o{(int32_t *)counts, (int32_t *)offsets, (int32_t *)slot, (int32_t *)src};
+  const Route o{(int32_t *)counts, (int32_t *)offsets, (int32_t *)order, (int32_t *)slot, (int32_t *)src};
   const int E = (int)experts, bits = bits_of((uint32_t)E - 1), wide = ids_bytes == 8;
   if (n <= kSmallMax) {
     with_items(n, [&](auto items) {

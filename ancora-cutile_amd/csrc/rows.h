@@ -22,6 +22,7 @@ template <> struct Raw<ANC_BF16, 8> { anc_u32x4 q; };
 template <> struct Raw<ANC_BF16, 2> { uint32_t q; };
 template <> struct Raw<ANC_BF16, 1> { uint16_t q; };
 template <> struct Raw<ANC_F32, 8> { anc_f32x4 a, b; };
+template <> struct Raw<ANC_F32, 4> { anc_f32x4 a; };
 template <> struct Raw<ANC_F32, 2> { anc_f32x2 a; };
 template <> struct Raw<ANC_F32, 1> { float a; };
 
@@ -44,6 +45,8 @@ template <int T, int VEC> __device__ __forceinline__ void widen(const Raw<T, VEC
   } else if constexpr (VEC == 8) {
     x[0] = r.a.x; x[1] = r.a.y; x[2] = r.a.z; x[3] = r.a.w;
     x[4] = r.b.x; x[5] = r.b.y; x[6] = r.b.z; x[7] = r.b.w;
+  } else if constexpr (VEC == 4) {
+    x[0] = r.a.x; x[1] = r.a.y; x[2] = r.a.z; x[3] = r.a.w;
   } else if constexpr (VEC == 2) {
     x[0] = r.a.x; x[1] = r.a.y;
   } else {
@@ -61,6 +64,8 @@ template <int T, int VEC> __device__ __forceinline__ Raw<T, VEC> narrow(const fl
   } else if constexpr (VEC == 8) {
     r.a = anc_f32x4{x[0], x[1], x[2], x[3]};
     r.b = anc_f32x4{x[4], x[5], x[6], x[7]};
+  } else if constexpr (VEC == 4) {
+    r.a = anc_f32x4{x[0], x[1], x[2], x[3]};
   } else if constexpr (VEC == 2) {
     r.a = anc_f32x2{x[0], x[1]};
   } else {
@@ -73,7 +78,25 @@ template <int T, int VEC> __device__ __forceinline__ void store(elem_t<T> *p, co
   *(Raw<T, VEC> *)p = narrow<T, VEC>(x);
 }
 
+// i / d for i < 2^31 as one multiplication (64-bit division by a value that is not known to the compiler is some hundred instructions):
+// m = ceil(2^(31 + s) / d) with 2^s >= d is below 2^32 + 1 and m i / 2^(31 + s) exceeds i / d by less than 1 / d.
+struct FastDiv {
+  uint32_t d, mul;
+  int shift;
+  __device__ __forceinline__ uint32_t div(uint32_t i) const { return d == 1 ? i : __umulhi(i, mul) >> shift; }
+};
+inline FastDiv fast_div(uint32_t d) {
+  FastDiv f{d, 0, 0};
+  if (d == 1) return f;
+  int s = 0;
+  while ((1ull << s) < d) ++s;                       // 2^s >= d >= 2, s >= 1
+  f.mul = (uint32_t)(((1ull << (31 + s)) + d - 1) / d);
+  f.shift = s - 1;
+  return f;
+}
+
 // ---- host side: which piece a call's rows allow
+constexpr int64_t kMostPieces = (1ll << 31) - 1;     // of one launch (FastDiv)
 struct Ptr { uint64_t p; int type; };
 inline int64_t elem_size(int type) { return type == ANC_F32 ? 4 : 2; }
 inline bool type_ok(int type) { return type == ANC_F32 || type == ANC_BF16; }

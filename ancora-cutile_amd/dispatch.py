@@ -22,6 +22,7 @@ class RoutePlan:
 
     counts (E,) int32     tokens of each expert
     offsets (E + 1,)      first slot of each expert's segment, filled up to a multiple of `align` (a power of two up to 256)
+    order (E,)            the experts by falling number of tokens (as they are numbered beyond 256 experts)
     slot (tokens, k)      slot of token t's choice j, -1: none
     src (capacity,)       the assignment t * k + j of a slot, -1: filling, or behind the last segment
     capacity              slots (rows of xs, ys) that hold every routing of `tokens` tokens
@@ -39,12 +40,13 @@ class RoutePlan:
         if self.capacity < 0:
             raise ValueError("RoutePlan: " + _lib.load().anc_last_error().decode())
         nbytes = api.anc_route_workspace_bytes(A, self.E)
-        sizes = (self.E, self.E + 1, A, self.capacity)
+        sizes = (self.E, self.E + 1, self.E, A, self.capacity)
         self._block = DevBuf.empty((sum(sizes),), np.int32)
         self._ws = DevBuf.empty((nbytes,), np.uint8)
-        at = [self._block.ptr + 4 * sum(sizes[:i]) for i in range(4)]
-        shapes = ((self.E,), (self.E + 1,), (self.tokens, self.k), (self.capacity,))
-        self.counts, self.offsets, self.slot, self.src = (DevBuf(shape=sh, dtype=np.int32, ptr=p) for sh, p in zip(shapes, at))
+        at = [self._block.ptr + 4 * sum(sizes[:i]) for i in range(5)]
+        shapes = ((self.E,), (self.E + 1,), (self.E,), (self.tokens, self.k), (self.capacity,))
+        bufs = [DevBuf(shape=sh, dtype=np.int32, ptr=p) for sh, p in zip(shapes, at)]
+        self.counts, self.offsets, self.order, self.slot, self.src = bufs
         self._at = (*at, self.capacity, self._ws.ptr, nbytes)
         self.active = None                     # tokens of the last `route`
 
@@ -83,7 +85,7 @@ def dispatch(plan, x, si, xs):
     _rows_of(xs, plan.capacity, H, "dispatch", "xs")
     if x.dtype != xs.dtype:
         raise ValueError(f"dispatch: x is {x.dtype}, xs {xs.dtype}")
-    counts, offsets, slot = plan._at[:3]
+    counts, offsets, _, slot = plan._at[:4]
     api.anc_dispatch(slot, counts, offsets, plan.active, plan.k, plan.E, plan.align, x.ptr, xs.ptr, _type(x, "dispatch"), H, int(si))
 
 
@@ -102,7 +104,7 @@ def combine(plan, ys, weights, si, y):
     _rows_of(ys, plan.capacity, H, "combine", "ys")
     _rows_of(y, plan.active, H, "combine", "y")
     w = 0 if weights is None else _weights(plan, weights, "combine")
-    api.anc_combine(plan._at[2], w, plan.active, plan.k, ys.ptr, _type(ys, "combine"), y.ptr, _type(y, "combine"), H, int(si))
+    api.anc_combine(plan._at[3], w, plan.active, plan.k, ys.ptr, _type(ys, "combine"), y.ptr, _type(y, "combine"), H, int(si))
 
 
 def dispatch_grad(plan, dxs, si, dx):
@@ -120,7 +122,7 @@ def combine_grad(plan, dy, ys, weights, si, dys, dweights):
     _rows_of(dys, plan.capacity, H, "combine_grad", "dys")
     if ys.dtype != dys.dtype:
         raise ValueError(f"combine_grad: ys is {ys.dtype}, dys {dys.dtype}")
-    counts, offsets, slot = plan._at[:3]
+    counts, offsets, _, slot = plan._at[:4]
     api.anc_combine_grad(slot, _weights(plan, weights, "combine_grad"), counts, offsets, plan.active, plan.k, plan.E, plan.align, dy.ptr,
                          _type(dy, "combine_grad"), ys.ptr, dys.ptr, _type(ys, "combine_grad"),
                          _weights(plan, dweights, "combine_grad"), H, int(si))

@@ -140,7 +140,7 @@ def expert_dW(plan, problems, si=0):
     read. Asynchronous on stream `si`."""
     plan._used("expert_dW")
     shapes = [_expert_problem(plan, p) for p in problems]
-    counts, offsets = plan._at[:2]
+    counts, offsets, order = plan._at[:3]
     for i in range(0, len(problems), MAX_PER_CALL):
         group = problems[i:i + MAX_PER_CALL]
         arr = (ExpertDwProblem * len(group))()
@@ -148,4 +148,4 @@ def expert_dW(plan, problems, si=0):
             g16 = p.get("g16")
             _EDW.pack_into(arr, k * _EDW.size, p["x"].ptr, p["dy"].ptr, p["dW"].ptr, 0 if g16 is None else g16.ptr, K, N,
                            1 if p.get("accumulate", False) else 0, 0)
-        api.anc_expert_dw_multi(arr, len(group), counts, offsets, plan.E, int(si))
+        api.anc_expert_dw_multi(arr, len(group), counts, offsets, order, plan.E, int(si))

@@ -354,11 +354,12 @@ int anc_embed_dw(uint64_t srt, uint64_t start, uint64_t cnt, uint64_t key, uint6
  * filled up to a multiple of `align` (a power of two up to 256). An assignment outside [0, experts) has no slot.
  *   counts int32[experts], offsets int32[experts + 1], slot int32[n] (-1: none), src int32[capacity]: the assignment of a
  *   slot (-1: filling, or behind the last segment). capacity >= anc_route_capacity(n, experts, align) slots.
+ *   order int32[experts]: the experts by falling number of tokens (as they are numbered beyond 256 experts).
  * n <= 2^22, experts <= 512. The same expert may be named twice for one token. */
 int64_t anc_route_capacity(int64_t assignments, int64_t experts, int64_t align);
 int64_t anc_route_workspace_bytes(int64_t assignments, int64_t experts);
 int anc_route(uint64_t expert_ids, int32_t ids_bytes, int64_t n, int64_t experts, int64_t align, uint64_t counts,
-              uint64_t offsets, uint64_t slot, uint64_t src, int64_t capacity, uint64_t workspace, int64_t workspace_bytes,
+              uint64_t offsets, uint64_t order, uint64_t slot, uint64_t src, int64_t capacity, uint64_t workspace, int64_t workspace_bytes,
               uint64_t stream);
 
 /* Rows there and back over the slots of anc_route (slot int32[tokens * k]); types ANC_F32 or ANC_BF16, sums in fp32 with
@@ -490,15 +491,16 @@ int anc_gemm_dw_info(int64_t T, int64_t K, int64_t N, double *flops, int32_t *se
  * slot offsets[e] on (the arrays of anc_route, on the device: no host round trip), up to 8 weights per call. x (slots, K) and
  * dy (slots, N) bf16, dW (experts, K, N) fp32 overwritten, or added onto when `accumulate` is set; an expert without tokens gets zeros
  * (or keeps dW). g16, if not 0, receives the bf16 copy of the final dW. Rows that fill up a segment are not read, whatever they hold.
- * An expert's tokens are added in ascending order, one accumulator per element: its bits are a function of its own rows.
- * K, N multiples of 8; x, dy, dW 16-byte aligned. */
+ * An expert's tokens are added in ascending order, one accumulator per element: its bits are a function of its own rows. order: every
+ * expert once, best by falling number of tokens (anc_route's): the order in which they are taken up, no more.
+ * K, N multiples of 8 up to 2^17; x, dy, dW 16-byte aligned. */
 typedef struct {
   uint64_t x, dy, dW, g16;
   int64_t  K, N;
   int32_t  accumulate, reserved;
 } anc_expert_dw_problem_t;
 int anc_expert_dw_multi(const anc_expert_dw_problem_t *problems, int32_t n_problems, uint64_t counts, uint64_t offsets,
-                        int64_t experts, uint64_t stream);
+                        uint64_t order, int64_t experts, uint64_t stream);
 
 /* MXFP8 re-quantisation of bf16 weights (E, K, N) after the step: per block of 32 consecutive K
  * and per column one E8M0 scale byte = (biased fp32 exponent of the block's amax) - 7 (0 below

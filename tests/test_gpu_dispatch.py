@@ -51,7 +51,7 @@ def _experts(rng, T, k, E, how):
 
 
 ROUTES = [(1, 1, 1, 1), (1, 8, 128, 16), (3, 2, 5, 128), (700, 3, 7, 1), (1000, 4, 512, 4), (2048, 8, 64, 256), (5000, 8, 31, 16),
-          (33, 512, 300, 2), (60000, 2, 512, 1), (9001, 8, 160, 128)]
+          (33, 512, 300, 2), (500, 3, 256, 8), (9000, 2, 256, 1), (9000, 3, 257, 1), (60000, 2, 512, 1), (9001, 8, 160, 128)]
 
 
 @pytest.mark.parametrize("T,k,E,align", ROUTES)
@@ -71,6 +71,7 @@ def test_route(gpu, T, k, E, align):
             counts, offsets, slot, src = ref.route(np.where((e[:n] >= 0) & (e[:n] < E), e[:n], -1), E, align)
             assert np.array_equal(plan.counts.to_numpy(), counts), (how, n)
             assert np.array_equal(plan.offsets.to_numpy(), offsets), (how, n)
+            assert np.array_equal(plan.order.to_numpy(), np.argsort(-counts, kind="stable") if E <= 256 else np.arange(E)), (how, n)
             got = plan.slot.to_numpy()
             assert np.array_equal(got[:n], slot) and np.array_equal(got[n:], before[n:]), (how, n)
             full = np.full(plan.capacity, -1)

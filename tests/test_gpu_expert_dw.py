@@ -52,7 +52,7 @@ def _check(got, counts, offsets, x, dy, base=None):
     assert np.all(np.abs(got - want) <= bound), float((np.abs(got - want) - bound).max())
 
 
-@pytest.mark.parametrize("K,N", [(8, 8), (64, 264), (128, 256), (136, 1000), (640, 392), (264, 72), (1024, 512)])
+@pytest.mark.parametrize("K,N", [(8, 8), (1536, 2304), (64, 264), (128, 256), (136, 1000), (640, 392), (264, 72), (1024, 512)])
 @pytest.mark.parametrize("counts,align", [((0, 1, 31, 32, 33), 1), ((64, 0, 100, 5, 0, 95, 96, 97), 16), ((3,), 128), ((1000, 1, 257), 32)])
 def test_against_64_bits(gpu, K, N, counts, align):
     from ancora_cutile_amd import DevBuf, expert_dW
