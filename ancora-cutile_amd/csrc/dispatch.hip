@@ -93,7 +93,7 @@ k_combine(const int32_t *__restrict__ slot, const float *__restrict__ w, uint32_
 // One wavefront per token, four choices at a time: their rows are in flight together, dy comes from the caches for the next
 // four. The four products' sums over the lanes are made together: at the first two steps of the butterfly a lane hands half of its sums
 // on and keeps the other half, so that four sums take 7 exchanges instead of 24.
-template <int TY, int TS, int VEC>
+template <int TY, int TS, int VEC, bool ONCE>
 __global__ void __launch_bounds__(kLanes)
 k_combine_grad(const int32_t *__restrict__ slot, const float *__restrict__ w, const int32_t *__restrict__ counts,
                const int32_t *__restrict__ offsets, int64_t tokens, int k, int align, int64_t main_blocks, int64_t H,
@@ -124,7 +124,7 @@ k_combine_grad(const int32_t *__restrict__ slot, const float *__restrict__ w, co
       const Raw<TY, VEC> own = load<TY, VEC>(dy + t * H + col);
 #pragma unroll
       for (int j = 0; j < D; ++j)
-        if (s[j] >= 0) v[j] = load<TS, VEC>(ys + s[j] * H + col);
+        if (s[j] >= 0) v[j] = load<TS, VEC, ONCE>(ys + s[j] * H + col);
       widen<TY, VEC>(own, g);
 #pragma unroll
       for (int j = 0; j < D; ++j) {
@@ -136,7 +136,7 @@ k_combine_grad(const int32_t *__restrict__ slot, const float *__restrict__ w, co
           dot[j] = fmaf(g[q], a[q], dot[j]);
           o[q] = f[j] * g[q];
         }
-        store<TS, VEC>(dys + s[j] * H + col, o);
+        store<TS, VEC, ONCE>(dys + s[j] * H + col, o);
       }
     }
     // lane bit 5 chooses the pair (0, 1) or (2, 3), bit 4 the one of the pair
@@ -241,7 +241,9 @@ extern "C" int anc_combine_grad(uint64_t slot, uint64_t weights, uint64_t counts
     with_type(ys_type, [&](auto ts) {
       with_piece(vec, [&](auto v) {
         constexpr int TY = decltype(ty)::value, TS = decltype(ts)::value, VEC = decltype(v)::value;
-        hipLaunchKernelGGL((k_combine_grad<TY, TS, VEC>), dim3((unsigned)all), dim3(kLanes), 0, s, (const int32_t *)slot,
+        const bool once = tokens * k * H * elem_size(ys_type) > kCached;
+        auto kernel = once ? k_combine_grad<TY, TS, VEC, true> : k_combine_grad<TY, TS, VEC, false>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)all), dim3(kLanes), 0, s, (const int32_t *)slot,
                            (const float *)weights, (const int32_t *)counts, (const int32_t *)offsets, tokens, (int)k, (int)align, blocks, H,
                            (const elem_t<TY> *)dy, (const elem_t<TS> *)ys, (elem_t<TS> *)dys, (float *)dw);
       });

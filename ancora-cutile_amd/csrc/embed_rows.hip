@@ -10,7 +10,7 @@ using namespace anc_rows;
 
 // U pieces of VEC elements per lane, (row, piece) flattened over the grid. The U ids and then the U pieces are in flight together.
 constexpr int kLookupLanes = 256;
-template <int TT, int TO, int VEC, int U>
+template <int TT, int TO, int VEC, int U, bool ONCE>
 __global__ void __launch_bounds__(kLookupLanes)
 k_embed_lookup(const void *__restrict__ ids, int wide, uint32_t total, int64_t V, FastDiv pieces, int64_t H, float scale,
                const elem_t<TT> *__restrict__ table, elem_t<TO> *__restrict__ out) {
@@ -35,40 +35,58 @@ k_embed_lookup(const void *__restrict__ ids, int wide, uint32_t total, int64_t V
     const bool there = id[u] >= 0 && id[u] < V;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) x[k] = there ? x[k] * scale : 0.0f;
-    store<TO, VEC>(out + (int64_t)row[u] * H + col[u], x);
+    store<TO, VEC, ONCE>(out + (int64_t)row[u] * H + col[u], x);
   }
 }
 
-// The gradient walks the sorted positions in chunks of `chunk` (at most 64): a workgroup takes one chunk's rows of dy one after the
-// other, and a group that lies inside the chunk is finished there. Of a group that reaches over an edge the chunk leaves a partial row,
-// of the group that comes in (part 0) and of the one that goes out (part 1; a group that fills the chunk is part 0), and
-// k_embed_dw_join adds them up in ascending order. Work is even whatever the ids: one id may hold most of the batch.
+// The gradient walks the sorted positions in chunks: a workgroup of kSubs teams, each of which adds up the rows of dy of `sub` (at most 64)
+// positions one after the other. A group that lies inside a team's positions is finished there. Of one that reaches over an edge the team
+// leaves a row in LDS, of the group that comes in (head) and of the one that begins and goes out (tail), and the teams put
+// together what meets inside the chunk. What reaches over the chunk's edges goes to memory the same way, part 0 of the group that comes in and
+// part 1 of the one that begins and goes out, and k_embed_dw_join adds those up in ascending order. Work is even whatever the ids: one
+// id may hold most of the batch.
 struct EmbedDw {
   const int32_t *srt, *start, *cnt, *key, *grp;
   int64_t n, V, H;
-  int chunk;
+  int sub, chunk;                                    // chunk = kSubs * sub positions
   float scale;
   float *out, *compact, *part;
 };
-constexpr int kDwLanes = 256;
+constexpr int kSubs = 4;
+constexpr int kDwLanes = 256;                        // most lanes of a team, and of the join
 
-template <int TD, int VEC, bool DENSE>
-__global__ void __launch_bounds__(kDwLanes) k_embed_dw(EmbedDw p, const elem_t<TD> *__restrict__ dy) {
-  const int lane = (int)(threadIdx.x & 63);
-  const int64_t p0 = (int64_t)blockIdx.x * p.chunk, here = p0 + lane;
-  const bool in = lane < p.chunk && here < p.n;
+template <int VEC, bool DENSE>
+__device__ __forceinline__ void put_row(const EmbedDw &p, int64_t at, const float (&acc)[VEC]) {
+  float x[VEC];
+  float *to = (DENSE ? p.out : p.compact) + at;
+  if constexpr (DENSE) widen<ANC_F32, VEC>(load<ANC_F32, VEC>(to), x);
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) x[k] = DENSE ? x[k] + p.scale * acc[k] : p.scale * acc[k];
+  store<ANC_F32, VEC>(to, x);
+}
+
+template <int TD, int VEC, bool DENSE, bool ONCE>
+__global__ void __launch_bounds__(kDwLanes * kSubs) k_embed_dw(EmbedDw p, const elem_t<TD> *__restrict__ dy) {
+  extern __shared__ float edge[];                    // [kSubs][head, tail][lanes * VEC]
+  __shared__ int flags[kSubs];                       // 1: a head, 2: its group goes out again, 4: a tail
+  const int lane = (int)(threadIdx.x & 63), team = __builtin_amdgcn_readfirstlane((int)threadIdx.y);
+  const int64_t p0 = (int64_t)blockIdx.x * p.chunk + (int64_t)team * p.sub, here = p0 + lane;
+  const bool in = lane < p.sub && here < p.n;
   const int64_t at = in ? here : p.n - 1;
   const int idx = p.srt[at], key = p.key[at], read = p.grp[at], grp = in ? read : -1;
-  const int came = p0 > 0 ? p.grp[p0 - 1] : -1;                          // the group before the chunk
-  const int goes = p0 + p.chunk < p.n ? p.grp[p0 + p.chunk] : -1;        // ... and behind it
+  const int came = p0 > 0 && p0 < p.n ? p.grp[p0 - 1] : -1;              // the group before the team's positions
+  const int goes = p0 + p.sub < p.n ? p.grp[p0 + p.sub] : -1;            // ... and behind them
   const int m = __popcll(__ballot(grp >= 0));                            // (ids that name no row lie at the end)
   const int64_t col = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
   const bool live = col < p.H;
   const int64_t c0 = live ? col : 0;                                     // (every lane stays: its indices serve the others)
+  const int width = (int)blockDim.x * VEC;
+  float *head = edge + team * 2 * width + threadIdx.x * VEC, *tail = head + width;
   float acc[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
-  constexpr int D = 8;
+  int state = 0, tail_grp = -1, tail_key = 0;
+  constexpr int D = DENSE ? 4 : 8;
   for (int i = 0; i < m; i += D) {
     Raw<TD, VEC> v[D];
     Raw<ANC_F32, VEC> old[DENSE ? D : 1];
@@ -77,8 +95,8 @@ __global__ void __launch_bounds__(kDwLanes) k_embed_dw(EmbedDw p, const elem_t<T
     for (int j = 0; j < D; ++j) {
       const int q = i + j < m ? i + j : m - 1;
       g[j] = __builtin_amdgcn_readlane(grp, q);
-      next[j] = q + 1 < m ? __builtin_amdgcn_readlane(grp, q + 1) : -1;  // (a group that goes on behind the chunk ends here, too)
-      v[j] = load<TD, VEC>(dy + (int64_t)__builtin_amdgcn_readlane(idx, q) * p.H + c0);
+      next[j] = q + 1 < m ? __builtin_amdgcn_readlane(grp, q + 1) : -1;  // (a group that goes on behind ends here, too)
+      v[j] = load<TD, VEC, ONCE>(dy + (int64_t)__builtin_amdgcn_readlane(idx, q) * p.H + c0);
       if constexpr (DENSE)
         if (next[j] != g[j] && g[j] != came && g[j] != goes)
           old[j] = load<ANC_F32, VEC>(p.out + (int64_t)__builtin_amdgcn_readlane(key, q) * p.H + c0);
@@ -91,24 +109,57 @@ __global__ void __launch_bounds__(kDwLanes) k_embed_dw(EmbedDw p, const elem_t<T
 #pragma unroll
       for (int k = 0; k < VEC; ++k) acc[k] = acc[k] + x[k];
       if (next[j] == g[j]) continue;
-      if (live) {
-        if (g[j] == came || g[j] == goes) {
-          store<ANC_F32, VEC>(p.part + ((int64_t)blockIdx.x * 2 + (g[j] == came ? 0 : 1)) * p.H + c0, acc);
-        } else {
-          if constexpr (DENSE) widen<ANC_F32, VEC>(old[j], x);
+      if (g[j] == came) {
+        state |= g[j] == goes ? 3 : 1;
+        *(Raw<ANC_F32, VEC> *)head = narrow<ANC_F32, VEC>(acc);
+      } else if (g[j] == goes) {
+        state |= 4;
+        tail_grp = g[j];
+        tail_key = __builtin_amdgcn_readlane(key, i + j);
+        *(Raw<ANC_F32, VEC> *)tail = narrow<ANC_F32, VEC>(acc);
+      } else if (live) {
+        if constexpr (DENSE) widen<ANC_F32, VEC>(old[j], x);
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) x[k] = DENSE ? x[k] + p.scale * acc[k] : p.scale * acc[k];
-          store<ANC_F32, VEC>(DENSE ? p.out + (int64_t)__builtin_amdgcn_readlane(key, i + j) * p.H + c0 : p.compact + (int64_t)g[j] * p.H + c0, x);
-        }
+        for (int k = 0; k < VEC; ++k) x[k] = DENSE ? x[k] + p.scale * acc[k] : p.scale * acc[k];
+        store<ANC_F32, VEC>(DENSE ? p.out + (int64_t)__builtin_amdgcn_readlane(key, i + j) * p.H + c0 : p.compact + (int64_t)g[j] * p.H + c0, x);
       }
 #pragma unroll
       for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
     }
   }
+  if (threadIdx.x == 0) flags[team] = state;
+  __syncthreads();
+  auto add_head = [&](int t) {
+    float x[VEC];
+    widen<ANC_F32, VEC>(*(const Raw<ANC_F32, VEC> *)(edge + t * 2 * width + threadIdx.x * VEC), x);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] = acc[k] + x[k];
+  };
+  if (state & 4) {                                   // what begins here and goes on
+    widen<ANC_F32, VEC>(*(const Raw<ANC_F32, VEC> *)tail, acc);
+    int t = team + 1;
+    for (; t < kSubs; ++t) {
+      add_head(t);
+      if (!(flags[t] & 2)) break;
+    }
+    if (live) {
+      if (t < kSubs) put_row<VEC, DENSE>(p, (DENSE ? (int64_t)tail_key : (int64_t)tail_grp) * p.H + c0, acc);
+      else store<ANC_F32, VEC>(p.part + ((int64_t)blockIdx.x * 2 + 1) * p.H + c0, acc);
+    }
+  }
+  if (team == 0 && (state & 1)) {                    // what came into the chunk
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
+    for (int t = 0; t < kSubs; ++t) {
+      add_head(t);
+      if (!(flags[t] & 2)) break;
+    }
+    if (live) store<ANC_F32, VEC>(p.part + (int64_t)blockIdx.x * 2 * p.H + c0, acc);
+  }
 }
 
 // Chunk c's part 1 begins a group that goes on: the parts of it, in order. The four wavefronts take a quarter of the list each
-// (a third of 65536 positions on one id: 338 partial rows of 64 positions), 16 rows in flight, and their sums meet in LDS.
+// (a third of 65536 positions on one id: 338 rows of 64 ... ), 8 rows in flight, and their sums meet in LDS.
 template <int VEC>
 __global__ void __launch_bounds__(kDwLanes) k_embed_dw_join(EmbedDw p) {
   constexpr int W = kDwLanes / 64;
@@ -129,7 +180,7 @@ __global__ void __launch_bounds__(kDwLanes) k_embed_dw_join(EmbedDw p) {
   float acc[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
-  constexpr int D = 16;
+  constexpr int D = 8;
   for (int64_t i = lo; i < hi; i += D) {
     Raw<ANC_F32, VEC> v[D];
 #pragma unroll
@@ -162,9 +213,9 @@ __global__ void __launch_bounds__(kDwLanes) k_embed_dw_join(EmbedDw p) {
   store<ANC_F32, VEC>(to, x);
 }
 
-// Positions per chunk: enough chunks to fill the card, at most 64 (one index per lane).
-constexpr int64_t kChunk16Most = 16384, kChunk32Most = 32768;
-int dw_chunk(int64_t n) { return n <= kChunk16Most ? 16 : n <= kChunk32Most ? 32 : 64; }
+// Positions per team: enough chunks to fill the card.
+constexpr int64_t kSub8Most = 8192, kSub16Most = 32768;
+int dw_chunk(int64_t n) { return kSubs * (n <= kSub8Most ? 8 : n <= kSub16Most ? 16 : 64); }
 int64_t dw_chunks(int64_t n) { return (n + dw_chunk(n) - 1) / dw_chunk(n); }
 constexpr int64_t kMostPositions = 1ll << 20;
 constexpr int64_t kFewPieces = 1 << 19;              // of a lookup: below, one piece per lane
@@ -189,12 +240,13 @@ extern "C" int anc_embed_lookup(uint64_t ids, int32_t ids_bytes, int64_t n, uint
   for (int64_t r = 0; r < n; r += most) {
     const int64_t rows = n - r < most ? n - r : most, total = rows * per_row;
     const int u = total >= kFewPieces ? 4 : 1;
+    const bool once = n * H * elem_size(out_type) > kCached;
     const dim3 grid((unsigned)((total + u * kLookupLanes - 1) / (u * kLookupLanes)));
     with_type(table_type, [&](auto tt) {
       with_type(out_type, [&](auto to) {
         with_piece(vec, [&](auto v) {
           constexpr int TT = decltype(tt)::value, TO = decltype(to)::value, VEC = decltype(v)::value;
-          auto kernel = u == 4 ? k_embed_lookup<TT, TO, VEC, 4> : k_embed_lookup<TT, TO, VEC, 1>;
+          auto kernel = u == 1 ? k_embed_lookup<TT, TO, VEC, 1, false> : once ? k_embed_lookup<TT, TO, VEC, 4, true> : k_embed_lookup<TT, TO, VEC, 4, false>;
           hipLaunchKernelGGL(kernel, grid, dim3(kLookupLanes), 0, s, (const void *)(ids + (uint64_t)(r * ids_bytes)), ids_bytes == 8,
                              (uint32_t)total, V, fast_div((uint32_t)per_row), H, scale, (const elem_t<TT> *)table,
                              (elem_t<TO> *)out + r * H);
@@ -213,7 +265,7 @@ extern "C" int64_t anc_embed_dw_workspace_bytes(int64_t M, int64_t H) {
     return -1;
   }
   int64_t most = dw_chunks(M);
-  for (int64_t edge : {kChunk16Most, kChunk32Most})
+  for (int64_t edge : {kSub8Most, kSub16Most})
     if (edge < M && dw_chunks(edge) > most) most = dw_chunks(edge);
   return most * 2 * H * 4;
 }
@@ -231,22 +283,26 @@ extern "C" int anc_embed_dw(uint64_t srt, uint64_t start, uint64_t cnt, uint64_t
               "anc_embed_dw: misaligned pointers");
   const int64_t chunks = dw_chunks(n), need = chunks * 2 * H * 4;
   ANC_REQUIRE(workspace_bytes >= need, "anc_embed_dw: workspace holds %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
-  const Ptr ps[2] = {{dy, dy_type}, {out | compact, ANC_F32}};
-  const int vec = piece(H, ps);
+  const Ptr ps[1] = {{dy, dy_type}};
+  const int rows = piece(H, ps), vec = ((out | compact) & (uint64_t)(rows >= 4 ? 15 : 4 * rows - 1)) == 0 ? rows : 1;
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_MISC, s);
   EmbedDw p{(const int32_t *)srt, (const int32_t *)start, (const int32_t *)cnt, (const int32_t *)key, (const int32_t *)grp,
-            n, V, H, dw_chunk(n), scale, (float *)out, (float *)compact, (float *)workspace};
+            n, V, H, dw_chunk(n) / kSubs, dw_chunk(n), scale, (float *)out, (float *)compact, (float *)workspace};
   with_piece(vec, [&](auto v) {
     constexpr int VEC = decltype(v)::value;
-    const int64_t waves = (H + 64 * VEC - 1) / (64 * VEC), wide = waves < kDwLanes / 64 ? waves : kDwLanes / 64;
+    // (a team is at most 1024 columns wide: 32 KiB of LDS for the edges)
+    constexpr int64_t widest = VEC == 8 ? 2 : kDwLanes / 64;
+    const int64_t waves = (H + 64 * VEC - 1) / (64 * VEC), wide = waves < widest ? waves : widest;
     with_type(dy_type, [&](auto t) {
       constexpr int T = decltype(t)::value;
-      auto kernel = out != 0 ? k_embed_dw<T, VEC, true> : k_embed_dw<T, VEC, false>;
-      hipLaunchKernelGGL(kernel, dim3((unsigned)chunks, (unsigned)((waves + wide - 1) / wide)), dim3((unsigned)(64 * wide)), 0, s, p,
-                         (const elem_t<T> *)dy);
+      const bool once = n * H * elem_size(dy_type) > kCached;
+      auto kernel = out != 0 ? (once ? k_embed_dw<T, VEC, true, true> : k_embed_dw<T, VEC, true, false>)
+                             : (once ? k_embed_dw<T, VEC, false, true> : k_embed_dw<T, VEC, false, false>);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)chunks, (unsigned)((waves + wide - 1) / wide)), dim3((unsigned)(64 * wide), kSubs),
+                         (unsigned)(kSubs * 2 * 64 * wide * VEC * sizeof(float)), s, p, (const elem_t<T> *)dy);
     });
-    constexpr int JV = VEC == 8 ? 4 : VEC;           // narrower pieces: more wavefronts on a long list
+    constexpr int JV = VEC < 4 ? VEC : 4;            // narrower pieces: more wavefronts on a long list
     if (chunks > 1)
       hipLaunchKernelGGL((k_embed_dw_join<JV>), dim3((unsigned)(chunks - 1), (unsigned)((H + 64 * JV - 1) / (64 * JV))), dim3(kDwLanes), 0, s, p);
   });

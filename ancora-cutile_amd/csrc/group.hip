@@ -6,23 +6,27 @@
 // per bit of the digit; an item's rank is the number of earlier lanes among them plus the wavefront's count of the digit
 // so far, a counter in LDS. Items of different wavefronts meet in an exclusive sum over (digit, wavefront).
 //
-// Up to 1024 x kMostItems items one workgroup does everything in one launch: the keys stay in LDS and only 16-bit positions are
-// permuted, 9 bits a pass (two passes for a vocabulary of 152 K). Beyond, the same passes run over blocks of kBlock items
-// with the blocks' digit counts in memory: a block adds up the counts before it itself (no launch in between), and the
-// count for the next pass is made by the scatter, with integer atomics, which have no order to lose.
+// Ids of up to kMostSplit positions are grouped in one launch: every workgroup looks at all ids, takes those of its share of the order
+// (shares cut by a sample), sorts them in LDS and writes them where they belong; what lies before its share it has counted on the
+// way. A launch costs as much as looking at some ten thousand ids. Beyond, passes of 9 bits over blocks of kBlock items with the
+// blocks' digit counts in memory: a block adds up the counts before it itself (no launch in between), and the count for the next pass is
+// made by the scatter, with integer atomics, which have no order to lose.
 #include "common.h"
 
 namespace {
 
+typedef int anc_i32x4 __attribute__((ext_vector_type(4)));
+
 constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
-constexpr int kMostItems = 16;                       // per lane of the one-workgroup kernels
-constexpr int kSmallMax = 1024 * kMostItems;
+constexpr int kRouteItems = 4, kSmallRoute = 1024 * kRouteItems;       // assignments that one workgroup takes
 constexpr int kBlockLanes = 256, kBlockItems = 8, kBlock = kBlockLanes * kBlockItems;
 
 // Lanes of the wavefront that hold the same digit as this one, among those with `in`. (Six vector instructions a bit: the digit's bit
 // as 0 or -1, its ballot, and two words of agreement.)
 __device__ __forceinline__ uint64_t same_digit(uint32_t d, int bits, bool in) {
   const uint64_t all = __ballot(in);
+  const int first = all != 0 ? __builtin_ctzll(all) : 0;
+  if (__ballot(in && d == (uint32_t)__builtin_amdgcn_readlane((int)d, first)) == all) return all;      // (a frequent id's run)
   uint32_t lo = (uint32_t)all, hi = (uint32_t)(all >> 32);
   for (int b = 0; b < bits; ++b) {
     const uint32_t s = (uint32_t)__builtin_amdgcn_sbfe((int)d, b, 1);
@@ -73,6 +77,7 @@ __device__ __forceinline__ int block_scan(int v, int *tmp, int &total) {
     base += w < wave ? t : 0;
     total += t;
   }
+  total = __builtin_amdgcn_readfirstlane(total);
   return base + inc - v;
 }
 
@@ -105,102 +110,312 @@ struct Groups {
   int32_t *count;                                    // number of groups
 };
 
-// ---------------------------------------------------------------- token ids, one workgroup
-template <int ITEMS>
-__global__ void __launch_bounds__(1024)
-k_group_small(const void *__restrict__ ids, int wide, int n, int M, uint32_t V, int bits, Groups o) {
-  constexpr int W = 16, N = 1024 * ITEMS;
-  __shared__ uint32_t skey[N];
-  __shared__ uint16_t sidx[N];
-  __shared__ int count[W * kDigits];
+// ---------------------------------------------------------------- token ids, one launch
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// An item's place in the order, as a number: its id, then its position.
+__device__ __forceinline__ uint64_t place(uint32_t key, int p) { return (uint64_t)key << 32 | (uint32_t)p; }
+// A token id as a key: V for one that names no row.
+__device__ __forceinline__ uint32_t as_key(int32_t id, uint32_t V) { return (uint32_t)id < V ? (uint32_t)id : V; }
+__device__ __forceinline__ uint32_t as_key(int64_t id, uint32_t V) { return (uint64_t)id < V ? (uint32_t)id : V; }
+constexpr int kPartItems = 4, kTile = 8, kSamples = 256;
+constexpr int64_t kFewAlone = 512, kMostAlone = 4096, kMostSplit = 1 << 16;             // positions: of one workgroup, of several
+constexpr int64_t kMostMarked = 1 << 18;                               // ids, where several workgroups share them (one bit each in LDS)
+
+// SPLIT: gridDim.x workgroups share the order; else one takes all of it (n <= CAP, and any V).
+template <int LANES, bool SPLIT, typename ID>
+__global__ void __launch_bounds__(LANES)
+k_group_part(const ID *__restrict__ ids, int n, int64_t M, uint32_t V, Groups o) {
+  constexpr int W = LANES / 64, CAP = LANES * kPartItems, PER = kDigits > LANES ? kDigits / LANES : 1;
+  __shared__ uint32_t skey[CAP];
+  __shared__ int spos[SPLIT ? CAP : 1];
+  __shared__ uint16_t sidx[CAP];
+  __shared__ __attribute__((aligned(16))) int count[W * kDigits];      // (also the sample, and where the groups begin)
   __shared__ int tmp[W];
-  const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63, first = wave * (64 * ITEMS) + lane;
-  int idx[ITEMS];
-  uint32_t key[ITEMS];
-  if (n > 0) {
-    load_keys<ITEMS>(ids, wide, first, 64, n, V, key);       // (what lies behind the last id stays behind the ids that name no row)
-  } else {
+  __shared__ anc_i32x4 four[W];
+  __shared__ int cut[4];
+  __shared__ uint32_t last_id;
+  __shared__ uint32_t marks[SPLIT ? kMostMarked / 32 : 1];
+  static_assert(W * kDigits >= CAP && W * kDigits >= kSamples, "count is used three ways");
+  const int tid = (int)threadIdx.x, wave = uniform(tid >> 6), lane = tid & 63, parts = (int)gridDim.x, part = (int)blockIdx.x;
+  uint32_t id_lo = 0, id_hi = V + 1;                 // this workgroup's share: from (id_lo, p_lo) to (id_hi, p_hi)
+  int p_lo = 0, p_hi = 0;
+  const int words = (int)((V + 31) / 32);
+  // A wavefront looks at `share` positions next to each other (64 times 64 at most), kTile times 64 at a time.
+  const int share = ((n + W - 1) / W + 63) / 64 * 64, w0 = wave * share, w1 = w0 + share < n ? w0 + share : n;
+  uint32_t key[kTile];
+  ID raw[kTile];
+  auto fetch = [&](int t) {
 #pragma unroll
-    for (int j = 0; j < ITEMS; ++j) key[j] = V;
-  }
+    for (int j = 0; j < kTile; ++j) raw[j] = ids[t + 64 * j + lane < w1 ? t + 64 * j + lane : w1 - 1];
+  };
+  // f(a tile's first position) for all tiles of the wavefront, its keys there, the next tile's ids on their way; the first is fetched again.
+  auto each_tile = [&](auto f) {
+#pragma unroll 1
+    for (int t = w0; t < w1; t += 64 * kTile) {
 #pragma unroll
-  for (int j = 0; j < ITEMS; ++j) {
-    idx[j] = first + 64 * j;
-    skey[first + 64 * j] = key[j];
-  }
-  for (int shift = 0; shift < bits; shift += kDigitBits) {
-    const int b = bits - shift < kDigitBits ? bits - shift : kDigitBits, digits = 1 << b;
-    for (int i = tid; i < W << b; i += 1024) count[i] = 0;
+      for (int j = 0; j < kTile; ++j) key[j] = as_key(raw[j], V);
+      fetch(t + 64 * kTile < w1 ? t + 64 * kTile : w0);
+      f(t);
+    }
+  };
+  if (w0 < w1) fetch(w0);
+  if constexpr (SPLIT) {
+    // Every workgroup sorts the same sample, a position of every n / kSamples, spread by a multiplicative hash, by looking at all of it, and
+    // cuts the order at its own two of the shares.
+    constexpr int L = LANES / kSamples;              // lanes per sample, neighbours, each looking at a run of the others
+    uint32_t *sample = (uint32_t *)count;
+    const int i = tid / L, at = (int)((int64_t)i * n / kSamples) + (int)(((uint32_t)i * 2654435761u >> 8) % (uint32_t)(n / kSamples));
+    const uint32_t id = as_key(ids[at], V), mine = id << 8 | (uint32_t)i;  // (at most 19 bits of id, and the sample's own order)
+    for (int w = tid; w < words; w += LANES) marks[w] = 0;
+    if (tid % L == 0) sample[i] = mine;
+    if (tid < 4) cut[tid] = tid == 2 ? (int)(V + 1) : 0;
     __syncthreads();
-    int rank[ITEMS];
+    int before = 0;
+    const anc_u32x4 *run = (const anc_u32x4 *)sample + (tid % L) * (kSamples / L / 4);
 #pragma unroll
-    for (int j = 0; j < ITEMS; ++j)
-      rank[j] = take_rank(count + (wave << b), (key[j] >> shift) & (digits - 1), b, true);
+    for (int j = 0; j < kSamples / L / 4; ++j) {
+      const anc_u32x4 v = run[j];
+      before += (v.x < mine ? 1 : 0) + (v.y < mine ? 1 : 0) + (v.z < mine ? 1 : 0) + (v.w < mine ? 1 : 0);
+    }
+#pragma unroll
+    for (int s = 1; s < L; s <<= 1) before += __shfl_xor(before, s, 64);
+    if (tid % L == 0) {
+      if (part > 0 && before == part * kSamples / parts) { cut[0] = (int)id; cut[1] = at; }
+      if (part + 1 < parts && before == (part + 1) * kSamples / parts) { cut[2] = (int)id; cut[3] = at; }
+    }
     __syncthreads();
-    int c[W], sum = 0, total;
+    id_lo = (uint32_t)uniform(cut[0]);
+    p_lo = uniform(cut[1]);
+    id_hi = (uint32_t)uniform(cut[2]);
+    p_hi = uniform(cut[3]);
+  }
+  bool marked = false;
+  int groups = 0;                                    // of the whole batch
+  while (place(id_lo, p_lo) < place(id_hi, p_hi)) {
+    uint32_t id_to = id_hi;                          // the piece that is done at once ends at (id_to, p_to)
+    uint64_t mask = 0;
+    int p_to = p_hi, size = n, put = 0, base = 0, came = 0, goes = 0, smaller = 0;
+    if constexpr (SPLIT) {
+      const uint64_t lo = place(id_lo, p_lo);
+      for (;;) {
+        // Lane i keeps which of the wavefront's i-th 64 positions belong to the piece. Counted are the items before it, those of its first
+        // id before it and those of the id it ends in behind it.
+        const uint64_t to = place(id_to, p_to);
+        mask = 0;
+        int low = 0, came_goes = 0;                  // (of a lane, then of a wavefront: at most 64 and 4096)
+        each_tile([&](int t) {
+          if (!marked) {                             // (a frequent id is read, not set, from its second item on)
+            uint32_t seen[kTile];
 #pragma unroll
-    for (int w = 0; w < W; ++w) c[w] = tid < digits ? count[(w << b) + tid] : 0;
+            for (int j = 0; j < kTile; ++j) seen[j] = ((volatile uint32_t *)marks)[key[j] < V ? key[j] >> 5 : 0];
 #pragma unroll
-    for (int w = 0; w < W; ++w) sum += c[w];
-    int at = block_scan<1024>(sum, tmp, total);
-    if (tid < digits) {
+            for (int j = 0; j < kTile; ++j)
+              if (key[j] < V && !(seen[j] >> (key[j] & 31) & 1u)) atomicOr(&marks[key[j] >> 5], 1u << (key[j] & 31));
+          }
+#pragma unroll
+          for (int j = 0; j < kTile; ++j) {
+            if (t + 64 * j >= w1) break;
+            const int p = t + 64 * j + lane;
+            const uint64_t r = place(key[j], p);
+            const bool there = p < w1, is_low = r < lo, is_high = r >= to;
+            const uint64_t m = __ballot(there && !is_low && !is_high);
+            if (lane == (t - w0) / 64 + j) mask = m;
+            low += there && is_low ? 1 : 0;
+            if (__ballot(key[j] == id_lo || key[j] == id_to) != 0)
+              came_goes += there && is_low && key[j] == id_lo ? 1 : there && is_high && key[j] == id_to ? 0x10000 : 0;
+          }
+        });
+        marked = true;
+        const int own = __popcll(mask), upto = wave_scan(own);
+#pragma unroll
+        for (int s = 32; s >= 1; s >>= 1) {
+          low += __shfl_xor(low, s, 64);
+          came_goes += __shfl_xor(came_goes, s, 64);
+        }
+        if (lane == 63) four[wave] = anc_i32x4{upto, low, came_goes & 0xFFFF, came_goes >> 16};
+        __syncthreads();
+        anc_i32x4 sum = {0, 0, 0, 0};
+        put = upto - own;                            // this lane's first
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const anc_i32x4 v = four[w];
+          put += w < wave ? v.x : 0;
+          sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+        }
+        size = uniform(sum.x);
+        base = uniform(sum.y);
+        came = uniform(sum.z);
+        goes = uniform(sum.w);
+        __syncthreads();
+        if (size <= CAP) break;
+        // More than LDS holds (hardly ever: a share is a quarter of that or less on average): the largest beginning that fits.
+        uint64_t fits = lo, over = to;
+        while (over - fits > 1) {
+          const uint64_t mid = fits + (over - fits) / 2;
+          int some = 0, total;
+          each_tile([&](int t) {
+#pragma unroll
+            for (int j = 0; j < kTile; ++j) {
+              const uint64_t r = place(key[j], t + 64 * j + lane);
+              some += t + 64 * j + lane < w1 && r >= lo && r < mid ? 1 : 0;
+            }
+          });
+          block_scan<LANES>(some, tmp, total);
+          if (total <= CAP) fits = mid; else over = mid;
+        }
+        id_to = (uint32_t)(fits >> 32);
+        p_to = (int)(uint32_t)fits;
+      }
+      int low_every = 0;                             // ids below the piece's first; all of them (a wavefront's are at most 2^15 - 1 ... 2^14)
+      for (int i = tid; i < words; i += LANES) {
+        const uint32_t w = marks[i], i32 = (uint32_t)i * 32;
+        low_every += __popc(w) << 16 | (i32 + 32 <= id_lo ? __popc(w) : i32 >= id_lo ? 0 : __popc(w & ((1u << (id_lo - i32)) - 1)));
+      }
+#pragma unroll
+      for (int s = 32; s >= 1; s >>= 1) low_every += __shfl_xor(low_every, s, 64);
+      if (lane == 0) tmp[wave] = low_every;
+      for (; mask != 0; mask &= mask - 1) spos[put++] = w0 + lane * 64 + (int)__builtin_ctzll(mask);
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kPartItems; ++j)
+        if (tid + j * LANES < size) skey[tid + j * LANES] = as_key(ids[spos[tid + j * LANES]], V);
+      groups = 0;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        count[(w << b) + tid] = at;
-        at += c[w];
+        smaller += tmp[w] & 0xFFFF;
+        groups += (int)((uint32_t)tmp[w] >> 16);
+      }
+      smaller = uniform(smaller);
+      groups = uniform(groups);
+      __syncthreads();
+    } else {
+      each_tile([&](int t) {
+#pragma unroll
+        for (int j = 0; j < kTile; ++j)
+          if (t + 64 * j + lane < w1) skey[t + 64 * j + lane] = key[j];
+      });
+      __syncthreads();
+    }
+    // The piece by its ids, relative to the first. Up to RANKED items are counted against each other: an item's rank is the number of smaller
+    // (id, place in the piece), L lanes look for it. More go by up to 9 bits a pass. `items` per lane, a wavefront's next to each other.
+    const int items = (size + LANES - 1) / LANES, first = wave * 64 * items + lane;
+    const int bits = 32 - __builtin_clz((id_to - id_lo) | 1);
+    const int passes = (bits + kDigitBits - 1) / kDigitBits, per = (bits + passes - 1) / passes;
+    int idx[kPartItems], rank[kPartItems];
+    uint32_t k[kPartItems];
+#pragma unroll
+    for (int j = 0; j < kPartItems; ++j) {
+      idx[j] = first + 64 * j;
+      k[j] = j < items && idx[j] < size ? skey[idx[j]] : 0;
+    }
+    constexpr int RANKED = LANES < 512 ? LANES : 512, L = LANES / RANKED;
+    const bool by_rank = size <= RANKED && bits <= 22;
+    if (by_rank) {
+      uint32_t *numbers = (uint32_t *)count;
+      if (tid < RANKED) numbers[tid] = tid < size ? (k[0] - id_lo) << 9 | (uint32_t)tid : ~0u;
+      __syncthreads();
+      const uint32_t mine = numbers[tid / L];
+      int smaller_ones = 0;
+      for (int v = tid % L; v * 4 < size; v += L) {
+        const anc_u32x4 q = ((const anc_u32x4 *)numbers)[v];
+        smaller_ones += (q.x < mine ? 1 : 0) + (q.y < mine ? 1 : 0) + (q.z < mine ? 1 : 0) + (q.w < mine ? 1 : 0);
+      }
+#pragma unroll
+      for (int s = 1; s < L; s <<= 1) smaller_ones += __shfl_xor(smaller_ones, s, 64);
+      if (tid % L == 0 && tid / L < size) sidx[smaller_ones] = (uint16_t)(tid / L);
+      __syncthreads();
+      if (tid < size) {
+        idx[0] = sidx[tid];
+        k[0] = skey[idx[0]];
+      }
+    }
+    for (int shift = by_rank ? bits : 0; shift < bits; shift += per) {
+      const int b = bits - shift < per ? bits - shift : per, digits = 1 << b;
+      for (int i = tid; i < W << b; i += LANES) count[i] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kPartItems; ++j)
+        if (j < items) rank[j] = take_rank(count + (wave << b), ((k[j] - id_lo) >> shift) & (digits - 1), b, first + 64 * j < size);
+      __syncthreads();
+      int c[PER][W], sum = 0, total;                 // PER digits of a lane, next to each other
+#pragma unroll
+      for (int q = 0; q < PER; ++q)
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          c[q][w] = tid * PER + q < digits ? count[(w << b) + tid * PER + q] : 0;
+          sum += c[q][w];
+        }
+      int at = block_scan<LANES>(sum, tmp, total);
+#pragma unroll
+      for (int q = 0; q < PER; ++q)
+        if (tid * PER + q < digits) {
+#pragma unroll
+          for (int w = 0; w < W; ++w) {
+            count[(w << b) + tid * PER + q] = at;
+            at += c[q][w];
+          }
+        }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kPartItems; ++j)
+        if (j < items && first + 64 * j < size)
+          sidx[count[(wave << b) + (((k[j] - id_lo) >> shift) & (digits - 1))] + rank[j]] = (uint16_t)idx[j];
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kPartItems; ++j)
+        if (j < items && first + 64 * j < size) {
+          idx[j] = sidx[first + 64 * j];
+          k[j] = skey[idx[j]];
+        }
+    }
+    // Heads: the first item of an id. Their number up to an item is its group, counted from the ids below the piece.
+    int heads = 0, mine = 0, valid = 0;
+#pragma unroll
+    for (int j = 0; j < kPartItems; ++j) {
+      const int p = first + 64 * j;
+      if (j >= items || p >= size) continue;
+      const bool head = k[j] < V && (p == 0 ? came == 0 || k[j] != id_lo : skey[sidx[p - 1]] != k[j]);
+      heads |= head ? 1 << j : 0;
+      mine += head ? 1 : 0;
+      valid += k[j] < V ? 1 : 0;
+    }
+    int both;                                        // heads and items that name a row (CAP at most)
+    int run = uniform(block_scan<LANES>(mine | valid << 16, tmp, both)) & 0xFFFF;        // (lane 0's: heads of the wavefronts before this one)
+    const int n_heads = both & 0xFFFF, n_valid = both >> 16;
+    const int group0 = smaller + (came > 0 && id_lo < V ? 1 : 0);
+#pragma unroll
+    for (int j = 0; j < kPartItems; ++j) {
+      const int p = first + 64 * j;
+      const bool head = (heads >> j) & 1;
+      const uint64_t m = __ballot(head);
+      const int h = run + lanes_before(m) + (head ? 1 : 0);
+      run += __popcll(m);
+      if (j >= items || p >= size) continue;
+      const int g = group0 + h - 1;
+      o.srt[base + p] = SPLIT ? spos[idx[j]] : idx[j];
+      o.key[base + p] = (int32_t)k[j];
+      o.grp[base + p] = k[j] < V ? g : -1;
+      if (head) {
+        count[h - 1] = p;
+        if (h == n_heads) last_id = k[j];
+        o.start[g] = base + p;
+        o.gid[g] = (int32_t)k[j];
       }
     }
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < ITEMS; ++j)
-      sidx[count[(wave << b) + ((key[j] >> shift) & (digits - 1))] + rank[j]] = (uint16_t)idx[j];
+    for (int h = tid; h < n_heads; h += LANES)       // (the last group may go on behind the piece)
+      o.cnt[group0 + h] = (h + 1 < n_heads ? count[h + 1] : n_valid + (last_id == id_to ? goes : 0)) - count[h];
+    if constexpr (!SPLIT) groups = n_heads;
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < ITEMS; ++j) {
-      idx[j] = sidx[first + 64 * j];
-      key[j] = skey[idx[j]];
-    }
+    id_lo = id_to;
+    p_lo = p_to;
   }
-  // The number of heads (first items of an id) up to an item is its group.
-  int heads = 0, valid = 0, mine = 0;
-#pragma unroll
-  for (int j = 0; j < ITEMS; ++j) {
-    const int p = first + 64 * j;
-    const bool head = key[j] < V && (p == 0 || skey[sidx[p - 1]] != key[j]);
-    heads |= head ? 1 << j : 0;
-    mine += head ? 1 : 0;
-    valid += key[j] < V ? 1 : 0;
+  for (int64_t g = groups + (int64_t)part * LANES + tid; g < M; g += (int64_t)parts * LANES) {
+    o.start[g] = 0;
+    o.cnt[g] = 0;
+    o.gid[g] = -1;
   }
-  int total, n_valid;
-  const int before = block_scan<1024>(mine, tmp, total) - (wave_scan(mine) - mine);    // heads of the wavefronts before this one
-  block_scan<1024>(valid, tmp, n_valid);             // (its barriers also end the reads of skey above)
-  int run = before;
-#pragma unroll
-  for (int j = 0; j < ITEMS; ++j) {
-    const int p = first + 64 * j;
-    const bool head = (heads >> j) & 1;
-    const uint64_t m = __ballot(head);
-    const int g = run + __popcll(m & ((1ull << lane) - 1)) - (head ? 0 : 1);
-    run += __popcll(m);
-    if (p < n) {
-      o.srt[p] = idx[j];
-      o.key[p] = (int32_t)key[j];
-      o.grp[p] = key[j] < V ? g : -1;
-    }
-    if (head) {
-      skey[g] = (uint32_t)p;
-      o.gid[g] = (int32_t)key[j];
-    }
-  }
-  __syncthreads();
-  for (int g = tid; g < M; g += 1024) {
-    const bool used = g < total;
-    const int at = used ? (int)skey[g] : 0;
-    o.start[g] = at;
-    o.cnt[g] = used ? (g + 1 < total ? (int)skey[g + 1] : n_valid) - at : 0;
-    if (!used) o.gid[g] = -1;
-  }
-  if (tid == 0) *o.count = total;
+  if (part == 0 && tid == 0) *o.count = groups;
 }
 
 // ---------------------------------------------------------------- token ids, many workgroups
@@ -227,7 +442,7 @@ k_radix_count(const void *__restrict__ ids, int wide, int64_t n, int64_t M, uint
   for (int64_t i = b * kBlockLanes + tid; i < M; i += blocks * kBlockLanes) cnt[i] = 0;
 }
 
-// Items [lo, lo + 64 * ITEMS) of a wavefront in rank order; `base`: first place of every digit for this block.
+// One stable pass over bits shift .. of the keys.
 __global__ void __launch_bounds__(kBlockLanes)
 k_radix_scatter(const void *__restrict__ ids, int wide, const int32_t *__restrict__ key_in,
                 const int32_t *__restrict__ idx_in, int64_t n, uint32_t V, int shift, int bits,
@@ -259,14 +474,20 @@ k_radix_scatter(const void *__restrict__ ids, int wide, const int32_t *__restric
   int all[PER], below[PER];
 #pragma unroll
   for (int q = 0; q < PER; ++q) all[q] = below[q] = 0;
-#pragma unroll 8
-  for (int64_t c = 0; c < blocks; ++c) {
+  constexpr int D = 16;
+  for (int64_t c = 0; c < blocks; c += D) {
+    int v[D][PER];
 #pragma unroll
-    for (int q = 0; q < PER; ++q) {
-      const int v = hist[c * kDigits + tid * PER + q];
-      all[q] += v;
-      below[q] += c < b ? v : 0;
-    }
+    for (int i = 0; i < D; ++i)
+#pragma unroll
+      for (int q = 0; q < PER; ++q) v[i][q] = hist[(c + i < blocks ? c + i : blocks - 1) * kDigits + tid * PER + q];
+#pragma unroll
+    for (int i = 0; i < D; ++i)
+#pragma unroll
+      for (int q = 0; q < PER; ++q) {
+        all[q] += c + i < blocks ? v[i][q] : 0;
+        below[q] += c + i < b ? v[i][q] : 0;
+      }
   }
   __syncthreads();
   int rank[kBlockItems];
@@ -487,30 +708,44 @@ k_route_place(const void *__restrict__ ids, int wide, int64_t n, int E, int bits
   constexpr int W = kBlockLanes / 64, PER = kMostExperts / kBlockLanes;
   __shared__ int count[W * kMostExperts];
   __shared__ int tmp[W];
-  __shared__ int soff[kMostExperts + 1], scnt[kMostExperts];
+  __shared__ int soff[kMostExperts + 1], scnt[kMostExperts], sall[kMostExperts], sbelow[kMostExperts];
   const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63, blocks = (int)gridDim.x, b = (int)blockIdx.x;
   const int64_t first = (int64_t)b * kBlock + wave * (64 * kBlockItems) + lane;
   uint32_t e[kBlockItems];
   int rank[kBlockItems], all[PER], below[PER];
   load_keys<kBlockItems>(ids, wide, first, 64, n, (uint32_t)E, e);
   for (int i = tid; i < W * E; i += kBlockLanes) count[i] = 0;
+  // counts of every expert over all blocks and over the blocks before this one: `parts` lanes share an expert's column
+  for (int i = tid; i < E; i += kBlockLanes) sall[i] = sbelow[i] = 0;
+  __syncthreads();
+  const int parts = E < kBlockLanes ? kBlockLanes / E : 1;
+  for (int d = tid % E; d < E && tid < parts * E; d += kBlockLanes) {
+    constexpr int D = 8;
+    int a = 0, u = 0;
+    for (int c = tid / E; c < blocks; c += D * parts) {
+      int v[D];
 #pragma unroll
-  for (int q = 0; q < PER; ++q) {
-    all[q] = below[q] = 0;
-    const int d = tid * PER + q;
-    if (d < E) {
-#pragma unroll 8
-      for (int c = 0; c < blocks; ++c) {
-        const int v = hist[(int64_t)c * E + d];
-        all[q] += v;
-        below[q] += c < b ? v : 0;
+      for (int i = 0; i < D; ++i) v[i] = hist[(int64_t)(c + i * parts < blocks ? c + i * parts : c) * E + d];
+#pragma unroll
+      for (int i = 0; i < D; ++i) {
+        a += c + i * parts < blocks ? v[i] : 0;
+        u += c + i * parts < b ? v[i] : 0;
       }
     }
+    atomicAdd(&sall[d], a);
+    atomicAdd(&sbelow[d], u);
   }
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kBlockItems; ++j)
     rank[j] = take_rank(count + wave * E, e[j], bits, e[j] < (uint32_t)E);
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < PER; ++q) {
+    const int d = tid * PER + q;
+    all[q] = d < E ? sall[d] : 0;
+    below[q] = d < E ? sbelow[d] : 0;
+  }
   int sum = 0, total;
 #pragma unroll
   for (int q = 0; q < PER; ++q) sum += filled_up(all[q], align);
@@ -559,10 +794,7 @@ int bits_of(uint32_t most) {                         // bits that hold 0 .. most
 int64_t n_blocks(int64_t n) { return (n + kBlock - 1) / kBlock; }
 constexpr int64_t kMostIds = 1ll << 20, kMostAssignments = 1ll << 22;
 
-template <int V> struct IC { static constexpr int value = V; };
-template <typename F> void with_items(int64_t n, F &&f) {
-  if (n <= 1024) f(IC<1>{}); else if (n <= 4096) f(IC<4>{}); else if (n <= 8192) f(IC<8>{}); else f(IC<kMostItems>{});
-}
+bool one_launch(int64_t n, int64_t V) { return n <= kMostAlone || (n <= kMostSplit && V <= kMostMarked); }
 
 }  // namespace
 
@@ -572,8 +804,9 @@ extern "C" int64_t anc_id_groups_device_workspace_bytes(int64_t M, int64_t V) {
                   (long long)V);
     return -1;
   }
+  if (one_launch(M, V)) return 16;
   const int64_t passes = (bits_of((uint32_t)V) + kDigitBits - 1) / kDigitBits;
-  return M <= kSmallMax ? 4 : 4 * (n_blocks(M) * (kDigits * passes + 1) + 4 * M);
+  return 4 * (n_blocks(M) * (kDigits * passes + 1) + 4 * M);
 }
 
 extern "C" int anc_id_groups_device(uint64_t ids, int32_t ids_bytes, int64_t n, int64_t M, int64_t V, uint64_t srt, uint64_t start,
@@ -584,7 +817,7 @@ extern "C" int anc_id_groups_device(uint64_t ids, int32_t ids_bytes, int64_t n, 
   ANC_REQUIRE(ids_bytes == 4 || ids_bytes == 8, "anc_id_groups_device: ids of %d bytes (4 or 8)", (int)ids_bytes);
   ANC_REQUIRE((ids != 0 || n == 0) && srt && start && cnt && gid && key && grp && count && workspace,
               "anc_id_groups_device: null pointer");
-  ANC_REQUIRE(ids % (uint64_t)ids_bytes == 0 && ((srt | start | cnt | gid | key | grp | count | workspace) & 3) == 0,
+  ANC_REQUIRE(ids % (uint64_t)ids_bytes == 0 && ((srt | start | cnt | gid | key | grp | count) & 3) == 0 && (workspace & 15) == 0,
               "anc_id_groups_device: misaligned pointers");
   ANC_REQUIRE(workspace_bytes >= anc_id_groups_device_workspace_bytes(n > 0 ? n : 1, V), "anc_id_groups_device: workspace holds %lld bytes, %lld needed",
               (long long)workspace_bytes, (long long)anc_id_groups_device_workspace_bytes(n > 0 ? n : 1, V));
@@ -592,27 +825,39 @@ extern "C" int anc_id_groups_device(uint64_t ids, int32_t ids_bytes, int64_t n, 
   AncProfScope prof(ANC_PROF_MISC, s);
   const Groups o{(int32_t *)srt, (int32_t *)start, (int32_t *)cnt, (int32_t *)gid, (int32_t *)key, (int32_t *)grp, (int32_t *)count};
   const int bits = bits_of((uint32_t)V), wide = ids_bytes == 8;
-  if (n <= kSmallMax) {
-    with_items(n, [&](auto items) {
-      hipLaunchKernelGGL(k_group_small<decltype(items)::value>, dim3(1), dim3(1024), 0, s, (const void *)ids, wide, (int)n, (int)M,
-                         (uint32_t)V, bits, o);
-    });
+  if (n <= kFewAlone) {
+    if (wide) hipLaunchKernelGGL((k_group_part<256, false, int64_t>), dim3(1), dim3(256), 0, s, (const int64_t *)ids, (int)n, M, (uint32_t)V, o);
+    else      hipLaunchKernelGGL((k_group_part<256, false, int32_t>), dim3(1), dim3(256), 0, s, (const int32_t *)ids, (int)n, M, (uint32_t)V, o);
+    ANC_LAUNCH_CHECK();
+    return ANC_OK;
+  }
+  if (n <= kMostAlone) {
+    if (wide) hipLaunchKernelGGL((k_group_part<1024, false, int64_t>), dim3(1), dim3(1024), 0, s, (const int64_t *)ids, (int)n, M, (uint32_t)V, o);
+    else      hipLaunchKernelGGL((k_group_part<1024, false, int32_t>), dim3(1), dim3(1024), 0, s, (const int32_t *)ids, (int)n, M, (uint32_t)V, o);
+    ANC_LAUNCH_CHECK();
+    return ANC_OK;
+  }
+  if (one_launch(n, V)) {
+    const int64_t parts = (n + 63) / 64;
+    const dim3 grid((unsigned)(parts < 128 ? parts : 128)), lanes(1024);
+    if (wide) hipLaunchKernelGGL((k_group_part<1024, true, int64_t>), grid, lanes, 0, s, (const int64_t *)ids, (int)n, M, (uint32_t)V, o);
+    else      hipLaunchKernelGGL((k_group_part<1024, true, int32_t>), grid, lanes, 0, s, (const int32_t *)ids, (int)n, M, (uint32_t)V, o);
     ANC_LAUNCH_CHECK();
     return ANC_OK;
   }
   const int64_t blocks = n_blocks(n);
+  const dim3 grid((unsigned)blocks), lanes(kBlockLanes);
   const int passes = (bits + kDigitBits - 1) / kDigitBits;
   int *hist = (int *)workspace, *heads = hist + blocks * kDigits * passes;
   int32_t *buf = heads + blocks;                     // two (key, position) pairs of arrays
-  const dim3 grid((unsigned)blocks), lanes(kBlockLanes);
   hipLaunchKernelGGL(k_radix_count, grid, lanes, 0, s, (const void *)ids, wide, n, M, (uint32_t)V, bits, passes, hist, o.cnt);
   const int32_t *key_in = nullptr, *idx_in = nullptr;
   for (int q = 0; q < passes; ++q) {
     const bool last = q + 1 == passes;
     int32_t *key_out = last ? o.key : buf + (q & 1) * 2 * n, *idx_out = last ? o.srt : key_out + n;
     hipLaunchKernelGGL(k_radix_scatter, grid, lanes, 0, s, (const void *)ids, wide, key_in, idx_in, n, (uint32_t)V,
-                       q * kDigitBits, bits, hist + q * blocks * kDigits, last ? (int *)nullptr : hist + (q + 1) * blocks * kDigits,
-                       key_out, idx_out);
+                       q * kDigitBits, bits, (const int *)(hist + q * blocks * kDigits),
+                       last ? (int *)nullptr : hist + (q + 1) * blocks * kDigits, key_out, idx_out);
     key_in = key_out;
     idx_in = idx_out;
   }
@@ -638,7 +883,7 @@ extern "C" int64_t anc_route_capacity(int64_t assignments, int64_t experts, int6
 extern "C" int64_t anc_route_workspace_bytes(int64_t assignments, int64_t experts) {
   int64_t c;
   if (check_route("anc_route_workspace_bytes", assignments, experts, 1, c)) return -1;
-  return assignments <= kSmallMax ? 4 : 4 * n_blocks(assignments) * experts;
+  return assignments <= kSmallRoute ? 4 : 4 * n_blocks(assignments) * experts;
 }
 
 extern "C" int anc_route(uint64_t expert_ids, int32_t ids_bytes, int64_t n, int64_t experts, int64_t align, uint64_t counts,
@@ -658,11 +903,9 @@ extern "C" int anc_route(uint64_t expert_ids, int32_t ids_bytes, int64_t n, int6
   AncProfScope prof(ANC_PROF_MISC, s);
   const Route o{(int32_t *)counts, (int32_t *)offsets, (int32_t *)order, (int32_t *)slot, (int32_t *)src};
   const int E = (int)experts, bits = bits_of((uint32_t)E - 1), wide = ids_bytes == 8;
-  if (n <= kSmallMax) {
-    with_items(n, [&](auto items) {
-      hipLaunchKernelGGL(k_route_small<decltype(items)::value>, dim3(1), dim3(1024), 0, s, (const void *)expert_ids, wide, (int)n, E,
-                         bits, (int)align, (int)capacity, o);
-    });
+  if (n <= kSmallRoute) {
+    auto kernel = n <= 1024 ? k_route_small<1> : k_route_small<kRouteItems>;
+    hipLaunchKernelGGL(kernel, dim3(1), dim3(1024), 0, s, (const void *)expert_ids, wide, (int)n, E, bits, (int)align, (int)capacity, o);
   } else {
     const dim3 grid((unsigned)n_blocks(n)), lanes(kBlockLanes);
     hipLaunchKernelGGL(k_route_count, grid, lanes, 0, s, (const void *)expert_ids, wide, n, E, (int *)workspace);

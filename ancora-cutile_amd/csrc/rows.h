@@ -19,9 +19,10 @@ template <int T> using elem_t = typename Elem<T>::type;
 // VEC elements at p, in registers as they lie in memory: loads first, widening where the values are needed.
 template <int T, int VEC> struct Raw;
 template <> struct Raw<ANC_BF16, 8> { anc_u32x4 q; };
+template <> struct Raw<ANC_BF16, 4> { anc_u32x2 q; };
 template <> struct Raw<ANC_BF16, 2> { uint32_t q; };
 template <> struct Raw<ANC_BF16, 1> { uint16_t q; };
-template <> struct Raw<ANC_F32, 8> { anc_f32x4 a, b; };
+template <> struct Raw<ANC_F32, 8> { anc_f32x4 a, b; };      // (sums of bf16 rows)
 template <> struct Raw<ANC_F32, 4> { anc_f32x4 a; };
 template <> struct Raw<ANC_F32, 2> { anc_f32x2 a; };
 template <> struct Raw<ANC_F32, 1> { float a; };
@@ -37,6 +38,11 @@ template <int T, int VEC> __device__ __forceinline__ void widen(const Raw<T, VEC
       x[2 * i] = __uint_as_float(w[i] << 16);
       x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
     }
+  } else if constexpr (T == ANC_BF16 && VEC == 4) {
+    x[0] = __uint_as_float(r.q.x << 16);
+    x[1] = __uint_as_float(r.q.x & 0xFFFF0000u);
+    x[2] = __uint_as_float(r.q.y << 16);
+    x[3] = __uint_as_float(r.q.y & 0xFFFF0000u);
   } else if constexpr (T == ANC_BF16 && VEC == 2) {
     x[0] = __uint_as_float(r.q << 16);
     x[1] = __uint_as_float(r.q & 0xFFFF0000u);
@@ -57,6 +63,8 @@ template <int T, int VEC> __device__ __forceinline__ Raw<T, VEC> narrow(const fl
   Raw<T, VEC> r;
   if constexpr (T == ANC_BF16 && VEC == 8) {
     r.q = anc_u32x4{bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]), bf16_pair(x[4], x[5]), bf16_pair(x[6], x[7])};
+  } else if constexpr (T == ANC_BF16 && VEC == 4) {
+    r.q = anc_u32x2{bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3])};
   } else if constexpr (T == ANC_BF16 && VEC == 2) {
     r.q = bf16_pair(x[0], x[1]);
   } else if constexpr (T == ANC_BF16) {
@@ -72,6 +80,32 @@ template <int T, int VEC> __device__ __forceinline__ Raw<T, VEC> narrow(const fl
     r.a = x[0];
   }
   return r;
+}
+// ONCE: past the caches, for rows so large that whoever reads them next does not find them there anyway (see kCached).
+template <int T, int VEC, bool ONCE> __device__ __forceinline__ Raw<T, VEC> load(const elem_t<T> *p) {
+  Raw<T, VEC> r;
+  if constexpr (!ONCE) {
+    r = *(const Raw<T, VEC> *)p;
+  } else if constexpr (T == ANC_BF16) {
+    r.q = anc_ld_stream((const decltype(r.q) *)p);
+  } else {
+    r.a = anc_ld_stream((const decltype(r.a) *)p);
+    if constexpr (VEC == 8) r.b = anc_ld_stream((const anc_f32x4 *)p + 1);
+  }
+  return r;
+}
+template <int T, int VEC, bool ONCE> __device__ __forceinline__ void store(elem_t<T> *p, const Raw<T, VEC> &r) {
+  if constexpr (!ONCE) {
+    *(Raw<T, VEC> *)p = r;
+  } else if constexpr (T == ANC_BF16) {
+    anc_st_stream((decltype(Raw<T, VEC>::q) *)p, r.q);
+  } else {
+    anc_st_stream((decltype(Raw<T, VEC>::a) *)p, r.a);
+    if constexpr (VEC == 8) anc_st_stream((anc_f32x4 *)p + 1, r.b);
+  }
+}
+template <int T, int VEC, bool ONCE> __device__ __forceinline__ void store(elem_t<T> *p, const float (&x)[VEC]) {
+  store<T, VEC, ONCE>(p, narrow<T, VEC>(x));
 }
 template <int T, int VEC> __device__ __forceinline__ void store(elem_t<T> *p, const Raw<T, VEC> &r) { *(Raw<T, VEC> *)p = r; }
 template <int T, int VEC> __device__ __forceinline__ void store(elem_t<T> *p, const float (&x)[VEC]) {
@@ -97,24 +131,31 @@ inline FastDiv fast_div(uint32_t d) {
 
 // ---- host side: which piece a call's rows allow
 constexpr int64_t kMostPieces = (1ll << 31) - 1;     // of one launch (FastDiv)
+// Bytes up to which rows go through the caches. A lookup of 16 MiB and a copy of it afterwards: 12.6 us, with its stores past the caches 14.7;
+// one of 199 MB: 149 us, past the caches 145, and the lookup alone 72 and 66.
+constexpr int64_t kCached = 64ll << 20;
 struct Ptr { uint64_t p; int type; };
 inline int64_t elem_size(int type) { return type == ANC_F32 ? 4 : 2; }
 inline bool type_ok(int type) { return type == ANC_F32 || type == ANC_BF16; }
-// 8 elements where every row starts 16-byte aligned, else pairs where H is even and the pointers allow them, else single elements.
+// 16 bytes of the widest type where every row starts so aligned (a lane's neighbour then reads the next 16 bytes): 8 elements of bf16 rows, 4
+// where fp32 rows take part; else pairs where H is even and the pointers allow them, else single elements.
 template <int N> inline int piece(int64_t H, const Ptr (&ps)[N]) {
-  bool by8 = H % 8 == 0, by2 = H % 2 == 0;
+  int wide = 8;
+  for (const Ptr &q : ps)
+    if (q.type == ANC_F32) wide = 4;
+  bool wides = H % wide == 0, by2 = H % 2 == 0;
   for (const Ptr &q : ps) {
-    by8 = by8 && (q.p & 15) == 0;
+    wides = wides && q.p % (uint64_t)(wide * elem_size(q.type)) == 0;
     by2 = by2 && q.p % (uint64_t)(2 * elem_size(q.type)) == 0;
   }
-  return by8 ? 8 : by2 ? 2 : 1;
+  return wides ? wide : by2 ? 2 : 1;
 }
 template <int V> struct Int { static constexpr int value = V; };
 template <typename F> inline void with_type(int type, F &&f) {
   if (type == ANC_F32) f(Int<ANC_F32>{}); else f(Int<ANC_BF16>{});
 }
 template <typename F> inline void with_piece(int vec, F &&f) {
-  if (vec == 8) f(Int<8>{}); else if (vec == 2) f(Int<2>{}); else f(Int<1>{});
+  if (vec == 8) f(Int<8>{}); else if (vec == 4) f(Int<4>{}); else if (vec == 2) f(Int<2>{}); else f(Int<1>{});
 }
 
 }  // namespace anc_rows

@@ -114,7 +114,8 @@ def test_lookup_and_gradient_of_rows_beyond_32_bit_offsets(gpu):
         b.free()
 
 
-BATCHES = [(1, 1), (2, 700), (63, 4), (64, 1), (65, 511), (1024, 512), (1025, 100000), (4097, 20), (8192, 151936), (9000, 262144),
+BATCHES = [(1, 1), (2, 700), (63, 4), (64, 1), (65, 511), (1000, (1 << 31) - 1), (1024, 512), (1025, 100000), (4097, 20), (8192, 151936),
+           (9000, 262144), (9000, 262145), (3000, 1 << 30), (65536, 50257), (65537, 151936),
            (16384, 3000), (16385, 151936), (40001, 600), (70001, 1 << 20), (140000, 40)]
 
 
@@ -146,8 +147,36 @@ def test_groups_are_the_hosts(gpu, M, V):
             assert np.array_equal(np.sort(got[0][:n]), np.arange(n)), (dist, n)
             assert np.array_equal(got[1][:g], start) and np.array_equal(got[2][:g], cnt) and np.array_equal(got[3][:g], gid), (dist, n)
             assert not got[1][g:].any() and not got[2][g:].any() and np.all(got[3][g:] == -1), (dist, n)
+            inner = [a.to_numpy().reshape(-1)[:n] for a in (groups._key, groups._grp)]
+            assert np.array_equal(inner[0], np.concatenate([np.repeat(gid, cnt), np.full(n - srt.size, V)])), (dist, n)
+            assert np.array_equal(inner[1], np.concatenate([np.repeat(np.arange(g), cnt), np.full(n - srt.size, -1)])), (dist, n)
         buf.free()
     groups.free()
+
+
+def test_groups_whatever_the_sample_sees(gpu):
+    """Several workgroups share the order by a sample of the positions (one of every n / 256, spread by a hash). Here the sampled
+    positions hold the table's last id and all others lie below it, or the first id and above: one workgroup's share is
+    nearly everything, many times what it holds at once."""
+    from ancora_cutile_amd import DevBuf, DeviceIdGroups
+    for n, V in ((20000, 5000), (65536, 262144), (8192, 300)):
+        rng = np.random.default_rng(n)
+        i = np.arange(256, dtype=np.int64)
+        at = i * n // 256 + (((i * 2654435761) & 0xFFFFFFFF) >> 8) % (n // 256)
+        groups = DeviceIdGroups(n, V)
+        for end in (0, V - 1, -1):
+            ids = rng.integers(1, V - 1, n).astype(np.int32)
+            ids[at] = end
+            buf = DevBuf(ids)
+            groups.group(buf, 0)
+            srt, start, cnt, gid = _groups_want(ids, V)
+            got = [a.to_numpy().reshape(-1) for a in (groups.srt, groups.start, groups.cnt, groups.gid)]
+            g = gid.size
+            assert groups.count.to_numpy()[0] == g and np.array_equal(got[0][:srt.size], srt), (n, end)
+            assert np.array_equal(got[1][:g], start) and np.array_equal(got[2][:g], cnt) and np.array_equal(got[3][:g], gid), (n, end)
+            assert np.array_equal(groups._grp.to_numpy().reshape(-1)[:srt.size], np.repeat(np.arange(g), cnt)), (n, end)
+            buf.free()
+        groups.free()
 
 
 def _dw_check(groups, ids, V, val, got_rows, scale, base=None):
