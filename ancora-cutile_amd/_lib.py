@@ -151,9 +151,9 @@ _PROTOS = {
     "anc_route_capacity": (i64, [i64, i64, i64]),
     "anc_route_workspace_bytes": (i64, [i64, i64]),
     "anc_route": (None, [u64, i32, i64, i64, i64, u64, u64, u64, u64, u64, i64, u64, i64, u64]),
-    "anc_dispatch": (None, [u64, u64, u64, i64, i64, i64, i64, u64, u64, C.c_int, i64, u64]),
-    "anc_combine": (None, [u64, u64, i64, i64, u64, C.c_int, u64, C.c_int, i64, u64]),
-    "anc_combine_grad": (None, [u64, u64, u64, u64, i64, i64, i64, i64, u64, C.c_int, u64, u64, C.c_int, u64, i64, u64]),
+    "anc_dispatch": (None, [u64, u64, u64, i64, i64, i64, i64, u64, u64, i64, C.c_int, i64, u64]),
+    "anc_combine": (None, [u64, u64, i64, i64, u64, i64, C.c_int, u64, C.c_int, i64, u64]),
+    "anc_combine_grad": (None, [u64, u64, u64, u64, i64, i64, i64, i64, u64, C.c_int, u64, u64, i64, C.c_int, u64, i64, u64]),
     "anc_cast_bf16": (None, [u64, u64, i64, C.c_int, u32, u64]),
     "anc_muon_momentum": (None, [u64, u64, u64, i64, i64, f32, C.c_int, C.c_int, C.c_int,
                                  C.c_int, u64, u64]),
@@ -169,7 +169,7 @@ _PROTOS = {
     "anc_quant_mxfp8_w_multi": (None, [u64, i32, i64, C.c_int, u64]),
     "anc_gemm_dw_workspace_bytes": (i64, [i64, i64, i64]),
     "anc_gemm_dw_multi": (None, [C.POINTER(DwProblem), i32, u64]),
-    "anc_expert_dw_multi": (None, [C.POINTER(ExpertDwProblem), i32, u64, u64, u64, i64, u64]),
+    "anc_expert_dw_multi": (None, [C.POINTER(ExpertDwProblem), i32, u64, u64, u64, i64, i64, u64]),
     "anc_gemm_dw_info": (None, [i64, i64, i64, C.POINTER(C.c_double), C.POINTER(i32)]),
     "anc_ns_workspace_bytes": (i64, [i64, i64, i64, C.c_int]),
     "anc_ns_batched": (None, [u64, i64, i64, i64, C.c_int, C.POINTER(f32), f32, C.c_int, u64, i64,

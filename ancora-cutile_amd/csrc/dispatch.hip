@@ -3,7 +3,8 @@
 //     dispatch:      xs[slot] = x[t]; the rows that fill up a segment become zero
 //     combine:       y[t] = sum over j of w[t, j] * ys[slot]          (w = 1: the gradient of dispatch)
 //     combine_grad:  dys[slot] = w[t, j] * dy[t];  dw[t, j] = <dy[t], ys[slot]>
-// All are bound by memory. They go by token, not by slot: a token's own row is read or written once for its k choices.
+// All are bound by memory. They go by token, not by slot: a token's own row is read or written once for its k choices. A slot outside
+// [0, capacity) is taken for none, whatever the array holds.
 #include "rows.h"
 
 namespace {
@@ -13,13 +14,17 @@ using namespace anc_rows;
 constexpr int kLanes = 256;
 constexpr int kPadRows = 8;                 // rows that one workgroup clears
 
+__device__ __forceinline__ int64_t in_range(int64_t slot, int64_t capacity) { return slot < capacity ? slot : -1; }
+
 // Rows between an expert's last token and the end of its segment: workgroup `b` of those that clear them.
 template <int T, int VEC>
-__device__ __forceinline__ void clear_padding(int b, int align, const int32_t *counts, const int32_t *offsets, int64_t H, elem_t<T> *out) {
+__device__ __forceinline__ void clear_padding(int b, int align, const int32_t *counts, const int32_t *offsets, int64_t capacity, int64_t H,
+                                              elem_t<T> *out) {
   const int per = (align - 1 + kPadRows - 1) / kPadRows, e = b / per;
-  const int64_t from = (int64_t)offsets[e] + counts[e] + (int64_t)(b - e * per) * kPadRows, end = offsets[e + 1];
+  const int64_t from = (int64_t)offsets[e] + counts[e] + (int64_t)(b - e * per) * kPadRows, last = offsets[e + 1];
+  const int64_t end = last < capacity ? last : capacity;
   const int64_t to = from + kPadRows < end ? from + kPadRows : end;
-  if (from >= to) return;
+  if (from < 0 || from >= to) return;
   float zero[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) zero[k] = 0.0f;
@@ -29,10 +34,10 @@ __device__ __forceinline__ void clear_padding(int b, int align, const int32_t *c
 template <int T, int VEC>
 __global__ void __launch_bounds__(kLanes)
 k_dispatch(const int32_t *__restrict__ slot, const int32_t *__restrict__ counts, const int32_t *__restrict__ offsets, uint32_t total,
-           int k, int align, uint32_t main_blocks, FastDiv pieces, int64_t H, const elem_t<T> *__restrict__ x,
+           int k, int align, uint32_t main_blocks, FastDiv pieces, int64_t capacity, int64_t H, const elem_t<T> *__restrict__ x,
            elem_t<T> *__restrict__ xs) {
   if (blockIdx.x >= main_blocks) {
-    clear_padding<T, VEC>((int)(blockIdx.x - main_blocks), align, counts, offsets, H, xs);
+    clear_padding<T, VEC>((int)(blockIdx.x - main_blocks), align, counts, offsets, capacity, H, xs);
     return;
   }
   const uint32_t i = blockIdx.x * (uint32_t)kLanes + threadIdx.x;
@@ -45,7 +50,7 @@ k_dispatch(const int32_t *__restrict__ slot, const int32_t *__restrict__ counts,
   for (int j0 = 0; j0 < k; j0 += D) {
     int64_t s[D];
 #pragma unroll
-    for (int j = 0; j < D; ++j) s[j] = to[j0 + j < k ? j0 + j : k - 1];
+    for (int j = 0; j < D; ++j) s[j] = in_range(to[j0 + j < k ? j0 + j : k - 1], capacity);
 #pragma unroll
     for (int j = 0; j < D; ++j)
       if (j0 + j < k && s[j] >= 0) store<T, VEC>(xs + s[j] * H + col, v);
@@ -54,7 +59,7 @@ k_dispatch(const int32_t *__restrict__ slot, const int32_t *__restrict__ counts,
 
 template <int TI, int TO, int VEC, bool WEIGHTS>
 __global__ void __launch_bounds__(kLanes)
-k_combine(const int32_t *__restrict__ slot, const float *__restrict__ w, uint32_t total, int k, FastDiv pieces, int64_t H,
+k_combine(const int32_t *__restrict__ slot, const float *__restrict__ w, uint32_t total, int k, FastDiv pieces, int64_t capacity, int64_t H,
           const elem_t<TI> *__restrict__ ys, elem_t<TO> *__restrict__ y) {
   const uint32_t i = blockIdx.x * (uint32_t)kLanes + threadIdx.x;
   if (i >= total) return;
@@ -71,7 +76,7 @@ k_combine(const int32_t *__restrict__ slot, const float *__restrict__ w, uint32_
 #pragma unroll
     for (int j = 0; j < D; ++j) {
       const int64_t a = t * k + (j0 + j < k ? j0 + j : k - 1);
-      const int64_t at = slot[a];
+      const int64_t at = in_range(slot[a], capacity);
       f[j] = WEIGHTS ? w[a] : 1.0f;
       s[j] = j0 + j < k ? at : -1;
     }
@@ -96,11 +101,11 @@ k_combine(const int32_t *__restrict__ slot, const float *__restrict__ w, uint32_
 template <int TY, int TS, int VEC, bool ONCE>
 __global__ void __launch_bounds__(kLanes)
 k_combine_grad(const int32_t *__restrict__ slot, const float *__restrict__ w, const int32_t *__restrict__ counts,
-               const int32_t *__restrict__ offsets, int64_t tokens, int k, int align, int64_t main_blocks, int64_t H,
+               const int32_t *__restrict__ offsets, int64_t tokens, int k, int align, int64_t main_blocks, int64_t capacity, int64_t H,
                const elem_t<TY> *__restrict__ dy, const elem_t<TS> *__restrict__ ys, elem_t<TS> *__restrict__ dys,
                float *__restrict__ dw) {
   if ((int64_t)blockIdx.x >= main_blocks) {
-    clear_padding<TS, VEC>((int)((int64_t)blockIdx.x - main_blocks), align, counts, offsets, H, dys);
+    clear_padding<TS, VEC>((int)((int64_t)blockIdx.x - main_blocks), align, counts, offsets, capacity, H, dys);
     return;
   }
   const int lane = (int)(threadIdx.x & 63);
@@ -113,7 +118,7 @@ k_combine_grad(const int32_t *__restrict__ slot, const float *__restrict__ w, co
 #pragma unroll
     for (int j = 0; j < D; ++j) {
       const int64_t a = t * k + (j0 + j < k ? j0 + j : k - 1);
-      s[j] = slot[a];
+      s[j] = in_range(slot[a], capacity);
       f[j] = w[a];
       dot[j] = 0.0f;
       if (j0 + j >= k) s[j] = -1;
@@ -151,10 +156,11 @@ k_combine_grad(const int32_t *__restrict__ slot, const float *__restrict__ w, co
   }
 }
 
-int check_rows(const char *who, uint64_t slot, int64_t tokens, int64_t k, int64_t H) {
+int check_rows(const char *who, uint64_t slot, int64_t tokens, int64_t k, int64_t capacity, int64_t H) {
   ANC_REQUIRE(tokens >= 0 && tokens < (1ll << 31) && k > 0 && k <= 512 && H > 0 && H <= (1ll << 20) && tokens * H < (1ll << 38),
               "%s: %lld tokens of width %lld with %lld choices", who, (long long)tokens, (long long)H, (long long)k);
   ANC_REQUIRE(slot != 0 && (slot & 3) == 0, "%s: null or misaligned slots", who);
+  ANC_REQUIRE(capacity > 0 && capacity < (1ll << 31), "%s: room for %lld slots", who, (long long)capacity);
   return ANC_OK;
 }
 int check_segments(const char *who, uint64_t counts, uint64_t offsets, int64_t experts, int64_t align) {
@@ -167,8 +173,8 @@ int64_t pad_blocks(int64_t experts, int64_t align) { return experts * ((align - 
 }  // namespace
 
 extern "C" int anc_dispatch(uint64_t slot, uint64_t counts, uint64_t offsets, int64_t tokens, int64_t k, int64_t experts, int64_t align,
-                            uint64_t x, uint64_t xs, int type, int64_t H, uint64_t stream) {
-  if (int rc = check_rows("anc_dispatch", slot, tokens, k, H)) return rc;
+                            uint64_t x, uint64_t xs, int64_t capacity, int type, int64_t H, uint64_t stream) {
+  if (int rc = check_rows("anc_dispatch", slot, tokens, k, capacity, H)) return rc;
   if (int rc = check_segments("anc_dispatch", counts, offsets, experts, align)) return rc;
   ANC_REQUIRE(type_ok(type), "anc_dispatch: type %d", type);
   ANC_REQUIRE(x && xs && (x | xs) % (uint64_t)elem_size(type) == 0, "anc_dispatch: null or misaligned pointers");
@@ -185,7 +191,7 @@ extern "C" int anc_dispatch(uint64_t slot, uint64_t counts, uint64_t offsets, in
         constexpr int T = decltype(t)::value, VEC = decltype(v)::value;
         hipLaunchKernelGGL((k_dispatch<T, VEC>), dim3((unsigned)all), dim3(kLanes), 0, s, (const int32_t *)slot + r * k,
                            (const int32_t *)counts, (const int32_t *)offsets, (uint32_t)total, (int)k, (int)align, (uint32_t)blocks,
-                           fast_div((uint32_t)per_row), H, (const elem_t<T> *)x + r * H, (elem_t<T> *)xs);
+                           fast_div((uint32_t)per_row), capacity, H, (const elem_t<T> *)x + r * H, (elem_t<T> *)xs);
       });
     });
   }
@@ -193,9 +199,9 @@ extern "C" int anc_dispatch(uint64_t slot, uint64_t counts, uint64_t offsets, in
   return ANC_OK;
 }
 
-extern "C" int anc_combine(uint64_t slot, uint64_t weights, int64_t tokens, int64_t k, uint64_t ys, int ys_type, uint64_t y, int y_type,
+extern "C" int anc_combine(uint64_t slot, uint64_t weights, int64_t tokens, int64_t k, uint64_t ys, int64_t capacity, int ys_type, uint64_t y, int y_type,
                            int64_t H, uint64_t stream) {
-  if (int rc = check_rows("anc_combine", slot, tokens, k, H)) return rc;
+  if (int rc = check_rows("anc_combine", slot, tokens, k, capacity, H)) return rc;
   ANC_REQUIRE(type_ok(ys_type) && type_ok(y_type), "anc_combine: types %d and %d", ys_type, y_type);
   ANC_REQUIRE(ys && y && ys % (uint64_t)elem_size(ys_type) == 0 && y % (uint64_t)elem_size(y_type) == 0 && (weights & 3) == 0,
               "anc_combine: null or misaligned pointers");
@@ -213,7 +219,7 @@ extern "C" int anc_combine(uint64_t slot, uint64_t weights, int64_t tokens, int6
           auto kernel = weights != 0 ? k_combine<TI, TO, VEC, true> : k_combine<TI, TO, VEC, false>;
           hipLaunchKernelGGL(kernel, dim3((unsigned)((total + kLanes - 1) / kLanes)), dim3(kLanes), 0, s, (const int32_t *)slot + r * k,
                              weights != 0 ? (const float *)weights + r * k : (const float *)nullptr, (uint32_t)total, (int)k,
-                             fast_div((uint32_t)per_row), H, (const elem_t<TI> *)ys, (elem_t<TO> *)y + r * H);
+                             fast_div((uint32_t)per_row), capacity, H, (const elem_t<TI> *)ys, (elem_t<TO> *)y + r * H);
         });
       });
     });
@@ -223,9 +229,9 @@ extern "C" int anc_combine(uint64_t slot, uint64_t weights, int64_t tokens, int6
 }
 
 extern "C" int anc_combine_grad(uint64_t slot, uint64_t weights, uint64_t counts, uint64_t offsets, int64_t tokens, int64_t k,
-                                int64_t experts, int64_t align, uint64_t dy, int dy_type, uint64_t ys, uint64_t dys, int ys_type,
-                                uint64_t dw, int64_t H, uint64_t stream) {
-  if (int rc = check_rows("anc_combine_grad", slot, tokens, k, H)) return rc;
+                                int64_t experts, int64_t align, uint64_t dy, int dy_type, uint64_t ys, uint64_t dys, int64_t capacity,
+                                int ys_type, uint64_t dw, int64_t H, uint64_t stream) {
+  if (int rc = check_rows("anc_combine_grad", slot, tokens, k, capacity, H)) return rc;
   if (int rc = check_segments("anc_combine_grad", counts, offsets, experts, align)) return rc;
   ANC_REQUIRE(type_ok(dy_type) && type_ok(ys_type), "anc_combine_grad: types %d and %d", dy_type, ys_type);
   ANC_REQUIRE(weights && dy && ys && dys && dw && ((weights | dw) & 3) == 0 && dy % (uint64_t)elem_size(dy_type) == 0 &&
@@ -244,7 +250,7 @@ extern "C" int anc_combine_grad(uint64_t slot, uint64_t weights, uint64_t counts
         const bool once = tokens * k * H * elem_size(ys_type) > kCached;
         auto kernel = once ? k_combine_grad<TY, TS, VEC, true> : k_combine_grad<TY, TS, VEC, false>;
         hipLaunchKernelGGL(kernel, dim3((unsigned)all), dim3(kLanes), 0, s, (const int32_t *)slot,
-                           (const float *)weights, (const int32_t *)counts, (const int32_t *)offsets, tokens, (int)k, (int)align, blocks, H,
+                           (const float *)weights, (const int32_t *)counts, (const int32_t *)offsets, tokens, (int)k, (int)align, blocks, capacity, H,
                            (const elem_t<TY> *)dy, (const elem_t<TS> *)ys, (elem_t<TS> *)dys, (float *)dw);
       });
     });

@@ -73,7 +73,8 @@ __global__ void __launch_bounds__(kDwLanes * kSubs) k_embed_dw(EmbedDw p, const 
   const int64_t p0 = (int64_t)blockIdx.x * p.chunk + (int64_t)team * p.sub, here = p0 + lane;
   const bool in = lane < p.sub && here < p.n;
   const int64_t at = in ? here : p.n - 1;
-  const int idx = p.srt[at], key = p.key[at], read = p.grp[at], grp = in ? read : -1;
+  const int row = p.srt[at], key = p.key[at], read = p.grp[at], idx = (uint32_t)row < (uint32_t)p.n ? row : 0;
+  const int grp = in && (uint32_t)read < (uint32_t)p.n && (uint32_t)key < (uint64_t)p.V ? read : -1;      // (whatever the arrays hold, no other row is touched)
   const int came = p0 > 0 && p0 < p.n ? p.grp[p0 - 1] : -1;              // the group before the team's positions
   const int goes = p0 + p.sub < p.n ? p.grp[p0 + p.sub] : -1;            // ... and behind them
   const int m = __popcll(__ballot(grp >= 0));                            // (ids that name no row lie at the end)
@@ -98,7 +99,7 @@ __global__ void __launch_bounds__(kDwLanes * kSubs) k_embed_dw(EmbedDw p, const 
       next[j] = q + 1 < m ? __builtin_amdgcn_readlane(grp, q + 1) : -1;  // (a group that goes on behind ends here, too)
       v[j] = load<TD, VEC, ONCE>(dy + (int64_t)__builtin_amdgcn_readlane(idx, q) * p.H + c0);
       if constexpr (DENSE)
-        if (next[j] != g[j] && g[j] != came && g[j] != goes)
+        if (next[j] != g[j] && g[j] != came && g[j] != goes && g[j] >= 0)
           old[j] = load<ANC_F32, VEC>(p.out + (int64_t)__builtin_amdgcn_readlane(key, q) * p.H + c0);
     }
 #pragma unroll
@@ -109,7 +110,8 @@ __global__ void __launch_bounds__(kDwLanes * kSubs) k_embed_dw(EmbedDw p, const 
 #pragma unroll
       for (int k = 0; k < VEC; ++k) acc[k] = acc[k] + x[k];
       if (next[j] == g[j]) continue;
-      if (g[j] == came) {
+      if (g[j] < 0) {                                // (arrays out of order only)
+      } else if (g[j] == came) {
         state |= g[j] == goes ? 3 : 1;
         *(Raw<ANC_F32, VEC> *)head = narrow<ANC_F32, VEC>(acc);
       } else if (g[j] == goes) {
@@ -159,7 +161,7 @@ __global__ void __launch_bounds__(kDwLanes * kSubs) k_embed_dw(EmbedDw p, const 
 }
 
 // Chunk c's part 1 begins a group that goes on: the parts of it, in order. The four wavefronts take a quarter of the list each
-// (a third of 65536 positions on one id: 338 rows of 64 ... ), 8 rows in flight, and their sums meet in LDS.
+// (a third of 65536 positions on one id: 85 rows), 8 rows in flight, and their sums meet in LDS.
 template <int VEC>
 __global__ void __launch_bounds__(kDwLanes) k_embed_dw_join(EmbedDw p) {
   constexpr int W = kDwLanes / 64;
@@ -167,8 +169,9 @@ __global__ void __launch_bounds__(kDwLanes) k_embed_dw_join(EmbedDw p) {
   const int64_t c = blockIdx.x, last = (c + 1) * p.chunk - 1;
   if (last + 1 >= p.n) return;
   const int g = p.grp[last], behind = p.grp[last + 1], before = c > 0 ? p.grp[last - p.chunk] : -1;
-  if (g < 0 || behind != g || before == g) return;     // (uniform over the workgroup)
-  const int64_t key = p.key[last], ce = ((int64_t)p.start[g] + p.cnt[g] - 1) / p.chunk;
+  if ((uint32_t)g >= (uint32_t)p.n || behind != g || before == g) return;     // (uniform over the workgroup)
+  const int64_t key = p.key[last], end = (int64_t)p.start[g] + p.cnt[g], ce = ((end < p.n ? end : p.n) - 1) / p.chunk;
+  if (ce < c || key < 0 || key >= p.V) return;
   const int lane = (int)(threadIdx.x & 63), wave = (int)(threadIdx.x >> 6);
   const int64_t col = ((int64_t)blockIdx.y * 64 + lane) * VEC;
   const bool live = col < p.H;
@@ -273,7 +276,7 @@ extern "C" int64_t anc_embed_dw_workspace_bytes(int64_t M, int64_t H) {
 extern "C" int anc_embed_dw(uint64_t srt, uint64_t start, uint64_t cnt, uint64_t key, uint64_t grp, int64_t n, uint64_t dy, int dy_type,
                             int64_t H, float scale, uint64_t out, uint64_t compact, int64_t V, uint64_t workspace,
                             int64_t workspace_bytes, uint64_t stream) {
-  ANC_REQUIRE(n >= 0 && n <= kMostPositions && H > 0 && H <= (1ll << 20) && (out == 0 || V > 0), "anc_embed_dw: n=%lld (at most %lld), V=%lld, H=%lld",
+  ANC_REQUIRE(n >= 0 && n <= kMostPositions && H > 0 && H <= (1ll << 20) && V > 0 && V < (1ll << 31), "anc_embed_dw: n=%lld (at most %lld), V=%lld, H=%lld",
               (long long)n, (long long)kMostPositions, (long long)V, (long long)H);
   ANC_REQUIRE(type_ok(dy_type), "anc_embed_dw: type %d", dy_type);
   ANC_REQUIRE((out != 0) != (compact != 0), "anc_embed_dw: one of out and compact");

@@ -30,6 +30,7 @@ struct DwOne {
 };
 struct DwMulti {
   const int32_t *counts, *offsets, *order;
+  int64_t capacity;                                            // slots
   int count, experts, unit;                                    // tiles that follow each other on one XCD
   int unit0[kMostProblems + 1];                                // first unit of each problem among an expert's
   DwOne p[kMostProblems];
@@ -72,14 +73,16 @@ __global__ void __launch_bounds__(TM * 2, 2) k_expert_dw(DwMulti m) {
   const int unit = round * kXcds + ((round & 1) ? kXcds - 1 - xcd : xcd), per = m.unit0[m.count], rank = unit / per, mine = unit - rank * per;
   if (rank >= m.experts) return;
   const int e = m.order[rank];
+  if ((uint32_t)e >= (uint32_t)m.experts) return;
   int pi = 0;
   while (pi + 1 < m.count && mine >= m.unit0[pi + 1]) ++pi;
   const DwOne &p = m.p[pi];
   const int tile = (mine - m.unit0[pi]) * m.unit + q % m.unit;
   if (tile >= p.tiles) return;
   const int m0 = tile / p.tn * TM, n0 = (tile % p.tn) * TN;
-  const int K = p.K, N = p.N, rows = m.counts[e];
-  const int64_t first = m.offsets[e];
+  const int K = p.K, N = p.N, at = m.offsets[e], tokens = m.counts[e];
+  const int64_t first = at < 0 ? 0 : at < m.capacity ? at : m.capacity, room = m.capacity - first;      // (a segment stays inside x and dy, whatever the arrays hold)
+  const int rows = tokens < room ? tokens : (int)room;
   const int lane = (int)(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
 
   Feed fa{(const char *)(p.x + first * K + m0), ((int64_t)rows * K - m0) * 2, (int64_t)TK * K * 2};
@@ -214,11 +217,13 @@ __global__ void __launch_bounds__(TM * 2, 2) k_expert_dw(DwMulti m) {
 }  // namespace
 
 extern "C" int anc_expert_dw_multi(const anc_expert_dw_problem_t *probs, int32_t n_probs, uint64_t counts, uint64_t offsets,
-                                   uint64_t order, int64_t experts, uint64_t stream) {
+                                   uint64_t order, int64_t experts, int64_t capacity, uint64_t stream) {
   ANC_REQUIRE(probs != nullptr && n_probs >= 1 && n_probs <= kMostProblems, "anc_expert_dw_multi: 1..%d problems", kMostProblems);
   ANC_REQUIRE(counts && offsets && order && ((counts | offsets | order) & 3) == 0 && experts > 0 && experts <= 512,
               "anc_expert_dw_multi: bad segments (%lld experts)", (long long)experts);
+  ANC_REQUIRE(capacity > 0 && capacity < (1ll << 31), "anc_expert_dw_multi: room for %lld slots", (long long)capacity);
   DwMulti m{};
+  m.capacity = capacity;
   m.counts = (const int32_t *)counts;
   m.offsets = (const int32_t *)offsets;
   m.order = (const int32_t *)order;

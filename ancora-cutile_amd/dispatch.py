@@ -86,7 +86,8 @@ def dispatch(plan, x, si, xs):
     if x.dtype != xs.dtype:
         raise ValueError(f"dispatch: x is {x.dtype}, xs {xs.dtype}")
     counts, offsets, _, slot = plan._at[:4]
-    api.anc_dispatch(slot, counts, offsets, plan.active, plan.k, plan.E, plan.align, x.ptr, xs.ptr, _type(x, "dispatch"), H, int(si))
+    api.anc_dispatch(slot, counts, offsets, plan.active, plan.k, plan.E, plan.align, x.ptr, xs.ptr, plan.capacity,
+                     _type(x, "dispatch"), H, int(si))
 
 
 def _weights(plan, w, who):
@@ -104,7 +105,8 @@ def combine(plan, ys, weights, si, y):
     _rows_of(ys, plan.capacity, H, "combine", "ys")
     _rows_of(y, plan.active, H, "combine", "y")
     w = 0 if weights is None else _weights(plan, weights, "combine")
-    api.anc_combine(plan._at[3], w, plan.active, plan.k, ys.ptr, _type(ys, "combine"), y.ptr, _type(y, "combine"), H, int(si))
+    api.anc_combine(plan._at[3], w, plan.active, plan.k, ys.ptr, plan.capacity, _type(ys, "combine"), y.ptr,
+                    _type(y, "combine"), H, int(si))
 
 
 def dispatch_grad(plan, dxs, si, dx):
@@ -124,5 +126,5 @@ def combine_grad(plan, dy, ys, weights, si, dys, dweights):
         raise ValueError(f"combine_grad: ys is {ys.dtype}, dys {dys.dtype}")
     counts, offsets, _, slot = plan._at[:4]
     api.anc_combine_grad(slot, _weights(plan, weights, "combine_grad"), counts, offsets, plan.active, plan.k, plan.E, plan.align, dy.ptr,
-                         _type(dy, "combine_grad"), ys.ptr, dys.ptr, _type(ys, "combine_grad"),
+                         _type(dy, "combine_grad"), ys.ptr, dys.ptr, plan.capacity, _type(ys, "combine_grad"),
                          _weights(plan, dweights, "combine_grad"), H, int(si))

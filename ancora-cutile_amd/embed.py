@@ -268,11 +268,13 @@ class DeviceIdGroups:
         api.anc_id_groups_device(ids.ptr, nbytes, n, self.M, self.V, *self._at, int(si))
         self.n = n
 
-    def _part(self, H):
+    def _part(self, H, si):
         nbytes = api.anc_embed_dw_workspace_bytes(self.M, H)
         for b in self._parts:
             if b.nbytes >= nbytes:
                 return b
+        if _lib.stream_is_capturing(si):
+            raise _lib.AncoraError(f"embed_dw: the first gradient of width {H} allocates; make it before the stream is captured")
         self._parts.append(DevBuf.empty((nbytes,), np.uint8))
         return self._parts[-1]
 
@@ -298,7 +300,7 @@ def embed_dw(groups, dy, si, out=None, compact=None, scale=1.0):
     if compact is None and tuple(out.shape) != (groups.V, H):
         raise ValueError(f"embed_dw: out is {out.shape}, ({groups.V}, {H}) expected")
     _rows_of(target, 0 if compact is None else groups.n, H, "embed_dw", "compact")
-    part = groups._part(H)
+    part = groups._part(H, si)
     srt, start, cnt, _, key, grp = groups._at[:6]
     api.anc_embed_dw(srt, start, cnt, key, grp, groups.n, dy.ptr, _type(dy, "embed_dw"), H, float(scale),
                      0 if out is None else out.ptr, 0 if compact is None else compact.ptr, groups.V, part.ptr, part.nbytes, int(si))

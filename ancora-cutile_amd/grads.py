@@ -148,4 +148,4 @@ def expert_dW(plan, problems, si=0):
             g16 = p.get("g16")
             _EDW.pack_into(arr, k * _EDW.size, p["x"].ptr, p["dy"].ptr, p["dW"].ptr, 0 if g16 is None else g16.ptr, K, N,
                            1 if p.get("accumulate", False) else 0, 0)
-        api.anc_expert_dw_multi(arr, len(group), counts, offsets, order, plan.E, int(si))
+        api.anc_expert_dw_multi(arr, len(group), counts, offsets, order, plan.E, plan.capacity, int(si))

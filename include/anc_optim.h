@@ -339,7 +339,8 @@ int anc_id_groups_device(uint64_t ids, int32_t ids_bytes, int64_t n, int64_t M, 
 
 /* anc_embed_dw: the table's gradient over those groups, dy (n, H).
  *   out != 0:     out[id] += scale * sum of the id's rows, out (V, H) fp32; rows that no id names are not touched
- *   compact != 0: compact[g] = scale * that sum, (n, H) fp32; rows behind the last group are left as they were
+ *   compact != 0: compact[g] = scale * that sum, (n, H) fp32; rows behind the last group are left as they were (V as when the ids were
+ *                 grouped)
  * Rows are added in fp32 in sorted order within runs of 8, 16 or 64 positions (by n), the runs in a fixed order: the same
  * bits on every run, a function of n, the ids and dy. One id may hold most of the batch at no loss of speed (a group of
  * anc_embed_dw_scatter, whose bits are the sequential sum's, is one workgroup's). */
@@ -362,8 +363,8 @@ int anc_route(uint64_t expert_ids, int32_t ids_bytes, int64_t n, int64_t experts
               uint64_t offsets, uint64_t order, uint64_t slot, uint64_t src, int64_t capacity, uint64_t workspace, int64_t workspace_bytes,
               uint64_t stream);
 
-/* Rows there and back over the slots of anc_route (slot int32[tokens * k]); types ANC_F32 or ANC_BF16, sums in fp32 with
- * one rounding at the end, choices in ascending order.
+/* Rows there and back over the slots of anc_route (slot int32[tokens * k]; xs, ys, dys hold `capacity` rows, a slot beyond them is
+ * taken for none); types ANC_F32 or ANC_BF16, sums in fp32 with one rounding at the end, choices in ascending order, k <= 512.
  *   anc_dispatch:      xs[slot[t, j]] = x[t]; the rows that fill up a segment become zero, rows behind the last segment and
  *                      without a slot are left as they were
  *   anc_combine:       y[t] = sum over j of weights[t, j] * ys[slot[t, j]] (weights fp32; 0: all one, which is the gradient
@@ -371,12 +372,12 @@ int anc_route(uint64_t expert_ids, int32_t ids_bytes, int64_t n, int64_t experts
  *   anc_combine_grad:  dys[slot[t, j]] = weights[t, j] * dy[t], filling rows zero as in anc_dispatch;
  *                      dw[t, j] = <dy[t], ys[slot[t, j]]> fp32, 0 for a choice without a slot */
 int anc_dispatch(uint64_t slot, uint64_t counts, uint64_t offsets, int64_t tokens, int64_t k, int64_t experts, int64_t align,
-                 uint64_t x, uint64_t xs, int type, int64_t H, uint64_t stream);
-int anc_combine(uint64_t slot, uint64_t weights, int64_t tokens, int64_t k, uint64_t ys, int ys_type, uint64_t y, int y_type,
-                int64_t H, uint64_t stream);
+                 uint64_t x, uint64_t xs, int64_t capacity, int type, int64_t H, uint64_t stream);
+int anc_combine(uint64_t slot, uint64_t weights, int64_t tokens, int64_t k, uint64_t ys, int64_t capacity, int ys_type, uint64_t y,
+                int y_type, int64_t H, uint64_t stream);
 int anc_combine_grad(uint64_t slot, uint64_t weights, uint64_t counts, uint64_t offsets, int64_t tokens, int64_t k,
-                     int64_t experts, int64_t align, uint64_t dy, int dy_type, uint64_t ys, uint64_t dys, int ys_type,
-                     uint64_t dw, int64_t H, uint64_t stream);
+                     int64_t experts, int64_t align, uint64_t dy, int dy_type, uint64_t ys, uint64_t dys, int64_t capacity,
+                     int ys_type, uint64_t dw, int64_t H, uint64_t stream);
 
 /* p16 = bf16(p32): replaces `_cast_bf16` (ancora/kernels/fused.py:285-290). */
 int anc_cast_bf16(uint64_t p32, uint64_t p16, int64_t n, int sr, uint32_t seed,
@@ -500,7 +501,7 @@ typedef struct {
   int32_t  accumulate, reserved;
 } anc_expert_dw_problem_t;
 int anc_expert_dw_multi(const anc_expert_dw_problem_t *problems, int32_t n_problems, uint64_t counts, uint64_t offsets,
-                        uint64_t order, int64_t experts, uint64_t stream);
+                        uint64_t order, int64_t experts, int64_t capacity, uint64_t stream);
 
 /* MXFP8 re-quantisation of bf16 weights (E, K, N) after the step: per block of 32 consecutive K
  * and per column one E8M0 scale byte = (biased fp32 exponent of the block's amax) - 7 (0 below

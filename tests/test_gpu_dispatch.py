@@ -195,6 +195,35 @@ def test_rows_beyond_32_bit_offsets(gpu):
         b.free()
 
 
+def test_slots_and_segments_that_hold_anything_touch_no_other_row(gpu):
+    from ancora_cutile_amd import DevBuf, RoutePlan, combine, combine_grad, expert_dW
+    from ancora_cutile_amd.dispatch import dispatch
+    T, k, E, H, align, guard = 500, 3, 7, 40, 8, 64
+    rng = np.random.default_rng(1)
+    plan = RoutePlan(T, k, E, align)
+    S = plan.capacity
+    ge = DevBuf(np.zeros((T, k), np.int32))
+    plan.route(ge, 0)
+    outer = {n: DevBuf(np.full((S + 2 * guard, H), 0x4040, np.uint16)) for n in ("xs", "dys")}
+    inner = {n: DevBuf(shape=(S, H), dtype=np.uint16, ptr=b.ptr + guard * H * 2) for n, b in outer.items()}
+    x, y, w = DevBuf.zeros((T, H), np.uint16), DevBuf.zeros((T, H), np.float32), DevBuf(np.ones((T, k), np.float32))
+    dw, dW = DevBuf.zeros((T, k), np.float32), DevBuf.zeros((E, H, H), np.float32)
+    for _ in range(3):
+        for a in (plan.slot, plan.counts, plan.offsets, plan.order):
+            r = rng.integers(-2 ** 31, 2 ** 31 - 1, a.shape) >> rng.integers(0, 31, a.shape)
+            a.upload(r.astype(np.int32))
+        dispatch(plan, x, 0, inner["xs"])
+        combine(plan, inner["xs"], w, 0, y)
+        combine_grad(plan, y, inner["xs"], w, 0, inner["dys"], dw)
+        expert_dW(plan, [dict(x=inner["xs"], dy=inner["dys"], dW=dW)], 0)
+    gpu.stream_sync(0)
+    for b in outer.values():
+        host = b.to_numpy()
+        assert np.all(host[:guard] == 0x4040) and np.all(host[guard + S:] == 0x4040)
+    for b in (plan, ge, x, y, w, dw, dW, *outer.values()):
+        b.free()
+
+
 @pytest.mark.parametrize("T", [50, 6000])
 def test_captured_and_replayed_on_new_routes(gpu, T):
     from ancora_cutile_amd import DevBuf, RoutePlan, combine, combine_grad, dispatch_grad

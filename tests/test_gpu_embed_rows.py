@@ -115,7 +115,7 @@ def test_lookup_and_gradient_of_rows_beyond_32_bit_offsets(gpu):
 
 
 BATCHES = [(1, 1), (2, 700), (63, 4), (64, 1), (65, 511), (1000, (1 << 31) - 1), (1024, 512), (1025, 100000), (4097, 20), (8192, 151936),
-           (9000, 262144), (9000, 262145), (3000, 1 << 30), (65536, 50257), (65537, 151936),
+           (9000, 1), (9000, 2), (9000, 262144), (9000, 262145), (1 << 20, 1000000), (3000, 1 << 30), (65536, 50257), (65537, 151936),
            (16384, 3000), (16385, 151936), (40001, 600), (70001, 1 << 20), (140000, 40)]
 
 
@@ -311,6 +311,33 @@ def test_captured_and_replayed_on_new_ids(gpu, M):
     for b in (table, dy, ids, mine, other, *x, *rows):
         b.free()
     gpu.api.anc_stream_destroy(s)
+
+
+def test_arrays_that_hold_anything_touch_no_other_row(gpu):
+    """Sorted indices, groups and ids outside the batch and the table (a batch that was never grouped, say): no row outside the
+    buffers is read or written."""
+    from ancora_cutile_amd import DevBuf, DeviceIdGroups, embed_dw
+    M, V, H = 3000, 50, 72
+    rng = np.random.default_rng(1)
+    groups = DeviceIdGroups(M, V)
+    ids, dy = DevBuf(np.zeros(M, np.int32)), DevBuf(np.ones((M, H), np.float32))
+    guard = 64
+    big = DevBuf(np.full((V + 2 * guard, H), 3.0, np.float32))
+    out = DevBuf(shape=(V, H), dtype=np.float32, ptr=big.ptr + guard * H * 4)
+    rows = DevBuf(np.full((M + 2 * guard, H), 3.0, np.float32))
+    compact = DevBuf(shape=(M, H), dtype=np.float32, ptr=rows.ptr + guard * H * 4)
+    groups.group(ids, 0)
+    for _ in range(3):
+        for a in (groups.srt, groups.start, groups.cnt, groups._key, groups._grp):
+            a.upload(rng.integers(-2 ** 31, 2 ** 31 - 1, (M, 1)).astype(np.int32) >> rng.integers(0, 31, (M, 1)).astype(np.int32))
+        embed_dw(groups, dy, 0, out=out)
+        embed_dw(groups, dy, 0, compact=compact)
+    gpu.stream_sync(0)
+    for b, n in ((big, V), (rows, M)):
+        host = b.to_numpy()
+        assert np.all(host[:guard] == 3.0) and np.all(host[guard + n:] == 3.0)
+    for b in (groups, ids, dy, big, rows):
+        b.free()
 
 
 def test_two_batches_at_once_on_two_streams(gpu):

@@ -119,6 +119,19 @@ def test_more_weights_than_one_call_takes_and_non_finite_rows(gpu):
         b.free()
 
 
+def test_no_tokens_at_all(gpu):
+    from ancora_cutile_amd import DevBuf, RoutePlan, expert_dW
+    plan, ids = RoutePlan(20, 2, 3, 16), DevBuf(np.zeros((20, 2), np.int32))
+    plan.route(ids, 0, 0)
+    x, dy = DevBuf(np.full((plan.capacity, 16), 0x7FFF, np.uint16)), DevBuf(np.full((plan.capacity, 24), 0x7FFF, np.uint16))
+    base = np.arange(3 * 16 * 24, dtype=np.float32).reshape(3, 16, 24)
+    W, A, g16 = DevBuf(base), DevBuf(base), DevBuf.zeros((3, 16, 24), np.uint16)
+    expert_dW(plan, [dict(x=x, dy=dy, dW=W), dict(x=x, dy=dy, dW=A, g16=g16, accumulate=True)], 0)
+    assert not W.to_numpy().any() and bits_equal(A.to_numpy(), base) and bits_equal(g16.to_numpy(), bf16_rne_bits(base).reshape(base.shape))
+    for b in (plan, ids, x, dy, W, A, g16):
+        b.free()
+
+
 def test_captured_and_replayed_on_new_segments(gpu):
     from ancora_cutile_amd import DevBuf, RoutePlan, expert_dW
     hip = ctypes.CDLL("libamdhip64.so")

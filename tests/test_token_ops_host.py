@@ -51,7 +51,7 @@ def test_gradient_refusals(lib):
         assert lib.anc_embed_dw_workspace_bytes(M, H) == -1
     ok = (P, P, P, P, P, 1000, P, 1, 64, 1.0, P, 0, 500, P, ws, 0)
     for at, value, word in ((5, -1, "n="), (5, (1 << 20) + 1, "n="), (6, 0, "null"), (6, P + 1, "misaligned"), (7, 7, "type"), (8, 0, "H="),
-                            (10, 0, "one of"), (10, P + 2, "misaligned"), (11, P, "one of"), (12, 0, "V="), (13, 0, "null"), (13, P + 8, "misaligned"),
+                            (10, 0, "one of"), (10, P + 2, "misaligned"), (11, P, "one of"), (12, 0, "V="), (12, 1 << 31, "V="), (13, 0, "null"), (13, P + 8, "misaligned"),
                             (14, ws - 1, "workspace holds")) + tuple((i, 0, "null") for i in range(5)):
         _refused(lib, "anc_embed_dw", _but(ok, at, value), word)
 
@@ -70,18 +70,18 @@ def test_route_refusals(lib):
 
 
 def test_row_mover_refusals(lib):
-    ok = (P, P, P, 10, 2, 4, 16, P, P, 1, 64, 0)
+    ok = (P, P, P, 10, 2, 4, 16, P, P, 200, 1, 64, 0)
     for at, value, word in ((0, 0, "slots"), (0, P + 2, "slots"), (1, 0, "segments"), (2, P + 1, "segments"), (3, -1, "tokens"), (4, 0, "choices"),
                             (4, 513, "choices"), (5, 0, "segments"), (5, 513, "segments"), (6, 0, "segments"), (7, 0, "null"), (8, 0, "null"),
-                            (8, P + 1, "misaligned"), (9, 5, "type"), (10, 0, "width")):
+                            (8, P + 1, "misaligned"), (9, 0, "room"), (9, 1 << 31, "room"), (10, 5, "type"), (11, 0, "width")):
         _refused(lib, "anc_dispatch", _but(ok, at, value), word)
-    ok = (P, P, 10, 2, P, 1, P, 0, 64, 0)
-    for at, value, word in ((0, 0, "slots"), (1, P + 2, "misaligned"), (2, -1, "tokens"), (3, 0, "choices"), (4, 0, "null"), (5, 9, "types"), (6, 0, "null"),
-                            (6, P + 2, "misaligned"), (7, 9, "types"), (8, 0, "width")):
+    ok = (P, P, 10, 2, P, 200, 1, P, 0, 64, 0)
+    for at, value, word in ((0, 0, "slots"), (1, P + 2, "misaligned"), (2, -1, "tokens"), (3, 0, "choices"), (4, 0, "null"), (5, 0, "room"), (6, 9, "types"), (7, 0, "null"),
+                            (7, P + 2, "misaligned"), (8, 9, "types"), (9, 0, "width")):
         _refused(lib, "anc_combine", _but(ok, at, value), word)
-    ok = (P, P, P, P, 10, 2, 4, 16, P, 0, P, P, 1, P, 64, 0)
+    ok = (P, P, P, P, 10, 2, 4, 16, P, 0, P, P, 200, 1, P, 64, 0)
     for at, value, word in ((0, 0, "slots"), (1, 0, "null"), (2, 0, "segments"), (3, 0, "segments"), (4, -1, "tokens"), (8, 0, "null"), (8, P + 2, "misaligned"),
-                            (9, 3, "types"), (10, 0, "null"), (11, P + 1, "misaligned"), (12, 3, "types"), (13, 0, "null"), (13, P + 2, "misaligned")):
+                            (9, 3, "types"), (10, 0, "null"), (11, P + 1, "misaligned"), (12, 0, "room"), (13, 3, "types"), (14, 0, "null"), (14, P + 2, "misaligned")):
         _refused(lib, "anc_combine_grad", _but(ok, at, value), word)
 
 
@@ -132,6 +132,13 @@ def test_embedding_calls_that_do_not_fit_launch_nothing(fake_device):
     assert fake_device.calls("anc_embed_dw")[-1][13] != first and first in fake_device.blocks
     embed_dw(g, dy, 0, out=dE)
     assert fake_device.calls("anc_embed_dw")[-1][13] == first
+    # a width that would allocate inside a capture is refused before anything is launched
+    fake_device.capturing.add(7)
+    before = len(fake_device.calls("anc_embed_dw"))
+    with pytest.raises(AncoraError, match="before the stream is captured"):
+        embed_dw(g, _buf((M, 9 * H), np.uint16), 7, compact=_buf((M, 9 * H), np.float32))
+    assert len(fake_device.calls("anc_embed_dw")) == before
+    embed_dw(g, dy, 7, out=dE)
     g.free()
     g.free()
     assert first not in fake_device.blocks
@@ -188,16 +195,16 @@ def test_expert_gradient_refusals(lib):
     from ancora_cutile_amd._lib import ExpertDwProblem
     fields = dict(x=P, dy=P, dW=P, g16=0, K=64, N=128, accumulate=0, reserved=0)
 
-    def call(n=1, counts=P, offsets=P, order=P, experts=4, **kw):
+    def call(n=1, counts=P, offsets=P, order=P, experts=4, capacity=100, **kw):
         arr = (ExpertDwProblem * 9)(*[ExpertDwProblem(**{**fields, **kw}) for _ in range(9)])
-        return lib.anc_expert_dw_multi(arr, n, counts, offsets, order, experts, 0)
+        return lib.anc_expert_dw_multi(arr, n, counts, offsets, order, experts, capacity, 0)
 
     for kw, word in ((dict(n=0), "problems"), (dict(n=9), "problems"), (dict(counts=0), "segments"), (dict(offsets=P + 2), "segments"), (dict(order=0), "segments"),
-                     (dict(experts=0), "segments"), (dict(experts=513), "segments"), (dict(K=12), "K % 8"), (dict(N=0), "K % 8"),
+                     (dict(experts=0), "segments"), (dict(capacity=0), "room"), (dict(experts=513), "segments"), (dict(K=12), "K % 8"), (dict(N=0), "K % 8"),
                      (dict(N=(1 << 17) + 8), "K % 8"), (dict(x=0), "null"), (dict(dy=P + 8), "misaligned"), (dict(dW=P + 4), "misaligned"),
                      (dict(g16=P + 4), "misaligned")):
         assert call(**kw) == 2 and word in lib.anc_last_error().decode(), (kw, lib.anc_last_error())
-    assert lib.anc_expert_dw_multi(ctypes.POINTER(ExpertDwProblem)(), 1, P, P, P, 4, 0) == 2
+    assert lib.anc_expert_dw_multi(ctypes.POINTER(ExpertDwProblem)(), 1, P, P, P, 4, 100, 0) == 2
 
 
 def test_expert_gradient_calls_that_do_not_fit_launch_nothing(fake_device):
