@@ -18,7 +18,6 @@ namespace {
 typedef int anc_i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
-constexpr int kRouteItems = 4, kSmallRoute = 1024 * kRouteItems;       // assignments that one workgroup takes
 constexpr int kBlockLanes = 256, kBlockItems = 8, kBlock = kBlockLanes * kBlockItems;
 
 // Lanes of the wavefront that hold the same digit as this one, among those with `in`. (Six vector instructions a bit: the digit's bit
@@ -633,59 +632,84 @@ __device__ __forceinline__ void order_experts(const int *scnt, int E, int32_t *o
 }
 __device__ __forceinline__ int filled_up(int c, int align) { return (c + align - 1) & -align; }
 
-template <int ITEMS>
-__global__ void __launch_bounds__(1024)
-k_route_small(const void *__restrict__ ids, int wide, int n, int E, int bits, int align, int capacity, Route o) {
-  constexpr int W = 16;
+// Up to kMostCounted assignments in one launch: every workgroup counts all of them per expert, and those before its own kBlock, as the two
+// halves of a word; four copies of the counters keep the lanes that meet on one apart.
+// (16384 to 16 experts 7.5 us, counted and placed in two launches 9.9; 32768 9.6 and 10.0, to 128 experts 11.6 and 13.4)
+constexpr int kMostCounted = 1 << 15, kOneLanes = 1024, kOneItems = kBlock / kOneLanes, kCopies = 4;
+__global__ void __launch_bounds__(kOneLanes)
+k_route_one(const void *__restrict__ ids, int wide, int n, int E, int bits, int align, int capacity, Route o) {
+  constexpr int W = kOneLanes / 64;
   __shared__ int count[W * kMostExperts];
+  __shared__ uint32_t hist[kCopies * kMostExperts];
   __shared__ int tmp[W];
   __shared__ int soff[kMostExperts + 1], scnt[kMostExperts];
-  const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63, first = wave * (64 * ITEMS) + lane;
-  uint32_t e[ITEMS];                                 // E: no expert
-  int rank[ITEMS];
+  const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63, blocks = (int)gridDim.x, b = (int)blockIdx.x;
+  const int first = b * kBlock + wave * (64 * kOneItems) + lane;
+  uint32_t e[kOneItems];                             // E: no expert
+  int rank[kOneItems];
   if (n > 0) {
-    load_keys<ITEMS>(ids, wide, first, 64, n, (uint32_t)E, e);
+    load_keys<kOneItems>(ids, wide, first, 64, n, (uint32_t)E, e);
   } else {
 #pragma unroll
-    for (int j = 0; j < ITEMS; ++j) e[j] = (uint32_t)E;
+    for (int j = 0; j < kOneItems; ++j) e[j] = (uint32_t)E;
   }
-  for (int i = tid; i < W * E; i += 1024) count[i] = 0;
+  for (int i = tid; i < W * E; i += kOneLanes) count[i] = 0;
+  for (int i = tid; i < kCopies * E; i += kOneLanes) hist[i] = 0;
   __syncthreads();
+  constexpr int D = 8;
+  for (int t = tid; blocks > 1 && t < n; t += D * kOneLanes) {
+    uint32_t k[D];
+    load_keys<D>(ids, wide, t, kOneLanes, n, (uint32_t)E, k);
 #pragma unroll
-  for (int j = 0; j < ITEMS; ++j) rank[j] = take_rank(count + wave * E, e[j], bits, e[j] < (uint32_t)E);
+    for (int j = 0; j < D; ++j)
+      if (k[j] < (uint32_t)E) atomicAdd(&hist[k[j] * kCopies + (lane & (kCopies - 1))], t + j * kOneLanes < b * kBlock ? 0x10001u : 1u);
+  }
+#pragma unroll
+  for (int j = 0; j < kOneItems; ++j) rank[j] = take_rank(count + wave * E, e[j], bits, e[j] < (uint32_t)E);
   __syncthreads();
-  int c[W], sum = 0, total;
+  int all = 0, below = 0, c[W], total;
 #pragma unroll
   for (int w = 0; w < W; ++w) c[w] = tid < E ? count[w * E + tid] : 0;
+  if (blocks == 1) {
 #pragma unroll
-  for (int w = 0; w < W; ++w) sum += c[w];
-  const int base = block_scan<1024>(filled_up(sum, align), tmp, total);
+    for (int w = 0; w < W; ++w) all += c[w];
+  } else if (tid < E) {
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) {
+      const uint32_t h = hist[tid * kCopies + i];
+      all += (int)(h & 0xFFFF);
+      below += (int)(h >> 16);
+    }
+  }
+  const int base = block_scan<kOneLanes>(filled_up(all, align), tmp, total);
   if (tid < E) {
-    int at = base;
+    int at = base + below;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       count[w * E + tid] = at;
       at += c[w];
     }
     soff[tid] = base;
-    scnt[tid] = sum;
-    o.counts[tid] = sum;
-    o.offsets[tid] = base;
+    scnt[tid] = all;
+    if (b == 0) { o.counts[tid] = all; o.offsets[tid] = base; }
   }
-  if (tid == 0) { soff[E] = total; o.offsets[E] = total; }
+  if (tid == 0) {
+    soff[E] = total;
+    if (b == 0) o.offsets[E] = total;
+  }
   __syncthreads();
-  order_experts<1024>(scnt, E, o.order);
 #pragma unroll
-  for (int j = 0; j < ITEMS; ++j) {
+  for (int j = 0; j < kOneItems; ++j) {
     const int p = first + 64 * j;
     if (p >= n) continue;
     const int s = e[j] < (uint32_t)E ? count[wave * E + e[j]] + rank[j] : -1;
     o.slot[p] = s;
     if (s >= 0) o.src[s] = p;
   }
-  for (int q = wave; q < E; q += W)
+  if (b == blocks - 1) order_experts<kOneLanes>(scnt, E, o.order);
+  for (int q = b * W + wave; q < E; q += blocks * W)
     for (int s = soff[q] + scnt[q] + lane; s < soff[q + 1]; s += 64) o.src[s] = -1;
-  for (int s = total + tid; s < capacity; s += 1024) o.src[s] = -1;
+  for (int64_t s = total + (int64_t)b * kOneLanes + tid; s < capacity; s += (int64_t)blocks * kOneLanes) o.src[s] = -1;
 }
 
 __global__ void __launch_bounds__(kBlockLanes)
@@ -883,7 +907,7 @@ extern "C" int64_t anc_route_capacity(int64_t assignments, int64_t experts, int6
 extern "C" int64_t anc_route_workspace_bytes(int64_t assignments, int64_t experts) {
   int64_t c;
   if (check_route("anc_route_workspace_bytes", assignments, experts, 1, c)) return -1;
-  return assignments <= kSmallRoute ? 4 : 4 * n_blocks(assignments) * experts;
+  return assignments <= kMostCounted ? 4 : 4 * n_blocks(assignments) * experts;
 }
 
 extern "C" int anc_route(uint64_t expert_ids, int32_t ids_bytes, int64_t n, int64_t experts, int64_t align, uint64_t counts,
@@ -903,9 +927,9 @@ extern "C" int anc_route(uint64_t expert_ids, int32_t ids_bytes, int64_t n, int6
   AncProfScope prof(ANC_PROF_MISC, s);
   const Route o{(int32_t *)counts, (int32_t *)offsets, (int32_t *)order, (int32_t *)slot, (int32_t *)src};
   const int E = (int)experts, bits = bits_of((uint32_t)E - 1), wide = ids_bytes == 8;
-  if (n <= kSmallRoute) {
-    auto kernel = n <= 1024 ? k_route_small<1> : k_route_small<kRouteItems>;
-    hipLaunchKernelGGL(kernel, dim3(1), dim3(1024), 0, s, (const void *)expert_ids, wide, (int)n, E, bits, (int)align, (int)capacity, o);
+  if (n <= kMostCounted) {
+    hipLaunchKernelGGL(k_route_one, dim3((unsigned)(n > 0 ? n_blocks(n) : 1)), dim3(kOneLanes), 0, s, (const void *)expert_ids, wide, (int)n, E,
+                       bits, (int)align, (int)capacity, o);
   } else {
     const dim3 grid((unsigned)n_blocks(n)), lanes(kBlockLanes);
     hipLaunchKernelGGL(k_route_count, grid, lanes, 0, s, (const void *)expert_ids, wide, n, E, (int *)workspace);

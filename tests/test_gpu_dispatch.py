@@ -50,7 +50,7 @@ def _experts(rng, T, k, E, how):
     return e
 
 
-ROUTES = [(1, 1, 1, 1), (1, 8, 128, 16), (3, 2, 5, 128), (700, 3, 7, 1), (1000, 4, 512, 4), (2048, 8, 64, 256), (5000, 8, 31, 16),
+ROUTES = [(1, 1, 1, 1), (32768, 1, 16, 16), (16385, 2, 3, 1), (4096, 8, 512, 2), (2049, 1, 1, 256), (1, 8, 128, 16), (3, 2, 5, 128), (700, 3, 7, 1), (1000, 4, 512, 4), (2048, 8, 64, 256), (5000, 8, 31, 16),
           (33, 512, 300, 2), (500, 3, 256, 8), (9000, 2, 256, 1), (9000, 3, 257, 1), (60000, 2, 512, 1), (9001, 8, 160, 128)]
 
 
