@@ -17,7 +17,7 @@ constexpr int kPadRows = 8;                 // rows that one workgroup clears
 __device__ __forceinline__ int64_t in_range(int64_t slot, int64_t capacity) { return slot < capacity ? slot : -1; }
 
 // Rows between an expert's last token and the end of its segment: workgroup `b` of those that clear them.
-template <int T, int VEC>
+template <int T, int VEC, bool TAIL>
 __device__ __forceinline__ void clear_padding(int b, int align, const int32_t *counts, const int32_t *offsets, int64_t capacity, int64_t H,
                                               elem_t<T> *out) {
   const int per = (align - 1 + kPadRows - 1) / kPadRows, e = b / per;
@@ -28,23 +28,25 @@ __device__ __forceinline__ void clear_padding(int b, int align, const int32_t *c
   float zero[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) zero[k] = 0.0f;
-  for (int64_t i = threadIdx.x; i < (to - from) * (H / VEC); i += kLanes) store<T, VEC>(out + from * H + i * VEC, zero);
+  const Raw<T, VEC> r = narrow<T, VEC>(zero);        // (the rows lie behind each other: one long row)
+  for (int64_t i = threadIdx.x * VEC; i < (to - from) * H; i += kLanes * VEC) store<T, VEC, TAIL>(out + from * H, r, piece_at<VEC, TAIL>(i, (to - from) * H));
 }
 
-template <int T, int VEC>
+template <int T, bool TAIL>
 __global__ void __launch_bounds__(kLanes)
 k_dispatch(const int32_t *__restrict__ slot, const int32_t *__restrict__ counts, const int32_t *__restrict__ offsets, uint32_t total,
            int k, int align, uint32_t main_blocks, FastDiv pieces, int64_t capacity, int64_t H, const elem_t<T> *__restrict__ x,
            elem_t<T> *__restrict__ xs) {
+  constexpr int VEC = piece_of<T, T>;
   if (blockIdx.x >= main_blocks) {
-    clear_padding<T, VEC>((int)(blockIdx.x - main_blocks), align, counts, offsets, capacity, H, xs);
+    clear_padding<T, VEC, TAIL>((int)(blockIdx.x - main_blocks), align, counts, offsets, capacity, H, xs);
     return;
   }
   const uint32_t i = blockIdx.x * (uint32_t)kLanes + threadIdx.x;
   if (i >= total) return;
   const uint32_t t = pieces.div(i);
-  const int64_t col = (int64_t)(i - t * pieces.d) * VEC;
-  const Raw<T, VEC> v = load<T, VEC>(x + (int64_t)t * H + col);
+  const Piece c = piece_at<VEC, TAIL>((int64_t)(i - t * pieces.d) * VEC, H);
+  const Raw<T, VEC> v = load<T, VEC, TAIL>(x + (int64_t)t * H, c);
   const int32_t *to = slot + (int64_t)t * k;
   constexpr int D = 4;
   for (int j0 = 0; j0 < k; j0 += D) {
@@ -53,18 +55,20 @@ k_dispatch(const int32_t *__restrict__ slot, const int32_t *__restrict__ counts,
     for (int j = 0; j < D; ++j) s[j] = in_range(to[j0 + j < k ? j0 + j : k - 1], capacity);
 #pragma unroll
     for (int j = 0; j < D; ++j)
-      if (j0 + j < k && s[j] >= 0) store<T, VEC>(xs + s[j] * H + col, v);
+      if (j0 + j < k && s[j] >= 0) store<T, VEC, TAIL>(xs + s[j] * H, v, c);
   }
 }
 
-template <int TI, int TO, int VEC, bool WEIGHTS>
+template <int TI, int TO, bool TAIL, bool WEIGHTS>
 __global__ void __launch_bounds__(kLanes)
 k_combine(const int32_t *__restrict__ slot, const float *__restrict__ w, uint32_t total, int k, FastDiv pieces, int64_t capacity, int64_t H,
           const elem_t<TI> *__restrict__ ys, elem_t<TO> *__restrict__ y) {
+  constexpr int VEC = piece_of<TI, TO>;
   const uint32_t i = blockIdx.x * (uint32_t)kLanes + threadIdx.x;
   if (i >= total) return;
   const uint32_t row = pieces.div(i);
-  const int64_t t = row, col = (int64_t)(i - row * pieces.d) * VEC;
+  const int64_t t = row;
+  const Piece c = piece_at<VEC, TAIL>((int64_t)(i - row * pieces.d) * VEC, H);
   float acc[VEC];
 #pragma unroll
   for (int q = 0; q < VEC; ++q) acc[q] = 0.0f;
@@ -82,7 +86,7 @@ k_combine(const int32_t *__restrict__ slot, const float *__restrict__ w, uint32_
     }
 #pragma unroll
     for (int j = 0; j < D; ++j)
-      if (s[j] >= 0) v[j] = load<TI, VEC>(ys + s[j] * H + col);
+      if (s[j] >= 0) v[j] = load<TI, VEC, TAIL>(ys + s[j] * H, c);
 #pragma unroll
     for (int j = 0; j < D; ++j) {
       if (s[j] < 0) continue;
@@ -92,20 +96,21 @@ k_combine(const int32_t *__restrict__ slot, const float *__restrict__ w, uint32_
       for (int q = 0; q < VEC; ++q) acc[q] = WEIGHTS ? fmaf(f[j], a[q], acc[q]) : acc[q] + a[q];
     }
   }
-  store<TO, VEC>(y + t * H + col, acc);
+  store<TO, VEC, TAIL>(y + t * H, narrow<TO, VEC>(acc), c);
 }
 
 // One wavefront per token, four choices at a time: their rows are in flight together, dy comes from the caches for the next
 // four. The four products' sums over the lanes are made together: at the first two steps of the butterfly a lane hands half of its sums
 // on and keeps the other half, so that four sums take 7 exchanges instead of 24.
-template <int TY, int TS, int VEC, bool ONCE>
+template <int TY, int TS, bool TAIL, bool ONCE>
 __global__ void __launch_bounds__(kLanes)
 k_combine_grad(const int32_t *__restrict__ slot, const float *__restrict__ w, const int32_t *__restrict__ counts,
                const int32_t *__restrict__ offsets, int64_t tokens, int k, int align, int64_t main_blocks, int64_t capacity, int64_t H,
                const elem_t<TY> *__restrict__ dy, const elem_t<TS> *__restrict__ ys, elem_t<TS> *__restrict__ dys,
                float *__restrict__ dw) {
+  constexpr int VEC = piece_of<TY, TS>;
   if ((int64_t)blockIdx.x >= main_blocks) {
-    clear_padding<TS, VEC>((int)((int64_t)blockIdx.x - main_blocks), align, counts, offsets, capacity, H, dys);
+    clear_padding<TS, VEC, TAIL>((int)((int64_t)blockIdx.x - main_blocks), align, counts, offsets, capacity, H, dys);
     return;
   }
   const int lane = (int)(threadIdx.x & 63);
@@ -126,10 +131,11 @@ k_combine_grad(const int32_t *__restrict__ slot, const float *__restrict__ w, co
     for (int64_t col = (int64_t)lane * VEC; col < H; col += 64 * VEC) {
       float g[VEC];
       Raw<TS, VEC> v[D];
-      const Raw<TY, VEC> own = load<TY, VEC>(dy + t * H + col);
+      const Piece c = piece_at<VEC, TAIL>(col, H);
+      const Raw<TY, VEC> own = load<TY, VEC, TAIL>(dy + t * H, c);
 #pragma unroll
       for (int j = 0; j < D; ++j)
-        if (s[j] >= 0) v[j] = load<TS, VEC, ONCE>(ys + s[j] * H + col);
+        if (s[j] >= 0) v[j] = load<TS, VEC, TAIL, ONCE>(ys + s[j] * H, c);
       widen<TY, VEC>(own, g);
 #pragma unroll
       for (int j = 0; j < D; ++j) {
@@ -138,10 +144,10 @@ k_combine_grad(const int32_t *__restrict__ slot, const float *__restrict__ w, co
         widen<TS, VEC>(v[j], a);
 #pragma unroll
         for (int q = 0; q < VEC; ++q) {
-          dot[j] = fmaf(g[q], a[q], dot[j]);
+          if (!TAIL || q >= c.first) dot[j] = fmaf(g[q], a[q], dot[j]);
           o[q] = f[j] * g[q];
         }
-        store<TS, VEC, ONCE>(dys + s[j] * H + col, o);
+        store<TS, VEC, TAIL, ONCE>(dys + s[j] * H, narrow<TS, VEC>(o), c);
       }
     }
     // lane bit 5 chooses the pair (0, 1) or (2, 3), bit 4 the one of the pair
@@ -178,18 +184,16 @@ extern "C" int anc_dispatch(uint64_t slot, uint64_t counts, uint64_t offsets, in
   if (int rc = check_segments("anc_dispatch", counts, offsets, experts, align)) return rc;
   ANC_REQUIRE(type_ok(type), "anc_dispatch: type %d", type);
   ANC_REQUIRE(x && xs && (x | xs) % (uint64_t)elem_size(type) == 0, "anc_dispatch: null or misaligned pointers");
-  const Ptr ps[2] = {{x, type}, {xs, type}};
-  const int vec = piece(H, ps);
-  const int64_t per_row = H / vec, most = kMostPieces / per_row;
+  const int64_t vec = type == ANC_F32 ? 4 : 8, per_row = pieces_of(H, vec), most = kMostPieces / per_row;
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_MISC, s);
   for (int64_t r = 0; r < tokens; r += most) {       // (the first launch clears the padding)
     const int64_t rows = tokens - r < most ? tokens - r : most, total = rows * per_row;
     const int64_t blocks = (total + kLanes - 1) / kLanes, all = blocks + (r == 0 ? pad_blocks(experts, align) : 0);
     with_type(type, [&](auto t) {
-      with_piece(vec, [&](auto v) {
-        constexpr int T = decltype(t)::value, VEC = decltype(v)::value;
-        hipLaunchKernelGGL((k_dispatch<T, VEC>), dim3((unsigned)all), dim3(kLanes), 0, s, (const int32_t *)slot + r * k,
+      with_flag(H % vec != 0, [&](auto tail) {
+        constexpr int T = decltype(t)::value;
+        hipLaunchKernelGGL((k_dispatch<T, decltype(tail)::value != 0>), dim3((unsigned)all), dim3(kLanes), 0, s, (const int32_t *)slot + r * k,
                            (const int32_t *)counts, (const int32_t *)offsets, (uint32_t)total, (int)k, (int)align, (uint32_t)blocks,
                            fast_div((uint32_t)per_row), capacity, H, (const elem_t<T> *)x + r * H, (elem_t<T> *)xs);
       });
@@ -205,18 +209,17 @@ extern "C" int anc_combine(uint64_t slot, uint64_t weights, int64_t tokens, int6
   ANC_REQUIRE(type_ok(ys_type) && type_ok(y_type), "anc_combine: types %d and %d", ys_type, y_type);
   ANC_REQUIRE(ys && y && ys % (uint64_t)elem_size(ys_type) == 0 && y % (uint64_t)elem_size(y_type) == 0 && (weights & 3) == 0,
               "anc_combine: null or misaligned pointers");
-  const Ptr ps[2] = {{ys, ys_type}, {y, y_type}};
-  const int vec = piece(H, ps);
-  const int64_t per_row = H / vec, most = kMostPieces / per_row;
+  const int64_t vec = ys_type == ANC_F32 || y_type == ANC_F32 ? 4 : 8, per_row = pieces_of(H, vec), most = kMostPieces / per_row;
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_MISC, s);
   for (int64_t r = 0; r < tokens; r += most) {
     const int64_t rows = tokens - r < most ? tokens - r : most, total = rows * per_row;
     with_type(ys_type, [&](auto ti) {
       with_type(y_type, [&](auto to) {
-        with_piece(vec, [&](auto v) {
-          constexpr int TI = decltype(ti)::value, TO = decltype(to)::value, VEC = decltype(v)::value;
-          auto kernel = weights != 0 ? k_combine<TI, TO, VEC, true> : k_combine<TI, TO, VEC, false>;
+        with_flag(H % vec != 0, [&](auto tail) {
+          constexpr int TI = decltype(ti)::value, TO = decltype(to)::value;
+          constexpr bool TAIL = decltype(tail)::value != 0;
+          auto kernel = weights != 0 ? k_combine<TI, TO, TAIL, true> : k_combine<TI, TO, TAIL, false>;
           hipLaunchKernelGGL(kernel, dim3((unsigned)((total + kLanes - 1) / kLanes)), dim3(kLanes), 0, s, (const int32_t *)slot + r * k,
                              weights != 0 ? (const float *)weights + r * k : (const float *)nullptr, (uint32_t)total, (int)k,
                              fast_div((uint32_t)per_row), capacity, H, (const elem_t<TI> *)ys, (elem_t<TO> *)y + r * H);
@@ -237,18 +240,18 @@ extern "C" int anc_combine_grad(uint64_t slot, uint64_t weights, uint64_t counts
   ANC_REQUIRE(weights && dy && ys && dys && dw && ((weights | dw) & 3) == 0 && dy % (uint64_t)elem_size(dy_type) == 0 &&
                   (ys | dys) % (uint64_t)elem_size(ys_type) == 0,
               "anc_combine_grad: null or misaligned pointers");
-  const Ptr ps[3] = {{dy, dy_type}, {ys, ys_type}, {dys, ys_type}};
-  const int vec = piece(H, ps);
+  const int64_t vec = dy_type == ANC_F32 || ys_type == ANC_F32 ? 4 : 8;
   const int64_t blocks = (tokens + kLanes / 64 - 1) / (kLanes / 64), all = blocks + pad_blocks(experts, align);
   if (tokens == 0) return ANC_OK;
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_MISC, s);
   with_type(dy_type, [&](auto ty) {
     with_type(ys_type, [&](auto ts) {
-      with_piece(vec, [&](auto v) {
-        constexpr int TY = decltype(ty)::value, TS = decltype(ts)::value, VEC = decltype(v)::value;
+      with_flag(H % vec != 0, [&](auto tail) {
+        constexpr int TY = decltype(ty)::value, TS = decltype(ts)::value;
+        constexpr bool TAIL = decltype(tail)::value != 0;
         const bool once = tokens * k * H * elem_size(ys_type) > kCached;
-        auto kernel = once ? k_combine_grad<TY, TS, VEC, true> : k_combine_grad<TY, TS, VEC, false>;
+        auto kernel = once ? k_combine_grad<TY, TS, TAIL, true> : k_combine_grad<TY, TS, TAIL, false>;
         hipLaunchKernelGGL(kernel, dim3((unsigned)all), dim3(kLanes), 0, s, (const int32_t *)slot,
                            (const float *)weights, (const int32_t *)counts, (const int32_t *)offsets, tokens, (int)k, (int)align, blocks, capacity, H,
                            (const elem_t<TY> *)dy, (const elem_t<TS> *)ys, (elem_t<TS> *)dys, (float *)dw);

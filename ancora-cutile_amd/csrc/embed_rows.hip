@@ -10,23 +10,25 @@ using namespace anc_rows;
 
 // U pieces of VEC elements per lane, (row, piece) flattened over the grid. The U ids and then the U pieces are in flight together.
 constexpr int kLookupLanes = 256;
-template <int TT, int TO, int VEC, int U, bool ONCE>
+template <int TT, int TO, bool TAIL, int U, bool ONCE>
 __global__ void __launch_bounds__(kLookupLanes)
 k_embed_lookup(const void *__restrict__ ids, int wide, uint32_t total, int64_t V, FastDiv pieces, int64_t H, float scale,
                const elem_t<TT> *__restrict__ table, elem_t<TO> *__restrict__ out) {
+  constexpr int VEC = piece_of<TT, TO>;
   const uint32_t first = blockIdx.x * (uint32_t)(kLookupLanes * U) + threadIdx.x;
   uint32_t row[U];
-  int64_t id[U], col[U];
+  int64_t id[U];
+  Piece c[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const uint32_t i = first + u * kLookupLanes < total ? first + u * kLookupLanes : total - 1;
     row[u] = pieces.div(i);
-    col[u] = (int64_t)(i - row[u] * pieces.d) * VEC;
+    c[u] = piece_at<VEC, TAIL>((int64_t)(i - row[u] * pieces.d) * VEC, H);
     id[u] = wide ? ((const int64_t *)ids)[row[u]] : (int64_t)((const int32_t *)ids)[row[u]];
   }
   Raw<TT, VEC> r[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) r[u] = load<TT, VEC>(table + (id[u] >= 0 && id[u] < V ? id[u] : 0) * H + col[u]);
+  for (int u = 0; u < U; ++u) r[u] = load<TT, VEC, TAIL>(table + (id[u] >= 0 && id[u] < V ? id[u] : 0) * H, c[u]);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     if (first + u * kLookupLanes >= total) return;
@@ -35,7 +37,7 @@ k_embed_lookup(const void *__restrict__ ids, int wide, uint32_t total, int64_t V
     const bool there = id[u] >= 0 && id[u] < V;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) x[k] = there ? x[k] * scale : 0.0f;
-    store<TO, VEC, ONCE>(out + (int64_t)row[u] * H + col[u], x);
+    store<TO, VEC, TAIL, ONCE>(out + (int64_t)row[u] * H, narrow<TO, VEC>(x), c[u]);
   }
 }
 
@@ -47,7 +49,7 @@ k_embed_lookup(const void *__restrict__ ids, int wide, uint32_t total, int64_t V
 // id may hold most of the batch.
 struct EmbedDw {
   const int32_t *srt, *start, *cnt, *key, *grp;
-  int64_t n, V, H;
+  int64_t n, V, H, pitch;                            // pitch: between rows of part, whole pieces
   int sub, chunk;                                    // chunk = kSubs * sub positions
   float scale;
   float *out, *compact, *part;
@@ -55,19 +57,20 @@ struct EmbedDw {
 constexpr int kSubs = 4;
 constexpr int kDwLanes = 256;                        // most lanes of a team, and of the join
 
-template <int VEC, bool DENSE>
-__device__ __forceinline__ void put_row(const EmbedDw &p, int64_t at, const float (&acc)[VEC]) {
+template <int VEC, bool TAIL, bool DENSE>
+__device__ __forceinline__ void put_row(const EmbedDw &p, int64_t row, const Piece &c, const float (&acc)[VEC]) {
   float x[VEC];
-  float *to = (DENSE ? p.out : p.compact) + at;
-  if constexpr (DENSE) widen<ANC_F32, VEC>(load<ANC_F32, VEC>(to), x);
+  float *to = (DENSE ? p.out : p.compact) + row * p.H;
+  if constexpr (DENSE) widen<ANC_F32, VEC>(load<ANC_F32, VEC, TAIL>(to, c), x);
 #pragma unroll
   for (int k = 0; k < VEC; ++k) x[k] = DENSE ? x[k] + p.scale * acc[k] : p.scale * acc[k];
-  store<ANC_F32, VEC>(to, x);
+  store<ANC_F32, VEC, TAIL, false, DENSE>(to, narrow<ANC_F32, VEC>(x), c);
 }
 
-template <int TD, int VEC, bool DENSE, bool ONCE>
+template <int TD, bool TAIL, bool DENSE, bool ONCE>
 __global__ void __launch_bounds__(kDwLanes * kSubs) k_embed_dw(EmbedDw p, const elem_t<TD> *__restrict__ dy) {
-  extern __shared__ float edge[];                    // [kSubs][head, tail][lanes * VEC]
+  constexpr int VEC = piece_of<TD, TD>;
+  extern __shared__ __attribute__((aligned(16))) float edge[];                    // [kSubs][head, tail][lanes * VEC]
   __shared__ int flags[kSubs];                       // 1: a head, 2: its group goes out again, 4: a tail
   const int lane = (int)(threadIdx.x & 63), team = __builtin_amdgcn_readfirstlane((int)threadIdx.y);
   const int64_t p0 = (int64_t)blockIdx.x * p.chunk + (int64_t)team * p.sub, here = p0 + lane;
@@ -80,7 +83,7 @@ __global__ void __launch_bounds__(kDwLanes * kSubs) k_embed_dw(EmbedDw p, const 
   const int m = __popcll(__ballot(grp >= 0));                            // (ids that name no row lie at the end)
   const int64_t col = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * VEC;
   const bool live = col < p.H;
-  const int64_t c0 = live ? col : 0;                                     // (every lane stays: its indices serve the others)
+  const Piece c = piece_at<VEC, TAIL>(live ? col : 0, p.H);              // (every lane stays: its indices serve the others)
   const int width = (int)blockDim.x * VEC;
   float *head = edge + team * 2 * width + threadIdx.x * VEC, *tail = head + width;
   float acc[VEC];
@@ -97,10 +100,10 @@ __global__ void __launch_bounds__(kDwLanes * kSubs) k_embed_dw(EmbedDw p, const 
       const int q = i + j < m ? i + j : m - 1;
       g[j] = __builtin_amdgcn_readlane(grp, q);
       next[j] = q + 1 < m ? __builtin_amdgcn_readlane(grp, q + 1) : -1;  // (a group that goes on behind ends here, too)
-      v[j] = load<TD, VEC, ONCE>(dy + (int64_t)__builtin_amdgcn_readlane(idx, q) * p.H + c0);
+      v[j] = load<TD, VEC, TAIL, ONCE>(dy + (int64_t)__builtin_amdgcn_readlane(idx, q) * p.H, c);
       if constexpr (DENSE)
         if (next[j] != g[j] && g[j] != came && g[j] != goes && g[j] >= 0)
-          old[j] = load<ANC_F32, VEC>(p.out + (int64_t)__builtin_amdgcn_readlane(key, q) * p.H + c0);
+          old[j] = load<ANC_F32, VEC, TAIL>(p.out + (int64_t)__builtin_amdgcn_readlane(key, q) * p.H, c);
     }
 #pragma unroll
     for (int j = 0; j < D; ++j) {
@@ -123,7 +126,8 @@ __global__ void __launch_bounds__(kDwLanes * kSubs) k_embed_dw(EmbedDw p, const 
         if constexpr (DENSE) widen<ANC_F32, VEC>(old[j], x);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) x[k] = DENSE ? x[k] + p.scale * acc[k] : p.scale * acc[k];
-        store<ANC_F32, VEC>(DENSE ? p.out + (int64_t)__builtin_amdgcn_readlane(key, i + j) * p.H + c0 : p.compact + (int64_t)g[j] * p.H + c0, x);
+        float *to = DENSE ? p.out + (int64_t)__builtin_amdgcn_readlane(key, i + j) * p.H : p.compact + (int64_t)g[j] * p.H;
+        store<ANC_F32, VEC, TAIL, false, DENSE>(to, narrow<ANC_F32, VEC>(x), c);
       }
 #pragma unroll
       for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
@@ -145,8 +149,8 @@ __global__ void __launch_bounds__(kDwLanes * kSubs) k_embed_dw(EmbedDw p, const 
       if (!(flags[t] & 2)) break;
     }
     if (live) {
-      if (t < kSubs) put_row<VEC, DENSE>(p, (DENSE ? (int64_t)tail_key : (int64_t)tail_grp) * p.H + c0, acc);
-      else store<ANC_F32, VEC>(p.part + ((int64_t)blockIdx.x * 2 + 1) * p.H + c0, acc);
+      if (t < kSubs) put_row<VEC, TAIL, DENSE>(p, DENSE ? (int64_t)tail_key : (int64_t)tail_grp, c, acc);
+      else store<ANC_F32, VEC, TAIL>(p.part + ((int64_t)blockIdx.x * 2 + 1) * p.pitch, narrow<ANC_F32, VEC>(acc), c);
     }
   }
   if (team == 0 && (state & 1)) {                    // what came into the chunk
@@ -156,15 +160,15 @@ __global__ void __launch_bounds__(kDwLanes * kSubs) k_embed_dw(EmbedDw p, const 
       add_head(t);
       if (!(flags[t] & 2)) break;
     }
-    if (live) store<ANC_F32, VEC>(p.part + (int64_t)blockIdx.x * 2 * p.H + c0, acc);
+    if (live) store<ANC_F32, VEC, TAIL>(p.part + (int64_t)blockIdx.x * 2 * p.pitch, narrow<ANC_F32, VEC>(acc), c);
   }
 }
 
 // Chunk c's part 1 begins a group that goes on: the parts of it, in order. The four wavefronts take a quarter of the list each
 // (a third of 65536 positions on one id: 85 rows), 8 rows in flight, and their sums meet in LDS.
-template <int VEC>
+template <bool TAIL>
 __global__ void __launch_bounds__(kDwLanes) k_embed_dw_join(EmbedDw p) {
-  constexpr int W = kDwLanes / 64;
+  constexpr int W = kDwLanes / 64, VEC = 4;           // (narrow pieces: more wavefronts on a long list)
   __shared__ float sums[W][64 * VEC];
   const int64_t c = blockIdx.x, last = (c + 1) * p.chunk - 1;
   if (last + 1 >= p.n) return;
@@ -175,11 +179,12 @@ __global__ void __launch_bounds__(kDwLanes) k_embed_dw_join(EmbedDw p) {
   const int lane = (int)(threadIdx.x & 63), wave = (int)(threadIdx.x >> 6);
   const int64_t col = ((int64_t)blockIdx.y * 64 + lane) * VEC;
   const bool live = col < p.H;
-  const int64_t c0 = live ? col : 0, many = ce - c + 1, per = (many + W - 1) / W;
+  const Piece pc = piece_at<VEC, TAIL>(live ? col : 0, p.H);
+  const int64_t many = ce - c + 1, per = (many + W - 1) / W;
   const int64_t lo = wave * per < many ? wave * per : many, hi = lo + per < many ? lo + per : many;
-  float *to = p.compact != nullptr ? p.compact + (int64_t)g * p.H + c0 : p.out + key * p.H + c0;
+  float *to = p.compact != nullptr ? p.compact + (int64_t)g * p.H : p.out + key * p.H;
   Raw<ANC_F32, VEC> old;
-  if (p.compact == nullptr) old = load<ANC_F32, VEC>(to);
+  if (p.compact == nullptr) old = load<ANC_F32, VEC, TAIL>(to, pc);
   float acc[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
@@ -189,7 +194,7 @@ __global__ void __launch_bounds__(kDwLanes) k_embed_dw_join(EmbedDw p) {
 #pragma unroll
     for (int j = 0; j < D; ++j) {
       const int64_t q = i + j < hi ? i + j : hi - 1;
-      v[j] = load<ANC_F32, VEC>(p.part + ((c + q) * 2 + (q == 0 ? 1 : 0)) * p.H + c0);
+      v[j] = load<ANC_F32, VEC, TAIL>(p.part + ((c + q) * 2 + (q == 0 ? 1 : 0)) * p.pitch, pc);
     }
 #pragma unroll
     for (int j = 0; j < D; ++j) {
@@ -213,13 +218,14 @@ __global__ void __launch_bounds__(kDwLanes) k_embed_dw_join(EmbedDw p) {
   if (p.compact == nullptr) widen<ANC_F32, VEC>(old, x);
 #pragma unroll
   for (int k = 0; k < VEC; ++k) x[k] = p.compact == nullptr ? x[k] + p.scale * acc[k] : p.scale * acc[k];
-  store<ANC_F32, VEC>(to, x);
+  store<ANC_F32, VEC, TAIL, false, true>(to, narrow<ANC_F32, VEC>(x), pc);
 }
 
 // Positions per team: enough chunks to fill the card.
 constexpr int64_t kSub8Most = 8192, kSub16Most = 32768;
 int dw_chunk(int64_t n) { return kSubs * (n <= kSub8Most ? 8 : n <= kSub16Most ? 16 : 64); }
 int64_t dw_chunks(int64_t n) { return (n + dw_chunk(n) - 1) / dw_chunk(n); }
+int64_t dw_pitch(int64_t H) { return (H + 7) / 8 * 8; }
 constexpr int64_t kMostPositions = 1ll << 20;
 constexpr int64_t kFewPieces = 1 << 19;              // of a lookup: below, one piece per lane
 
@@ -235,9 +241,8 @@ extern "C" int anc_embed_lookup(uint64_t ids, int32_t ids_bytes, int64_t n, uint
   ANC_REQUIRE(ids && table && out, "anc_embed_lookup: null pointer");
   ANC_REQUIRE(ids % (uint64_t)ids_bytes == 0 && table % (uint64_t)elem_size(table_type) == 0 && out % (uint64_t)elem_size(out_type) == 0,
               "anc_embed_lookup: misaligned pointers");
-  const Ptr ps[2] = {{table, table_type}, {out, out_type}};
-  const int vec = piece(H, ps);
-  const int64_t per_row = H / vec, most = kMostPieces / per_row;
+  const int vec = table_type == ANC_F32 || out_type == ANC_F32 ? 4 : 8;
+  const int64_t per_row = pieces_of(H, vec), most = kMostPieces / per_row;
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_MISC, s);
   for (int64_t r = 0; r < n; r += most) {
@@ -247,9 +252,11 @@ extern "C" int anc_embed_lookup(uint64_t ids, int32_t ids_bytes, int64_t n, uint
     const dim3 grid((unsigned)((total + u * kLookupLanes - 1) / (u * kLookupLanes)));
     with_type(table_type, [&](auto tt) {
       with_type(out_type, [&](auto to) {
-        with_piece(vec, [&](auto v) {
-          constexpr int TT = decltype(tt)::value, TO = decltype(to)::value, VEC = decltype(v)::value;
-          auto kernel = u == 1 ? k_embed_lookup<TT, TO, VEC, 1, false> : once ? k_embed_lookup<TT, TO, VEC, 4, true> : k_embed_lookup<TT, TO, VEC, 4, false>;
+        with_flag(H % vec != 0, [&](auto tail) {
+          constexpr int TT = decltype(tt)::value, TO = decltype(to)::value;
+          constexpr bool TAIL = decltype(tail)::value != 0;
+          auto kernel = u == 1 ? k_embed_lookup<TT, TO, TAIL, 1, false>
+                        : once ? k_embed_lookup<TT, TO, TAIL, 4, true> : k_embed_lookup<TT, TO, TAIL, 4, false>;
           hipLaunchKernelGGL(kernel, grid, dim3(kLookupLanes), 0, s, (const void *)(ids + (uint64_t)(r * ids_bytes)), ids_bytes == 8,
                              (uint32_t)total, V, fast_div((uint32_t)per_row), H, scale, (const elem_t<TT> *)table,
                              (elem_t<TO> *)out + r * H);
@@ -270,7 +277,7 @@ extern "C" int64_t anc_embed_dw_workspace_bytes(int64_t M, int64_t H) {
   int64_t most = dw_chunks(M);
   for (int64_t edge : {kSub8Most, kSub16Most})
     if (edge < M && dw_chunks(edge) > most) most = dw_chunks(edge);
-  return most * 2 * H * 4;
+  return most * 2 * dw_pitch(H) * 4;
 }
 
 extern "C" int anc_embed_dw(uint64_t srt, uint64_t start, uint64_t cnt, uint64_t key, uint64_t grp, int64_t n, uint64_t dy, int dy_type,
@@ -284,31 +291,30 @@ extern "C" int anc_embed_dw(uint64_t srt, uint64_t start, uint64_t cnt, uint64_t
   ANC_REQUIRE(srt && start && cnt && key && grp && dy && workspace, "anc_embed_dw: null pointer");
   ANC_REQUIRE(((srt | start | cnt | key | grp | out | compact) & 3) == 0 && dy % (uint64_t)elem_size(dy_type) == 0 && (workspace & 15) == 0,
               "anc_embed_dw: misaligned pointers");
-  const int64_t chunks = dw_chunks(n), need = chunks * 2 * H * 4;
+  const int64_t chunks = dw_chunks(n), need = chunks * 2 * dw_pitch(H) * 4;
   ANC_REQUIRE(workspace_bytes >= need, "anc_embed_dw: workspace holds %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
-  const Ptr ps[1] = {{dy, dy_type}};
-  const int rows = piece(H, ps), vec = ((out | compact) & (uint64_t)(rows >= 4 ? 15 : 4 * rows - 1)) == 0 ? rows : 1;
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_MISC, s);
-  EmbedDw p{(const int32_t *)srt, (const int32_t *)start, (const int32_t *)cnt, (const int32_t *)key, (const int32_t *)grp,
-            n, V, H, dw_chunk(n) / kSubs, dw_chunk(n), scale, (float *)out, (float *)compact, (float *)workspace};
-  with_piece(vec, [&](auto v) {
-    constexpr int VEC = decltype(v)::value;
-    // (a team is at most 1024 columns wide: 32 KiB of LDS for the edges)
-    constexpr int64_t widest = VEC == 8 ? 2 : kDwLanes / 64;
-    const int64_t waves = (H + 64 * VEC - 1) / (64 * VEC), wide = waves < widest ? waves : widest;
-    with_type(dy_type, [&](auto t) {
-      constexpr int T = decltype(t)::value;
-      const bool once = n * H * elem_size(dy_type) > kCached;
-      auto kernel = out != 0 ? (once ? k_embed_dw<T, VEC, true, true> : k_embed_dw<T, VEC, true, false>)
-                             : (once ? k_embed_dw<T, VEC, false, true> : k_embed_dw<T, VEC, false, false>);
+  const EmbedDw p{(const int32_t *)srt, (const int32_t *)start, (const int32_t *)cnt, (const int32_t *)key, (const int32_t *)grp,
+                  n, V, H, dw_pitch(H), dw_chunk(n) / kSubs, dw_chunk(n), scale, (float *)out, (float *)compact, (float *)workspace};
+  const bool once = n * H * elem_size(dy_type) > kCached;
+  with_type(dy_type, [&](auto t) {
+    with_flag(H % piece_of<decltype(t)::value, decltype(t)::value> != 0, [&](auto tail) {
+      constexpr int T = decltype(t)::value, VEC = piece_of<T, T>;
+      constexpr bool TAIL = decltype(tail)::value != 0;
+      // (a team is at most 1024 columns wide: 32 KiB of LDS for the edges)
+      const int64_t waves = (H + 64 * VEC - 1) / (64 * VEC), widest = 1024 / (64 * VEC), wide = waves < widest ? waves : widest;
+      auto kernel = out != 0 ? (once ? k_embed_dw<T, TAIL, true, true> : k_embed_dw<T, TAIL, true, false>)
+                             : (once ? k_embed_dw<T, TAIL, false, true> : k_embed_dw<T, TAIL, false, false>);
       hipLaunchKernelGGL(kernel, dim3((unsigned)chunks, (unsigned)((waves + wide - 1) / wide)), dim3((unsigned)(64 * wide), kSubs),
                          (unsigned)(kSubs * 2 * 64 * wide * VEC * sizeof(float)), s, p, (const elem_t<T> *)dy);
     });
-    constexpr int JV = VEC < 4 ? VEC : 4;            // narrower pieces: more wavefronts on a long list
-    if (chunks > 1)
-      hipLaunchKernelGGL((k_embed_dw_join<JV>), dim3((unsigned)(chunks - 1), (unsigned)((H + 64 * JV - 1) / (64 * JV))), dim3(kDwLanes), 0, s, p);
   });
+  if (chunks > 1)
+    with_flag(H % 4 != 0, [&](auto tail) {
+      hipLaunchKernelGGL((k_embed_dw_join<decltype(tail)::value != 0>), dim3((unsigned)(chunks - 1), (unsigned)((H + 255) / 256)), dim3(kDwLanes), 0,
+                         s, p);
+    });
   ANC_LAUNCH_CHECK();
   return ANC_OK;
 }
