@@ -14,7 +14,7 @@ import numpy as np
 from . import _lib
 from ._lib import api
 from .devbuf import DevBuf
-from .embed import _ids, _rows_of, _type
+from .embed import _TYPES, _ids, _rows_of, _type
 
 
 class RoutePlan:
@@ -47,7 +47,8 @@ class RoutePlan:
         shapes = ((self.E,), (self.E + 1,), (self.E,), (self.tokens, self.k), (self.capacity,))
         bufs = [DevBuf(shape=sh, dtype=np.int32, ptr=p) for sh, p in zip(shapes, at)]
         self.counts, self.offsets, self.order, self.slot, self.src = bufs
-        self._at = (*at, self.capacity, self._ws.ptr, nbytes)
+        # (as the library takes them: converting a number of every call's arguments was a tenth of a small call)
+        self._at = (*(_lib.u64(p) for p in at), _lib.i64(self.capacity), _lib.u64(self._ws.ptr), _lib.i64(nbytes))
         self.active = None                     # tokens of the last `route`
 
     def _used(self, who):
@@ -86,12 +87,12 @@ def dispatch(plan, x, si, xs):
     if x.dtype != xs.dtype:
         raise ValueError(f"dispatch: x is {x.dtype}, xs {xs.dtype}")
     counts, offsets, _, slot = plan._at[:4]
-    api.anc_dispatch(slot, counts, offsets, plan.active, plan.k, plan.E, plan.align, x.ptr, xs.ptr, plan.capacity,
+    api.anc_dispatch(slot, counts, offsets, plan.active, plan.k, plan.E, plan.align, x.ptr, xs.ptr, plan._at[5],
                      _type(x, "dispatch"), H, int(si))
 
 
 def _weights(plan, w, who):
-    if w.dtype != np.float32 or len(w.shape) != 2 or w.shape[1] != plan.k or w.shape[0] < plan.active:
+    if _TYPES.get(w.dtype) != _lib.F32 or len(w.shape) != 2 or w.shape[1] != plan.k or w.shape[0] < plan.active:
         raise ValueError(f"{who}: weights are {w.shape} {w.dtype}, ({plan.active}, {plan.k}) float32 expected")
     return w.ptr
 
@@ -105,7 +106,7 @@ def combine(plan, ys, weights, si, y):
     _rows_of(ys, plan.capacity, H, "combine", "ys")
     _rows_of(y, plan.active, H, "combine", "y")
     w = 0 if weights is None else _weights(plan, weights, "combine")
-    api.anc_combine(plan._at[3], w, plan.active, plan.k, ys.ptr, plan.capacity, _type(ys, "combine"), y.ptr,
+    api.anc_combine(plan._at[3], w, plan.active, plan.k, ys.ptr, plan._at[5], _type(ys, "combine"), y.ptr,
                     _type(y, "combine"), H, int(si))
 
 
@@ -126,5 +127,5 @@ def combine_grad(plan, dy, ys, weights, si, dys, dweights):
         raise ValueError(f"combine_grad: ys is {ys.dtype}, dys {dys.dtype}")
     counts, offsets, _, slot = plan._at[:4]
     api.anc_combine_grad(slot, _weights(plan, weights, "combine_grad"), counts, offsets, plan.active, plan.k, plan.E, plan.align, dy.ptr,
-                         _type(dy, "combine_grad"), ys.ptr, dys.ptr, plan.capacity, _type(ys, "combine_grad"),
+                         _type(dy, "combine_grad"), ys.ptr, dys.ptr, plan._at[5], _type(ys, "combine_grad"),
                          _weights(plan, dweights, "combine_grad"), H, int(si))

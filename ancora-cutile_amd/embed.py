@@ -180,26 +180,32 @@ def embed_dw_scatter(groups, dy, si, out=None, compact=None, V=None):
                              M, 0 if V is None else V, H, int(si))
 
 
+_ID_BYTES = {np.dtype(np.int32): 4, np.dtype(np.int64): 8}
+_TYPES = {np.dtype(np.uint16): _lib.BF16, np.dtype(np.float32): _lib.F32}
+
+
 def _ids(buf, who, most=None):
     """(bytes per id, number of ids) of a device array of ids."""
-    if buf.dtype not in (np.int32, np.int64):
+    nbytes = _ID_BYTES.get(buf.dtype)
+    if nbytes is None:
         raise ValueError(f"{who}: ids are int32 or int64, got {buf.dtype}")
-    if most is not None and buf.size > most:
-        raise ValueError(f"{who}: {buf.size} ids, room for {most}")
-    return buf.dtype.itemsize, buf.size
+    have = buf.nbytes // nbytes
+    if most is not None and have > most:
+        raise ValueError(f"{who}: {have} ids, room for {most}")
+    return nbytes, have
 
 
 def _type(buf, who):
-    if buf.dtype == np.uint16:
-        return _lib.BF16
-    if buf.dtype == np.float32:
-        return _lib.F32
-    raise ValueError(f"{who}: rows are float32 or bf16 bits (uint16), got {buf.dtype}")
+    t = _TYPES.get(buf.dtype)
+    if t is None:
+        raise ValueError(f"{who}: rows are float32 or bf16 bits (uint16), got {buf.dtype}")
+    return t
 
 
 def _rows_of(buf, rows, H, who, name):
     """`buf` holds at least `rows` rows of H elements."""
-    if len(buf.shape) != 2 or buf.shape[1] != H or buf.shape[0] < rows:
+    shape = buf.shape
+    if len(shape) != 2 or shape[1] != H or shape[0] < rows:
         raise ValueError(f"{who}: {name} is {buf.shape}, ({rows}, {H}) expected")
 
 
@@ -244,7 +250,8 @@ class DeviceIdGroups:
         arrays = [DevBuf(shape=(self.M, 1), dtype=np.int32, ptr=self._block.ptr + 4 * i * self.M) for i in range(6)]
         self.srt, self.start, self.cnt, self.gid, self._key, self._grp = arrays
         self.count = DevBuf(shape=(1,), dtype=np.int32, ptr=self._block.ptr + 24 * self.M)
-        self._at = tuple(a.ptr for a in arrays) + (self.count.ptr, self._ws.ptr, nbytes)
+        # (as the library takes them: converting a number of every call's arguments was a tenth of a small call)
+        self._at = tuple(_lib.u64(a.ptr) for a in arrays) + (_lib.u64(self.count.ptr), _lib.u64(self._ws.ptr), _lib.i64(nbytes))
         self.n = None                          # ids of the last `group`
 
     def base_on(self, si):
