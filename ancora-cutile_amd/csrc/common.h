@@ -23,6 +23,11 @@ int anc_hip_fail(hipError_t e, const char *what, const char *file, int line);
 // Launch check: hipGetLastError right after a launch catches bad configurations.
 #define ANC_LAUNCH_CHECK() ANC_HIP(hipGetLastError())
 
+// Two buffers have no byte in common.
+static inline bool anc_apart(uint64_t a, int64_t a_bytes, uint64_t b, int64_t b_bytes) {
+  return a + (uint64_t)a_bytes <= b || b + (uint64_t)b_bytes <= a;
+}
+
 static inline hipStream_t anc_stream(uint64_t s) { return reinterpret_cast<hipStream_t>(s); }
 
 // Optional per-launch timing (anc_profile_enable): when on, every kernel launch of the

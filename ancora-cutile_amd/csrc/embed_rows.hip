@@ -241,6 +241,8 @@ extern "C" int anc_embed_lookup(uint64_t ids, int32_t ids_bytes, int64_t n, uint
   ANC_REQUIRE(ids && table && out, "anc_embed_lookup: null pointer");
   ANC_REQUIRE(ids % (uint64_t)ids_bytes == 0 && table % (uint64_t)elem_size(table_type) == 0 && out % (uint64_t)elem_size(out_type) == 0,
               "anc_embed_lookup: misaligned pointers");
+  ANC_REQUIRE(anc_apart(out, n * H * elem_size(out_type), table, V * H * elem_size(table_type)) && anc_apart(out, n * H * elem_size(out_type), ids, n * ids_bytes),
+              "anc_embed_lookup: out overlaps an input");
   const int vec = table_type == ANC_F32 || out_type == ANC_F32 ? 4 : 8;
   const int64_t per_row = pieces_of(H, vec), most = kMostPieces / per_row;
   hipStream_t s = anc_stream(stream);
@@ -293,6 +295,10 @@ extern "C" int anc_embed_dw(uint64_t srt, uint64_t start, uint64_t cnt, uint64_t
               "anc_embed_dw: misaligned pointers");
   const int64_t chunks = dw_chunks(n), need = chunks * 2 * dw_pitch(H) * 4;
   ANC_REQUIRE(workspace_bytes >= need, "anc_embed_dw: workspace holds %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  const uint64_t to = out != 0 ? out : compact;       // (a compact gradient is n rows at most)
+  const int64_t to_bytes = (out != 0 ? V : n) * H * 4, dy_bytes = n * H * elem_size(dy_type);
+  ANC_REQUIRE(anc_apart(to, to_bytes, dy, dy_bytes) && anc_apart(workspace, need, dy, dy_bytes) && anc_apart(workspace, need, to, to_bytes),
+              "anc_embed_dw: dy, the gradient and the workspace overlap");
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_MISC, s);
   const EmbedDw p{(const int32_t *)srt, (const int32_t *)start, (const int32_t *)cnt, (const int32_t *)key, (const int32_t *)grp,

@@ -230,16 +230,27 @@ extern "C" int anc_expert_dw_multi(const anc_expert_dw_problem_t *probs, int32_t
   m.count = n_probs;
   m.experts = (int)experts;
   int64_t wide = 0;                                  // tiles of 256x256
+  struct { uint64_t at; int64_t bytes; } span[kMostProblems][4];       // outputs, then inputs
   for (int i = 0; i < n_probs; ++i) {
     const anc_expert_dw_problem_t &b = probs[i];
     ANC_REQUIRE(b.K > 0 && b.N > 0 && b.K % 8 == 0 && b.N % 8 == 0 && b.K <= (1 << 17) && b.N <= (1 << 17),
                 "anc_expert_dw_multi: needs K %% 8 == 0 and N %% 8 == 0 (K=%lld N=%lld)", (long long)b.K, (long long)b.N);
     ANC_REQUIRE(b.x && b.dy && b.dW && ((b.x | b.dy | b.dW) & 15) == 0 && (b.g16 & 7) == 0,
                 "anc_expert_dw_multi: null or misaligned pointer");
+    span[i][0] = {b.dW, experts * b.K * b.N * 4};
+    span[i][1] = {b.g16, b.g16 != 0 ? experts * b.K * b.N * 2 : 0};
+    span[i][2] = {b.x, capacity * b.K * 2};
+    span[i][3] = {b.dy, capacity * b.N * 2};
     m.p[i] = DwOne{(const uint16_t *)b.x, (const uint16_t *)b.dy, (float *)b.dW, (uint16_t *)b.g16, (int)b.K, (int)b.N,
                    (int)((b.N + TN - 1) / TN), 0, b.accumulate != 0};
     wide += (b.K + 255) / 256 * m.p[i].tn * experts;
   }
+  for (int i = 0; i < n_probs; ++i)                  // (workgroups run in any order: an output meets no other buffer of the call)
+    for (int a = 0; a < 2; ++a)
+      for (int j = 0; j < n_probs; ++j)
+        for (int c = 0; c < 4; ++c)
+          ANC_REQUIRE((i == j && a == c) || anc_apart(span[i][a].at, span[i][a].bytes, span[j][c].at, span[j][c].bytes),
+                      "anc_expert_dw_multi: an output of problem %d overlaps a buffer of problem %d", i, j);
   // 256x256 tiles where they give every CU one; fewer, and twice as many of 128x256 are at work.
   const int TM = wide >= 256 ? 256 : 128;
   for (int i = 0; i < n_probs; ++i) m.p[i].tiles = (m.p[i].K + TM - 1) / TM * m.p[i].tn;
@@ -250,7 +261,7 @@ extern "C" int anc_expert_dw_multi(const anc_expert_dw_problem_t *probs, int32_t
     if (m.unit == 4 || m.unit0[n_probs] * experts >= 6 * kXcds) break;
   }
   const int64_t units = m.unit0[n_probs] * experts, grid = (units + kXcds - 1) / kXcds * kXcds * m.unit;
-  ANC_REQUIRE(grid < (1ll << 31), "anc_expert_dw_multi: too large for one call");
+  ANC_REQUIRE(grid * TM * 2 < (1ll << 32), "anc_expert_dw_multi: too large for one call");
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_DW_GEMM, s);
   if (TM == 256) hipLaunchKernelGGL(k_expert_dw<256>, dim3((unsigned)grid), dim3(512), 0, s, m);

@@ -7,7 +7,8 @@
     combine(plan, ys, weights, si, y)                # y[t] = sum over j of weights[t, j] * ys[slot[t, j]]
 
 and backwards `combine_grad` (rows and weights), `grads.expert_dW` (the experts' weights, over the ragged segments) and
-`dispatch_grad`. Everything is decided on the device: no copy to the host, and each call may be captured into a graph.
+`dispatch_grad`. Everything is decided on the device: no copy to the host, and each call may be captured into a graph. Outputs
+overlap no input.
 """
 import numpy as np
 

@@ -321,7 +321,7 @@ int anc_unique_ids(const int32_t *ids, int64_t n, int32_t *out, int64_t *n_out);
 
 /* The input embedding from ids that lie on the device. Ids are int32 or int64 (ids_bytes 4 or 8); one outside
  * [0, V) names no row: its lookup is a zero row, its gradient is left out. Types are ANC_F32 or ANC_BF16, rows are
- * contiguous, any H; rows that start 16-byte aligned with H % 8 == 0 move fastest.
+ * contiguous, any H. No output may overlap an input or another output, here and in the calls below.
  *
  * anc_embed_lookup: out[i] = scale * table[ids[i]] for i < n, product in fp32, one rounding. */
 int anc_embed_lookup(uint64_t ids, int32_t ids_bytes, int64_t n, uint64_t table, int table_type, int64_t V, int64_t H,
@@ -494,7 +494,7 @@ int anc_gemm_dw_info(int64_t T, int64_t K, int64_t N, double *flops, int32_t *se
  * (or keeps dW). g16, if not 0, receives the bf16 copy of the final dW. Rows that fill up a segment are not read, whatever they hold.
  * An expert's tokens are added in ascending order, one accumulator per element: its bits are a function of its own rows. order: every
  * expert once, best by falling number of tokens (anc_route's): the order in which they are taken up, no more.
- * K, N multiples of 8 up to 2^17; x, dy, dW 16-byte aligned. */
+ * K, N multiples of 8 up to 2^17; x, dy, dW 16-byte aligned. No output overlaps another buffer of the call. */
 typedef struct {
   uint64_t x, dy, dW, g16;
   int64_t  K, N;

@@ -227,3 +227,38 @@ def test_expert_gradient_calls_that_do_not_fit_launch_nothing(fake_device):
     assert [a[1] for a in fake_device.calls("anc_expert_dw_multi")] == [8, 3]
     expert_dW(p, [], 0)
     assert len(fake_device.calls("anc_expert_dw_multi")) == 2
+
+
+def test_outputs_that_overlap_are_refused(lib):
+    from ancora_cutile_amd._lib import ExpertDwProblem
+    a = [P * (16 + i) for i in range(12)]                                          # far apart
+    look = (a[0], 4, 10, a[1], 1, 100, 64, 1.0, a[2], 1, 0)
+    for out in (a[1], a[1] + 100 * 128 - 2, a[1] - 10 * 128 + 2, a[0], a[0] + 36):
+        _refused(lib, "anc_embed_lookup", _but(look, 8, out), "overlaps")
+    ws = lib.anc_embed_dw_workspace_bytes(1000, 64)
+    grad = (a[0], a[1], a[2], a[3], a[4], 1000, a[5], 1, 64, 1.0, a[6], 0, 500, a[7], ws, 0)
+    for at, value in ((10, a[5]), (10, a[5] + 1000 * 128 - 4), (10, a[7] + ws - 4), (13, a[5]), (13, a[6] + 500 * 256 - 16)):
+        _refused(lib, "anc_embed_dw", _but(grad, at, value), "overlap")
+    move = (a[0], a[1], a[2], 10, 2, 4, 16, a[3], a[4], 200, 1, 64, 0)
+    for x in (a[4], a[4] + 200 * 128 - 2, a[4] - 10 * 128 + 2):
+        _refused(lib, "anc_dispatch", _but(move, 7, x), "overlap")
+    back = (a[0], a[1], 10, 2, a[2], 200, 1, a[3], 1, 64, 0)
+    for y in (a[2], a[2] + 200 * 128 - 2, a[1] - 2, a[1] + 78):
+        _refused(lib, "anc_combine", _but(back, 7, y), "overlaps")
+    both = (a[0], a[1], a[2], a[3], 10, 2, 4, 16, a[4], 1, a[5], a[6], 200, 1, a[7], 64, 0)
+    for at, value in ((11, a[5]), (11, a[4] + 1278), (11, a[1] + 78), (14, a[1]), (14, a[5] + 4), (14, a[4]), (14, a[6])):
+        _refused(lib, "anc_combine_grad", _but(both, at, value), "overlaps")
+    for name, args in (("anc_dispatch", move), ("anc_combine", back), ("anc_combine_grad", both)):
+        at = 2 if name == "anc_combine" else 3 if name == "anc_dispatch" else 4
+        _refused(lib, name, _but(_but(args, at, (1 << 21) + 1), at + 1, 2), "tokens")      # more than can be routed
+
+    def call(*problems):
+        fields = dict(x=a[0], dy=a[1], dW=a[2], g16=0, K=64, N=128, accumulate=0, reserved=0)
+        arr = (ExpertDwProblem * len(problems))(*[ExpertDwProblem(**{**fields, **p}) for p in problems])
+        return lib.anc_expert_dw_multi(arr, len(problems), a[8], a[9], a[10], 4, 100, 0)
+
+    weight = 4 * 64 * 128 * 4
+    for ps in ((dict(dW=a[0]),), (dict(dW=a[1] + 100 * 256 - 16),), (dict(g16=a[2] + weight - 8),), (dict(g16=a[0]),), (dict(g16=a[1]),), ({}, {}),
+               ({}, dict(dW=a[2] + weight - 16)), (dict(g16=a[3]), dict(dW=a[3])), (dict(g16=a[3]), dict(dW=a[4], g16=a[3])), ({}, dict(dW=a[3], x=a[2])),
+               (dict(x=a[4]), dict(dW=a[4])), (dict(dy=a[4]), dict(dW=a[3], g16=a[4]))):
+        assert call(*ps) == 2 and "overlaps" in lib.anc_last_error().decode(), (ps, lib.anc_last_error())
