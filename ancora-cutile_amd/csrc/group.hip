@@ -50,13 +50,22 @@ __device__ __forceinline__ int take_rank(volatile int *count, uint32_t d, int bi
   __builtin_amdgcn_wave_barrier();
   return old + before;
 }
+// Sums across lanes within registers: DPP moves feed the addition itself (through LDS a step is some hundred clocks: the three
+// sums of a grouping of 8192 ids took 2.3 us).
 __device__ __forceinline__ int wave_scan(int v) {          // inclusive
-  const int lane = (int)(threadIdx.x & 63);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(v, o, 64);
-    if (lane >= o) v += u;
-  }
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);      // from 1, 2, 4, 8 lanes below, within 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);      // lane 15 of a row of 16 to the next row, rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);      // lane 31 to rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ int wave_sum(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+template <int L> __device__ __forceinline__ int sum_of(int v) {        // over L neighbours
+  static_assert(L == 1 || L == 2 || L == 4, "within four lanes");
+  if constexpr (L >= 2) v += __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, true);         // lanes 1 0 3 2
+  if constexpr (L == 4) v += __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, true);         // lanes 2 3 0 1
   return v;
 }
 // Exclusive sum over the workgroup's lanes, in lane order; every lane calls. total: the sum over all.
@@ -116,15 +125,18 @@ __device__ __forceinline__ uint64_t place(uint32_t key, int p) { return (uint64_
 // A token id as a key: V for one that names no row.
 __device__ __forceinline__ uint32_t as_key(int32_t id, uint32_t V) { return (uint32_t)id < V ? (uint32_t)id : V; }
 __device__ __forceinline__ uint32_t as_key(int64_t id, uint32_t V) { return (uint64_t)id < V ? (uint32_t)id : V; }
-constexpr int kPartItems = 4, kTile = 8, kSamples = 256;
-constexpr int64_t kFewAlone = 512, kMostAlone = 4096, kMostSplit = 1 << 16;             // positions: of one workgroup, of several
+constexpr int kPartItems = 4, kSamples = 256;
+// Both sides measured, ids of 152 K rows, a call in a row of calls: 512 alone on 256 lanes 7.0 us (on 1024 7.7), 1024 alone on 512 lanes 7.5 (on
+// 1024 8.4; in shares 9.2), 1500 alone 8.8, 2048 alone 10.2 and in shares 9.3; shares on 512 and on 1024 lanes: 8192 12.4 and 13.8, 24000 20.1 and
+// 20.8, 32768 23.2 and 23.0; 65536 in shares 31, by passes 47.
+constexpr int64_t kFewAlone = 512, kMostAlone = 1536, kFewSplit = 1 << 14, kMostSplit = 1 << 16;             // positions: of one workgroup, of several
 constexpr int64_t kMostMarked = 1 << 18;                               // ids, where several workgroups share them (one bit each in LDS)
 
 // SPLIT: gridDim.x workgroups share the order; else one takes all of it (n <= CAP, and any V).
 template <int LANES, bool SPLIT, typename ID>
 __global__ void __launch_bounds__(LANES)
 k_group_part(const ID *__restrict__ ids, int n, int64_t M, uint32_t V, Groups o) {
-  constexpr int W = LANES / 64, CAP = LANES * kPartItems, PER = kDigits > LANES ? kDigits / LANES : 1;
+  constexpr int W = LANES / 64, CAP = LANES * kPartItems, PER = kDigits > LANES ? kDigits / LANES : 1, kTile = 8;
   __shared__ uint32_t skey[CAP];
   __shared__ int spos[SPLIT ? CAP : 1];
   __shared__ uint16_t sidx[CAP];
@@ -147,13 +159,16 @@ k_group_part(const ID *__restrict__ ids, int n, int64_t M, uint32_t V, Groups o)
 #pragma unroll
     for (int j = 0; j < kTile; ++j) raw[j] = ids[t + 64 * j + lane < w1 ? t + 64 * j + lane : w1 - 1];
   };
-  // f(a tile's first position) for all tiles of the wavefront, its keys there, the next tile's ids on their way; the first is fetched again.
+  // f(a tile's first position) for all tiles of the wavefront, its keys there, the next tile's ids on their way.
+  bool ready = true;
   auto each_tile = [&](auto f) {
+    if (!ready && w0 < w1) fetch(w0);
+    ready = false;
 #pragma unroll 1
     for (int t = w0; t < w1; t += 64 * kTile) {
 #pragma unroll
       for (int j = 0; j < kTile; ++j) key[j] = as_key(raw[j], V);
-      fetch(t + 64 * kTile < w1 ? t + 64 * kTile : w0);
+      if (t + 64 * kTile < w1) fetch(t + 64 * kTile);
       f(t);
     }
   };
@@ -176,8 +191,7 @@ k_group_part(const ID *__restrict__ ids, int n, int64_t M, uint32_t V, Groups o)
       const anc_u32x4 v = run[j];
       before += (v.x < mine ? 1 : 0) + (v.y < mine ? 1 : 0) + (v.z < mine ? 1 : 0) + (v.w < mine ? 1 : 0);
     }
-#pragma unroll
-    for (int s = 1; s < L; s <<= 1) before += __shfl_xor(before, s, 64);
+    before = sum_of<L>(before);
     if (tid % L == 0) {
       if (part > 0 && before == part * kSamples / parts) { cut[0] = (int)id; cut[1] = at; }
       if (part + 1 < parts && before == (part + 1) * kSamples / parts) { cut[2] = (int)id; cut[3] = at; }
@@ -203,13 +217,15 @@ k_group_part(const ID *__restrict__ ids, int n, int64_t M, uint32_t V, Groups o)
         mask = 0;
         int low = 0, came_goes = 0;                  // (of a lane, then of a wavefront: at most 64 and 4096)
         each_tile([&](int t) {
-          if (!marked) {                             // (a frequent id is read, not set, from its second item on)
-            uint32_t seen[kTile];
+          // (Lanes that meet on a word take turns: of a run of one id its first lane goes, of an id that is frequent everywhere, padding, the
+          // wavefront's first. 65536 ids in runs of 16: 33 us; with every item reading first whether its bit is set 67.)
+          if (!marked) {
 #pragma unroll
-            for (int j = 0; j < kTile; ++j) seen[j] = ((volatile uint32_t *)marks)[key[j] < V ? key[j] >> 5 : 0];
-#pragma unroll
-            for (int j = 0; j < kTile; ++j)
-              if (key[j] < V && !(seen[j] >> (key[j] & 31) & 1u)) atomicOr(&marks[key[j] >> 5], 1u << (key[j] & 31));
+            for (int j = 0; j < kTile; ++j) {
+              const uint32_t left = (uint32_t)__builtin_amdgcn_update_dpp((int)V, (int)key[j], 0x138, 0xF, 0xF, false);
+              const uint32_t of_lane0 = (uint32_t)uniform((int)key[j]);          // (read while every lane is active)
+              if (key[j] < V && key[j] != left && (lane == 0 || key[j] != of_lane0)) atomicOr(&marks[key[j] >> 5], 1u << (key[j] & 31));
+            }
           }
 #pragma unroll
           for (int j = 0; j < kTile; ++j) {
@@ -226,11 +242,8 @@ k_group_part(const ID *__restrict__ ids, int n, int64_t M, uint32_t V, Groups o)
         });
         marked = true;
         const int own = __popcll(mask), upto = wave_scan(own);
-#pragma unroll
-        for (int s = 32; s >= 1; s >>= 1) {
-          low += __shfl_xor(low, s, 64);
-          came_goes += __shfl_xor(came_goes, s, 64);
-        }
+        low = wave_sum(low);
+        came_goes = wave_sum(came_goes);
         if (lane == 63) four[wave] = anc_i32x4{upto, low, came_goes & 0xFFFF, came_goes >> 16};
         __syncthreads();
         anc_i32x4 sum = {0, 0, 0, 0};
@@ -270,8 +283,7 @@ k_group_part(const ID *__restrict__ ids, int n, int64_t M, uint32_t V, Groups o)
         const uint32_t w = marks[i], i32 = (uint32_t)i * 32;
         low_every += __popc(w) << 16 | (i32 + 32 <= id_lo ? __popc(w) : i32 >= id_lo ? 0 : __popc(w & ((1u << (id_lo - i32)) - 1)));
       }
-#pragma unroll
-      for (int s = 32; s >= 1; s >>= 1) low_every += __shfl_xor(low_every, s, 64);
+      low_every = wave_sum(low_every);
       if (lane == 0) tmp[wave] = low_every;
       for (; mask != 0; mask &= mask - 1) spos[put++] = w0 + lane * 64 + (int)__builtin_ctzll(mask);
       __syncthreads();
@@ -319,8 +331,7 @@ k_group_part(const ID *__restrict__ ids, int n, int64_t M, uint32_t V, Groups o)
         const anc_u32x4 q = ((const anc_u32x4 *)numbers)[v];
         smaller_ones += (q.x < mine ? 1 : 0) + (q.y < mine ? 1 : 0) + (q.z < mine ? 1 : 0) + (q.w < mine ? 1 : 0);
       }
-#pragma unroll
-      for (int s = 1; s < L; s <<= 1) smaller_ones += __shfl_xor(smaller_ones, s, 64);
+      smaller_ones = sum_of<L>(smaller_ones);
       if (tid % L == 0 && tid / L < size) sidx[smaller_ones] = (uint16_t)(tid / L);
       __syncthreads();
       if (tid < size) {
@@ -626,8 +637,7 @@ __device__ __forceinline__ void order_experts(const int *scnt, int E, int32_t *o
     const int c = scnt[j];
     before += c > mine || (c == mine && j < e) ? 1 : 0;
   }
-#pragma unroll
-  for (int o = 1; o < L; o <<= 1) before += __shfl_xor(before, o, 64);
+  before = sum_of<L>(before);
   if (e < E && (int)threadIdx.x % L == 0) order[before] = e;
 }
 __device__ __forceinline__ int filled_up(int c, int align) { return (c + align - 1) & -align; }
@@ -856,16 +866,19 @@ extern "C" int anc_id_groups_device(uint64_t ids, int32_t ids_bytes, int64_t n, 
     return ANC_OK;
   }
   if (n <= kMostAlone) {
-    if (wide) hipLaunchKernelGGL((k_group_part<1024, false, int64_t>), dim3(1), dim3(1024), 0, s, (const int64_t *)ids, (int)n, M, (uint32_t)V, o);
-    else      hipLaunchKernelGGL((k_group_part<1024, false, int32_t>), dim3(1), dim3(1024), 0, s, (const int32_t *)ids, (int)n, M, (uint32_t)V, o);
+    if (wide) hipLaunchKernelGGL((k_group_part<512, false, int64_t>), dim3(1), dim3(512), 0, s, (const int64_t *)ids, (int)n, M, (uint32_t)V, o);
+    else      hipLaunchKernelGGL((k_group_part<512, false, int32_t>), dim3(1), dim3(512), 0, s, (const int32_t *)ids, (int)n, M, (uint32_t)V, o);
     ANC_LAUNCH_CHECK();
     return ANC_OK;
   }
   if (one_launch(n, V)) {
-    const int64_t parts = (n + 63) / 64;
-    const dim3 grid((unsigned)(parts < 128 ? parts : 128)), lanes(1024);
-    if (wide) hipLaunchKernelGGL((k_group_part<1024, true, int64_t>), grid, lanes, 0, s, (const int64_t *)ids, (int)n, M, (uint32_t)V, o);
-    else      hipLaunchKernelGGL((k_group_part<1024, true, int32_t>), grid, lanes, 0, s, (const int32_t *)ids, (int)n, M, (uint32_t)V, o);
+    const int64_t parts = (n + 31) / 32;
+    const dim3 grid((unsigned)(parts < 128 ? parts : 128));
+    const bool few = n <= kFewSplit;
+    auto kernel = few ? k_group_part<512, true, int64_t> : k_group_part<1024, true, int64_t>;
+    auto narrow = few ? k_group_part<512, true, int32_t> : k_group_part<1024, true, int32_t>;
+    if (wide) hipLaunchKernelGGL(kernel, grid, dim3(few ? 512 : 1024), 0, s, (const int64_t *)ids, (int)n, M, (uint32_t)V, o);
+    else      hipLaunchKernelGGL(narrow, grid, dim3(few ? 512 : 1024), 0, s, (const int32_t *)ids, (int)n, M, (uint32_t)V, o);
     ANC_LAUNCH_CHECK();
     return ANC_OK;
   }
