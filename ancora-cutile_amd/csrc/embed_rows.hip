@@ -41,7 +41,7 @@ k_embed_lookup(const void *__restrict__ ids, int wide, uint32_t total, int64_t V
   }
 }
 
-// The gradient walks the sorted positions in chunks: a workgroup of kSubs teams, each of which adds up the rows of dy of `sub` (at most 64)
+// The gradient walks the sorted positions in chunks: a workgroup of SUBS teams, each of which adds up the rows of dy of `sub` (at most 64)
 // positions one after the other. A group that lies inside a team's positions is finished there. Of one that reaches over an edge the team
 // leaves a row in LDS, of the group that comes in (head) and of the one that begins and goes out (tail), and the teams put
 // together what meets inside the chunk. What reaches over the chunk's edges goes to memory the same way, part 0 of the group that comes in and
@@ -50,11 +50,11 @@ k_embed_lookup(const void *__restrict__ ids, int wide, uint32_t total, int64_t V
 struct EmbedDw {
   const int32_t *srt, *start, *cnt, *key, *grp;
   int64_t n, V, H, pitch;                            // pitch: between rows of part, whole pieces
-  int sub, chunk;                                    // chunk = kSubs * sub positions
+  int sub, chunk;                                    // positions of a team, of a workgroup
   float scale;
   float *out, *compact, *part;
 };
-constexpr int kSubs = 4;
+constexpr int kSubs = 4, kFewSubs = 16;              // teams; of the one workgroup that few positions make
 constexpr int kDwLanes = 256;                        // most lanes of a team, and of the join
 
 template <int VEC, bool TAIL, bool DENSE>
@@ -67,11 +67,11 @@ __device__ __forceinline__ void put_row(const EmbedDw &p, int64_t row, const Pie
   store<ANC_F32, VEC, TAIL, false, DENSE>(to, narrow<ANC_F32, VEC>(x), c);
 }
 
-template <int TD, bool TAIL, bool DENSE, bool ONCE>
+template <int TD, bool TAIL, bool DENSE, bool ONCE, int SUBS>
 __global__ void __launch_bounds__(kDwLanes * kSubs) k_embed_dw(EmbedDw p, const elem_t<TD> *__restrict__ dy) {
   constexpr int VEC = piece_of<TD, TD>;
-  extern __shared__ __attribute__((aligned(16))) float edge[];                    // [kSubs][head, tail][lanes * VEC]
-  __shared__ int flags[kSubs];                       // 1: a head, 2: its group goes out again, 4: a tail
+  extern __shared__ __attribute__((aligned(16))) float edge[];                    // [SUBS][head, tail][lanes * VEC]
+  __shared__ int flags[SUBS];                       // 1: a head, 2: its group goes out again, 4: a tail
   const int lane = (int)(threadIdx.x & 63), team = __builtin_amdgcn_readfirstlane((int)threadIdx.y);
   const int64_t p0 = (int64_t)blockIdx.x * p.chunk + (int64_t)team * p.sub, here = p0 + lane;
   const bool in = lane < p.sub && here < p.n;
@@ -144,19 +144,19 @@ __global__ void __launch_bounds__(kDwLanes * kSubs) k_embed_dw(EmbedDw p, const 
   if (state & 4) {                                   // what begins here and goes on
     widen<ANC_F32, VEC>(*(const Raw<ANC_F32, VEC> *)tail, acc);
     int t = team + 1;
-    for (; t < kSubs; ++t) {
+    for (; t < SUBS; ++t) {
       add_head(t);
       if (!(flags[t] & 2)) break;
     }
     if (live) {
-      if (t < kSubs) put_row<VEC, TAIL, DENSE>(p, DENSE ? (int64_t)tail_key : (int64_t)tail_grp, c, acc);
+      if (t < SUBS) put_row<VEC, TAIL, DENSE>(p, DENSE ? (int64_t)tail_key : (int64_t)tail_grp, c, acc);
       else store<ANC_F32, VEC, TAIL>(p.part + ((int64_t)blockIdx.x * 2 + 1) * p.pitch, narrow<ANC_F32, VEC>(acc), c);
     }
   }
   if (team == 0 && (state & 1)) {                    // what came into the chunk
 #pragma unroll
     for (int k = 0; k < VEC; ++k) acc[k] = 0.0f;
-    for (int t = 0; t < kSubs; ++t) {
+    for (int t = 0; t < SUBS; ++t) {
       add_head(t);
       if (!(flags[t] & 2)) break;
     }
@@ -221,9 +221,12 @@ __global__ void __launch_bounds__(kDwLanes) k_embed_dw_join(EmbedDw p) {
   store<ANC_F32, VEC, TAIL, false, true>(to, narrow<ANC_F32, VEC>(x), pc);
 }
 
-// Positions per team: enough chunks to fill the card.
-constexpr int64_t kSub8Most = 8192, kSub16Most = 32768;
-int dw_chunk(int64_t n) { return kSubs * (n <= kSub8Most ? 8 : n <= kSub16Most ? 16 : 64); }
+// Positions per team: enough chunks to fill the card (8192 positions of 16 or of 8: 28.1 and 27.1 us with the grouping; 65536 of 32 or of 64: 91 and 87).
+// Up to kFewMost all are one workgroup's, for 64 pieces of the rows each, and nothing is left to join (77 rows into a dense gradient 6.7 us, by
+// the join 8.8; 128 rows 9.1 and 8.9, into compact rows 7.1 and 8.8; 200 rows, 16 to a team, 12.2 and 9.0).
+constexpr int64_t kFewMost = kFewSubs * 8, kSub8Most = 8192, kSub16Most = 32768;
+int dw_sub(int64_t n) { return n <= kFewSubs * 4 ? 4 : n <= kSub8Most ? 8 : n <= kSub16Most ? 16 : 64; }
+int dw_chunk(int64_t n) { return (n <= kFewMost ? kFewSubs : kSubs) * dw_sub(n); }
 int64_t dw_chunks(int64_t n) { return (n + dw_chunk(n) - 1) / dw_chunk(n); }
 int64_t dw_pitch(int64_t H) { return (H + 7) / 8 * 8; }
 constexpr int64_t kMostPositions = 1ll << 20;
@@ -302,18 +305,21 @@ extern "C" int anc_embed_dw(uint64_t srt, uint64_t start, uint64_t cnt, uint64_t
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_MISC, s);
   const EmbedDw p{(const int32_t *)srt, (const int32_t *)start, (const int32_t *)cnt, (const int32_t *)key, (const int32_t *)grp,
-                  n, V, H, dw_pitch(H), dw_chunk(n) / kSubs, dw_chunk(n), scale, (float *)out, (float *)compact, (float *)workspace};
+                  n, V, H, dw_pitch(H), dw_sub(n), dw_chunk(n), scale, (float *)out, (float *)compact, (float *)workspace};
   const bool once = n * H * elem_size(dy_type) > kCached;
   with_type(dy_type, [&](auto t) {
     with_flag(H % piece_of<decltype(t)::value, decltype(t)::value> != 0, [&](auto tail) {
       constexpr int T = decltype(t)::value, VEC = piece_of<T, T>;
       constexpr bool TAIL = decltype(tail)::value != 0;
-      // (a team is at most 1024 columns wide: 32 KiB of LDS for the edges)
-      const int64_t waves = (H + 64 * VEC - 1) / (64 * VEC), widest = 1024 / (64 * VEC), wide = waves < widest ? waves : widest;
-      auto kernel = out != 0 ? (once ? k_embed_dw<T, TAIL, true, true> : k_embed_dw<T, TAIL, true, false>)
-                             : (once ? k_embed_dw<T, TAIL, false, true> : k_embed_dw<T, TAIL, false, false>);
-      hipLaunchKernelGGL(kernel, dim3((unsigned)chunks, (unsigned)((waves + wide - 1) / wide)), dim3((unsigned)(64 * wide), kSubs),
-                         (unsigned)(kSubs * 2 * 64 * wide * VEC * sizeof(float)), s, p, (const elem_t<T> *)dy);
+      // (a team is at most 1024 columns wide: 32 KiB of LDS for the edges; one of few positions has one wavefront: 64 KiB)
+      const bool few = n <= kFewMost;
+      const int64_t waves = (H + 64 * VEC - 1) / (64 * VEC), widest = few ? 1 : 1024 / (64 * VEC), wide = waves < widest ? waves : widest;
+      const int subs = few ? kFewSubs : kSubs;
+      auto kernel = few ? (out != 0 ? k_embed_dw<T, TAIL, true, false, kFewSubs> : k_embed_dw<T, TAIL, false, false, kFewSubs>)
+                    : out != 0 ? (once ? k_embed_dw<T, TAIL, true, true, kSubs> : k_embed_dw<T, TAIL, true, false, kSubs>)
+                               : (once ? k_embed_dw<T, TAIL, false, true, kSubs> : k_embed_dw<T, TAIL, false, false, kSubs>);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)chunks, (unsigned)((waves + wide - 1) / wide)), dim3((unsigned)(64 * wide), subs),
+                         (unsigned)(subs * 2 * 64 * wide * VEC * sizeof(float)), s, p, (const elem_t<T> *)dy);
     });
   });
   if (chunks > 1)

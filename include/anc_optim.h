@@ -341,7 +341,7 @@ int anc_id_groups_device(uint64_t ids, int32_t ids_bytes, int64_t n, int64_t M, 
  *   out != 0:     out[id] += scale * sum of the id's rows, out (V, H) fp32; rows that no id names are not touched
  *   compact != 0: compact[g] = scale * that sum, (n, H) fp32; rows behind the last group are left as they were (V as when the ids were
  *                 grouped)
- * Rows are added in fp32 in sorted order within runs of 8, 16 or 64 positions (by n), the runs in a fixed order: the same
+ * Rows are added in fp32 in sorted order within runs of 4, 8, 16 or 64 positions (by n), the runs in a fixed order: the same
  * bits on every run, a function of n, the ids and dy. One id may hold most of the batch at no loss of speed (a group of
  * anc_embed_dw_scatter, whose bits are the sequential sum's, is one workgroup's). */
 int64_t anc_embed_dw_workspace_bytes(int64_t M, int64_t H);        /* enough for every n <= M */

@@ -397,3 +397,14 @@ def test_device_groups_feed_the_sequential_scatter_and_the_row_sparse_step(gpu):
         assert bits_equal(a.to_numpy(), b.to_numpy())
     for b in (dev, *rows, *opts):
         b.free()
+
+
+@pytest.mark.parametrize("M,V,H,kind", [(63, 5, 520, "bf16"), (64, 900, 257, "f32"), (65, 12, 1003, "bf16"), (127, 40, 24, "f32"), (128, 3, 2050, "bf16"),
+                                        (129, 3, 520, "bf16")])
+def test_gradient_of_few_positions(gpu, M, V, H, kind):
+    """Up to 128 positions one workgroup holds all of them, 4 or 8 to a wavefront, and no second kernel joins anything."""
+    test_gradient_against_64_bits(gpu, M, V, H, kind)
+
+
+def test_few_positions_captured_and_replayed(gpu):
+    test_captured_and_replayed_on_new_ids(gpu, 100)
