@@ -620,8 +620,8 @@ struct Route {
   int32_t *counts, *offsets, *order, *slot, *src;
 };
 // The experts by falling number of tokens, lower ones first where equal: an expert's place is the number of experts before it, found
-// by looking at all of them (LANES / E lanes share the looking). Beyond kMostOrdered that would take longer than it gives: many
-// short segments even out in any order.
+// by looking at all of them (LANES / kMostOrdered lanes share the looking; behind the last expert scnt holds -1 up to a multiple of 4).
+// Beyond kMostOrdered that would take longer than it gives: many short segments even out in any order.
 constexpr int kMostOrdered = 256;
 template <int LANES>
 __device__ __forceinline__ void order_experts(const int *scnt, int E, int32_t *order) {
@@ -633,36 +633,33 @@ __device__ __forceinline__ void order_experts(const int *scnt, int E, int32_t *o
   const int e = (int)threadIdx.x / L;
   const int mine = e < E ? scnt[e] : 0;
   int before = 0;
-  for (int j = (int)threadIdx.x % L; j < E; j += L) {
-    const int c = scnt[j];
-    before += c > mine || (c == mine && j < e) ? 1 : 0;
+  for (int j = (int)threadIdx.x % L * 4; j < E; j += L * 4) {
+    const anc_i32x4 c = *(const anc_i32x4 *)(scnt + j);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) before += c[q] > mine || (c[q] == mine && j + q < e) ? 1 : 0;
   }
   before = sum_of<L>(before);
   if (e < E && (int)threadIdx.x % L == 0) order[before] = e;
 }
 __device__ __forceinline__ int filled_up(int c, int align) { return (c + align - 1) & -align; }
 
-// Up to kMostCounted assignments in one launch: every workgroup counts all of them per expert, and those before its own kBlock, as the two
+// Up to kMostCounted assignments in one launch: every workgroup counts all of them per expert, and those before its own, one to a lane, as the two
 // halves of a word; four copies of the counters keep the lanes that meet on one apart.
-// (16384 to 16 experts 7.5 us, counted and placed in two launches 9.9; 32768 9.6 and 10.0, to 128 experts 11.6 and 13.4)
-constexpr int kMostCounted = 1 << 15, kOneLanes = 1024, kOneItems = kBlock / kOneLanes, kCopies = 4;
+// (16384 to 16 experts 6.3 us, two to a lane 7.0, counted and placed in two launches 9.9; 32768 8.5, 9.3 and 10.0)
+constexpr int kMostCounted = 1 << 15, kOneLanes = 1024, kCopies = 4;
 __global__ void __launch_bounds__(kOneLanes)
 k_route_one(const void *__restrict__ ids, int wide, int n, int E, int bits, int align, int capacity, Route o) {
   constexpr int W = kOneLanes / 64;
   __shared__ int count[W * kMostExperts];
   __shared__ uint32_t hist[kCopies * kMostExperts];
   __shared__ int tmp[W];
-  __shared__ int soff[kMostExperts + 1], scnt[kMostExperts];
+  __shared__ int soff[kMostExperts + 1];
+  __shared__ __attribute__((aligned(16))) int scnt[kMostExperts];
   const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63, blocks = (int)gridDim.x, b = (int)blockIdx.x;
-  const int first = b * kBlock + wave * (64 * kOneItems) + lane;
-  uint32_t e[kOneItems];                             // E: no expert
-  int rank[kOneItems];
-  if (n > 0) {
-    load_keys<kOneItems>(ids, wide, first, 64, n, (uint32_t)E, e);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kOneItems; ++j) e[j] = (uint32_t)E;
-  }
+  const int p = b * kOneLanes + tid;
+  uint32_t own[1] = {(uint32_t)E};                   // E: no expert
+  if (n > 0) load_keys<1>(ids, wide, p, 0, n, (uint32_t)E, own);
+  const uint32_t e = own[0];
   for (int i = tid; i < W * E; i += kOneLanes) count[i] = 0;
   for (int i = tid; i < kCopies * E; i += kOneLanes) hist[i] = 0;
   __syncthreads();
@@ -672,10 +669,9 @@ k_route_one(const void *__restrict__ ids, int wide, int n, int E, int bits, int 
     load_keys<D>(ids, wide, t, kOneLanes, n, (uint32_t)E, k);
 #pragma unroll
     for (int j = 0; j < D; ++j)
-      if (k[j] < (uint32_t)E) atomicAdd(&hist[k[j] * kCopies + (lane & (kCopies - 1))], t + j * kOneLanes < b * kBlock ? 0x10001u : 1u);
+      if (k[j] < (uint32_t)E) atomicAdd(&hist[k[j] * kCopies + (lane & (kCopies - 1))], t + j * kOneLanes < b * kOneLanes ? 0x10001u : 1u);
   }
-#pragma unroll
-  for (int j = 0; j < kOneItems; ++j) rank[j] = take_rank(count + wave * E, e[j], bits, e[j] < (uint32_t)E);
+  const int rank = take_rank(count + wave * E, e, bits, e < (uint32_t)E);
   __syncthreads();
   int all = 0, below = 0, c[W], total;
 #pragma unroll
@@ -702,17 +698,16 @@ k_route_one(const void *__restrict__ ids, int wide, int n, int E, int bits, int 
     soff[tid] = base;
     scnt[tid] = all;
     if (b == 0) { o.counts[tid] = all; o.offsets[tid] = base; }
+  } else if (tid < kMostExperts) {
+    scnt[tid] = -1;
   }
   if (tid == 0) {
     soff[E] = total;
     if (b == 0) o.offsets[E] = total;
   }
   __syncthreads();
-#pragma unroll
-  for (int j = 0; j < kOneItems; ++j) {
-    const int p = first + 64 * j;
-    if (p >= n) continue;
-    const int s = e[j] < (uint32_t)E ? count[wave * E + e[j]] + rank[j] : -1;
+  if (p < n) {
+    const int s = e < (uint32_t)E ? count[wave * E + e] + rank : -1;
     o.slot[p] = s;
     if (s >= 0) o.src[s] = p;
   }
@@ -742,7 +737,8 @@ k_route_place(const void *__restrict__ ids, int wide, int64_t n, int E, int bits
   constexpr int W = kBlockLanes / 64, PER = kMostExperts / kBlockLanes;
   __shared__ int count[W * kMostExperts];
   __shared__ int tmp[W];
-  __shared__ int soff[kMostExperts + 1], scnt[kMostExperts], sall[kMostExperts], sbelow[kMostExperts];
+  __shared__ int soff[kMostExperts + 1], sall[kMostExperts], sbelow[kMostExperts];
+  __shared__ __attribute__((aligned(16))) int scnt[kMostExperts];
   const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63, blocks = (int)gridDim.x, b = (int)blockIdx.x;
   const int64_t first = (int64_t)b * kBlock + wave * (64 * kBlockItems) + lane;
   uint32_t e[kBlockItems];
@@ -798,6 +794,8 @@ k_route_place(const void *__restrict__ ids, int wide, int64_t n, int E, int bits
         count[w * E + d] = at;
         at += c;
       }
+    } else if (d < kMostExperts) {
+      scnt[d] = -1;
     }
     base += filled_up(all[q], align);
   }
@@ -941,7 +939,7 @@ extern "C" int anc_route(uint64_t expert_ids, int32_t ids_bytes, int64_t n, int6
   const Route o{(int32_t *)counts, (int32_t *)offsets, (int32_t *)order, (int32_t *)slot, (int32_t *)src};
   const int E = (int)experts, bits = bits_of((uint32_t)E - 1), wide = ids_bytes == 8;
   if (n <= kMostCounted) {
-    hipLaunchKernelGGL(k_route_one, dim3((unsigned)(n > 0 ? n_blocks(n) : 1)), dim3(kOneLanes), 0, s, (const void *)expert_ids, wide, (int)n, E,
+    hipLaunchKernelGGL(k_route_one, dim3((unsigned)(n > 0 ? (n + kOneLanes - 1) / kOneLanes : 1)), dim3(kOneLanes), 0, s, (const void *)expert_ids, wide, (int)n, E,
                        bits, (int)align, (int)capacity, o);
   } else {
     const dim3 grid((unsigned)n_blocks(n)), lanes(kBlockLanes);
