@@ -232,8 +232,10 @@ class DeviceIdGroups:
 
         groups = DeviceIdGroups(M, V)
         groups.group(ids, si)                              # every step
+        opt.catch_up(groups, si)                           # RowSparseAdamW: the rows that the forward looks up
+        embed_lookup(ids, opt.p16, si, x)
         embed_dw(groups, dy, si, compact=rows)             # or out=dE
-        opt.step(groups.gid, groups.M, rows, si)           # RowSparseAdamW: M rows, those behind the last group left out
+        opt.step(groups.gid, groups.M, rows, si)           # M rows, those behind the last group left out
 
     The arrays and the gradient's partial rows are one set of buffers: calls on different streams (or replays of graphs)
     that use one object are put in order by the caller; work that overlaps takes an object each."""
@@ -393,7 +395,15 @@ class RowSparseAdamW:
                            float(self.wd), self.tensor_seed, int(ctl), int(si))
 
     def catch_up(self, row_ids, si):
-        """Replay, on the distinct rows in `row_ids` (host integers), the steps they missed."""
+        """Replay, on the distinct rows in `row_ids` (host integers, or a `DeviceIdGroups` of ids on the device, grouped on
+        the same stream), the steps they missed."""
+        if isinstance(row_ids, DeviceIdGroups):
+            row_ids._used("RowSparseAdamW.catch_up")
+            if row_ids.V != self.V:
+                raise ValueError(f"RowSparseAdamW.catch_up: ids of {row_ids.V} rows, the table has {self.V}")
+            if self.t and row_ids.n:                 # (entries behind the last group name no row)
+                self._launch(row_ids.gid.ptr, row_ids.n, 0, self.t, 0, si)
+            return
         if self.t == 0:
             return
         ids = _ids32(row_ids)

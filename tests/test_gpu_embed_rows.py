@@ -408,3 +408,37 @@ def test_gradient_of_few_positions(gpu, M, V, H, kind):
 
 def test_few_positions_captured_and_replayed(gpu):
     test_captured_and_replayed_on_new_ids(gpu, 100)
+
+
+def test_row_sparse_training_without_the_host_seeing_an_id(gpu):
+    """Group, catch up, look up, gradient, step, all from ids on the device: rows looked up and final state have the bits of a run whose ids
+    are known to the host."""
+    from ancora_cutile_amd import DevBuf, DeviceIdGroups, embed_dw, embed_lookup
+    from ancora_cutile_amd.embed import RowSparseAdamW
+    M, V, H = 300, 500, 64
+    rng = np.random.default_rng(12)
+    W0 = (0.02 * rng.standard_normal((V, H))).astype(np.float32)
+    known, opt = (RowSparseAdamW(W0, lr=1e-2, wd=0.1, sr=True, seed=5) for _ in range(2))
+    groups, x, rows = DeviceIdGroups(M, V), [DevBuf.zeros((M, H), np.float32) for _ in range(2)], DevBuf.zeros((M, H), np.float32)
+    for step, n in enumerate((M, 1, 0, 200, M)):
+        ids = np.where(rng.random(M) < 0.1, -1, V * rng.random(M) ** 2).astype(np.int64)
+        host, _ = _rows(rng, (M, H), "f32", 1e-2)
+        buf, dy = DevBuf(ids), DevBuf(host)
+        groups.group(buf, 0, n)
+        opt.catch_up(groups, 0)
+        if (ids[:n] >= 0).any():
+            known.catch_up(ids[:n][ids[:n] >= 0], 0)
+        for o, out in ((known, x[0]), (opt, x[1])):
+            embed_lookup(buf, o.p32, 0, out, n=n)
+        assert bits_equal(x[0].to_numpy(), x[1].to_numpy()), step
+        embed_dw(groups, dy, 0, compact=rows)
+        g = int(groups.count.to_numpy()[0])
+        known.step(groups.gid, g, rows, 0)
+        opt.step(groups.gid, groups.M, rows, 0)
+        buf.free(); dy.free()
+    for o in (known, opt):
+        o.flush(0)
+    for a, b in ((known.p32, opt.p32), (known.m, opt.m), (known.v, opt.v), (known.p16, opt.p16), (known.last, opt.last)):
+        assert bits_equal(a.to_numpy(), b.to_numpy())
+    for b in (groups, rows, *x, known, opt):
+        b.free()

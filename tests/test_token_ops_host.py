@@ -262,3 +262,26 @@ def test_outputs_that_overlap_are_refused(lib):
                ({}, dict(dW=a[2] + weight - 16)), (dict(g16=a[3]), dict(dW=a[3])), (dict(g16=a[3]), dict(dW=a[4], g16=a[3])), ({}, dict(dW=a[3], x=a[2])),
                (dict(x=a[4]), dict(dW=a[4])), (dict(dy=a[4]), dict(dW=a[3], g16=a[4]))):
         assert call(*ps) == 2 and "overlaps" in lib.anc_last_error().decode(), (ps, lib.anc_last_error())
+
+
+def test_catch_up_from_groups_on_the_device(fake_device):
+    from ancora_cutile_amd import DeviceIdGroups
+    from ancora_cutile_amd._lib import AncoraError
+    from ancora_cutile_amd.embed import RowSparseAdamW
+    opt = RowSparseAdamW(np.zeros((40, 64), np.float32))
+    g, other = DeviceIdGroups(30, 40), DeviceIdGroups(30, 41)
+    with pytest.raises(AncoraError, match="no ids were grouped"):
+        opt.catch_up(g, 0)
+    g.group(_buf((30,), np.int32), 0, 20)
+    other.group(_buf((30,), np.int32), 0)
+    with pytest.raises(ValueError):
+        opt.catch_up(other, 0)
+    opt.catch_up(g, 0)                                                # no step yet: nothing was missed
+    assert not fake_device.calls("anc_adamw_rows")
+    opt.t = 3
+    opt.catch_up(g, 0)
+    (call,) = fake_device.calls("anc_adamw_rows")
+    assert call[0] == g.gid.ptr and call[1] == 20 and call[2] == 0
+    g.group(_buf((30,), np.int32), 0, 0)
+    opt.catch_up(g, 0)
+    assert len(fake_device.calls("anc_adamw_rows")) == 1
