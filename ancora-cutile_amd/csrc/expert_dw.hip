@@ -251,8 +251,11 @@ extern "C" int anc_expert_dw_multi(const anc_expert_dw_problem_t *probs, int32_t
         for (int c = 0; c < 4; ++c)
           ANC_REQUIRE((i == j && a == c) || anc_apart(span[i][a].at, span[i][a].bytes, span[j][c].at, span[j][c].bytes),
                       "anc_expert_dw_multi: an output of problem %d overlaps a buffer of problem %d", i, j);
-  // 256x256 tiles where they give every CU one; fewer, and twice as many of 128x256 are at work.
-  const int TM = wide >= 256 ? 256 : 128;
+  // 256x256 tiles where they give every CU one and segments are long (256 rows on average, by the room for them): fewer operand bytes for a
+  // product. With fewer tiles twice as many of 128x256 are at work; with short segments the two workgroups of a CU hide each other's ends.
+  // 16 experts, three weights of 1024x1024 with bf16 copies, from HBM, 256x256 and 128x256: 1024 rows each 142 and 152 us, 512 104 and 113, 256
+  // 76 and 72, 128 66 and 62; 64 experts, 512x1024, 256 rows 169 and 181; 8 experts, one weight of 512x512, 512 rows 19.0 and 14.5.
+  const int TM = wide >= 256 && capacity >= 256 * experts ? 256 : 128;
   for (int i = 0; i < n_probs; ++i) m.p[i].tiles = (m.p[i].K + TM - 1) / TM * m.p[i].tn;
   // The tiles that stay together: a whole weight of 16 or 32 tiles, fewer where that leaves an XCD less than six units to even out.
   for (m.unit = 32;; m.unit /= 2) {

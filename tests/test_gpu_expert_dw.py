@@ -164,3 +164,9 @@ def test_captured_and_replayed_on_new_segments(gpu):
     for b in (*plans, e, gx, gdy, *outs):
         b.free()
     gpu.api.anc_stream_destroy(s)
+
+
+@pytest.mark.parametrize("counts,align", [((1100, 1, 0, 31), 1), ((33, 700, 0, 320), 64)])
+def test_large_ragged_weights_with_long_and_short_segments(gpu, counts, align):
+    """Enough outputs and long enough segments for the widest tiles, which reach over the weight's edges here."""
+    test_against_64_bits(gpu, 2296, 2056, counts, align)
