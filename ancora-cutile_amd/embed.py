@@ -170,8 +170,16 @@ class IdGroups:
 
 def embed_dw_scatter(groups, dy, si, out=None, compact=None, V=None):
     """dy: (M, H) bf16 DevBuf. out: (V, H) fp32 DevBuf, added onto in place (the reference's
-    launch); or compact: (M, H) fp32 DevBuf that receives one summed row per group."""
+    launch); or compact: (M, H) fp32 DevBuf that receives one summed row per group. Over a `DeviceIdGroups` dy and
+    compact hold at least the rows that were grouped, and at most (dy) those there is room for."""
     M, H = dy.shape
+    if M > groups.M:                                       # (a group per row of dy is launched)
+        raise ValueError(f"embed_dw_scatter: dy has {M} rows, the groups have room for {groups.M}")
+    if isinstance(groups, DeviceIdGroups):
+        groups._used("embed_dw_scatter")
+        groups._fits("embed_dw_scatter", dy, out, compact)
+        if dy.dtype != np.uint16:
+            raise ValueError(f"embed_dw_scatter: dy is {dy.dtype}, bf16 bits (uint16) expected")
     if out is not None:
         V = out.shape[0] if V is None else V
     base, step = groups.base_on(si), 4 * groups.M          # srt, start, cnt, gid
@@ -277,6 +285,19 @@ class DeviceIdGroups:
         api.anc_id_groups_device(ids.ptr, nbytes, n, self.M, self.V, *self._at, int(si))
         self.n = n
 
+    def _fits(self, who, dy, out, compact):
+        """dy and the gradient belong to the ids of the last `group`."""
+        if (out is None) == (compact is None):
+            raise ValueError(f"{who}: one of out and compact")
+        H = dy.shape[-1]
+        _rows_of(dy, self.n, H, who, "dy")
+        target = out if compact is None else compact
+        if target.dtype != np.float32:
+            raise ValueError(f"{who}: the gradient is float32, got {target.dtype}")
+        if compact is None and tuple(out.shape) != (self.V, H):
+            raise ValueError(f"{who}: out is {out.shape}, ({self.V}, {H}) expected")
+        _rows_of(target, 0 if compact is None else self.n, H, who, "compact")
+
     def _part(self, H, si):
         nbytes = api.anc_embed_dw_workspace_bytes(self.M, H)
         for b in self._parts:
@@ -299,16 +320,8 @@ def embed_dw(groups, dy, si, out=None, compact=None, scale=1.0):
     out: (V, H) fp32, added onto in place, or compact: (>= n, H) fp32 that receives one summed row per group (rows
     behind the last group are left as they were). Sums are fp32 in a fixed order: the same bits on every run."""
     groups._used("embed_dw")
-    if (out is None) == (compact is None):
-        raise ValueError("embed_dw: one of out and compact")
+    groups._fits("embed_dw", dy, out, compact)
     H = dy.shape[-1]
-    _rows_of(dy, groups.n, H, "embed_dw", "dy")
-    target = out if compact is None else compact
-    if target.dtype != np.float32:
-        raise ValueError(f"embed_dw: the gradient is float32, got {target.dtype}")
-    if compact is None and tuple(out.shape) != (groups.V, H):
-        raise ValueError(f"embed_dw: out is {out.shape}, ({groups.V}, {H}) expected")
-    _rows_of(target, 0 if compact is None else groups.n, H, "embed_dw", "compact")
     part = groups._part(H, si)
     srt, start, cnt, _, key, grp = groups._at[:6]
     api.anc_embed_dw(srt, start, cnt, key, grp, groups.n, dy.ptr, _type(dy, "embed_dw"), H, float(scale),
