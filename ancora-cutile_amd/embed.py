@@ -337,7 +337,8 @@ class RowSparseAdamW:
         opt.flush(si)                      # every row current (before a checkpoint / evaluation)
 
     State after `flush` equals the dense `AdamW` run on gradients that are zero outside the touched
-    rows, bit for bit (stochastic rounding included). `lr` may change between steps."""
+    rows, bit for bit (stochastic rounding included). `lr` may change between steps. Steps are counted on the host:
+    `catch_up`, `step` and `flush` refuse a stream that is being captured into a graph."""
 
     def __init__(self, W, lr=3e-4, betas=(0.9, 0.95), eps=1e-8, wd=0.01, form="div", sr=False, seed=0,
                  tensor_seed=0, max_steps=1 << 16):
@@ -360,6 +361,10 @@ class RowSparseAdamW:
         self.last_skipped = False
         self._filled_to = 0          # table entries 1 .. _filled_to hold the scalars of their steps
         self._filled_lr = None       # ... computed with this learning rate
+
+    def _not_captured(self, who, si):
+        if _lib.stream_is_capturing(si):             # (the number of the step is the launch's: a replay would be the same step)
+            raise _lib.AncoraError(f"RowSparseAdamW.{who}: a step cannot be captured into a graph")
 
     def _hyper(self):
         return AdamWHyper(beta1=self.b1, beta2=self.b2, omb1=1 - self.b1, omb2=1 - self.b2, eps=self.eps,
@@ -410,6 +415,7 @@ class RowSparseAdamW:
     def catch_up(self, row_ids, si):
         """Replay, on the distinct rows in `row_ids` (host integers, or a `DeviceIdGroups` of ids on the device, grouped on
         the same stream), the steps they missed."""
+        self._not_captured("catch_up", si)
         if isinstance(row_ids, DeviceIdGroups):
             row_ids._used("RowSparseAdamW.catch_up")
             if row_ids.V != self.V:
@@ -428,6 +434,7 @@ class RowSparseAdamW:
     def step(self, gid, n_groups, grads, si, guard=None):
         """gid: device int32 array of distinct row ids (e.g. `IdGroups.gid`), the first n_groups
         valid; grads: (>= n_groups, H) fp32 DevBuf, row i the gradient of gid[i]."""
+        self._not_captured("step", si)
         if self.t + 1 > self._cap:             # before the counter moves: t always matches the table
             raise RuntimeError(f"RowSparseAdamW: step table holds {self._cap} steps; raise max_steps")
         self._ensure_step(self.t + 1, si)
@@ -443,6 +450,7 @@ class RowSparseAdamW:
 
     def flush(self, si):
         """Bring every row up to date."""
+        self._not_captured("flush", si)
         if self.t:
             self._launch(0, self.V, 0, self.t, 0, si)
 

@@ -39,3 +39,28 @@ def test_sequential_scatter_takes_the_rows_its_groups_have_room_for(fake_device)
     embed_dw_scatter(host, _buf((M - 1, H), u16), 0, out=out, V=V)
     calls = fake_device.calls("anc_embed_dw_scatter")
     assert [c[7] for c in calls] == [M, M, M, M, 20, M - 1] and calls[0][0] == g.cnt.ptr and calls[0][2] == g.gid.ptr
+
+
+def test_a_row_sparse_step_is_not_captured(fake_device):
+    """A launch carries the step's number, and replays would carry it again: no row it has stepped would move any more. A catch-up before
+    the first step launches nothing, so that its graph would never replay a step."""
+    from ancora_cutile_amd import DeviceIdGroups
+    from ancora_cutile_amd._lib import AncoraError
+    from ancora_cutile_amd.embed import IdGroups, RowSparseAdamW
+    V, H, M = 40, 64, 30
+    opt, g = RowSparseAdamW(np.zeros((V, H), np.float32)), DeviceIdGroups(M, V)
+    host, rows = IdGroups(np.arange(M)), _buf((M, H), np.float32)
+    g.group(_buf((M,), np.int32), 0)
+    fake_device.capturing = {7}
+    calls = (lambda: opt.catch_up(g, 7), lambda: opt.catch_up(np.arange(M), 7), lambda: opt.step(g.gid, M, rows, 7),
+             lambda: opt.step(host.gid, M, rows, 7), lambda: opt.step(g.gid, 0, rows, 7), lambda: opt.flush(7))
+    for t in (0, 1):
+        before = len(fake_device.log)
+        for call in calls:
+            with pytest.raises(AncoraError, match="captured"):
+                call()
+        assert opt.t == t and {n for n, _ in fake_device.log[before:]} == {"anc_stream_is_capturing"}
+        opt.catch_up(g, 0)                                       # another stream than the captured one
+        opt.step(g.gid, M, rows, 0)
+    opt.flush(0)
+    assert opt.t == 2
