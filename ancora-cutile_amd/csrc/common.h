@@ -25,7 +25,15 @@ int anc_hip_fail(hipError_t e, const char *what, const char *file, int line);
 
 // Two buffers have no byte in common.
 static inline bool anc_apart(uint64_t a, int64_t a_bytes, uint64_t b, int64_t b_bytes) {
-  return a + (uint64_t)a_bytes <= b || b + (uint64_t)b_bytes <= a;
+  return a_bytes == 0 || b_bytes == 0 || a + (uint64_t)a_bytes <= b || b + (uint64_t)b_bytes <= a;
+}
+// The first `outputs` of `n` buffers have no byte in common with another one of them.
+struct AncSpan { uint64_t at; int64_t bytes; };
+template <int N> static inline bool anc_outputs_apart(const AncSpan (&s)[N], int outputs) {
+  for (int i = 0; i < outputs; ++i)
+    for (int j = i + 1; j < N; ++j)
+      if (!anc_apart(s[i].at, s[i].bytes, s[j].at, s[j].bytes)) return false;
+  return true;
 }
 
 static inline hipStream_t anc_stream(uint64_t s) { return reinterpret_cast<hipStream_t>(s); }

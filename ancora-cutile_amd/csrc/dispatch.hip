@@ -186,7 +186,9 @@ extern "C" int anc_dispatch(uint64_t slot, uint64_t counts, uint64_t offsets, in
   if (int rc = check_segments("anc_dispatch", counts, offsets, experts, align)) return rc;
   ANC_REQUIRE(type_ok(type), "anc_dispatch: type %d", type);
   ANC_REQUIRE(x && xs && (x | xs) % (uint64_t)elem_size(type) == 0, "anc_dispatch: null or misaligned pointers");
-  ANC_REQUIRE(anc_apart(x, tokens * H * elem_size(type), xs, capacity * H * elem_size(type)), "anc_dispatch: x and xs overlap");
+  ANC_REQUIRE(anc_outputs_apart({{xs, capacity * H * elem_size(type)}, {x, tokens * H * elem_size(type)}, {slot, 4 * tokens * k}, {counts, 4 * experts},
+                                 {offsets, 4 * experts + 4}}, 1),
+              "anc_dispatch: xs overlaps an input");
   const int64_t vec = type == ANC_F32 ? 4 : 8, per_row = pieces_of(H, vec), most = kMostPieces / per_row;
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_MISC, s);
@@ -212,8 +214,8 @@ extern "C" int anc_combine(uint64_t slot, uint64_t weights, int64_t tokens, int6
   ANC_REQUIRE(type_ok(ys_type) && type_ok(y_type), "anc_combine: types %d and %d", ys_type, y_type);
   ANC_REQUIRE(ys && y && ys % (uint64_t)elem_size(ys_type) == 0 && y % (uint64_t)elem_size(y_type) == 0 && (weights & 3) == 0,
               "anc_combine: null or misaligned pointers");
-  ANC_REQUIRE(anc_apart(y, tokens * H * elem_size(y_type), ys, capacity * H * elem_size(ys_type)) &&
-                  anc_apart(y, tokens * H * elem_size(y_type), weights, weights != 0 ? tokens * k * 4 : 0),
+  ANC_REQUIRE(anc_outputs_apart({{y, tokens * H * elem_size(y_type)}, {ys, capacity * H * elem_size(ys_type)}, {weights, weights != 0 ? 4 * tokens * k : 0},
+                                 {slot, 4 * tokens * k}}, 1),
               "anc_combine: y overlaps an input");
   const int64_t vec = ys_type == ANC_F32 || y_type == ANC_F32 ? 4 : 8, per_row = pieces_of(H, vec), most = kMostPieces / per_row;
   hipStream_t s = anc_stream(stream);
@@ -247,9 +249,8 @@ extern "C" int anc_combine_grad(uint64_t slot, uint64_t weights, uint64_t counts
                   (ys | dys) % (uint64_t)elem_size(ys_type) == 0,
               "anc_combine_grad: null or misaligned pointers");
   const int64_t dy_bytes = tokens * H * elem_size(dy_type), ys_bytes = capacity * H * elem_size(ys_type), w_bytes = tokens * k * 4;
-  ANC_REQUIRE(anc_apart(dys, ys_bytes, ys, ys_bytes) && anc_apart(dys, ys_bytes, dy, dy_bytes) && anc_apart(dys, ys_bytes, weights, w_bytes) &&
-                  anc_apart(dw, w_bytes, ys, ys_bytes) && anc_apart(dw, w_bytes, dy, dy_bytes) && anc_apart(dw, w_bytes, weights, w_bytes) &&
-                  anc_apart(dw, w_bytes, dys, ys_bytes),
+  ANC_REQUIRE(anc_outputs_apart({{dys, ys_bytes}, {dw, w_bytes}, {ys, ys_bytes}, {dy, dy_bytes}, {weights, w_bytes}, {slot, w_bytes}, {counts, 4 * experts},
+                                 {offsets, 4 * experts + 4}}, 2),
               "anc_combine_grad: an output overlaps another buffer");
   const int64_t vec = dy_type == ANC_F32 || ys_type == ANC_F32 ? 4 : 8;
   const int64_t blocks = (tokens + kLanes / 64 - 1) / (kLanes / 64), all = blocks + pad_blocks(experts, align);

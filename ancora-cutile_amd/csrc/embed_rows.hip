@@ -302,8 +302,8 @@ extern "C" int anc_embed_dw(uint64_t srt, uint64_t start, uint64_t cnt, uint64_t
   ANC_REQUIRE(workspace_bytes >= need, "anc_embed_dw: workspace holds %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
   const uint64_t to = out != 0 ? out : compact;       // (a compact gradient is n rows at most)
   const int64_t to_bytes = (out != 0 ? V : n) * H * 4, dy_bytes = n * H * elem_size(dy_type);
-  ANC_REQUIRE(anc_apart(to, to_bytes, dy, dy_bytes) && anc_apart(workspace, need, dy, dy_bytes) && anc_apart(workspace, need, to, to_bytes),
-              "anc_embed_dw: dy, the gradient and the workspace overlap");
+  ANC_REQUIRE(anc_outputs_apart({{to, to_bytes}, {workspace, need}, {dy, dy_bytes}, {srt, 4 * n}, {start, 4 * n}, {cnt, 4 * n}, {key, 4 * n}, {grp, 4 * n}}, 2),
+              "anc_embed_dw: the gradient or the workspace overlaps another buffer");
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_MISC, s);
   const EmbedDw p{(const int32_t *)srt, (const int32_t *)start, (const int32_t *)cnt, (const int32_t *)key, (const int32_t *)grp,

@@ -230,7 +230,7 @@ extern "C" int anc_expert_dw_multi(const anc_expert_dw_problem_t *probs, int32_t
   m.count = n_probs;
   m.experts = (int)experts;
   int64_t wide = 0;                                  // tiles of 256x256
-  struct { uint64_t at; int64_t bytes; } span[kMostProblems][4];       // outputs, then inputs
+  AncSpan span[kMostProblems][4];                    // outputs, then inputs
   for (int i = 0; i < n_probs; ++i) {
     const anc_expert_dw_problem_t &b = probs[i];
     ANC_REQUIRE(b.K > 0 && b.N > 0 && b.K % 8 == 0 && b.N % 8 == 0 && b.K <= (1 << 17) && b.N <= (1 << 17),
@@ -251,6 +251,9 @@ extern "C" int anc_expert_dw_multi(const anc_expert_dw_problem_t *probs, int32_t
         for (int c = 0; c < 4; ++c)
           ANC_REQUIRE((i == j && a == c) || anc_apart(span[i][a].at, span[i][a].bytes, span[j][c].at, span[j][c].bytes),
                       "anc_expert_dw_multi: an output of problem %d overlaps a buffer of problem %d", i, j);
+  for (int i = 0; i < n_probs; ++i)
+    ANC_REQUIRE(anc_outputs_apart({span[i][0], span[i][1], {counts, 4 * experts}, {offsets, 4 * experts + 4}, {order, 4 * experts}}, 2),
+                "anc_expert_dw_multi: an output of problem %d overlaps the segments", i);
   // 256x256 tiles where they give every CU one and segments are long (256 rows on average, by the room for them): fewer operand bytes for a
   // product. With fewer tiles twice as many of 128x256 are at work; with short segments the two workgroups of a CU hide each other's ends.
   // 16 experts, three weights of 1024x1024 with bf16 copies, from HBM, 256x256 and 128x256: 1024 rows each 142 and 152 us, 512 104 and 113, 256

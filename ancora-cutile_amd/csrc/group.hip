@@ -851,8 +851,12 @@ extern "C" int anc_id_groups_device(uint64_t ids, int32_t ids_bytes, int64_t n, 
               "anc_id_groups_device: null pointer");
   ANC_REQUIRE(ids % (uint64_t)ids_bytes == 0 && ((srt | start | cnt | gid | key | grp | count) & 3) == 0 && (workspace & 15) == 0,
               "anc_id_groups_device: misaligned pointers");
-  ANC_REQUIRE(workspace_bytes >= anc_id_groups_device_workspace_bytes(n > 0 ? n : 1, V), "anc_id_groups_device: workspace holds %lld bytes, %lld needed",
-              (long long)workspace_bytes, (long long)anc_id_groups_device_workspace_bytes(n > 0 ? n : 1, V));
+  const int64_t ws = anc_id_groups_device_workspace_bytes(n > 0 ? n : 1, V);
+  ANC_REQUIRE(workspace_bytes >= ws, "anc_id_groups_device: workspace holds %lld bytes, %lld needed", (long long)workspace_bytes, (long long)ws);
+  // (workgroups read the ids more than once and write by what they found)
+  ANC_REQUIRE(anc_outputs_apart({{srt, 4 * M}, {start, 4 * M}, {cnt, 4 * M}, {gid, 4 * M}, {key, 4 * M}, {grp, 4 * M}, {count, 4}, {workspace, ws},
+                                 {ids, n * ids_bytes}}, 8),
+              "anc_id_groups_device: an output or the workspace overlaps another buffer");
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_MISC, s);
   const Groups o{(int32_t *)srt, (int32_t *)start, (int32_t *)cnt, (int32_t *)gid, (int32_t *)key, (int32_t *)grp, (int32_t *)count};
@@ -934,6 +938,9 @@ extern "C" int anc_route(uint64_t expert_ids, int32_t ids_bytes, int64_t n, int6
               "anc_route: misaligned pointers");
   const int64_t ws = anc_route_workspace_bytes(n > 0 ? n : 1, experts);
   ANC_REQUIRE(workspace_bytes >= ws, "anc_route: workspace holds %lld bytes, %lld needed", (long long)workspace_bytes, (long long)ws);
+  ANC_REQUIRE(anc_outputs_apart({{counts, 4 * experts}, {offsets, 4 * experts + 4}, {order, 4 * experts}, {slot, 4 * n}, {src, 4 * capacity},
+                                 {workspace, ws}, {expert_ids, n * ids_bytes}}, 6),
+              "anc_route: an output or the workspace overlaps another buffer");
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_MISC, s);
   const Route o{(int32_t *)counts, (int32_t *)offsets, (int32_t *)order, (int32_t *)slot, (int32_t *)src};

@@ -64,3 +64,65 @@ def test_a_row_sparse_step_is_not_captured(fake_device):
         opt.step(g.gid, M, rows, 0)
     opt.flush(0)
     assert opt.t == 2
+
+
+P = 1 << 20          # an address that is aligned and never read
+
+
+def _refused(lib, name, args, word):
+    assert getattr(lib, name)(*args) == 2, (name, args)
+    assert word in lib.anc_last_error().decode(), lib.anc_last_error()
+
+
+def _but(args, at, value):
+    return args[:at] + (value,) + args[at + 1:]
+
+
+def test_indices_that_a_call_would_write_over_are_refused():
+    """Ids, slots and segments are read by workgroups while others write: an output on top of them would place rows by half-written
+    numbers (a routing of ids that change on the way has slots beyond its capacity)."""
+    from ancora_cutile_amd import _lib
+    lib = _lib.load()
+    a = [P * (16 + i) for i in range(16)]                                         # far apart
+    n, M, V = 3000, 4000, 500000
+    ws = lib.anc_id_groups_device_workspace_bytes(M, V)
+    group = (a[0], 8, n, M, V, *a[1:9], ws, 0)
+    for at in range(5, 13):
+        _refused(lib, "anc_id_groups_device", _but(group, 0, group[at] - 8 * n + 8), "overlap")
+        if at != 11:
+            _refused(lib, "anc_id_groups_device", _but(group, 0, group[at] + (4 * M if at < 11 else lib.anc_id_groups_device_workspace_bytes(n, V) // 8 * 8) - 8), "overlap")
+        for other in range(5, at):
+            _refused(lib, "anc_id_groups_device", _but(group, at, group[other]), "overlap")
+    T, k, E = 30000, 2, 60
+    A = T * k
+    ws, cap = lib.anc_route_workspace_bytes(A, E), lib.anc_route_capacity(A, E, 32)
+    route = (a[0], 4, A, E, 32, a[1], a[2], a[3], a[4], a[5], cap, a[6], ws, 0)
+    for at, nbytes in ((5, 4 * E), (6, 4 * E + 4), (7, 4 * E), (8, 4 * A), (9, 4 * cap), (11, ws)):
+        _refused(lib, "anc_route", _but(route, 0, route[at] + nbytes - 4), "overlap")
+        _refused(lib, "anc_route", _but(route, 0, route[at] - 4 * A + 4), "overlap")
+        for other in (5, 6, 7, 8, 9, 11):
+            if other < at:
+                _refused(lib, "anc_route", _but(route, at, route[other]), "overlap")
+    ws = lib.anc_embed_dw_workspace_bytes(1000, 64)
+    grad = (a[0], a[1], a[2], a[3], a[4], 1000, a[5], 1, 64, 1.0, a[6], 0, 500, a[7], ws, 0)
+    for at in range(5):
+        for value in (a[6] + 500 * 256 - 4, a[6] - 3996, a[7] + ws - 4):
+            _refused(lib, "anc_embed_dw", _but(grad, at, value), "overlap")
+    move = (a[0], a[1], a[2], 10, 2, 4, 16, a[3], a[4], 200, 1, 64, 0)
+    for at, nbytes in ((0, 80), (1, 16), (2, 20)):
+        for value in (a[4] - nbytes + 4, a[4] + 200 * 128 - 4):
+            _refused(lib, "anc_dispatch", _but(move, at, value), "overlap")
+    back = (a[0], a[1], 10, 2, a[2], 200, 1, a[3], 1, 64, 0)
+    for value in (a[3] - 76, a[3] + 1276):
+        _refused(lib, "anc_combine", _but(back, 0, value), "overlap")
+    both = (a[0], a[1], a[2], a[3], 10, 2, 4, 16, a[4], 1, a[5], a[6], 200, 1, a[7], 64, 0)
+    for at, nbytes in ((0, 80), (2, 16), (3, 20)):
+        for value in (a[6] - nbytes + 4, a[6] + 200 * 128 - 4, a[7] - nbytes + 4, a[7] + 76):
+            _refused(lib, "anc_combine_grad", _but(both, at, value), "overlap")
+    weight = 4 * 64 * 128
+    for g16 in (0, a[3]):
+        arr = (_lib.ExpertDwProblem * 1)(_lib.ExpertDwProblem(x=a[0], dy=a[1], dW=a[2], g16=g16, K=64, N=128, accumulate=0, reserved=0))
+        for at, nbytes in ((0, 16), (1, 20), (2, 16)):
+            for value in (a[2] - nbytes + 4, a[2] + 4 * weight - 4) + ((g16 + 2 * weight - 4,) if g16 else ()):
+                segments = _but((a[8], a[9], a[10]), at, value)
+                _refused(lib, "anc_expert_dw_multi", (arr, 1, *segments, 4, 100, 0), "overlap")
