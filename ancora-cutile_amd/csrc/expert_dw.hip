@@ -36,26 +36,12 @@ struct DwMulti {
   DwOne p[kMostProblems];
 };
 
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-
-// `records` bytes from `base` on are there, the rest reads as zero.
-__device__ __forceinline__ i32x4 descriptor(const char *base, uint32_t records) {
-  const uint64_t b = (uint64_t)base;
-  return i32x4{__builtin_amdgcn_readfirstlane((int)(uint32_t)b), __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32) & 0xFFFF),
-               __builtin_amdgcn_readfirstlane((int)records), 0x00020000};
-}
-// 16 bytes per lane from descriptor + off (per lane) to LDS address lds_base + 16 * lane.
-__device__ __forceinline__ void dma16_bounded(i32x4 desc, uint32_t off, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds_base), "v"(off), "s"(desc)
-               : "memory", "m0");
-}
-
 // One operand's rows of a tile: where the next stage starts and how many bytes of the segment are left from there.
 struct Feed {
   const char *at;
   int64_t left, step;
-  __device__ __forceinline__ i32x4 desc() const {
-    return descriptor(at, left <= 0 ? 0u : left < 0xFFFFFFFFll ? (uint32_t)left : 0xFFFFFFFFu);
+  __device__ __forceinline__ anc_i32x4 desc() const {
+    return buffer_of(at, left <= 0 ? 0u : left < 0xFFFFFFFFll ? (uint32_t)left : 0xFFFFFFFFu);
   }
   __device__ __forceinline__ void next() { at += step; left -= step; }
 };
@@ -100,12 +86,12 @@ __global__ void __launch_bounds__(TM * 2, 2) k_expert_dw(DwMulti m) {
     const int row = (wave * kPiecesB + i) * 2 + (lane >> 5);
     vb[i] = (uint32_t)(row * N * 2 + (((lane & 31) ^ ((row & 3) << 2)) * 16));
   }
-  auto issue = [&](int i, const i32x4 &da, const i32x4 &db, unsigned char *stage) {
+  auto issue = [&](int i, const anc_i32x4 &da, const anc_i32x4 &db, unsigned char *stage) {
     if (i < kPiecesA) dma16_bounded(da, va[i], lds_addr(stage + (wave * kPiecesA + i) * 1024));
     else dma16_bounded(db, vb[i - kPiecesA], lds_addr(stage + kBytesA + (wave * kPiecesB + i - kPiecesA) * 1024));
   };
   auto issue_all = [&](unsigned char *stage) {
-    const i32x4 da = fa.desc(), db = fb.desc();
+    const anc_i32x4 da = fa.desc(), db = fb.desc();
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) issue(i, da, db, stage);
     fa.next();
@@ -159,7 +145,7 @@ __global__ void __launch_bounds__(TM * 2, 2) k_expert_dw(DwMulti m) {
       }
       wait_vm<(kStages - 2) * kPieces>();
       lds_barrier();
-      const i32x4 da = fa.desc(), db = fb.desc();
+      const anc_i32x4 da = fa.desc(), db = fb.desc();
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         multiply(1, i);
