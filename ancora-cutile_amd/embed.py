@@ -337,8 +337,9 @@ class RowSparseAdamW:
         opt.flush(si)                      # every row current (before a checkpoint / evaluation)
 
     State after `flush` equals the dense `AdamW` run on gradients that are zero outside the touched
-    rows, bit for bit (stochastic rounding included). `lr` may change between steps. Steps are counted on the host:
-    `catch_up`, `step` and `flush` refuse a stream that is being captured into a graph."""
+    rows, bit for bit (stochastic rounding included); until the first step p16 is W rounded to nearest. `lr` may change
+    between steps. Steps are counted on the host: `catch_up`, `step` and `flush` refuse a stream that is being captured into a
+    graph."""
 
     def __init__(self, W, lr=3e-4, betas=(0.9, 0.95), eps=1e-8, wd=0.01, form="div", sr=False, seed=0,
                  tensor_seed=0, max_steps=1 << 16):
@@ -351,7 +352,8 @@ class RowSparseAdamW:
         self.form, self.sr, self.seed, self.tensor_seed = form, bool(sr), int(seed), int(tensor_seed)
         self.t = 0
         self.p32 = DevBuf(W)
-        self.p16 = DevBuf.zeros(W.shape, np.uint16)
+        self.p16 = DevBuf.empty(W.shape, np.uint16)
+        api.anc_cast_bf16(self.p32.ptr, self.p16.ptr, W.size, 0, 0, 0)     # (the first forward reads it before any step has)
         self.m = DevBuf.zeros(W.shape, np.float32)
         self.v = DevBuf.zeros(W.shape, np.float32)
         self.last = DevBuf.zeros((self.V,), np.int32)

@@ -442,3 +442,27 @@ def test_row_sparse_training_without_the_host_seeing_an_id(gpu):
         assert bits_equal(a.to_numpy(), b.to_numpy())
     for b in (groups, rows, *x, known, opt):
         b.free()
+
+
+@pytest.mark.parametrize("sr", [False, True])
+def test_the_first_forward_reads_the_rounded_rows(gpu, sr):
+    """Nothing was missed before the first step: a lookup of the bf16 weights then gives the initial rows, rounded to nearest, and after a
+    step the rows that it did not name still are."""
+    from ancora_cutile_amd import DevBuf, DeviceIdGroups, embed_lookup
+    from ancora_cutile_amd.embed import RowSparseAdamW
+    V, H, M = 300, 192, 77
+    rng = np.random.default_rng(21)
+    W0 = rng.standard_normal((V, H)).astype(np.float32)
+    opt, groups = RowSparseAdamW(W0, lr=1e-2, wd=0.0, sr=sr, seed=3), DeviceIdGroups(M, V)
+    ids = rng.integers(0, V, M).astype(np.int32)
+    buf, x, rows = DevBuf(ids), DevBuf.zeros((M, H), np.uint16), DevBuf.zeros((M, H), np.float32)
+    groups.group(buf, 0)
+    opt.catch_up(groups, 0)
+    embed_lookup(buf, opt.p16, 0, x)
+    want = bf16_rne_bits(W0).reshape(V, H)
+    assert bits_equal(x.to_numpy(), want[ids])
+    opt.step(groups.gid, groups.M, rows, 0)
+    rest = np.setdiff1d(np.arange(V), ids)
+    assert bits_equal(opt.p16.to_numpy()[rest], want[rest])
+    for b in (opt, groups, buf, x, rows):
+        b.free()

@@ -126,3 +126,10 @@ def test_indices_that_a_call_would_write_over_are_refused():
             for value in (a[2] - nbytes + 4, a[2] + 4 * weight - 4) + ((g16 + 2 * weight - 4,) if g16 else ()):
                 segments = _but((a[8], a[9], a[10]), at, value)
                 _refused(lib, "anc_expert_dw_multi", (arr, 1, *segments, 4, 100, 0), "overlap")
+
+
+def test_row_sparse_weights_are_the_tables_from_the_start(fake_device):
+    """(not a refusal: the bf16 weights are made when the optimizer is, by one cast over the table)"""
+    from ancora_cutile_amd.embed import RowSparseAdamW
+    opt = RowSparseAdamW(np.ones((40, 64), np.float32), sr=True)
+    assert [c[:5] for c in fake_device.calls("anc_cast_bf16")] == [(opt.p32.ptr, opt.p16.ptr, 40 * 64, 0, 0)]
