@@ -257,24 +257,30 @@ def _buf(t):
     return DevBuf(shape=tuple(t.shape), dtype=kinds[t.dtype], ptr=t.data_ptr())
 
 
+class _Kept:
+    """A plan or groups, freed when the state and every tensor that shows one of its arrays are gone."""
+
+    def __init__(self, owner):
+        self.owner = owner
+
+    def __del__(self):
+        torch.cuda.synchronize()
+        self.owner.free()
+
+
 class _Shown:
-    def __init__(self, buf):
-        self.buf = buf              # (the memory lives as long as a tensor that shows it)
+    def __init__(self, buf, kept):
+        self.kept = kept            # (a tensor holds what it was made from)
         self.__cuda_array_interface__ = {"shape": buf.shape, "typestr": buf.dtype.str, "data": (buf.ptr, False), "version": 2}
 
 
-def _tensor(buf, shape):
-    return torch.as_tensor(_Shown(buf), device=DEV).view(shape)
+def _tensor(buf, kept, shape):
+    return torch.as_tensor(_Shown(buf, kept), device=DEV).view(shape)
 
 
 class State:
     def __init__(self, case, data):
         self.case, self.data, self.go, self.out, self.kept = case, data, None, None, None
-
-    def __del__(self):
-        if self.kept is not None:
-            torch.cuda.synchronize()
-            self.kept.free()
 
 
 def _ready(c, d, state):
@@ -289,8 +295,9 @@ def _ready(c, d, state):
         state.out = out
         return
     if kind == "embed_grad":
-        groups = state.kept = embed.DeviceIdGroups(c["M"], c["V"])
-        state.out = dict(n=_tensor(groups.count, ()), gid=_tensor(groups.gid, (c["M"],)))
+        groups = embed.DeviceIdGroups(c["M"], c["V"])
+        kept = state.kept = _Kept(groups)
+        state.out = dict(n=_tensor(groups.count, kept, ()), gid=_tensor(groups.gid, kept, (c["M"],)))
         if c["dense"]:
             state.out["dE"] = d["dE"]
 
@@ -308,13 +315,14 @@ def _ready(c, d, state):
         state.go = go
         return
     S, T, k, E, H = _capacity(c), c["T"], c["k"], c["E"], c["H"]
-    plan = state.kept = dispatch.RoutePlan(T, k, E, align=c["align"])
+    plan = dispatch.RoutePlan(T, k, E, align=c["align"])
+    kept = state.kept = _Kept(plan)
     assert plan.capacity == S
     if kind == "dispatch":
         xs = torch.zeros((S, H), device=DEV, dtype=_T[c["type"]])
         bxs = _buf(xs)
-        state.out = dict(counts=_tensor(plan.counts, (E,)), offsets=_tensor(plan.offsets, (E + 1,)),
-                         slot=_tensor(plan.slot, (T, k)), src=_tensor(plan.src, (S,)), xs=xs)
+        state.out = dict(counts=_tensor(plan.counts, kept, (E,)), offsets=_tensor(plan.offsets, kept, (E + 1,)),
+                         slot=_tensor(plan.slot, kept, (T, k)), src=_tensor(plan.src, kept, (S,)), xs=xs)
         if c["back"]:
             state.out["dx"] = torch.empty((T, H), device=DEV, dtype=_T[c["type"]])
             bdx = _buf(state.out["dx"])
