@@ -278,7 +278,10 @@ k_group_part(const ID *__restrict__ ids, int n, int64_t M, uint32_t V, Groups o)
         id_to = (uint32_t)(fits >> 32);
         p_to = (int)(uint32_t)fits;
       }
-      int low_every = 0;                             // ids below the piece's first; all of them (a wavefront's are at most 2^15 - 1 ... 2^14)
+      // Ids below the piece's first, and all of them << 16. A wavefront counts at most 2^14: on 1024 lanes its part of the words holds no
+      // more bits, on 512 the batch has no more ids.
+      static_assert(kMostMarked / W <= 1 << 14 || (LANES == 512 && kFewSplit <= 1 << 14), "two sums in a word");
+      int low_every = 0;
       for (int i = tid; i < words; i += LANES) {
         const uint32_t w = marks[i], i32 = (uint32_t)i * 32;
         low_every += __popc(w) << 16 | (i32 + 32 <= id_lo ? __popc(w) : i32 >= id_lo ? 0 : __popc(w & ((1u << (id_lo - i32)) - 1)));

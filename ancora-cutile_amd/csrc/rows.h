@@ -118,7 +118,8 @@ template <int T, int VEC> __device__ __forceinline__ Raw<T, VEC> narrow(const fl
 }
 
 // i / d for i < 2^31 as one multiplication (64-bit division by a value that is not known to the compiler is some hundred instructions):
-// m = ceil(2^(31 + s) / d) with 2^s >= d is below 2^32 + 1 and m i / 2^(31 + s) exceeds i / d by less than 1 / d.
+// m = ceil(2^(31 + s) / d) for the smallest s with 2^s >= d. From d >= 2^(s - 1) + 1 and d < 2^31 follows m < 2^32: 2^(31 + s) / d is at most
+// 2^32 - 2^32 / (2^(s - 1) + 1), 2^32 - 3 or less. And m d - 2^(31 + s) < d <= 2^s, so m i / 2^(31 + s) exceeds i / d by less than 1 / d.
 struct FastDiv {
   uint32_t d, mul;
   int shift;
