@@ -18,3 +18,4 @@ from .quant import Mxfp8WeightCache, quant_mxfp8_w                          # no
 from .grads import gemm_dW, transpose_acts, DwWorkspace, expert_dW            # noqa: F401
 from .embed import embed_lookup, DeviceIdGroups, embed_dw                     # noqa: F401
 from .dispatch import RoutePlan, dispatch_grad, combine, combine_grad         # noqa: F401
+from . import dispatch                  # (the module: the call of that name is dispatch.dispatch)     # noqa: F401

@@ -221,7 +221,12 @@ __global__ void __launch_bounds__(kDwLanes) k_embed_dw_join(EmbedDw p) {
   store<ANC_F32, VEC, TAIL, false, true>(to, narrow<ANC_F32, VEC>(x), pc);
 }
 
-// Positions per team: enough chunks to fill the card (8192 positions of 16 or of 8: 28.1 and 27.1 us with the grouping; 65536 of 32 or of 64: 91 and 87).
+// Positions per team: enough chunks to fill the card while there are few, fewer partial rows where there are many. By n alone, so that the bits
+// do not hang on the width. Gradient and join, us, mostly distinct ids, bf16 rows of 256, 1024 and 2048 values:
+//   runs of 8 and 16:   8192 positions 7.9 and 9.9, 16.2 and 20.0, 29 and 27; 12288 8.9 and 10.3, 24.8 and 22.8, 38 and 43; 16384 10.2 and 11.4, 26.7 and
+//                       26.0, 50 and 49
+//   runs of 16 and 64:  32768 16.0 and 29.7, 44 and 63, 85 and 79; 65536 24.7 and 34.3, 71 and 74, 163 and 154; with a third of the positions on one id
+//                       32768 17 and 28, 37 and 45, 72 and 67; 65536 28 and 33, 62 and 66, 151 and 147 (64 is right for wide rows only)
 // Up to kFewMost all are one workgroup's, for 64 pieces of the rows each, and nothing is left to join (77 rows into a dense gradient 6.7 us, by
 // the join 8.8; 128 rows 9.1 and 8.9, into compact rows 7.1 and 8.8; 200 rows, 16 to a team, 12.2 and 9.0).
 constexpr int64_t kFewMost = kFewSubs * 8, kSub8Most = 8192, kSub16Most = 32768;

@@ -240,10 +240,14 @@ extern "C" int anc_expert_dw_multi(const anc_expert_dw_problem_t *probs, int32_t
   for (int i = 0; i < n_probs; ++i)
     ANC_REQUIRE(anc_outputs_apart({span[i][0], span[i][1], {counts, 4 * experts}, {offsets, 4 * experts + 4}, {order, 4 * experts}}, 2),
                 "anc_expert_dw_multi: an output of problem %d overlaps the segments", i);
-  // 256x256 tiles where they give every CU one and segments are long (256 rows on average, by the room for them): fewer operand bytes for a
-  // product. With fewer tiles twice as many of 128x256 are at work; with short segments the two workgroups of a CU hide each other's ends.
-  // 16 experts, three weights of 1024x1024 with bf16 copies, from HBM, 256x256 and 128x256: 1024 rows each 142 and 152 us, 512 104 and 113, 256
-  // 76 and 72, 128 66 and 62; 64 experts, 512x1024, 256 rows 169 and 181; 8 experts, one weight of 512x512, 512 rows 19.0 and 14.5.
+  // 256x256 tiles where they give every CU one and there is room for 256 rows per expert: fewer operand bytes for a product. With fewer
+  // tiles twice as many of 128x256 are at work; with short segments the two workgroups of a CU hide each other's ends. Room is what
+  // the host knows: filling, tokens without an expert and tokens that the plan could hold count in it, so that segments may be much shorter
+  // than the line says, and around the line the better side hangs on the shape and on what is cached. A layer's three weights with bf16 copies
+  // and its five operands, us, 256x256 and 128x256: 16 experts of 1024x1024 with 1024 rows each 147 and 155, 768 125 and 134, 512 99 and 92 (with
+  // operands of each weight's own 102 and 114), 256 79 and 72, 128 68 and 63, 64 filled up to 256 62 and 60; 64 experts of 512x1024 with
+  // 512 rows 208 and 219, 256 168 and 182, 128 filled up to 256 135 and 132; 128 experts of 512x768 with 256 rows 265 and 249; 8 experts, one weight
+  // of 512x512, 512 rows 19.0 and 14.5.
   const int TM = wide >= 256 && capacity >= 256 * experts ? 256 : 128;
   for (int i = 0; i < n_probs; ++i) m.p[i].tiles = (m.p[i].K + TM - 1) / TM * m.p[i].tn;
   // The tiles that stay together: a whole weight of 16 or 32 tiles, fewer where that leaves an XCD less than six units to even out.

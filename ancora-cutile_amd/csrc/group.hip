@@ -128,7 +128,8 @@ __device__ __forceinline__ uint32_t as_key(int64_t id, uint32_t V) { return (uin
 constexpr int kPartItems = 4, kSamples = 256;
 // Both sides measured, ids of 152 K rows, a call in a row of calls: 512 alone on 256 lanes 7.0 us (on 1024 7.7), 1024 alone on 512 lanes 7.5 (on
 // 1024 8.4; in shares 9.2), 1500 alone 8.8, 2048 alone 10.2 and in shares 9.3; shares on 512 and on 1024 lanes: 8192 12.4 and 13.8, 24000 20.1 and
-// 20.8, 32768 23.2 and 23.0; 65536 in shares 31, by passes 47.
+// 20.8, 32768 23.2 and 23.0; 65536 in shares 31, by passes 47. Where a table has more rows than bits in LDS the passes are all there is: 2^18
+// rows and one more, 1537 ids 10 and 34 us, 8192 13 and 52, 65536 32 and 73; beyond 65536 ids 131072 take 52 (2 passes) and 82 (3), 2^20 143 and 227.
 constexpr int64_t kFewAlone = 512, kMostAlone = 1536, kFewSplit = 1 << 14, kMostSplit = 1 << 16;             // positions: of one workgroup, of several
 constexpr int64_t kMostMarked = 1 << 18;                               // ids, where several workgroups share them (one bit each in LDS)
 
@@ -260,7 +261,10 @@ k_group_part(const ID *__restrict__ ids, int n, int64_t M, uint32_t V, Groups o)
         goes = uniform(sum.w);
         __syncthreads();
         if (size <= CAP) break;
-        // More than LDS holds (hardly ever: a share is a quarter of that or less on average): the largest beginning that fits.
+        // More than LDS holds: the largest beginning that fits, by some 50 more looks at all ids. On average a share is a sixteenth (512
+        // lanes) or an eighth of that, and it spans two samples: of 65536 mostly distinct ids one call in some 6000 meets such a share, of
+        // 50000 one in a million. Where the sample sees nothing of the order (all sampled positions on one id) 8192 ids take 170 us, 20000 530,
+        // 65536 4800.
         uint64_t fits = lo, over = to;
         while (over - fits > 1) {
           const uint64_t mid = fits + (over - fits) / 2;

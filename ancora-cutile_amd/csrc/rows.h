@@ -137,8 +137,10 @@ inline FastDiv fast_div(uint32_t d) {
 
 // ---- host side
 constexpr int64_t kMostPieces = (1ll << 31) - 1;     // of one launch (FastDiv)
-// Bytes up to which rows go through the caches. A lookup of 16 MiB and a copy of it afterwards: 12.6 us, with its stores past the caches 14.7;
-// one of 199 MB: 149 us, past the caches 145, and the lookup alone 72 and 66.
+// Bytes up to which rows go through the caches; through them and past them, us, bf16 rows of 1024 values. A lookup and a copy of it afterwards: 32
+// MiB 20.3 and 22.9, 48 30.3 and 32.4, 64 47.7 and 42.2, 128 115 and 96. A gradient after the copy that made its dy: 32 MiB 28.9 both, 64 57 and 47, 128
+// 128 and 124. combine_grad by itself is faster past them from 16 MiB on (9.9 and 9.4; 64 MiB 35 and 28), together with the experts' gradient that
+// reads its dys from 256 MiB on (335 and 333; 16 MiB 36.3 and 36.9, 64 93.0 and 94.6, 128 173 and 176): the line is between the two.
 constexpr int64_t kCached = 64ll << 20;
 inline int64_t elem_size(int type) { return type == ANC_F32 ? 4 : 2; }
 inline bool type_ok(int type) { return type == ANC_F32 || type == ANC_BF16; }

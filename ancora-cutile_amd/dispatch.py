@@ -8,7 +8,7 @@
 
 and backwards `combine_grad` (rows and weights), `grads.expert_dW` (the experts' weights, over the ragged segments) and
 `dispatch_grad`. Everything is decided on the device: no copy to the host, and each call may be captured into a graph. Outputs
-overlap no input.
+that overlap an input are refused.
 """
 import numpy as np
 

@@ -7,7 +7,7 @@ it updates only the rows a step's tokens touch and replays the steps a row misse
 next needed, so that every row it hands out is bit-identical to the dense optimizer's.
 
 For ids that lie on the device: `embed_lookup` (rows times a scale), `DeviceIdGroups` (the group arrays, made there) and
-`embed_dw` (the gradient over them, whatever the ids' frequencies). Their outputs overlap none of their inputs.
+`embed_dw` (the gradient over them, whatever the ids' frequencies). Outputs that overlap an input are refused.
 """
 import ctypes
 import threading

@@ -321,7 +321,7 @@ int anc_unique_ids(const int32_t *ids, int64_t n, int32_t *out, int64_t *n_out);
 
 /* The input embedding from ids that lie on the device. Ids are int32 or int64 (ids_bytes 4 or 8); one outside
  * [0, V) names no row: its lookup is a zero row, its gradient is left out. Types are ANC_F32 or ANC_BF16, rows are
- * contiguous, any H. No output may overlap an input or another output, here and in the calls below.
+ * contiguous, any H. An output or a workspace that overlaps another buffer of the call is refused, here and in the calls below.
  *
  * anc_embed_lookup: out[i] = scale * table[ids[i]] for i < n, product in fp32, one rounding. */
 int anc_embed_lookup(uint64_t ids, int32_t ids_bytes, int64_t n, uint64_t table, int table_type, int64_t V, int64_t H,
