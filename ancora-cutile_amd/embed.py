@@ -170,14 +170,16 @@ class IdGroups:
 
 def embed_dw_scatter(groups, dy, si, out=None, compact=None, V=None):
     """dy: (M, H) bf16 DevBuf. out: (V, H) fp32 DevBuf, added onto in place (the reference's
-    launch); or compact: (M, H) fp32 DevBuf that receives one summed row per group. Over a `DeviceIdGroups` dy and
-    compact hold at least the rows that were grouped, and at most (dy) those there is room for."""
+    launch); or compact: (M, H) fp32 DevBuf that receives one summed row per group. Over a `DeviceIdGroups` dy has at
+    least the rows that were grouped and at most those there is room for, compact no fewer than dy."""
     M, H = dy.shape
     if M > groups.M:                                       # (a group per row of dy is launched)
         raise ValueError(f"embed_dw_scatter: dy has {M} rows, the groups have room for {groups.M}")
     if isinstance(groups, DeviceIdGroups):
         groups._used("embed_dw_scatter")
         groups._fits("embed_dw_scatter", dy, out, compact)
+        if compact is not None:                            # (whatever a replayed `group` has left there: a row per workgroup)
+            _rows_of(compact, M, H, "embed_dw_scatter", "compact")
         if dy.dtype != np.uint16:
             raise ValueError(f"embed_dw_scatter: dy is {dy.dtype}, bf16 bits (uint16) expected")
     if out is not None:

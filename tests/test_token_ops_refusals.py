@@ -25,6 +25,7 @@ def test_sequential_scatter_takes_the_rows_its_groups_have_room_for(fake_device)
     host = IdGroups(np.arange(M))
     for groups, dy, to in ((g, _buf((M + 1, H), u16), dict(out=out)), (g, _buf((7 * M, H), u16), dict(compact=_buf((7 * M, H), f32))),
                            (g, _buf((19, H), u16), dict(out=out)), (g, _buf((M, H), u16), dict(compact=_buf((19, H), f32))),
+                           (g, _buf((M, H), u16), dict(compact=_buf((M - 1, H), f32))),     # (a replayed `group` may have made more groups)
                            (g, _buf((M, H), u16), dict(out=_buf((V - 1, H), f32))), (g, _buf((M, H), u16), dict(out=_buf((V, 2 * H), f32))),
                            (g, _buf((M, H), u16), dict(compact=_buf((M, H), u16))), (g, _buf((M, H), f32), dict(out=out)),
                            (g, _buf((M, H), u16), {}), (g, _buf((M, H), u16), dict(out=out, compact=rows)),
