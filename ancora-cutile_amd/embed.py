@@ -361,6 +361,7 @@ class RowSparseAdamW:
         self.last = DevBuf.zeros((self.V,), np.int32)
         self._cap = int(max_steps)
         self.table = DevBuf.zeros((self._cap + 1, 4), np.uint32)
+        _lib.stream_sync(0)                    # (streams that do not wait for the null stream may use all of this at once)
         self._rows_buf, self._rows_si = None, 0
         self.last_skipped = False
         self._filled_to = 0          # table entries 1 .. _filled_to hold the scalars of their steps

@@ -134,3 +134,12 @@ def test_row_sparse_weights_are_the_tables_from_the_start(fake_device):
     from ancora_cutile_amd.embed import RowSparseAdamW
     opt = RowSparseAdamW(np.ones((40, 64), np.float32), sr=True)
     assert [c[:5] for c in fake_device.calls("anc_cast_bf16")] == [(opt.p32.ptr, opt.p16.ptr, 40 * 64, 0, 0)]
+
+
+def test_row_sparse_state_is_in_place_for_every_stream(fake_device):
+    """What the constructor fills and casts on the null stream is waited for: a stream that does not wait for that one may read it at once."""
+    from ancora_cutile_amd.embed import RowSparseAdamW
+    RowSparseAdamW(np.ones((40, 64), np.float32))
+    names = [n for n, _ in fake_device.log]
+    last = max(i for i, n in enumerate(names) if n in ("anc_cast_bf16", "anc_fill_u32"))
+    assert ("anc_stream_sync", (0,)) in fake_device.log[last:]
