@@ -13,7 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # ANCORA_OPTIM_LIB names another build of the same library (an ablation variant, see build.py)
 LIB_PATH = os.environ.get("ANCORA_OPTIM_LIB") or os.path.join(_HERE, "csrc", "libancora_optim.so")
 
-F32, BF16 = 0, 1                  # ANC_F32 / ANC_BF16
+F32, BF16, MXFP8 = 0, 1, 2        # ANC_F32 / ANC_BF16 / ANC_MXFP8
 FORM_DIV, FORM_IBC = 0, 1         # ANC_ADAMW_FORM_*
 NS_BF16, NS_FP32, NS_BF16_FAST, NS_BF16_X3, NS_BF16_LATE3 = 0, 1, 2, 3, 4   # ANC_NS_*
 GN_CHUNK = 8192                   # ANC_GN_CHUNK
@@ -54,6 +54,12 @@ class AdamWStepEntry(C.Structure):
 
 class AdamWDesc(C.Structure):
     _fields_ = [("g", u64), ("m", u64), ("v", u64), ("p32", u64), ("p16", u64), ("n", i64),
+                ("blk0", i64), ("wd", f32), ("seed", u32), ("g_dtype", i32), ("pad", i32)]
+
+
+class AdamW8Desc(C.Structure):
+    """anc_adamw8_desc_t: one tensor of the step with 8-bit moments."""
+    _fields_ = [("g", u64), ("m", u64), ("v", u64), ("ms", u64), ("vs", u64), ("p32", u64), ("p16", u64), ("n", i64),
                 ("blk0", i64), ("wd", f32), ("seed", u32), ("g_dtype", i32), ("pad", i32)]
 
 
@@ -140,6 +146,7 @@ _PROTOS = {
                          u64, u64]),
     "anc_adamw_num_blocks": (i64, [i64]),
     "anc_adamw_multi": (None, [u64, i32, i64, C.POINTER(AdamWHyper), u64, u64]),
+    "anc_adamw8_multi": (None, [u64, i32, i64, C.POINTER(AdamWHyper), u64, u64]),
     "anc_adamw_rows": (None, [u64, i64, u64, u64, u64, u64, u64, u64, i64, i64, u64, i32,
                               C.POINTER(AdamWHyper), f32, u32, u64, u64]),
     "anc_embed_dw_scatter": (None, [u64, u64, u64, u64, u64, u64, u64, i64, i64, i64, u64]),
@@ -167,6 +174,13 @@ _PROTOS = {
     "anc_quant_mxfp8_w": (None, [u64, u64, u64, i64, i64, i64, C.c_int, u64]),
     "anc_quant_mxfp8_num_tiles": (i64, [i64, i64, i64]),
     "anc_quant_mxfp8_w_multi": (None, [u64, i32, i64, C.c_int, u64]),
+    "anc_rms_norm": (None, [u64, C.c_int, u64, C.c_int, u64, C.c_int, i64, i64, f32, u64, C.c_int, u64, u64, u64, u64]),
+    "anc_rms_norm_grad_workspace_bytes": (i64, [i64, i64]),
+    "anc_rms_norm_grad": (None, [u64, C.c_int, u64, C.c_int, u64, C.c_int, u64, u64, i64, i64, u64, u64, C.c_int, u64, i64, u64]),
+    "anc_gated_ffn": (None, [u64, u64, u64, u64, u64, i64, i64, i64, i64, u64, u64, u64, u64]),
+    "anc_ffn_down": (None, [u64, u64, u64, u64, i64, i64, i64, i64, u64, u64, C.c_int, u64]),
+    "anc_gated_ffn_grad": (None, [u64, u64, u64, u64, u64, u64, i64, i64, i64, i64, u64, u64, u64, u64]),
+    "anc_gated_ffn_dx": (None, [u64, u64, u64, u64, u64, u64, i64, i64, i64, i64, u64, u64, C.c_int, u64]),
     "anc_gemm_dw_workspace_bytes": (i64, [i64, i64, i64]),
     "anc_gemm_dw_multi": (None, [C.POINTER(DwProblem), i32, u64]),
     "anc_expert_dw_multi": (None, [C.POINTER(ExpertDwProblem), i32, u64, u64, u64, i64, i64, u64]),

@@ -15,14 +15,16 @@ the host, so master weights and moments are bit-identical to that oracle;
 
 Extensions (all off by default): bf16 gradients (uint16 arrays), gradients already
 resident in DevBufs, stochastic-rounded bf16 downcast (`sr=True`, counter-based hash of
-ancora/kernels/fused.py:154-161), and a StepGuard (global clip + skip on non-finite).
+ancora/kernels/fused.py:154-161), a StepGuard (global clip + skip on non-finite), and moments in 8 bits
+(`state_bits=8`: E4M3 codes for m and E5M2 codes for v with a scale byte per 64 elements, stored by stochastic rounding:
+2 1/32 instead of 8 bytes per element of state, the same fp32 arithmetic in between).
 """
 import ctypes
 
 import numpy as np
 
 from . import _lib
-from ._lib import (api, AdamWHyper, AdamWDesc, AdamWStepEntry, F32, BF16, FORM_DIV, FORM_IBC, SR_ON,
+from ._lib import (api, AdamWHyper, AdamWDesc, AdamW8Desc, AdamWStepEntry, F32, BF16, FORM_DIV, FORM_IBC, SR_ON,
                    SR_STEP_SEED)
 from .bf16 import bf16_bits as _bf16_bits, bits_f32 as _bits_f32  # noqa: F401  (re-exported)
 from .devbuf import DevBuf, upload_table
@@ -82,14 +84,42 @@ def _adamw(stream_int, g, m, v, p32, p16, OTM, beta1, beta2, eps, lr, wd, ibc1, 
                   float(wd), 0, int(ctl), int(stream_int))
 
 
+def _codes(exponents, mantissa):
+    """The magnitudes of an 8-bit float's codes 0 .. 127: `exponents` values of the exponent field, subnormals at 0, the topmost
+    not finite (E5M2: infinity and NaN, E4M3: NaN alone)."""
+    e, m = np.divmod(np.arange(128), 1 << mantissa)
+    bias = exponents // 2 - 1
+    v = np.where(e == 0, np.ldexp(m / 2.0 ** mantissa, 1 - bias), np.ldexp(1 + m / 2.0 ** mantissa, e - bias)).astype(np.float32)
+    v[127] = np.nan
+    if exponents == 32:
+        v[124:] = (np.inf, np.nan, np.nan, np.nan)
+    return v
+
+
+_E4M3, _E5M2 = _codes(16, 3), _codes(32, 2)
+
+
+def moments8(codes, scales, values):
+    """fp32 values of 8-bit moments: codes (R, 64) and scale bytes (R,) as `AdamW(state_bits=8)` holds them; values: `_E4M3` for
+    m, `_E5M2` for v."""
+    codes = np.asarray(codes)
+    v = np.where(codes & 0x80, -values[codes & 0x7F], values[codes & 0x7F])
+    return (v * np.exp2(scales.astype(np.float64) - 127.0)[:, None]).astype(np.float32)
+
+
 class AdamW:
     """fp32-master AdamW. params: {name: fp32 ndarray}. no_decay: names with wd=0 (norm gains /
     biases). step(grads, stream) updates in place; .weights() returns the bf16-valued fp32
-    weights for the forward (ancora/optim/adamw.py:69-109)."""
+    weights for the forward (ancora/optim/adamw.py:69-109). state_bits=8 holds m and v as 8-bit codes `st[name]["m"]`, `["v"]`
+    (R, 64) with scale bytes `["ms"]`, `["vs"]` (R,); `seed` then decides their rounding too."""
 
     def __init__(self, params, lr=3e-4, betas=(0.9, 0.95), eps=1e-8, wd=0.01, no_decay=(),
-                 form="div", sr=False, seed=0, grad_dtype=np.float32):
+                 form="div", sr=False, seed=0, grad_dtype=np.float32, state_bits=32):
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits={state_bits}: 8 or 32")
         _lib.init()
+        self.state_bits = int(state_bits)
+        self._kept = ("p32", "m", "v", "p16") + (("ms", "vs") if state_bits == 8 else ())      # what a checkpoint holds
         self.lr, (self.b1, self.b2), self.eps, self.wd = lr, betas, eps, wd
         if form not in ("div", "ibc"):
             raise ValueError("form must be 'div' or 'ibc'")
@@ -104,11 +134,16 @@ class AdamW:
                 raise ValueError(f"AdamW: '{name}' has {p.size} elements, not a multiple of {C}")
             R = p.size // C
             flat = np.ascontiguousarray(p, dtype=np.float32).reshape(R, C)
+            sdt = np.float32 if state_bits == 32 else np.uint8
             self.st[name] = dict(
                 shape=p.shape, R=R, otm=_pick_otm(R), wd=0.0 if name in no_decay else wd,
                 g=DevBuf.zeros((R, C), gdt),
-                m=DevBuf.zeros((R, C), np.float32), v=DevBuf.zeros((R, C), np.float32),
+                m=DevBuf.zeros((R, C), sdt), v=DevBuf.zeros((R, C), sdt),
                 p32=DevBuf(flat), p16=DevBuf.zeros((R, C), np.uint16))
+            if state_bits == 8:
+                half = (R + 3) // 4 * 4
+                block = DevBuf.zeros((2 * half,), np.uint8)
+                self.st[name].update(scales=block, ms=block.view((R,)), vs=DevBuf(shape=(R,), dtype=np.uint8, ptr=block.ptr + half))
         self._table = None
         self._table_key = None
         self.last_skipped = False
@@ -158,15 +193,22 @@ class AdamW:
             n = s["R"] * C
             if g.size != n:
                 raise ValueError(f"AdamW: gradient of '{name}' has {g.size} elements, expected {n}")
-            descs.append(AdamWDesc(g.ptr, s["m"].ptr, s["v"].ptr, s["p32"].ptr, s["p16"].ptr, n,
-                                   blk0, s["wd"], seed, _g_code(g.dtype), 0))
+            if self.state_bits == 8:
+                code = _g_code(g.dtype)
+                if g.ptr % (16 if code == F32 else 8):
+                    raise ValueError(f"AdamW: gradient of '{name}' at {g.ptr:#x} is not aligned")
+                descs.append(AdamW8Desc(g.ptr, s["m"].ptr, s["v"].ptr, s["ms"].ptr, s["vs"].ptr, s["p32"].ptr, s["p16"].ptr, n,
+                                        blk0, s["wd"], seed, code, 0))
+            else:
+                descs.append(AdamWDesc(g.ptr, s["m"].ptr, s["v"].ptr, s["p32"].ptr, s["p16"].ptr, n,
+                                       blk0, s["wd"], seed, _g_code(g.dtype), 0))
             blk0 += api.anc_adamw_num_blocks(n)
         self._total_blocks = blk0
         self._table = upload_table(descs)
         self._table_key = key
 
     def _hyper(self):
-        sb = sr_seed_base(self.seed, self.t) if self.sr else 0
+        sb = sr_seed_base(self.seed, self.t) if self.sr or self.state_bits == 8 else 0
         if self.form == "div":
             return hyper_div(self.lr, self.b1, self.b2, self.eps, self.t, self.sr, sb)
         ibc1 = 1.0 / (1.0 - self.b1 ** self.t)
@@ -209,12 +251,12 @@ class AdamW:
                 h = hyper_div(self.lr, self.b1, self.b2, self.eps, 1, False, self.seed)
             else:
                 h = hyper_ibc(self.lr, self.b1, self.b2, self.eps, 1.0, 1.0, False, self.seed)
-            h.sr = (SR_ON | SR_STEP_SEED) if self.sr else 0
+            h.sr = (SR_ON | SR_STEP_SEED) if self.sr else SR_STEP_SEED if self.state_bits == 8 else 0
             h.step_table, h.step_cap = self._steps.ptr, self._steps_cap
         else:
             h = self._hyper()
-        api.anc_adamw_multi(self._table.ptr, len(self.st), self._total_blocks, ctypes.byref(h),
-                            ctl_ptr(guard), int(stream_int))
+        step = api.anc_adamw8_multi if self.state_bits == 8 else api.anc_adamw_multi
+        step(self._table.ptr, len(self.st), self._total_blocks, ctypes.byref(h), ctl_ptr(guard), int(stream_int))
 
     def unstep(self):
         """Undo the counter advance of a step the guard skipped (state was left untouched)."""
@@ -235,17 +277,19 @@ class AdamW:
 
     def state_dict(self):
         """Everything a resumed run needs, as host arrays: per tensor the fp32 master, both
-        moments and the bf16 weights, plus the step counter (it enters the bias corrections and
+        moments (8-bit ones as codes and scales) and the bf16 weights, plus the step counter (it enters the bias corrections and
         the stochastic-rounding seed). The reference has no optimizer checkpoint at all."""
         out = {"t": np.int64(self.t)}
         for n, s in self.st.items():
-            for k in ("p32", "m", "v", "p16"):
+            for k in self._kept:
                 out[f"{n}/{k}"] = s[k].to_numpy()
         return out
 
     def load_state_dict(self, sd, stream_int=0):
         for n, s in self.st.items():
-            for k in ("p32", "m", "v", "p16"):
+            for k in self._kept:
+                if f"{n}/{k}" not in sd:
+                    raise ValueError(f"AdamW.load_state_dict: '{n}/{k}' is missing (moments of {self.state_bits} bits are held here)")
                 a = np.asarray(sd[f"{n}/{k}"])
                 if a.size != s[k].size or a.dtype != s[k].dtype:
                     raise ValueError(f"AdamW.load_state_dict: '{n}/{k}' is {a.dtype}[{a.size}], "
@@ -257,12 +301,15 @@ class AdamW:
         return {n: s["p32"].numpy().reshape(s["shape"]) for n, s in self.st.items()}
 
     def moments(self):
+        if self.state_bits == 8:
+            return {n: tuple(moments8(s[k].numpy(), s[k + "s"].numpy(), values).reshape(s["shape"])
+                             for k, values in (("m", _E4M3), ("v", _E5M2))) for n, s in self.st.items()}
         return {n: (s["m"].numpy().reshape(s["shape"]), s["v"].numpy().reshape(s["shape"]))
                 for n, s in self.st.items()}
 
     def free(self):
         for s in self.st.values():
-            for k in ("g", "m", "v", "p32", "p16"):
+            for k in ("g", "m", "v", "p32", "p16") + (("scales", "ms", "vs") if self.state_bits == 8 else ()):
                 s[k].free()
         if self._table is not None:
             self._table.free()

@@ -62,12 +62,14 @@ __device__ __forceinline__ float anc_bf16_bits_to_f32(uint32_t b) {
 
 // Dither of the stochastic downcast (ancora/kernels/fused.py:154-161): a 16-bit
 // hash of the element's global (row, col) and the per-step seed, all uint32.
-__device__ __forceinline__ uint32_t anc_sr_dither(uint32_t row, uint32_t col, uint32_t seed) {
+__device__ __forceinline__ uint32_t anc_sr_hash(uint32_t row, uint32_t col, uint32_t seed) {
   uint32_t h = ((row * 73856093u) ^ (col * 19349663u) ^ seed) * 0x9E3779B1u;
   h ^= h >> 16;
   h *= 0x85EBCA6Bu;
-  h ^= h >> 13;
-  return h & 0xFFFFu;
+  return h ^ (h >> 13);
+}
+__device__ __forceinline__ uint32_t anc_sr_dither(uint32_t row, uint32_t col, uint32_t seed) {
+  return anc_sr_hash(row, col, seed) & 0xFFFFu;
 }
 // Stochastic rounding fp32 -> bf16 bits: (bits + dither) >> 16. Inf/NaN pass through
 // (a NaN keeps a non-zero mantissa) instead of carrying into the sign bit.

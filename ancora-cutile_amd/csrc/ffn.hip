@@ -1,0 +1,585 @@
+// The gated feed-forward block between two residual additions, dense or over tokens sorted by expert (anc_route), as four products:
+//
+//   gated   h = silu(x Wg) * (x Wu)                     x (rows, H), Wg, Wu (H, I), h (rows, I); optionally the pre-activations g, u
+//   down    y = h Wd + residual                         Wd (I, H)
+//   grad    dh = dy Wd^T;  dg = dh u s (1 + g (1 - s)), du = dh g s, h = g s u, s = sigmoid(g)
+//   dx      dx = dg Wg^T + du Wu^T + residual
+//
+// Weights lie (in, out), one after the other per expert, as the optimizer keeps its bf16 copies: forwards the contraction runs down their
+// columns, whose fragments come from transposing LDS reads, backwards along their rows, so no transposed copy exists. Products of bf16
+// accumulate in fp32 over ascending k (dx: all of dg, then all of du); each output is rounded once.
+//
+// k_ffn_tiles: a workgroup owns TM x 256 values of the product (gated: 128 columns of either weight, so that a lane holds g and u of the
+// same element) and runs k in steps of 32 through three LDS stages; wavefronts of 128 x 64. Operands go straight to LDS through descriptors
+// that end with the segment or the matrix: rows and columns beyond read zeros and are not stored.
+// k_ffn_few: up to 32 rows of a segment by 16 to 64 columns, the eight wavefronts of a workgroup taking every eighth step of k, each
+// with stages of its own and no barrier, and adding up at the end in a fixed order: with few rows the weights' bytes are the work, and
+// this way they are spread over as many CUs as there are.
+#include "lds_dma.h"
+#include "ns_common.h"
+
+namespace {
+
+enum { kGated, kDown, kGrad, kDx };
+constexpr int TK = 32;
+
+struct Ffn {
+  const uint16_t *A[2], *B[2];          // (rows, K) and per expert (K, N) forwards, (N, K) backwards
+  const int32_t *counts, *offsets;      // null: one segment of all rows
+  int64_t rows;                         // dense: rows; else slots
+  int K, N, experts, tn;                // tn: tiles side by side
+  const void *residual;
+  void *y;                              // down, dx; h otherwise
+  const uint16_t *gate, *up;
+  uint16_t *dgate, *dup;                // grad; gated: gate and up, null where not wanted
+  int y_f32;
+};
+
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+
+// Where a workgroup's tile lies: the expert, its first row in the buffers and how many of the segment's rows are left from there.
+struct Place { int e, n; int64_t row; int left; };
+
+// Workgroup id -> tile. The tiles of all segments, TM rows each, are counted on the device; ids go round the XCDs in equal runs, a run in
+// blocks of 8 row tiles by all columns, so that what an XCD works on at a time shares its L2.
+__device__ __forceinline__ bool place_of(const Ffn &p, int TM, Place &at) {
+  const int lane = (int)(threadIdx.x & 63);
+  int total = 0;
+  int tiles[8], upto[8], count[8], first[8];               // experts lane, lane + 64, ...: their tiles, and those up to and with them
+  if (p.counts == nullptr) {
+    total = (int)((p.rows + TM - 1) / TM);
+  } else {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      count[c] = first[c] = 0;
+      if (c * 64 < p.experts && c * 64 + lane < p.experts) {
+        count[c] = p.counts[c * 64 + lane];
+        first[c] = p.offsets[c * 64 + lane];
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      if (c * 64 >= p.experts) { tiles[c] = 0; upto[c] = total; continue; }
+      const int64_t f = first[c] < 0 ? 0 : first[c] < p.rows ? first[c] : p.rows, room = p.rows - f;      // (a segment stays inside its buffers, whatever the arrays hold)
+      first[c] = (int)f;
+      count[c] = count[c] < 0 ? 0 : count[c] < room ? count[c] : (int)room;
+      tiles[c] = (count[c] + TM - 1) / TM;
+      int v = tiles[c];
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int o = __shfl_up(v, off, 64);
+        v += lane >= off ? o : 0;
+      }
+      upto[c] = total + v;
+      total += __shfl(v, 63, 64);
+    }
+  }
+  total = __builtin_amdgcn_readfirstlane(total);
+  const int all = total * p.tn, share = (all + kXcds - 1) / kXcds, b = (int)blockIdx.x, q = b / kXcds;
+  const int id = b % kXcds * share + q;
+  if (q >= share || id >= all) return false;
+  const int group = id / (8 * p.tn), in = id - group * 8 * p.tn, high = total - group * 8 < 8 ? total - group * 8 : 8;
+  const int m = group * 8 + in % high;
+  at.n = in / high;
+  if (p.counts == nullptr) {
+    at.e = 0;
+    at.row = (int64_t)m * TM;
+    at.left = (int)(p.rows - at.row < 0x7FFFFFFF ? p.rows - at.row : 0x7FFFFFFF);
+    return true;
+  }
+  at.e = 0; at.row = 0; at.left = 0;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    const uint64_t hit = __ballot(c * 64 < p.experts && upto[c] > m && upto[c] - tiles[c] <= m);
+    if (hit == 0) continue;
+    const int l = __builtin_ctzll(hit);
+    const int mine = m - __builtin_amdgcn_readlane(upto[c] - tiles[c], l);
+    at.e = c * 64 + l;
+    at.row = (int64_t)__builtin_amdgcn_readlane(first[c], l) + (int64_t)mine * TM;
+    at.left = __builtin_amdgcn_readlane(count[c], l) - mine * TM;
+  }
+  at.e = __builtin_amdgcn_readfirstlane(at.e);
+  at.left = __builtin_amdgcn_readfirstlane(at.left);
+  return at.left > 0;
+}
+
+// One operand: where the next stage starts and how many bytes may be read from there on.
+struct Feed {
+  const char *at;
+  int64_t left, step;
+  __device__ __forceinline__ anc_i32x4 desc() const {
+    return buffer_of(at, left <= 0 ? 0u : left < 0x7FFFFFF0ll ? (uint32_t)left : 0x7FFFFFF0u);
+  }
+  __device__ __forceinline__ void next() { at += step; left -= step; }
+};
+constexpr uint32_t kNowhere = 0x80000000u;                 // an offset beyond every descriptor
+
+__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
+__device__ __forceinline__ void eight(const uint16_t *p, float (&f)[8]) {
+  const anc_u32x4 q = *(const anc_u32x4 *)p;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(q[i] << 16);
+    f[2 * i + 1] = __uint_as_float(q[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void put_eight(uint16_t *p, const float (&f)[8]) {
+  *(anc_u32x4 *)p = anc_u32x4{anc_pk_bf16(f[0], f[1]), anc_pk_bf16(f[2], f[3]), anc_pk_bf16(f[4], f[5]), anc_pk_bf16(f[6], f[7])};
+}
+// Eight neighbouring values of the product (gated: of both) at element `at` of the outputs.
+template <int MODE> __device__ __forceinline__ void finish(const Ffn &p, int64_t at, float (&v)[8], const float (&w)[8]) {
+  if constexpr (MODE == kGated) {
+    float h[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) h[k] = v[k] * sigmoid(v[k]) * w[k];
+    put_eight((uint16_t *)p.y + at, h);
+    if (p.dgate != nullptr) put_eight(p.dgate + at, v);
+    if (p.dup != nullptr) put_eight(p.dup + at, w);
+  } else if constexpr (MODE == kGrad) {
+    float g[8], u[8], dg[8], du[8], h[8];
+    eight(p.gate + at, g);
+    eight(p.up + at, u);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float s = sigmoid(g[k]), a = g[k] * s;
+      dg[k] = v[k] * u[k] * (s * (1.0f + g[k] * (1.0f - s)));
+      du[k] = v[k] * a;
+      h[k] = a * u[k];
+    }
+    put_eight(p.dgate + at, dg);
+    put_eight(p.dup + at, du);
+    if (p.y != nullptr) put_eight((uint16_t *)p.y + at, h);
+  } else if (p.y_f32) {
+    anc_f32x4 a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
+    if (p.residual != nullptr) {
+      const anc_f32x4 r = *(const anc_f32x4 *)((const float *)p.residual + at), s = *(const anc_f32x4 *)((const float *)p.residual + at + 4);
+      a = anc_f32x4{a.x + r.x, a.y + r.y, a.z + r.z, a.w + r.w};
+      b = anc_f32x4{b.x + s.x, b.y + s.y, b.z + s.z, b.w + s.w};
+    }
+    *(anc_f32x4 *)((float *)p.y + at) = a;
+    *(anc_f32x4 *)((float *)p.y + at + 4) = b;
+  } else {
+    if (p.residual != nullptr) {
+      float r[8];
+      eight((const uint16_t *)p.residual + at, r);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] += r[k];
+    }
+    put_eight((uint16_t *)p.y + at, v);
+  }
+}
+
+// ---------------------------------------------------------------- many rows
+template <int MODE, int TM> __global__ void __launch_bounds__(TM * 2, 2) k_ffn_tiles(Ffn p) {
+  constexpr bool kForward = MODE == kGated || MODE == kDown;
+  constexpr int kWaves = TM / 32, kBytesA = TM * 64, kBytesB = 256 * 64, kStage = kBytesA + kBytesB, kStages = 3;
+  constexpr int kPiecesA = kBytesA / 1024 / kWaves, kPiecesB = kBytesB / 1024 / kWaves, kPieces = kPiecesA + kPiecesB;
+  constexpr int kCols = MODE == kGated ? 128 : 256;         // columns of the outputs
+  static_assert(kWaves * 8192 <= kStages * kStage && kPieces <= 8, "room for the way out; pieces to a half step");
+  __shared__ __attribute__((aligned(1024))) unsigned char ring[kStages * kStage];
+  Place at;
+  if (!place_of(p, TM, at)) return;
+  const int K = p.K, N = p.N, lane = (int)(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int wm = wave >> 2, wn = wave & 3, n0 = at.n * kCols;
+  const int rows = at.left < TM ? at.left : TM, steps = (K + TK - 1) / TK, all = MODE == kDx ? 2 * steps : steps;
+
+  // Which of the B tile's two halves this wavefront fetches: forwards [32 k][128 columns] each (of either weight, or side by side), backwards rows.
+  const int half = wave * kPiecesB / 8;
+  Feed fa, fb;
+  auto term = [&](int t) {
+    fa = Feed{(const char *)(p.A[t] + at.row * K), (int64_t)rows * K * 2, TK * 2};
+    if constexpr (kForward) {
+      const int col = MODE == kGated ? n0 : n0 + half * 128;
+      fb = Feed{(const char *)(p.B[MODE == kGated ? half : 0] + (int64_t)at.e * K * N + col), ((int64_t)K * N - col) * 2, (int64_t)TK * N * 2};
+    } else {
+      const int high = N - n0 < 256 ? N - n0 : 256;
+      fb = Feed{(const char *)(p.B[t] + ((int64_t)at.e * N + n0) * K), (int64_t)high * K * 2, TK * 2};
+    }
+  };
+  term(0);
+  // Offsets of the pieces, 1 KiB of LDS each. Rows of 64 bytes: 16 to a piece, their four 16-byte chunks XORed with (row >> 2) & 3; rows of 256 bytes: 4 to a
+  // piece, chunks XORed with 4 * (row & 3). Of a row's last 32 k the chunks beyond K are sent nowhere, which reads zeros.
+  const int chunk = (lane & 3) ^ (lane >> 4);
+  const uint32_t beyond = chunk * 8 >= K - (steps - 1) * TK ? kNowhere : 0u;
+  uint32_t va[kPiecesA], vb[kPiecesB];
+#pragma unroll
+  for (int i = 0; i < kPiecesA; ++i) va[i] = (uint32_t)(((wave * kPiecesA + i) * 16 + (lane >> 2)) * K * 2 + chunk * 16);
+#pragma unroll
+  for (int i = 0; i < kPiecesB; ++i) {
+    const int piece = wave * kPiecesB + i;
+    if constexpr (kForward) vb[i] = (uint32_t)(((piece & 7) * 4 + (lane >> 4)) * N * 2 + (((lane & 15) ^ ((lane >> 4) << 2)) * 16));
+    else vb[i] = (uint32_t)((piece * 16 + (lane >> 2)) * K * 2 + chunk * 16);
+  }
+  int fetched = 0;
+  uint32_t mask = steps == 1 ? beyond : 0u;
+  auto issue = [&](int i, const anc_i32x4 &da, const anc_i32x4 &db, unsigned char *stage) {
+    if (i < kPiecesA) dma16_bounded(da, va[i] | mask, lds_addr(stage + (wave * kPiecesA + i) * 1024));
+    else dma16_bounded(db, kForward ? vb[i - kPiecesA] : vb[i - kPiecesA] | mask, lds_addr(stage + kBytesA + (wave * kPiecesB + i - kPiecesA) * 1024));
+  };
+  auto advance = [&]() {
+    ++fetched;
+    if (MODE == kDx && fetched == steps) term(1);
+    else if (fetched >= all) fa.left = fb.left = 0;
+    else { fa.next(); fb.next(); }
+    const int k = MODE == kDx && fetched >= steps ? fetched - steps : fetched;
+    mask = k == steps - 1 ? beyond : 0u;
+  };
+
+  int ta, tb[2];
+  ta = (wm * 128 + (lane & 31)) * 64;
+  if constexpr (kForward) {
+    const int s16 = lane & 15, g16 = lane >> 4, row = 8 * (g16 >> 1) + (s16 >> 2), sw = (s16 >> 2) << 2;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int sub = MODE == kGated ? j : wn >> 1, col = MODE == kGated ? wn * 4 : (wn & 1) * 8 + j * 4;     // (in chunks)
+      tb[j] = kBytesA + sub * 8192 + row * 256 + (((col + 2 * (g16 & 1) + ((s16 & 3) >> 1)) ^ sw) * 16) + (s16 & 1) * 8;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) tb[j] = kBytesA + (wn * 64 + j * 32 + (lane & 31)) * 64;
+  }
+  f32x16 acc[4][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+
+  bf16x8 a[2][4], c[2][2];
+  // fragment i (0 .. 5: b0 b1 a0 a1 a2 a3) of k 16 kk .. 16 kk + 15 of a stage
+  auto load = [&](int set, int i, const unsigned char *stage, int kk) {
+    const int sw = ((kk * 2 + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16;
+    if (i >= 2) a[set][i - 2] = *(const bf16x8 *)(stage + ta + (i - 2) * (32 * 64) + sw);
+    else if constexpr (kForward) c[set][i] = anc_lds_tr_frag(stage + tb[i] + kk * (16 * 256), stage + tb[i] + kk * (16 * 256) + 4 * 256);
+    else c[set][i] = *(const bf16x8 *)(stage + tb[i] + sw);
+  };
+  auto multiply = [&](int set, int idx) {        // operands exchanged: a lane holds runs of 4 columns of one row
+    acc[idx >> 1][idx & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c[set][idx & 1], a[set][idx >> 1], acc[idx >> 1][idx & 1], 0, 0, 0);
+  };
+  for (int i = 0; i < kStages; ++i) {
+    const anc_i32x4 da = fa.desc(), db = fb.desc();
+#pragma unroll
+    for (int q = 0; q < kPieces; ++q) issue(q, da, db, ring + i * kStage);
+    advance();
+  }
+  wait_vm<(kStages - 1) * kPieces>();
+  lds_barrier();
+#pragma unroll
+  for (int i = 0; i < 6; ++i) load(0, i, ring, 0);
+  // One step: the first half's products over the reads of the second half; then every wavefront has read the stage and the next
+  // one has landed for all; then the second half's products over the next stage's first reads and the fetches into the place just read.
+  auto step = [&](unsigned char *here, unsigned char *next) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      multiply(0, i);
+      __builtin_amdgcn_sched_barrier(0);
+      if (i < 6) load(1, i, here, 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    wait_vm<(kStages - 2) * kPieces>();
+    lds_barrier();
+    const anc_i32x4 da = fa.desc(), db = fb.desc();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      multiply(1, i);
+      __builtin_amdgcn_sched_barrier(0);
+      if (i < 6) load(0, i, next, 0);
+      if (i < kPieces) issue(i, da, db, here);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    advance();
+  };
+  int here = 0;
+  for (int t = 0; t < all; ++t) {
+    const int next = here + kStage < kStages * kStage ? here + kStage : 0;
+    step(ring + here, ring + next);
+    here = next;
+  }
+  wait_vm<0>();                                  // (zeros still on their way into the stages)
+  lds_barrier();
+
+  // Out through LDS, 32 rows of 64 values at a time: a lane then holds 8 neighbouring columns of a row.
+  unsigned char *r = ring + wave * 8192;
+  constexpr int kOcts = MODE == kGated ? 4 : 8;
+  const int col0 = n0 + wn * (MODE == kGated ? 32 : 64);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int rr = lane & 31, hh = lane >> 5;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *(anc_f32x4 *)(r + rr * 256 + (((j * 8 + 2 * g + hh) ^ (rr & 15)) * 16)) =
+            anc_f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+    lds_wave_sync();
+#pragma unroll
+    for (int z = 0; z < kOcts / 2; ++z) {
+      const int idx = z * 64 + lane, row = idx / kOcts, oct = idx % kOcts, in = wm * 128 + i * 32 + row, col = col0 + oct * 8;
+      auto values = [&](int ch, float (&f)[8]) {
+        const anc_f32x4 lo = *(const anc_f32x4 *)(r + row * 256 + ((ch ^ (row & 15)) * 16)), hi = *(const anc_f32x4 *)(r + row * 256 + (((ch + 1) ^ (row & 15)) * 16));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { f[k] = lo[k]; f[4 + k] = hi[k]; }
+      };
+      float v[8], w[8];
+      values(2 * oct, v);
+      if constexpr (MODE == kGated) values(8 + 2 * oct, w);
+      if (in < rows && col < N) finish<MODE>(p, (at.row + in) * N + col, v, w);
+    }
+    lds_wave_sync();
+  }
+}
+
+// ---------------------------------------------------------------- few rows
+// C blocks of 16 columns (gated: half of them of either weight).
+template <int MODE, int C> __global__ void __launch_bounds__(512, 2) k_ffn_few(Ffn p) {
+  constexpr bool kForward = MODE == kGated || MODE == kDown;
+  constexpr int TM = 32, kWaves = 8, kStages = C == 4 ? 2 : 3, kStage = 2048 + C * 1024, kPieces = 2 + C;
+  constexpr int kSub = MODE == kGated ? C / 2 : C;          // blocks of a row of one weight
+  constexpr int kRowB = kSub * 32, kPer = 1024 / kRowB;     // bytes of it, rows to a piece
+  constexpr int kCols = kSub * 16;
+  __shared__ __attribute__((aligned(1024))) unsigned char ring[kWaves * kStages * kStage];
+  static_assert(kWaves * 32 * C * 64 <= sizeof(ring), "room for the partial sums");
+  Place at;
+  if (!place_of(p, TM, at)) return;
+  const int K = p.K, N = p.N, lane = (int)(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int n0 = at.n * kCols, rows = at.left < TM ? at.left : TM, steps = (K + TK - 1) / TK, all = MODE == kDx ? 2 * steps : steps;
+  unsigned char *mine = ring + wave * kStages * kStage;
+  const int chunk = (lane & 3) ^ (lane >> 4);
+  const uint32_t beyond = chunk * 8 >= K - (steps - 1) * TK ? kNowhere : 0u;
+  const uint32_t va = (uint32_t)((lane >> 2) * K * 2 + chunk * 16);
+  const uint32_t vb = kForward ? (uint32_t)(lane / (kRowB / 16) * N * 2 + lane % (kRowB / 16) * 16) : va;
+  auto fetch = [&](int t, unsigned char *stage) {           // step t of all; beyond them nothing is read
+    const int second = MODE == kDx && t >= steps, k = t - (second ? steps : 0), k0 = k * TK;
+    const bool there = t < all;
+    const uint32_t mask = k == steps - 1 ? beyond : 0u;
+    const int64_t lefta = ((int64_t)rows * K - k0) * 2;
+    const anc_i32x4 da = buffer_of((const char *)(p.A[second] + at.row * K + (there ? k0 : 0)), there ? (uint32_t)lefta : 0u);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) dma16_bounded(da, (va + (uint32_t)(i * 16 * K * 2)) | mask, lds_addr(stage + i * 1024));
+    if constexpr (kForward) {
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        const int w = MODE == kGated ? i / (C / 2 > 0 ? C / 2 : 1) : 0, piece = MODE == kGated ? i % (C / 2 > 0 ? C / 2 : 1) : i;
+        const Feed f{(const char *)(p.B[w] + (int64_t)at.e * K * N + (there ? (int64_t)k0 * N : 0) + n0), there ? ((int64_t)(K - k0) * N - n0) * 2 : 0, 0};
+        dma16_bounded(f.desc(), vb + (uint32_t)(piece * kPer * N * 2), lds_addr(stage + 2048 + i * 1024));
+      }
+    } else {
+      const int high = N - n0 < kCols ? N - n0 : kCols;
+      const anc_i32x4 db = buffer_of((const char *)(p.B[second] + ((int64_t)at.e * N + n0) * K + (there ? k0 : 0)), there ? (uint32_t)(((int64_t)high * K - k0) * 2) : 0u);
+#pragma unroll
+      for (int i = 0; i < C; ++i) dma16_bounded(db, (vb + (uint32_t)(i * 16 * K * 2)) | mask, lds_addr(stage + 2048 + i * 1024));
+    }
+  };
+  f32x4v acc[2][C];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < C; ++j) acc[i][j] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
+  const int s16 = lane & 15, g16 = lane >> 4;
+  const int ta = s16 * 64 + ((g16 ^ ((s16 >> 2) & 3)) * 16);
+  for (int i = 0; i < kStages; ++i) fetch(wave + i * kWaves, mine + i * kStage);
+  int here = 0;
+  for (int t = wave; t < all; t += kWaves) {
+    const unsigned char *stage = mine + here;
+    wait_vm<(kStages - 1) * kPieces>();
+    bf16x8 a[2], b[C];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) a[i] = *(const bf16x8 *)(stage + i * 1024 + ta);
+#pragma unroll
+    for (int j = 0; j < C; ++j) {
+      if constexpr (kForward) {
+        const unsigned char *q = stage + 2048 + j / kSub * (kSub * 1024) + (8 * g16 + (s16 >> 2)) * kRowB + j % kSub * 32 + (s16 & 3) * 8;
+        b[j] = anc_lds_tr_frag(q, q + 4 * kRowB);
+      } else {
+        b[j] = *(const bf16x8 *)(stage + 2048 + j * 1024 + ta);
+      }
+    }
+    lds_wave_sync();                             // (read before the stage is fetched into again)
+    fetch(t + kStages * kWaves, mine + here);
+#pragma unroll
+    for (int j = 0; j < C; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
+    here = here + kStage < kStages * kStage ? here + kStage : 0;
+  }
+  wait_vm<0>();
+  lds_barrier();
+  // The wavefronts' sums, in ascending order: [wavefront][row][column] fp32.
+  float *sums = (float *)ring;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < C; ++j) *(f32x4v *)(sums + (wave * 32 + i * 16 + s16) * (C * 16) + j * 16 + g16 * 4) = acc[i][j];
+  lds_barrier();
+  constexpr int kOcts = kCols / 8;
+  for (int idx = (int)threadIdx.x; idx < 32 * kOcts; idx += kWaves * 64) {
+    const int row = idx / kOcts, oct = idx % kOcts, col = n0 + oct * 8;
+    if (row >= rows || col >= N) continue;
+    auto total = [&](int first, float (&f)[8]) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = sums[row * (C * 16) + first + k];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] += sums[(w * 32 + row) * (C * 16) + first + k];
+    };
+    float v[8], w[8];
+    total(oct * 8, v);
+    if constexpr (MODE == kGated) total(kCols + oct * 8, w);
+    finish<MODE>(p, (at.row + row) * N + col, v, w);
+  }
+}
+
+// ---------------------------------------------------------------- launch
+template <int MODE> int launch(Ffn p, const char *who, hipStream_t s) {
+  const int64_t E = p.experts > 0 ? p.experts : 1, mean = (p.rows + E - 1) / E;
+  const int64_t some = p.rows < E ? p.rows : E;              // segments that can hold a row
+  const int wide = MODE == kGated ? 128 : 256;
+  auto row_tiles = [&](int64_t TM) { return p.counts == nullptr ? (p.rows + TM - 1) / TM : p.rows / TM + some; };
+  auto grid_of = [&](int64_t TM) { return (row_tiles(TM) * p.tn + kXcds - 1) / kXcds * kXcds; };
+  AncProfScope prof(ANC_PROF_DW_GEMM, s);
+  if (mean <= 48) {
+    constexpr int kLeast = MODE == kGated ? 2 : 1;
+    int C = 4;
+    while (C > kLeast && row_tiles(32) * ((p.N + 16 * C / kLeast - 1) / (16 * C / kLeast)) < 256) C /= 2;
+    p.tn = (p.N + 16 * C / kLeast - 1) / (16 * C / kLeast);
+    ANC_REQUIRE(grid_of(32) < (1ll << 31) / 512, "%s: too large for one call", who);
+    const dim3 grid((unsigned)grid_of(32));
+    if (C == 4) hipLaunchKernelGGL((k_ffn_few<MODE, 4>), grid, dim3(512), 0, s, p);
+    else if (C == 2) hipLaunchKernelGGL((k_ffn_few<MODE, 2>), grid, dim3(512), 0, s, p);
+    else if constexpr (MODE != kGated) hipLaunchKernelGGL((k_ffn_few<MODE, 1>), grid, dim3(512), 0, s, p);
+  } else {
+    p.tn = (p.N + wide - 1) / wide;
+    const bool high = ((p.rows + 255) / 256) * p.tn >= 256;
+    const int TM = high ? 256 : 128;
+    ANC_REQUIRE(grid_of(TM) < (1ll << 31) / 512, "%s: too large for one call", who);
+    const dim3 grid((unsigned)grid_of(TM));
+    if (high) hipLaunchKernelGGL((k_ffn_tiles<MODE, 256>), grid, dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((k_ffn_tiles<MODE, 128>), grid, dim3(256), 0, s, p);
+  }
+  ANC_LAUNCH_CHECK();
+  return ANC_OK;
+}
+
+int check(const char *who, uint64_t counts, uint64_t offsets, int64_t experts, int64_t rows, int64_t H, int64_t I) {
+  ANC_REQUIRE(H > 0 && I > 0 && H % 8 == 0 && I % 8 == 0 && H <= (1 << 17) && I <= (1 << 17),
+              "%s: needs H %% 8 == 0 and I %% 8 == 0 (H=%lld I=%lld)", who, (long long)H, (long long)I);
+  ANC_REQUIRE(rows >= 0 && rows < (1ll << 31), "%s: %lld rows", who, (long long)rows);
+  ANC_REQUIRE((counts != 0) == (experts > 0) && (offsets != 0) == (experts > 0) && ((counts | offsets) & 3) == 0 && experts >= 0 && experts <= 512,
+              "%s: bad segments (%lld experts)", who, (long long)experts);
+  return ANC_OK;
+}
+// Outputs meet no other buffer of the call, but for the pairs that are one buffer on purpose (the same elements, read before they are written).
+template <int O, int I> int apart(const char *who, const AncSpan (&out)[O], const AncSpan (&in)[I], const int (&pair)[O]) {
+  ANC_REQUIRE(anc_outputs_apart(out, O), "%s: outputs overlap", who);
+  for (int i = 0; i < O; ++i)
+    for (int j = 0; j < I; ++j)
+      ANC_REQUIRE((pair[i] == j && out[i].at == in[j].at && out[i].bytes == in[j].bytes) || anc_apart(out[i].at, out[i].bytes, in[j].at, in[j].bytes),
+                  "%s: an output overlaps an input", who);
+  return ANC_OK;
+}
+AncSpan span(uint64_t at, int64_t bytes) { return AncSpan{at, at != 0 ? bytes : 0}; }
+
+}  // namespace
+
+extern "C" int anc_gated_ffn(uint64_t x, uint64_t Wg, uint64_t Wu, uint64_t counts, uint64_t offsets, int64_t experts, int64_t rows,
+                             int64_t H, int64_t I, uint64_t h, uint64_t gate, uint64_t up, uint64_t stream) {
+  const char *who = "anc_gated_ffn";
+  if (int rc = check(who, counts, offsets, experts, rows, H, I)) return rc;
+  if (rows == 0) return ANC_OK;
+  ANC_REQUIRE(x && Wg && Wu && h && ((x | Wg | Wu | h | gate | up) & 15) == 0, "%s: null or misaligned pointer", who);
+  const int64_t E = experts > 0 ? experts : 1, w = E * H * I * 2, n = rows * I * 2;
+  if (int rc = apart<3, 5>(who, {span(h, n), span(gate, n), span(up, n)},
+                           {span(x, rows * H * 2), span(Wg, w), span(Wu, w), span(counts, 4 * experts), span(offsets, 4 * experts + 4)}, {-1, -1, -1})) return rc;
+  Ffn p{};
+  p.A[0] = (const uint16_t *)x;
+  p.B[0] = (const uint16_t *)Wg;
+  p.B[1] = (const uint16_t *)Wu;
+  p.counts = (const int32_t *)counts;
+  p.offsets = (const int32_t *)offsets;
+  p.rows = rows;
+  p.K = (int)H;
+  p.N = (int)I;
+  p.experts = (int)experts;
+  p.y = (void *)h;
+  p.dgate = (uint16_t *)gate;
+  p.dup = (uint16_t *)up;
+  return launch<kGated>(p, who, anc_stream(stream));
+}
+
+extern "C" int anc_ffn_down(uint64_t h, uint64_t Wd, uint64_t counts, uint64_t offsets, int64_t experts, int64_t rows, int64_t I,
+                            int64_t H, uint64_t residual, uint64_t y, int y_type, uint64_t stream) {
+  const char *who = "anc_ffn_down";
+  if (int rc = check(who, counts, offsets, experts, rows, H, I)) return rc;
+  ANC_REQUIRE(y_type == ANC_F32 || y_type == ANC_BF16, "%s: bad y_type %d", who, y_type);
+  if (rows == 0) return ANC_OK;
+  ANC_REQUIRE(h && Wd && y && ((h | Wd | y | residual) & 15) == 0, "%s: null or misaligned pointer", who);
+  const int64_t E = experts > 0 ? experts : 1, n = rows * H * (y_type == ANC_F32 ? 4 : 2);
+  if (int rc = apart<1, 5>(who, {span(y, n)}, {span(residual, n), span(h, rows * I * 2), span(Wd, E * H * I * 2), span(counts, 4 * experts), span(offsets, 4 * experts + 4)}, {0})) return rc;
+  Ffn p{};
+  p.A[0] = (const uint16_t *)h;
+  p.B[0] = (const uint16_t *)Wd;
+  p.counts = (const int32_t *)counts;
+  p.offsets = (const int32_t *)offsets;
+  p.rows = rows;
+  p.K = (int)I;
+  p.N = (int)H;
+  p.experts = (int)experts;
+  p.residual = (const void *)residual;
+  p.y = (void *)y;
+  p.y_f32 = y_type == ANC_F32;
+  return launch<kDown>(p, who, anc_stream(stream));
+}
+
+extern "C" int anc_gated_ffn_grad(uint64_t dy, uint64_t Wd, uint64_t gate, uint64_t up, uint64_t counts, uint64_t offsets, int64_t experts,
+                                  int64_t rows, int64_t H, int64_t I, uint64_t dgate, uint64_t dup, uint64_t h, uint64_t stream) {
+  const char *who = "anc_gated_ffn_grad";
+  if (int rc = check(who, counts, offsets, experts, rows, H, I)) return rc;
+  if (rows == 0) return ANC_OK;
+  ANC_REQUIRE(dy && Wd && gate && up && dgate && dup && ((dy | Wd | gate | up | dgate | dup | h) & 15) == 0, "%s: null or misaligned pointer", who);
+  const int64_t E = experts > 0 ? experts : 1, n = rows * I * 2;
+  if (int rc = apart<3, 6>(who, {span(dgate, n), span(dup, n), span(h, n)},
+                           {span(gate, n), span(up, n), span(dy, rows * H * 2), span(Wd, E * H * I * 2), span(counts, 4 * experts), span(offsets, 4 * experts + 4)}, {0, 1, -1})) return rc;
+  Ffn p{};
+  p.A[0] = (const uint16_t *)dy;
+  p.B[0] = (const uint16_t *)Wd;
+  p.counts = (const int32_t *)counts;
+  p.offsets = (const int32_t *)offsets;
+  p.rows = rows;
+  p.K = (int)H;
+  p.N = (int)I;
+  p.experts = (int)experts;
+  p.gate = (const uint16_t *)gate;
+  p.up = (const uint16_t *)up;
+  p.dgate = (uint16_t *)dgate;
+  p.dup = (uint16_t *)dup;
+  p.y = (void *)h;
+  return launch<kGrad>(p, who, anc_stream(stream));
+}
+
+extern "C" int anc_gated_ffn_dx(uint64_t dgate, uint64_t dup, uint64_t Wg, uint64_t Wu, uint64_t counts, uint64_t offsets, int64_t experts,
+                                int64_t rows, int64_t H, int64_t I, uint64_t residual, uint64_t dx, int dx_type, uint64_t stream) {
+  const char *who = "anc_gated_ffn_dx";
+  if (int rc = check(who, counts, offsets, experts, rows, H, I)) return rc;
+  ANC_REQUIRE(dx_type == ANC_F32 || dx_type == ANC_BF16, "%s: bad dx_type %d", who, dx_type);
+  if (rows == 0) return ANC_OK;
+  ANC_REQUIRE(dgate && dup && Wg && Wu && dx && ((dgate | dup | Wg | Wu | dx | residual) & 15) == 0, "%s: null or misaligned pointer", who);
+  const int64_t E = experts > 0 ? experts : 1, w = E * H * I * 2, n = rows * H * (dx_type == ANC_F32 ? 4 : 2);
+  if (int rc = apart<1, 7>(who, {span(dx, n)}, {span(residual, n), span(dgate, rows * I * 2), span(dup, rows * I * 2), span(Wg, w), span(Wu, w), span(counts, 4 * experts), span(offsets, 4 * experts + 4)}, {0})) return rc;
+  Ffn p{};
+  p.A[0] = (const uint16_t *)dgate;
+  p.A[1] = (const uint16_t *)dup;
+  p.B[0] = (const uint16_t *)Wg;
+  p.B[1] = (const uint16_t *)Wu;
+  p.counts = (const int32_t *)counts;
+  p.offsets = (const int32_t *)offsets;
+  p.rows = rows;
+  p.K = (int)I;
+  p.N = (int)H;
+  p.experts = (int)experts;
+  p.residual = (const void *)residual;
+  p.y = (void *)dx;
+  p.y_f32 = dx_type == ANC_F32;
+  return launch<kDx>(p, who, anc_stream(stream));
+}

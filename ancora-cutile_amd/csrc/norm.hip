@@ -1,0 +1,394 @@
+// Root-mean-square norm of rows with the residual's addition in front of it and, for products in 8 bits, MXFP8 rows behind it; and its
+// backward pass. The reference's layers run it between the optimizer's weights; its gain is one of AdamW's tensors.
+//
+//   s = x + residual,  r = 1 / sqrt(mean(s^2) + eps),  y = s r gain                                (all in fp32, one rounding per output)
+//   MXFP8: per 32 elements of a row byte = (biased exponent of the largest |y|) - 7 (0 below 7), element = E4M3(y 2^(127 - byte)): the
+//   format of quant.hip with the blocks along the row, which is the axis that a product with the weights runs over
+//   a = dy gain,  dx = r (a - s r^2 mean(a s)) + carry,  dgain = sum over rows of dy s r
+//
+// HBM-bound. A row is held in registers by 16, 64 or 256 lanes, 8 elements (16 bytes of bf16) to a piece, so that it is read once.
+// The gain's gradient: workgroups add up their rows in registers, then their groups of lanes through LDS, and leave one fp32 row each; a
+// second launch adds those in a fixed order. The bits are a function of the inputs and the shape.
+#include "rows.h"
+
+namespace {
+
+using anc_rows::bf16_pair;
+constexpr int kThreads = 256;
+constexpr int kMostRows = 512;          // partial rows of dgain
+
+template <int T> struct Eight;
+template <> struct Eight<ANC_BF16> { anc_u32x4 q; };
+template <> struct Eight<ANC_F32> { anc_f32x4 q, r; };
+template <int T> __device__ __forceinline__ Eight<T> load8(uint64_t p, int64_t e) {
+  if constexpr (T == ANC_BF16) return {*(const anc_u32x4 *)((const uint16_t *)p + e)};
+  else return {*(const anc_f32x4 *)((const float *)p + e), *(const anc_f32x4 *)((const float *)p + e + 4)};
+}
+template <int T> __device__ __forceinline__ void widen(const Eight<T> &v, float (&f)[8]) {
+  if constexpr (T == ANC_BF16) {
+    const uint32_t w[4] = {v.q.x, v.q.y, v.q.z, v.q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[i] = v.q[i];
+      f[4 + i] = v.r[i];
+    }
+  }
+}
+template <int T> __device__ __forceinline__ void store8(uint64_t p, int64_t e, const float (&f)[8]) {
+  if constexpr (T == ANC_BF16) {
+    *(anc_u32x4 *)((uint16_t *)p + e) = anc_u32x4{bf16_pair(f[0], f[1]), bf16_pair(f[2], f[3]), bf16_pair(f[4], f[5]), bf16_pair(f[6], f[7])};
+  } else {
+    *(anc_f32x4 *)((float *)p + e) = anc_f32x4{f[0], f[1], f[2], f[3]};
+    *(anc_f32x4 *)((float *)p + e + 4) = anc_f32x4{f[4], f[5], f[6], f[7]};
+  }
+}
+
+// Sum over the LPR lanes of a row, in all of them, in a fixed order. LPR = 256: every lane of the workgroup calls it.
+template <int LPR> __device__ __forceinline__ float row_sum(float v, float *lds) {
+#pragma unroll
+  for (int off = LPR == 16 ? 8 : 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+  if constexpr (LPR == 256) {
+    __syncthreads();                                  // (the last call's values have been read)
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = (lds[0] + lds[1]) + (lds[2] + lds[3]);
+  }
+  return v;
+}
+
+struct NormArgs {
+  uint64_t x, residual, gain, y, scale, total, rstd;
+  int64_t T;
+  int H;
+  float eps;
+};
+constexpr int kMx8 = 2;                 // beside ANC_F32 and ANC_BF16
+
+template <int XT, int ST, int GT, int OT, bool RES, int LPR, int CH>
+__global__ void __launch_bounds__(kThreads) k_rms_norm(NormArgs a) {
+  __shared__ float lds[4];
+  const int sub = (int)threadIdx.x % LPR;
+  const int64_t row = (int64_t)blockIdx.x * (kThreads / LPR) + (int)threadIdx.x / LPR;
+  const bool live = row < a.T;                        // (a wavefront's other rows still take part in its shuffles)
+  const int64_t base = (live ? row : 0) * a.H;
+  Eight<XT> x8[CH];
+  Eight<ST> r8[CH];
+  Eight<GT> g8[CH];
+  bool on[CH];
+#pragma unroll
+  for (int j = 0; j < CH; ++j) {
+    const int col = (sub + j * LPR) * 8;
+    on[j] = live && col < a.H;
+    if (on[j]) {
+      x8[j] = load8<XT>(a.x, base + col);
+      if constexpr (RES) r8[j] = load8<ST>(a.residual, base + col);
+      g8[j] = load8<GT>(a.gain, col);
+    }
+  }
+  float s[CH][8], sum = 0.0f;
+#pragma unroll
+  for (int j = 0; j < CH; ++j) {
+    if (!on[j]) continue;
+    widen<XT>(x8[j], s[j]);
+    if constexpr (RES) {
+      float r[8];
+      widen<ST>(r8[j], r);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s[j][k] += r[k];
+      store8<ST>(a.total, base + (sub + j * LPR) * 8, s[j]);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum = __builtin_fmaf(s[j][k], s[j][k], sum);
+  }
+  sum = row_sum<LPR>(sum, lds);
+  const float r = 1.0f / sqrtf(sum / (float)a.H + a.eps);
+  if (a.rstd != 0 && live && sub == 0) ((float *)a.rstd)[row] = r;
+#pragma unroll
+  for (int j = 0; j < CH; ++j) {
+    if (!on[j]) continue;
+    const int64_t at = base + (sub + j * LPR) * 8;
+    float y[8], g[8];
+    widen<GT>(g8[j], g);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y[k] = s[j][k] * r * g[k];
+    if constexpr (OT != kMx8) {
+      store8<OT>(a.y, at, y);
+    } else {
+      uint32_t amax = 0u;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t b = __float_as_uint(y[k]) & 0x7FFFFFFFu;
+        amax = amax > b ? amax : b;
+      }
+      // four neighbouring lanes hold a block (H % 32 == 0: all of them or none)
+      uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)amax, 0xB1, 0xF, 0xF, true);      // lane ^ 1
+      amax = amax > o ? amax : o;
+      o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)amax, 0x4E, 0xF, 0xF, true);                // lane ^ 2
+      amax = amax > o ? amax : o;
+      const uint32_t ea = amax >> 23, byte = ea >= 7u ? ea - 7u : 0u;
+      const float up = __uint_as_float((254u - byte) << 23);
+      uint32_t w[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2] * up, y[4 * h + 3] * up,
+                                                         __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h] * up, y[4 * h + 1] * up, 0, false), true);
+      if (ea == 255u) {                                // something is not finite: those elements become NaN codes
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if ((__float_as_uint(y[k]) & 0x7F800000u) == 0x7F800000u)
+            w[k >> 2] = (w[k >> 2] & ~(0xFFu << (8 * (k & 3)))) | ((0x7Fu | ((__float_as_uint(y[k]) >> 24) & 0x80u)) << (8 * (k & 3)));
+      }
+      *(anc_u32x2 *)((uint8_t *)a.y + at) = anc_u32x2{w[0], w[1]};
+      if ((threadIdx.x & 3) == 0) ((uint8_t *)a.scale)[at >> 5] = (uint8_t)byte;
+    }
+  }
+}
+
+struct GradArgs {
+  uint64_t dy, x, gain, rstd, carry, dx, dgain, parts;
+  int64_t T;
+  int H, rows, accumulate;              // rows of dgain in parts: the grid
+};
+
+// Group g of workgroup b takes rows b * groups + g, then every rows * groups further.
+template <int DT, int ST, int GT, bool CARRY, int LPR, int CH>
+__global__ void __launch_bounds__(kThreads) k_rms_norm_grad(GradArgs a) {
+  constexpr int kGroups = kThreads / LPR;
+  __shared__ float lds[4];
+  __shared__ float sums[kGroups > 1 ? kGroups * LPR * CH * 8 : 1];
+  const int sub = (int)threadIdx.x % LPR, group = (int)threadIdx.x / LPR;
+  float g[CH][8], dg[CH][8];
+#pragma unroll
+  for (int j = 0; j < CH; ++j) {
+    const int col = (sub + j * LPR) * 8;
+    if (col < a.H) widen<GT>(load8<GT>(a.gain, col), g[j]);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) dg[j][k] = 0.0f;
+  }
+  for (int64_t row0 = (int64_t)blockIdx.x * kGroups; row0 < a.T; row0 += (int64_t)a.rows * kGroups) {
+    const int64_t row = row0 + group;
+    const bool live = row < a.T;
+    const int64_t base = (live ? row : 0) * a.H;
+    const float r = ((const float *)a.rstd)[live ? row : 0];
+    Eight<DT> d8[CH];
+    Eight<ST> s8[CH], c8[CH];
+    bool on[CH];
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      const int col = (sub + j * LPR) * 8;
+      on[j] = live && col < a.H;
+      if (on[j]) {
+        d8[j] = load8<DT>(a.dy, base + col);
+        s8[j] = load8<ST>(a.x, base + col);
+        if constexpr (CARRY) c8[j] = load8<ST>(a.carry, base + col);
+      }
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      if (!on[j]) continue;
+      float d[8], s[8];
+      widen<DT>(d8[j], d);
+      widen<ST>(s8[j], s);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float xh = s[k] * r;
+        dg[j][k] = __builtin_fmaf(d[k], xh, dg[j][k]);
+        sum = __builtin_fmaf(d[k] * g[j][k], xh, sum);
+      }
+    }
+    const float c = row_sum<LPR>(sum, lds) / (float)a.H;
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      if (!on[j]) continue;
+      float d[8], s[8], o[8];
+      widen<DT>(d8[j], d);
+      widen<ST>(s8[j], s);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) o[k] = r * (d[k] * g[j][k] - s[k] * r * c);
+      if constexpr (CARRY) {
+        float f[8];
+        widen<ST>(c8[j], f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] += f[k];
+      }
+      store8<ST>(a.dx, base + (sub + j * LPR) * 8, o);
+    }
+  }
+  // the groups' sums in ascending order
+  if constexpr (kGroups > 1) {
+#pragma unroll
+    for (int j = 0; j < CH; ++j)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sums[group * LPR * CH * 8 + (sub + j * LPR) * 8 + k] = dg[j][k];
+    __syncthreads();
+  }
+  float *out = a.rows > 1 ? (float *)a.parts + (int64_t)blockIdx.x * a.H : (float *)a.dgain;
+  const bool onto = a.rows == 1 && a.accumulate;
+  if constexpr (kGroups > 1) {
+    for (int col = (int)threadIdx.x; col < a.H; col += kThreads) {
+      float v = sums[col];
+#pragma unroll
+      for (int q = 1; q < kGroups; ++q) v += sums[q * LPR * CH * 8 + col];
+      out[col] = onto ? out[col] + v : v;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      const int col = (sub + j * LPR) * 8;
+      if (col >= a.H) continue;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) out[col + k] = onto ? out[col + k] + dg[j][k] : dg[j][k];
+    }
+  }
+}
+
+// dgain (+)= the sum of `rows` rows: 32 columns to a workgroup, 32 of its groups of 8 lanes taking every 32nd row.
+__global__ void __launch_bounds__(kThreads) k_gain_sum(const float *parts, float *dgain, int rows, int H, int accumulate) {
+  __shared__ float sums[32][33];
+  const int c4 = (int)threadIdx.x & 7, q = (int)threadIdx.x >> 3, col = (int)blockIdx.x * 32 + c4 * 4;
+  anc_f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (col < H) {
+#pragma unroll 4
+    for (int r = q; r < rows; r += 32) {
+      const anc_f32x4 p = *(const anc_f32x4 *)(parts + (int64_t)r * H + col);
+      v = anc_f32x4{v.x + p.x, v.y + p.y, v.z + p.z, v.w + p.w};
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) sums[q][c4 * 4 + k] = v[k];
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const int c = (int)blockIdx.x * 32 + (int)threadIdx.x;
+    if (c < H) {
+      float t = sums[0][threadIdx.x];
+#pragma unroll
+      for (int r = 1; r < 32; ++r) t += sums[r][threadIdx.x];
+      dgain[c] = accumulate ? dgain[c] + t : t;
+    }
+  }
+}
+
+constexpr int kWidest = 16384;
+template <int V> struct IC { static constexpr int value = V; };
+template <typename F> void with_type(int t, F &&f) {
+  if (t == ANC_BF16) f(IC<ANC_BF16>{}); else f(IC<ANC_F32>{});
+}
+// Lanes per row and pieces per lane.
+template <typename F> void with_layout(int H, F &&f) {
+  const int pieces = H / 8;
+  if (pieces <= 16) f(IC<16>{}, IC<1>{});
+  else if (pieces <= 32) f(IC<16>{}, IC<2>{});
+  else if (pieces <= 64) f(IC<64>{}, IC<1>{});
+  else if (pieces <= 128) f(IC<64>{}, IC<2>{});
+  else if (pieces <= 256) f(IC<64>{}, IC<4>{});
+  else if (pieces <= 512) f(IC<256>{}, IC<2>{});
+  else if (pieces <= 1024) f(IC<256>{}, IC<4>{});
+  else f(IC<256>{}, IC<8>{});
+}
+int lanes_of(int64_t H) { return H <= 256 ? 16 : H <= 2048 ? 64 : 256; }
+bool width_ok(int64_t H) { return H > 0 && H % 8 == 0 && H <= kWidest; }
+bool type_ok(int t) { return t == ANC_F32 || t == ANC_BF16; }
+int64_t elem(int t) { return t == ANC_BF16 ? 2 : 4; }
+// Partial rows of dgain: two rows of the batch per group of lanes at least, as many workgroups as keep the memory busy at most.
+int64_t parts_of(int64_t T, int64_t H) {
+  const int64_t per = 2 * (kThreads / lanes_of(H)), n = (T + per - 1) / per;
+  return n < 1 ? 1 : n > kMostRows ? kMostRows : n;
+}
+
+}  // namespace
+
+extern "C" int anc_rms_norm(uint64_t x, int x_type, uint64_t residual, int stream_type, uint64_t gain, int gain_type, int64_t T, int64_t H,
+                            float eps, uint64_t y, int y_type, uint64_t scale, uint64_t total, uint64_t rstd, uint64_t stream) {
+  ANC_REQUIRE(type_ok(x_type) && type_ok(stream_type) && type_ok(gain_type) && (type_ok(y_type) || y_type == ANC_MXFP8),
+              "anc_rms_norm: bad types (x %d, stream %d, gain %d, y %d)", x_type, stream_type, gain_type, y_type);
+  ANC_REQUIRE(width_ok(H), "anc_rms_norm: rows of %lld: a multiple of 8 up to %d", (long long)H, kWidest);
+  ANC_REQUIRE(T >= 0 && T < (1ll << 31), "anc_rms_norm: %lld rows", (long long)T);
+  if (T == 0) return ANC_OK;
+  const bool mx8 = y_type == ANC_MXFP8;
+  ANC_REQUIRE(x && gain && y && (scale != 0) == mx8 && (residual != 0) == (total != 0),
+              "anc_rms_norm: null device pointer (scale goes with 8-bit rows, total with residual)");
+  ANC_REQUIRE(!mx8 || H % 32 == 0, "anc_rms_norm: 8-bit rows of %lld: a multiple of 32", (long long)H);
+  ANC_REQUIRE(((x | residual | gain | y | total) & 15) == 0 && (rstd & 3) == 0, "anc_rms_norm: misaligned pointers");
+  const int64_t n = T * H;
+  // (a workgroup reads its rows before it writes them: total may be the residual itself, y or total the x of the same type)
+  const AncSpan out[4] = {{y, n * (mx8 ? 1 : elem(y_type))}, {total, total ? n * elem(stream_type) : 0}, {scale, mx8 ? n / 32 : 0}, {rstd, rstd ? 4 * T : 0}};
+  const AncSpan in[3] = {{x, n * elem(x_type)}, {residual, residual ? n * elem(stream_type) : 0}, {gain, H * elem(gain_type)}};
+  ANC_REQUIRE(anc_outputs_apart({out[0], out[1], out[2], out[3]}, 4), "anc_rms_norm: outputs overlap");
+  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 3; ++j) {
+      const bool same = out[i].at == in[j].at && out[i].bytes == in[j].bytes && i < 2 && j < 2 && !(i == 0 && mx8);
+      ANC_REQUIRE(same || anc_apart(out[i].at, out[i].bytes, in[j].at, in[j].bytes), "anc_rms_norm: an output overlaps an input");
+    }
+  const NormArgs a{x, residual, gain, y, scale, total, rstd, T, (int)H, eps};
+  hipStream_t s = anc_stream(stream);
+  AncProfScope prof(ANC_PROF_MISC, s);
+  with_layout((int)H, [&](auto L, auto C) {
+    constexpr int lpr = decltype(L)::value, ch = decltype(C)::value;
+    const unsigned grid = (unsigned)((T + kThreads / lpr - 1) / (kThreads / lpr));
+    with_type(x_type, [&](auto X) { with_type(stream_type, [&](auto S) { with_type(gain_type, [&](auto G) {
+      constexpr int xt = decltype(X)::value, st = decltype(S)::value, gt = decltype(G)::value;
+      auto go = [&](auto O) {
+        constexpr int ot = decltype(O)::value;
+        if (residual) hipLaunchKernelGGL((k_rms_norm<xt, st, gt, ot, true, lpr, ch>), dim3(grid), dim3(kThreads), 0, s, a);
+        else hipLaunchKernelGGL((k_rms_norm<xt, ANC_BF16, gt, ot, false, lpr, ch>), dim3(grid), dim3(kThreads), 0, s, a);
+      };
+      if (mx8) go(IC<kMx8>{});
+      else if (y_type == ANC_BF16) go(IC<ANC_BF16>{});
+      else go(IC<ANC_F32>{});
+    }); }); });
+  });
+  ANC_LAUNCH_CHECK();
+  return ANC_OK;
+}
+
+extern "C" int64_t anc_rms_norm_grad_workspace_bytes(int64_t T, int64_t H) {
+  if (!width_ok(H) || T < 0 || T >= (1ll << 31)) {
+    anc_set_error("anc_rms_norm_grad_workspace_bytes: %lld rows of %lld", (long long)T, (long long)H);
+    return -1;
+  }
+  return parts_of(T, H) * H * 4;
+}
+
+extern "C" int anc_rms_norm_grad(uint64_t dy, int dy_type, uint64_t x, int stream_type, uint64_t gain, int gain_type, uint64_t rstd,
+                                 uint64_t carry, int64_t T, int64_t H, uint64_t dx, uint64_t dgain, int accumulate, uint64_t workspace,
+                                 int64_t workspace_bytes, uint64_t stream) {
+  ANC_REQUIRE(type_ok(dy_type) && type_ok(stream_type) && type_ok(gain_type), "anc_rms_norm_grad: bad types (dy %d, stream %d, gain %d)",
+              dy_type, stream_type, gain_type);
+  ANC_REQUIRE(width_ok(H), "anc_rms_norm_grad: rows of %lld: a multiple of 8 up to %d", (long long)H, kWidest);
+  ANC_REQUIRE(T >= 0 && T < (1ll << 31), "anc_rms_norm_grad: %lld rows", (long long)T);
+  ANC_REQUIRE(gain && dgain && (T == 0 || (dy && x && rstd && dx)), "anc_rms_norm_grad: null device pointer");
+  ANC_REQUIRE(((dy | x | gain | carry | dx | dgain | workspace) & 15) == 0 && (rstd & 3) == 0, "anc_rms_norm_grad: misaligned pointers");
+  const int64_t need = parts_of(T, H) * H * 4, n = T * H;
+  ANC_REQUIRE(workspace != 0 && workspace_bytes >= need, "anc_rms_norm_grad: workspace holds %lld bytes, %lld needed",
+              (long long)workspace_bytes, (long long)need);
+  const AncSpan out[3] = {{dx, n * elem(stream_type)}, {dgain, 4 * H}, {workspace, need}};
+  const AncSpan in[5] = {{dy, n * elem(dy_type)}, {x, n * elem(stream_type)}, {carry, carry ? n * elem(stream_type) : 0}, {gain, H * elem(gain_type)}, {rstd, 4 * T}};
+  ANC_REQUIRE(anc_outputs_apart({out[0], out[1], out[2]}, 3), "anc_rms_norm_grad: outputs or workspace overlap");
+  for (int i = 0; i < 3; ++i)
+    for (int j = 0; j < 5; ++j) {                     // (dx may be dy, x or carry itself)
+      const bool same = i == 0 && j < 3 && out[0].at == in[j].at && out[0].bytes == in[j].bytes;
+      ANC_REQUIRE(same || anc_apart(out[i].at, out[i].bytes, in[j].at, in[j].bytes), "anc_rms_norm_grad: an output or the workspace overlaps an input");
+    }
+  GradArgs a{dy, x, gain, rstd, carry, dx, dgain, workspace, T, (int)H, (int)parts_of(T, H), accumulate != 0};
+  hipStream_t s = anc_stream(stream);
+  AncProfScope prof(ANC_PROF_MISC, s);
+  with_layout((int)H, [&](auto L, auto C) {
+    constexpr int lpr = decltype(L)::value, ch = decltype(C)::value;
+    with_type(dy_type, [&](auto D) { with_type(stream_type, [&](auto S) { with_type(gain_type, [&](auto G) {
+      constexpr int dt = decltype(D)::value, st = decltype(S)::value, gt = decltype(G)::value;
+      if (carry) hipLaunchKernelGGL((k_rms_norm_grad<dt, st, gt, true, lpr, ch>), dim3((unsigned)a.rows), dim3(kThreads), 0, s, a);
+      else hipLaunchKernelGGL((k_rms_norm_grad<dt, st, gt, false, lpr, ch>), dim3((unsigned)a.rows), dim3(kThreads), 0, s, a);
+    }); }); });
+  });
+  ANC_LAUNCH_CHECK();
+  if (a.rows > 1) hipLaunchKernelGGL(k_gain_sum, dim3((unsigned)((H + 31) / 32)), dim3(kThreads), 0, s, (const float *)workspace, (float *)dgain, a.rows, (int)H, a.accumulate);
+  ANC_LAUNCH_CHECK();
+  return ANC_OK;
+}

@@ -132,6 +132,7 @@ int anc_profile_read(float *ms /* [ANC_PROF_KINDS] */, int64_t *launches /* [ANC
 /* --------------------------------------------------------- element types --- */
 #define ANC_F32   0
 #define ANC_BF16  1
+#define ANC_MXFP8 2   /* E4M3 codes with an E8M0 byte per 32 (anc_rms_norm's y) */
 
 /* ------------------------------------------------- step control block -------
  * 32 bytes in device memory, written by anc_gradnorm_finalize and read by every
@@ -279,6 +280,28 @@ int64_t anc_adamw_num_blocks(int64_t n);   /* blocks one tensor of n elements oc
  * tensor, ancora/optim/adamw.py:92-97). Per-element results are identical to anc_adamw. */
 int anc_adamw_multi(uint64_t desc_table, int32_t n_tensors, int64_t total_blocks,
                     const anc_adamw_hyper_t *h, uint64_t ctl, uint64_t stream);
+
+/* AdamW with the moments in 8 bits (no counterpart in the reference): the step of anc_adamw_multi, operation by operation in fp32, on
+ * moments held as 8-bit floats with one scale byte per 64 consecutive elements (value = code * 2^(byte - 127)).
+ *   m: E4M3 codes, byte = (biased fp32 exponent of the block's largest |m|) - 7; v: E5M2 codes, byte = that of v - 14; at least 1 each.
+ * Moments are stored by stochastic rounding: with h = the 32-bit hash whose low half is the weights' dither (row = i/64, col = i%64, seed ^
+ * 0x3C6EF372), a code is the lower neighbour, plus one where the dropped part of the magnitude and 16 bits of h (m: low half, v: high half), as
+ * a fraction of the codes' distance, add up to one or more. A v above zero is stored as no less than the least code, so that the update's
+ * divisor does not vanish. A moment that is not finite gets the NaN code 0x7F (m: with its sign) and does not count in its block's
+ * largest. sr and seeds as in anc_adamw_multi, but seed_base always counts (it is the moments' too), and sr may be ANC_SR_STEP_SEED
+ * alone. Elements are independent of how tensors share a launch. blk0 and total_blocks count anc_adamw_num_blocks(n).
+ * Alignment: g, p32 16 bytes (bf16 g: 8), p16 8, m and v 4. */
+typedef struct {
+  uint64_t g, m, v, ms, vs, p32, p16;   /* ms, vs: the scale bytes, n / 64 each           */
+  int64_t  n;                           /* elements, multiple of 64                       */
+  int64_t  blk0;                        /* index of this tensor's first block             */
+  float    wd;
+  uint32_t seed;                        /* per-tensor offset, added to seed_base          */
+  int32_t  g_dtype;
+  int32_t  pad;
+} anc_adamw8_desc_t;
+int anc_adamw8_multi(uint64_t desc_table, int32_t n_tensors, int64_t total_blocks, const anc_adamw_hyper_t *h, uint64_t ctl,
+                     uint64_t stream);
 
 /* Row-sparse AdamW on a (V, H) tensor whose gradient touches few rows per step (an input
  * embedding not tied to the output head), with the results of the dense kernel. The
@@ -502,6 +525,47 @@ typedef struct {
 } anc_expert_dw_problem_t;
 int anc_expert_dw_multi(const anc_expert_dw_problem_t *problems, int32_t n_problems, uint64_t counts, uint64_t offsets,
                         uint64_t order, int64_t experts, int64_t capacity, uint64_t stream);
+
+/* ------------------------------------------------- the gated feed-forward block ---
+ * The block between two residual additions (SwiGLU, ancora/kernels/activation.py and the grouped products of
+ * ancora/kernels/moe.py around the weights the step updates), over all `rows` rows (counts = offsets = 0, experts = 0) or over tokens
+ * sorted by expert (anc_route's counts and offsets on the device, `rows` slots): rows that fill up a segment, or lie behind the last, are neither
+ * read nor written. Weights are bf16 as the step keeps them, (in, out) row-major, one after the other per expert: Wg, Wu (H, I), Wd (I, H).
+ *   anc_gated_ffn:       h = silu(x Wg) * (x Wu); gate, up (0: not kept) receive x Wg and x Wu for the backward pass. All bf16.
+ *   anc_ffn_down:        y = h Wd + residual (0: none), y and residual of y_type (ANC_F32 or ANC_BF16)
+ *   anc_gated_ffn_grad:  with dh = dy Wd^T and s = sigmoid(gate): dgate = dh up s (1 + gate (1 - s)), dup = dh gate s, h = gate s up (0: not
+ *                        wanted): what the weight gradients (x^T dgate, x^T dup, h^T dy) and anc_gated_ffn_dx read
+ *   anc_gated_ffn_dx:    dx = dgate Wg^T + dup Wu^T + residual (0: none), dx and residual of dx_type
+ * Products of bf16 accumulate in fp32, each output is rounded once. The order of a sum hangs on the sizes of the call (rows, experts, H, I)
+ * alone: ascending k, or eight interleaved runs of it where there are few rows; the same bits on every run.
+ * H, I multiples of 8 up to 2^17, at most 512 experts, pointers 16-byte aligned. residual may be the output itself, dgate may be gate and dup
+ * up; no other overlap. rows = 0 does nothing. */
+int anc_gated_ffn(uint64_t x, uint64_t Wg, uint64_t Wu, uint64_t counts, uint64_t offsets, int64_t experts, int64_t rows,
+                  int64_t H, int64_t I, uint64_t h, uint64_t gate, uint64_t up, uint64_t stream);
+int anc_ffn_down(uint64_t h, uint64_t Wd, uint64_t counts, uint64_t offsets, int64_t experts, int64_t rows, int64_t I,
+                 int64_t H, uint64_t residual, uint64_t y, int y_type, uint64_t stream);
+int anc_gated_ffn_grad(uint64_t dy, uint64_t Wd, uint64_t gate, uint64_t up, uint64_t counts, uint64_t offsets, int64_t experts,
+                       int64_t rows, int64_t H, int64_t I, uint64_t dgate, uint64_t dup, uint64_t h, uint64_t stream);
+int anc_gated_ffn_dx(uint64_t dgate, uint64_t dup, uint64_t Wg, uint64_t Wu, uint64_t counts, uint64_t offsets, int64_t experts,
+                     int64_t rows, int64_t H, int64_t I, uint64_t residual, uint64_t dx, int dx_type, uint64_t stream);
+
+/* ------------------------------------------------- the layer's norm ---
+ * Root-mean-square norm of T rows of H with the residual's addition (RMSNorm as `ancora/kernels/norm.py` has it for the models whose gains
+ * the step updates): s = x + residual (residual 0: s = x), r = 1 / sqrt(mean(s^2) + eps), y = s r gain, in fp32 with one rounding
+ * per output. x ANC_F32 or ANC_BF16; residual and total (s, written where residual is given) of stream_type; gain of gain_type; rstd
+ * fp32[T] or 0. y of y_type, or ANC_MXFP8: E4M3 codes (T, H) with scale (T, H/32), one E8M0 byte per 32 elements of a row by
+ * the rule of anc_quant_mxfp8_w (elements that are not finite become NaN codes).
+ * H a multiple of 8 (MXFP8: 32) up to 16384; rows contiguous, 16-byte aligned. y or total may be x or residual itself (same address, same
+ * type); no other overlap. T = 0 does nothing. */
+int anc_rms_norm(uint64_t x, int x_type, uint64_t residual, int stream_type, uint64_t gain, int gain_type, int64_t T, int64_t H,
+                 float eps, uint64_t y, int y_type, uint64_t scale, uint64_t total, uint64_t rstd, uint64_t stream);
+/* Its backward pass: x is what was normed (total, or x) of stream_type, a = dy gain, dx = r (a - x r^2 mean(a x)) + carry in stream_type (carry
+ * 0: none: the gradient that comes along the residual stream), dgain fp32[H] = (or +=, `accumulate`) the sum over rows of dy x r,
+ * rows added in fp32 in a fixed order that hangs on T and H alone. dx may be dy, x or carry itself where the types agree. */
+int64_t anc_rms_norm_grad_workspace_bytes(int64_t T, int64_t H);
+int anc_rms_norm_grad(uint64_t dy, int dy_type, uint64_t x, int stream_type, uint64_t gain, int gain_type, uint64_t rstd,
+                      uint64_t carry, int64_t T, int64_t H, uint64_t dx, uint64_t dgain, int accumulate, uint64_t workspace,
+                      int64_t workspace_bytes, uint64_t stream);
 
 /* MXFP8 re-quantisation of bf16 weights (E, K, N) after the step: per block of 32 consecutive K
  * and per column one E8M0 scale byte = (biased fp32 exponent of the block's amax) - 7 (0 below
