@@ -7,133 +7,197 @@
 // a block's largest v and its least normal one is 2^15 between gradients, and a v that is not zero never becomes zero.
 //
 // Both are stored by stochastic rounding, the code's lower neighbour plus one where the dropped bits and 16 bits of a hash
-// of (row, column, seed) carry: rounded to nearest, a moment that moves by a thousandth a step would stay where it is for ever, since a code's
-// step is an eighth (m) or a quarter (v); this way its expectation is the exact moment's.
+// of (row, column, seed) carry (v_cvt_sr_fp8_f32 / v_cvt_sr_bf8_f32 with the 16 bits in the upper half of their operand): rounded to nearest, a
+// moment that moves by a thousandth a step would stay where it is for ever, since a code's step is an eighth (m) or a quarter (v); this
+// way its expectation is the exact moment's.
 //
-// HBM-bound: 16 1/16 bytes per element (bf16 gradients; read g 2, m 1, v 1, p32 4, write m 1, v 1, p32 4, p16 2, scales) against the
-// 28 of 32-bit moments.
+// Bound: 16 1/16 bytes per element (bf16 gradients; read g 2, m 1, v 1, p32 4, write m 1, v 1, p32 4, p16 2, scales) against the 28 of 32-bit
+// moments, so little that the arithmetic counts as much: the first form took 173 instructions per element and 179 us for 51.5 M elements (4.6
+// TB/s), its three divisions, root and the bookkeeping of codes most of them.
 #include "adamw_elem.h"
 
 namespace {
 
-constexpr int kThreads = 256, kVec = 4, kUnroll = 4;
-constexpr int kSlab = kThreads * kVec, kBlockElems = kSlab * kUnroll;    // as adamw.hip: anc_adamw_num_blocks
+constexpr int kThreads = 256, kVec = 4, kSlabs = 4;
+constexpr int kSlab = kThreads * kVec, kBlockElems = kSlab * kSlabs;      // as adamw.hip: anc_adamw_num_blocks
 constexpr uint32_t kStateSeed = 0x3C6EF372u;                              // apart from the weights' dither
+constexpr uint32_t kInf = 0x7F800000u;
+constexpr int64_t kFewBlocks = 512;
 
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
 // The largest of 16 neighbouring lanes, in all of them: rotations within a row of the data-parallel moves.
 __device__ __forceinline__ uint32_t max_of_16(uint32_t x) {
-#define ANC_ROT(n) { const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + n, 0xF, 0xF, true); x = x > o ? x : o; }
+#define ANC_ROT(n) x = larger(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + n, 0xF, 0xF, true));
   ANC_ROT(8) ANC_ROT(4) ANC_ROT(2) ANC_ROT(1)
 #undef ANC_ROT
   return x;
-}
-// Magnitude bits of a finite number, 0 of any other: a NaN does not decide its block's scale.
-__device__ __forceinline__ uint32_t finite_bits(float x) {
-  const uint32_t b = __float_as_uint(x) & 0x7FFFFFFFu;
-  return b < 0x7F800000u ? b : 0u;
 }
 __device__ __forceinline__ uint32_t scale_byte(uint32_t amax, uint32_t top) {
   const uint32_t e = amax >> 23;
   return e > top ? e - top : 1u;
 }
-// Code (without sign) of x >= 0 times the power of two `up`; MANT mantissa bits, exponent field 1 stands for 2^(1 + BASE - 127), dither
-// of 16 bits. A subnormal code's steps are those of the least normal binade, into which the sum moves it. NaN and infinity: 0x7F.
-template <int MANT, int BASE>
-__device__ __forceinline__ uint32_t code_of(float x, float up, uint32_t dither) {
-  constexpr int kDrop = 23 - MANT;
-  const float low = __uint_as_float((uint32_t)(BASE + 1) << 23);
-  const float y = x * up;
-  const bool small = y < low;
-  const uint32_t b = __float_as_uint(small ? y + low : y) + (dither << (kDrop - 16));
-  const uint32_t c = (b >> kDrop) - ((uint32_t)(small ? BASE + 1 : BASE) << MANT);
-  return x < __uint_as_float(0x7F800000u) ? c : 0x7Fu;
+// a / b for a b that many elements share, y = 1 / b rounded to nearest: two corrections make the quotient the correctly rounded one (Markstein's
+// theorem: the first leaves it within a unit, the remainder of the second is exact), 6 instructions instead of 11. Below 2^-100 remainders leave
+// the range of fp32 and the last bit may differ.
+__device__ __forceinline__ float shared_div(float a, float b, float y) {
+  float q = a * y;
+  q = __builtin_fmaf(__builtin_fmaf(-b, q, a), y, q);
+  q = __builtin_fmaf(__builtin_fmaf(-b, q, a), y, q);
+  return __builtin_amdgcn_div_fixupf(q, b, a);                            // (infinities, NaN, zeros)
+}
+// adamw_elem of adamw_elem.h with the bias corrections' reciprocals at hand.
+template <int FORM>
+__device__ __forceinline__ void elem(float g, float &m, float &v, float &p, const anc_adamw_hyper_t &h, float y1, float y2, float wd, float clip) {
+  if constexpr (FORM == ANC_ADAMW_FORM_DIV) {
+    const float gs = g * clip;
+    m = h.beta1 * m + h.omb1 * gs;
+    v = h.beta2 * v + (h.omb2 * gs) * gs;
+    p = p - h.lr * (shared_div(m, h.bc1, y1) / (sqrtf(shared_div(v, h.bc2, y2)) + h.eps) + wd * p);
+  } else {
+    adamw_elem<FORM>(g, m, v, p, h, wd, clip);
+  }
 }
 
-template <int GD, int FORM, int SR>
-__device__ __forceinline__ void adamw8_block(const anc_adamw8_desc_t &t, int64_t blk, const anc_adamw_hyper_t &h, float clip, uint32_t seed) {
-  const int64_t base = blk * kBlockElems + (int64_t)threadIdx.x * kVec;
-  const uint8_t *tm = (const uint8_t *)t.m, *tv = (const uint8_t *)t.v, *tms = (const uint8_t *)t.ms, *tvs = (const uint8_t *)t.vs;
-  anc_f32x4 g4[kUnroll], p4[kUnroll];
-  uint32_t m4[kUnroll], v4[kUnroll], ms[kUnroll], vs[kUnroll];
-  bool live[kUnroll];
+// The hash of anc_sr_hash from its key.
+__device__ __forceinline__ uint32_t mixed(uint32_t key) {
+  uint32_t h = key * 0x9E3779B1u;
+  h ^= h >> 16;
+  h *= 0x85EBCA6Bu;
+  return h ^ (h >> 13);
+}
+
+template <int SLABS> struct Loaded {
+  anc_f32x4 g[SLABS], p[SLABS];
+  uint32_t m[SLABS], v[SLABS], ms[SLABS], vs[SLABS];
+};
+
+// 1024 elements at e (this lane's four of them), loaded in slab j.
+template <int FORM, int SR, int SLABS>
+__device__ __forceinline__ void adamw8_slab(const anc_adamw8_desc_t &t, const Loaded<SLABS> &in, int j, int64_t e, const anc_adamw_hyper_t &h, float y1,
+                                            float y2, float clip, uint32_t seed) {
+  const float sm = __uint_as_float(in.ms[j] << 23), sv = __uint_as_float(in.vs[j] << 23);
+  const auto ma = __builtin_amdgcn_cvt_pk_f32_fp8((int)in.m[j], false), mb = __builtin_amdgcn_cvt_pk_f32_fp8((int)in.m[j], true);
+  const auto va = __builtin_amdgcn_cvt_pk_f32_bf8((int)in.v[j], false), vb = __builtin_amdgcn_cvt_pk_f32_bf8((int)in.v[j], true);
+  float mm[4] = {ma[0] * sm, ma[1] * sm, mb[0] * sm, mb[1] * sm};
+  float vv[4] = {va[0] * sv, va[1] * sv, vb[0] * sv, vb[1] * sv};
+  float pp[4] = {in.p[j].x, in.p[j].y, in.p[j].z, in.p[j].w};
+  uint32_t am = 0u, av = 0u, ap = 0u;
 #pragma unroll
-  for (int j = 0; j < kUnroll; ++j) {
+  for (int k = 0; k < 4; ++k) {
+    elem<FORM>(in.g[j][k], mm[k], vv[k], pp[k], h, y1, y2, t.wd, clip);
+    am = larger(am, __float_as_uint(mm[k]) & 0x7FFFFFFFu);
+    av = larger(av, __float_as_uint(vv[k]));                              // (never negative; a NaN is larger than infinity either way)
+    ap = larger(ap, __float_as_uint(pp[k]) & 0x7FFFFFFFu);
+  }
+  am = max_of_16(am);
+  av = max_of_16(av);
+  const bool odd = am >= kInf || av >= kInf;                              // something in the block is not finite: it does not count
+  if (odd) {
+    am = av = 0u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t a = __float_as_uint(mm[k]) & 0x7FFFFFFFu, b = __float_as_uint(vv[k]);
+      am = larger(am, a < kInf ? a : 0u);
+      av = larger(av, b < kInf ? b : 0u);
+    }
+    am = max_of_16(am);
+    av = max_of_16(av);
+  }
+  const uint32_t bm = scale_byte(am, 7u), bv = scale_byte(av, 14u);
+  const float um = __uint_as_float((254u - bm) << 23), uv = __uint_as_float((254u - bv) << 23);
+  // keys of the hashes: (row * c1) ^ (column * c2) ^ seed, the column's part the same in every slab
+  const uint32_t row = (uint32_t)(e >> 6) * 73856093u, col = ((uint32_t)threadIdx.x & 15u) * (4u * 19349663u);
+  uint32_t mo = 0u, vo = 0u;
+#define ANC_CODE(k)                                                                                        \
+  {                                                                                                        \
+    const uint32_t d = mixed(row ^ (col + k * 19349663u) ^ (seed ^ kStateSeed));                           \
+    mo = (uint32_t)__builtin_amdgcn_cvt_sr_fp8_f32(mm[k] * um, (int)(d << 16), (int)mo, k);                \
+    vo = (uint32_t)__builtin_amdgcn_cvt_sr_bf8_f32(vv[k] * uv, (int)(d & 0xFFFF0000u), (int)vo, k);        \
+  }
+  ANC_CODE(0) ANC_CODE(1) ANC_CODE(2) ANC_CODE(3)
+#undef ANC_CODE
+  const uint32_t none = ~((vo & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) & 0x80808080u;     // bytes of v that became zero
+  if (odd || none != 0u) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (vv[k] > 0.0f && (vo >> (8 * k) & 0xFFu) == 0u) vo |= 1u << (8 * k);
+      if (!(__builtin_fabsf(mm[k]) < __uint_as_float(kInf)))
+        mo = (mo & ~(0xFFu << (8 * k))) | ((0x7Fu | (__float_as_uint(mm[k]) >> 24 & 0x80u)) << (8 * k));
+      if (!(vv[k] < __uint_as_float(kInf))) vo = (vo & ~(0xFFu << (8 * k))) | (0x7Fu << (8 * k));
+    }
+  }
+  uint32_t h2[2];
+  if constexpr (SR) {
+    uint32_t b[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) b[k] = __float_as_uint(pp[k]) + (mixed(row ^ (col + k * 19349663u) ^ seed) & 0xFFFFu);
+    if (ap >= kInf) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) b[k] = anc_bf16_sr_bits(pp[k], (uint32_t)(e >> 6), ((uint32_t)e & 63u) + k, seed) << 16;
+    }
+    h2[0] = __builtin_amdgcn_perm(b[1], b[0], 0x07060302u);
+    h2[1] = __builtin_amdgcn_perm(b[3], b[2], 0x07060302u);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) h2[i] = anc_bf16_rne_bits(pp[2 * i]) | (anc_bf16_rne_bits(pp[2 * i + 1]) << 16);
+  }
+  anc_st_stream((uint32_t *)((uint8_t *)t.m + e), mo);
+  anc_st_stream((uint32_t *)((uint8_t *)t.v + e), vo);
+  anc_st_stream((anc_f32x4 *)((float *)t.p32 + e), anc_f32x4{pp[0], pp[1], pp[2], pp[3]});
+  anc_st_stream((anc_u32x2 *)((uint16_t *)t.p16 + e), anc_u32x2{h2[0], h2[1]});
+  if ((threadIdx.x & 15) == 0) {
+    ((uint8_t *)t.ms)[e >> 6] = (uint8_t)bm;
+    ((uint8_t *)t.vs)[e >> 6] = (uint8_t)bv;
+  }
+}
+
+template <int GD, int FORM, int SR, int SLABS>
+__device__ __forceinline__ void adamw8_slabs(const anc_adamw8_desc_t &t, int64_t first, const anc_adamw_hyper_t &h, float clip, uint32_t seed) {
+  const int64_t base = first + (int64_t)threadIdx.x * kVec;
+  Loaded<SLABS> in;
+#pragma unroll
+  for (int j = 0; j < SLABS; ++j) {
     const int64_t e = base + (int64_t)j * kSlab;
-    live[j] = e < t.n;                                     // (n % 64 == 0: 16 lanes live or die together)
-    if (live[j]) {
-      if (GD == ANC_BF16) {
-        const anc_u32x2 gb = anc_ld_stream((const anc_u32x2 *)((const uint16_t *)t.g + e));
-        g4[j] = anc_f32x4{__uint_as_float(gb.x << 16), __uint_as_float(gb.x & 0xFFFF0000u), __uint_as_float(gb.y << 16),
+    if (e >= t.n) continue;                                // (n % 64 == 0: 16 lanes live or die together)
+    if (GD == ANC_BF16) {
+      const anc_u32x2 gb = anc_ld_stream((const anc_u32x2 *)((const uint16_t *)t.g + e));
+      in.g[j] = anc_f32x4{__uint_as_float(gb.x << 16), __uint_as_float(gb.x & 0xFFFF0000u), __uint_as_float(gb.y << 16),
                           __uint_as_float(gb.y & 0xFFFF0000u)};
-      } else {
-        g4[j] = anc_ld_stream((const anc_f32x4 *)((const float *)t.g + e));
-      }
-      m4[j] = anc_ld_stream((const uint32_t *)(tm + e));
-      v4[j] = anc_ld_stream((const uint32_t *)(tv + e));
-      p4[j] = anc_ld_stream((const anc_f32x4 *)((const float *)t.p32 + e));
-      ms[j] = tms[e >> 6];
-      vs[j] = tvs[e >> 6];
+    } else {
+      in.g[j] = anc_ld_stream((const anc_f32x4 *)((const float *)t.g + e));
     }
+    in.m[j] = anc_ld_stream((const uint32_t *)((const uint8_t *)t.m + e));
+    in.v[j] = anc_ld_stream((const uint32_t *)((const uint8_t *)t.v + e));
+    in.p[j] = anc_ld_stream((const anc_f32x4 *)((const float *)t.p32 + e));
+    in.ms[j] = ((const uint8_t *)t.ms)[e >> 6];
+    in.vs[j] = ((const uint8_t *)t.vs)[e >> 6];
   }
+  const float y1 = FORM == ANC_ADAMW_FORM_DIV ? 1.0f / h.bc1 : 0.0f, y2 = FORM == ANC_ADAMW_FORM_DIV ? 1.0f / h.bc2 : 0.0f;
 #pragma unroll
-  for (int j = 0; j < kUnroll; ++j) {
-    if (!live[j]) continue;
+  for (int j = 0; j < SLABS; ++j) {
     const int64_t e = base + (int64_t)j * kSlab;
-    const float gg[4] = {g4[j].x, g4[j].y, g4[j].z, g4[j].w};
-    float pp[4] = {p4[j].x, p4[j].y, p4[j].z, p4[j].w};
-    const float sm = __uint_as_float(ms[j] << 23), sv = __uint_as_float(vs[j] << 23);
-    const auto ma = __builtin_amdgcn_cvt_pk_f32_fp8((int)m4[j], false), mb = __builtin_amdgcn_cvt_pk_f32_fp8((int)m4[j], true);
-    const auto va = __builtin_amdgcn_cvt_pk_f32_bf8((int)v4[j], false), vb = __builtin_amdgcn_cvt_pk_f32_bf8((int)v4[j], true);
-    float mm[4] = {ma[0] * sm, ma[1] * sm, mb[0] * sm, mb[1] * sm};
-    float vv[4] = {va[0] * sv, va[1] * sv, vb[0] * sv, vb[1] * sv};
-    uint32_t hb[4], am = 0u, av = 0u;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      adamw_elem<FORM>(gg[k], mm[k], vv[k], pp[k], h, t.wd, clip);
-      const uint64_t i = (uint64_t)(e + k);
-      hb[k] = SR ? anc_bf16_sr_bits(pp[k], (uint32_t)(i >> 6), (uint32_t)(i & 63u), seed) : anc_bf16_rne_bits(pp[k]);
-      const uint32_t a = finite_bits(mm[k]), b = finite_bits(vv[k]);
-      am = am > a ? am : a;
-      av = av > b ? av : b;
-    }
-    const uint32_t bm = scale_byte(max_of_16(am), 7u), bv = scale_byte(max_of_16(av), 14u);
-    const float um = __uint_as_float((254u - bm) << 23), uv = __uint_as_float((254u - bv) << 23);
-    uint32_t mo = 0u, vo = 0u;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint64_t i = (uint64_t)(e + k);
-      const uint32_t d = anc_sr_hash((uint32_t)(i >> 6), (uint32_t)(i & 63u), seed ^ kStateSeed);
-      const uint32_t cm = code_of<3, 120>(__builtin_fabsf(mm[k]), um, d & 0xFFFFu) | ((__float_as_uint(mm[k]) >> 24) & 0x80u);
-      const uint32_t cv = code_of<2, 112>(vv[k], uv, d >> 16);
-      mo |= cm << (8 * k);
-      vo |= (vv[k] > 0.0f && cv == 0u ? 1u : cv) << (8 * k);
-    }
-    anc_st_stream((uint32_t *)((uint8_t *)t.m + e), mo);
-    anc_st_stream((uint32_t *)((uint8_t *)t.v + e), vo);
-    anc_st_stream((anc_f32x4 *)((float *)t.p32 + e), anc_f32x4{pp[0], pp[1], pp[2], pp[3]});
-    anc_st_stream((anc_u32x2 *)((uint16_t *)t.p16 + e), anc_u32x2{(hb[0] & 0xFFFFu) | (hb[1] << 16), (hb[2] & 0xFFFFu) | (hb[3] << 16)});
-    if ((threadIdx.x & 15) == 0) {
-      ((uint8_t *)t.ms)[e >> 6] = (uint8_t)bm;
-      ((uint8_t *)t.vs)[e >> 6] = (uint8_t)bv;
-    }
+    if (e < t.n) adamw8_slab<FORM, SR, SLABS>(t, in, j, e, h, y1, y2, clip, seed);
   }
 }
 
-template <int FORM, int SR>
+// SLABS = 4: a workgroup takes a whole block of 4096 elements, all of a lane's loads before its arithmetic; 1: a quarter of one, for
+// launches of few blocks.
+template <int FORM, int SR, int SLABS>
 __global__ void __launch_bounds__(kThreads)
 k_adamw8_multi(const anc_adamw8_desc_t *__restrict__ table, int n_tensors, anc_adamw_hyper_t h, const anc_step_ctl_t *__restrict__ ctl) {
   float clip;
   if (!load_ctl(ctl, clip)) return;
   step_scalars(h, ctl);
-  const int64_t blk = (int64_t)blockIdx.x;
+  const int64_t blk = (int64_t)(blockIdx.x / (kSlabs / SLABS));
   int lo = 0, hi = n_tensors - 1;                          // last tensor whose first block is <= blk
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (table[mid].blk0 <= blk) lo = mid; else hi = mid - 1;
   }
   const anc_adamw8_desc_t d = table[lo];
-  if (d.g_dtype == ANC_BF16) adamw8_block<ANC_BF16, FORM, SR>(d, blk - d.blk0, h, clip, h.seed_base + d.seed);
-  else                       adamw8_block<ANC_F32, FORM, SR>(d, blk - d.blk0, h, clip, h.seed_base + d.seed);
+  const int64_t first = (blk - d.blk0) * kBlockElems + (int64_t)(blockIdx.x % (kSlabs / SLABS)) * (SLABS * kSlab);
+  if (d.g_dtype == ANC_BF16) adamw8_slabs<ANC_BF16, FORM, SR, SLABS>(d, first, h, clip, h.seed_base + d.seed);
+  else                       adamw8_slabs<ANC_F32, FORM, SR, SLABS>(d, first, h, clip, h.seed_base + d.seed);
 }
 
 }  // namespace
@@ -153,8 +217,12 @@ extern "C" int anc_adamw8_multi(uint64_t desc_table, int32_t n_tensors, int64_t 
   AncProfScope prof(ANC_PROF_ADAMW, anc_stream(stream));
   dispatch_form_sr(hh.form, hh.sr & ANC_SR_ON, [&](auto F, auto S) {
     constexpr int f = decltype(F)::value, s = decltype(S)::value;
-    hipLaunchKernelGGL((k_adamw8_multi<f, s>), dim3((unsigned)total_blocks), dim3(kThreads), 0, anc_stream(stream),
-                       (const anc_adamw8_desc_t *)desc_table, (int)n_tensors, hh, (const anc_step_ctl_t *)ctl);
+    const auto *tab = (const anc_adamw8_desc_t *)desc_table;
+    const auto *c = (const anc_step_ctl_t *)ctl;
+    if (total_blocks < kFewBlocks)
+      hipLaunchKernelGGL((k_adamw8_multi<f, s, 1>), dim3((unsigned)(total_blocks * kSlabs)), dim3(kThreads), 0, anc_stream(stream), tab, (int)n_tensors, hh, c);
+    else
+      hipLaunchKernelGGL((k_adamw8_multi<f, s, kSlabs>), dim3((unsigned)total_blocks), dim3(kThreads), 0, anc_stream(stream), tab, (int)n_tensors, hh, c);
   });
   ANC_LAUNCH_CHECK();
   return ANC_OK;

@@ -38,8 +38,7 @@ def decode(codes, scales, mantissa):
 
 def encode(x, mantissa, dither):
     """(codes, scales) of fp32 x (R, 64): by search among the format's values. The lower neighbour, plus one where the
-    magnitude's place between the neighbours (to 2^-(23 - mantissa) of a binade, cut off) and dither / 2^16 make one or more. The sum
-    with the least normal number in the subnormal range is rounded to fp32 like the kernel's."""
+    magnitude's place between the neighbours and dither / 2^16 make one or more."""
     x = np.asarray(x, np.float32)
     top, table = (7, values(3)) if mantissa == 3 else (14, values(2))
     a = np.abs(x)
@@ -48,11 +47,9 @@ def encode(x, mantissa, dither):
     _, e = np.frexp(amax.astype(np.float64))
     byte = np.where(amax > 0, np.maximum(e - 1 + 127 - top, 1), 1).astype(np.int64)
     y = np.where(fin, a, 0).astype(np.float64) * np.exp2(127.0 - byte)[:, None]
-    low = table[1 << mantissa]                                   # least normal
-    y = np.where(y < low, (y.astype(np.float32) + np.float32(low)).astype(np.float64) - low, y)
     at = np.clip(np.searchsorted(table, y, side="right") - 1, 0, table.size - 2)
     place = (y - table[at]) / (table[at + 1] - table[at])
-    codes = at + (np.floor(place * 2.0 ** (23 - mantissa)) + dither * 2.0 ** (7 - mantissa) >= 2.0 ** (23 - mantissa))
+    codes = at + (place * 65536.0 + dither >= 65536.0)
     codes = np.where(fin, codes, 0x7F) | (np.signbit(x).astype(np.int64) << 7)
     return codes.astype(np.uint8), byte.astype(np.uint8)
 
