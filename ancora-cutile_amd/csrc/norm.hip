@@ -15,6 +15,7 @@ namespace {
 
 using anc_rows::bf16_pair;
 constexpr int kThreads = 256;
+constexpr int kGradThreads = 512;       // of the backward pass: twice the wavefronts to a partial row of dgain
 constexpr int kMostRows = 512;          // partial rows of dgain
 
 template <int T> struct Eight;
@@ -57,7 +58,8 @@ template <int LPR> __device__ __forceinline__ float row_sum(float v, float *lds)
     __syncthreads();                                  // (the last call's values have been read)
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = (lds[0] + lds[1]) + (lds[2] + lds[3]);
+    const float *w = lds + (threadIdx.x >> 8) * 4;
+    v = (w[0] + w[1]) + (w[2] + w[3]);
   }
   return v;
 }
@@ -156,69 +158,90 @@ struct GradArgs {
   int H, rows, accumulate;              // rows of dgain in parts: the grid
 };
 
-// Group g of workgroup b takes rows b * groups + g, then every rows * groups further.
-template <int DT, int ST, int GT, bool CARRY, int LPR, int CH>
-__global__ void __launch_bounds__(kThreads) k_rms_norm_grad(GradArgs a) {
-  constexpr int kGroups = kThreads / LPR;
-  __shared__ float lds[4];
+// One row's pieces in registers, as they lie in memory.
+template <int DT, int ST, bool CARRY, int CH> struct GradRow {
+  Eight<DT> d[CH];
+  Eight<ST> s[CH], c[CARRY && CH < 8 ? CH : 1];
+  float r;
+};
+
+// Group g of workgroup b takes rows b * groups + g, then every rows * groups further. The gain is kept, or read again where four or more
+// pieces leave no room for it. (8192 rows of 1024 in bf16 with carry, both launches: 256 lanes and 512 partial rows 16.2 us, 512 lanes 15.2, 256 partial
+// rows 16.1; the next row's loads ahead of this row's sums 16.7: the wavefronts that their registers displace were worth more.)
+template <int DT, int ST, int WT, bool CARRY, int LPR, int CH>
+__global__ void __launch_bounds__(kGradThreads, 1) k_rms_norm_grad(GradArgs a) {
+  constexpr int kGroups = kGradThreads / LPR;
+  constexpr bool kKeep = CH < 4;
+  __shared__ float lds[kGradThreads / 64];
   __shared__ float sums[kGroups > 1 ? kGroups * LPR * CH * 8 : 1];
   const int sub = (int)threadIdx.x % LPR, group = (int)threadIdx.x / LPR;
-  float g[CH][8], dg[CH][8];
+  Eight<WT> kept[kKeep ? CH : 1];
+  float dg[CH][8];
+  auto gain = [&](int j) {
+    if constexpr (kKeep) return kept[j];
+    else return load8<WT>(a.gain, (sub + j * LPR) * 8);
+  };
+  using Row = GradRow<DT, ST, CARRY, CH>;
+  auto fetch = [&](int64_t row, Row &v) {
+    if (row >= a.T) return;
+    v.r = ((const float *)a.rstd)[row];
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      const int col = (sub + j * LPR) * 8;
+      if (col >= a.H) continue;
+      v.d[j] = load8<DT>(a.dy, row * a.H + col);
+      v.s[j] = load8<ST>(a.x, row * a.H + col);
+      if constexpr (CARRY && CH < 8) v.c[j] = load8<ST>(a.carry, row * a.H + col);      // (eight pieces: no room, fetched where it is added)
+    }
+  };
+  Row now;
 #pragma unroll
   for (int j = 0; j < CH; ++j) {
     const int col = (sub + j * LPR) * 8;
-    if (col < a.H) widen<GT>(load8<GT>(a.gain, col), g[j]);
+    if constexpr (kKeep) {
+      if (col < a.H) kept[j] = load8<WT>(a.gain, col);
+    }
 #pragma unroll
     for (int k = 0; k < 8; ++k) dg[j][k] = 0.0f;
   }
   for (int64_t row0 = (int64_t)blockIdx.x * kGroups; row0 < a.T; row0 += (int64_t)a.rows * kGroups) {
     const int64_t row = row0 + group;
-    const bool live = row < a.T;
-    const int64_t base = (live ? row : 0) * a.H;
-    const float r = ((const float *)a.rstd)[live ? row : 0];
-    Eight<DT> d8[CH];
-    Eight<ST> s8[CH], c8[CH];
-    bool on[CH];
-#pragma unroll
-    for (int j = 0; j < CH; ++j) {
-      const int col = (sub + j * LPR) * 8;
-      on[j] = live && col < a.H;
-      if (on[j]) {
-        d8[j] = load8<DT>(a.dy, base + col);
-        s8[j] = load8<ST>(a.x, base + col);
-        if constexpr (CARRY) c8[j] = load8<ST>(a.carry, base + col);
-      }
-    }
+    const bool live = row < a.T;                      // (a wavefront's other rows still take part in its shuffles)
+    fetch(row, now);
+    const float r = now.r;
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
-      if (!on[j]) continue;
-      float d[8], s[8];
-      widen<DT>(d8[j], d);
-      widen<ST>(s8[j], s);
+      if (!live || (sub + j * LPR) * 8 >= a.H) continue;
+      float d[8], s[8], g[8];
+      widen<DT>(now.d[j], d);
+      widen<ST>(now.s[j], s);
+      widen<WT>(gain(j), g);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float xh = s[k] * r;
         dg[j][k] = __builtin_fmaf(d[k], xh, dg[j][k]);
-        sum = __builtin_fmaf(d[k] * g[j][k], xh, sum);
+        sum = __builtin_fmaf(d[k] * g[k], xh, sum);
       }
     }
     const float c = row_sum<LPR>(sum, lds) / (float)a.H;
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
-      if (!on[j]) continue;
-      float d[8], s[8], o[8];
-      widen<DT>(d8[j], d);
-      widen<ST>(s8[j], s);
+      if (!live || (sub + j * LPR) * 8 >= a.H) continue;
+      float d[8], s[8], g[8], o[8];
+      widen<DT>(now.d[j], d);
+      widen<ST>(now.s[j], s);
+      widen<WT>(gain(j), g);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) o[k] = r * (d[k] * g[j][k] - s[k] * r * c);
+      for (int k = 0; k < 8; ++k) o[k] = r * (d[k] * g[k] - s[k] * r * c);
       if constexpr (CARRY) {
         float f[8];
-        widen<ST>(c8[j], f);
+        if constexpr (CH < 8) widen<ST>(now.c[j], f);
+        else widen<ST>(load8<ST>(a.carry, row * a.H + (sub + j * LPR) * 8), f);
 #pragma unroll
         for (int k = 0; k < 8; ++k) o[k] += f[k];
       }
-      store8<ST>(a.dx, base + (sub + j * LPR) * 8, o);
+      store8<ST>(a.dx, row * a.H + (sub + j * LPR) * 8, o);
     }
   }
   // the groups' sums in ascending order
@@ -232,7 +255,7 @@ __global__ void __launch_bounds__(kThreads) k_rms_norm_grad(GradArgs a) {
   float *out = a.rows > 1 ? (float *)a.parts + (int64_t)blockIdx.x * a.H : (float *)a.dgain;
   const bool onto = a.rows == 1 && a.accumulate;
   if constexpr (kGroups > 1) {
-    for (int col = (int)threadIdx.x; col < a.H; col += kThreads) {
+    for (int col = (int)threadIdx.x; col < a.H; col += kGradThreads) {
       float v = sums[col];
 #pragma unroll
       for (int q = 1; q < kGroups; ++q) v += sums[q * LPR * CH * 8 + col];
@@ -249,14 +272,14 @@ __global__ void __launch_bounds__(kThreads) k_rms_norm_grad(GradArgs a) {
   }
 }
 
-// dgain (+)= the sum of `rows` rows: 32 columns to a workgroup, 32 of its groups of 8 lanes taking every 32nd row.
+// dgain (+)= the sum of `rows` rows: 16 columns to a workgroup, 64 groups of 4 lanes taking every 64th row.
 __global__ void __launch_bounds__(kThreads) k_gain_sum(const float *parts, float *dgain, int rows, int H, int accumulate) {
-  __shared__ float sums[32][33];
-  const int c4 = (int)threadIdx.x & 7, q = (int)threadIdx.x >> 3, col = (int)blockIdx.x * 32 + c4 * 4;
+  __shared__ float sums[64][17];
+  const int c4 = (int)threadIdx.x & 3, q = (int)threadIdx.x >> 2, col = (int)blockIdx.x * 16 + c4 * 4;
   anc_f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
   if (col < H) {
-#pragma unroll 4
-    for (int r = q; r < rows; r += 32) {
+#pragma unroll 8
+    for (int r = q; r < rows; r += 64) {
       const anc_f32x4 p = *(const anc_f32x4 *)(parts + (int64_t)r * H + col);
       v = anc_f32x4{v.x + p.x, v.y + p.y, v.z + p.z, v.w + p.w};
     }
@@ -264,15 +287,13 @@ __global__ void __launch_bounds__(kThreads) k_gain_sum(const float *parts, float
 #pragma unroll
   for (int k = 0; k < 4; ++k) sums[q][c4 * 4 + k] = v[k];
   __syncthreads();
-  if (threadIdx.x < 32) {
-    const int c = (int)blockIdx.x * 32 + (int)threadIdx.x;
-    if (c < H) {
-      float t = sums[0][threadIdx.x];
+  // 16 lanes to a column: four rows each, then across the lanes
+  const int c = (int)threadIdx.x >> 4, part = (int)threadIdx.x & 15;
+  float t = ((sums[part][c] + sums[part + 16][c]) + sums[part + 32][c]) + sums[part + 48][c];
 #pragma unroll
-      for (int r = 1; r < 32; ++r) t += sums[r][threadIdx.x];
-      dgain[c] = accumulate ? dgain[c] + t : t;
-    }
-  }
+  for (int off = 8; off >= 1; off >>= 1) t += __shfl_xor(t, off, 64);
+  const int out = (int)blockIdx.x * 16 + c;
+  if (part == 0 && out < H) dgain[out] = accumulate ? dgain[out] + t : t;
 }
 
 constexpr int kWidest = 16384;
@@ -296,10 +317,12 @@ int lanes_of(int64_t H) { return H <= 256 ? 16 : H <= 2048 ? 64 : 256; }
 bool width_ok(int64_t H) { return H > 0 && H % 8 == 0 && H <= kWidest; }
 bool type_ok(int t) { return t == ANC_F32 || t == ANC_BF16; }
 int64_t elem(int t) { return t == ANC_BF16 ? 2 : 4; }
-// Partial rows of dgain: two rows of the batch per group of lanes at least, as many workgroups as keep the memory busy at most.
+// Partial rows of dgain: two rows of the batch per group of lanes at least, as many workgroups as keep the memory busy at most, all with
+// as many rows as the fullest.
 int64_t parts_of(int64_t T, int64_t H) {
-  const int64_t per = 2 * (kThreads / lanes_of(H)), n = (T + per - 1) / per;
-  return n < 1 ? 1 : n > kMostRows ? kMostRows : n;
+  const int64_t groups = kGradThreads / lanes_of(H), most = kMostRows * groups;
+  const int64_t each = T <= 2 * most ? 2 : (T + most - 1) / most, n = (T + each * groups - 1) / (each * groups);
+  return n < 1 ? 1 : n;
 }
 
 }  // namespace
@@ -383,12 +406,12 @@ extern "C" int anc_rms_norm_grad(uint64_t dy, int dy_type, uint64_t x, int strea
     constexpr int lpr = decltype(L)::value, ch = decltype(C)::value;
     with_type(dy_type, [&](auto D) { with_type(stream_type, [&](auto S) { with_type(gain_type, [&](auto G) {
       constexpr int dt = decltype(D)::value, st = decltype(S)::value, gt = decltype(G)::value;
-      if (carry) hipLaunchKernelGGL((k_rms_norm_grad<dt, st, gt, true, lpr, ch>), dim3((unsigned)a.rows), dim3(kThreads), 0, s, a);
-      else hipLaunchKernelGGL((k_rms_norm_grad<dt, st, gt, false, lpr, ch>), dim3((unsigned)a.rows), dim3(kThreads), 0, s, a);
+      if (carry) hipLaunchKernelGGL((k_rms_norm_grad<dt, st, gt, true, lpr, ch>), dim3((unsigned)a.rows), dim3(kGradThreads), 0, s, a);
+      else hipLaunchKernelGGL((k_rms_norm_grad<dt, st, gt, false, lpr, ch>), dim3((unsigned)a.rows), dim3(kGradThreads), 0, s, a);
     }); }); });
   });
   ANC_LAUNCH_CHECK();
-  if (a.rows > 1) hipLaunchKernelGGL(k_gain_sum, dim3((unsigned)((H + 31) / 32)), dim3(kThreads), 0, s, (const float *)workspace, (float *)dgain, a.rows, (int)H, a.accumulate);
+  if (a.rows > 1) hipLaunchKernelGGL(k_gain_sum, dim3((unsigned)((H + 15) / 16)), dim3(kThreads), 0, s, (const float *)workspace, (float *)dgain, a.rows, (int)H, a.accumulate);
   ANC_LAUNCH_CHECK();
   return ANC_OK;
 }
