@@ -177,10 +177,10 @@ _PROTOS = {
     "anc_rms_norm": (None, [u64, C.c_int, u64, C.c_int, u64, C.c_int, i64, i64, f32, u64, C.c_int, u64, u64, u64, u64]),
     "anc_rms_norm_grad_workspace_bytes": (i64, [i64, i64]),
     "anc_rms_norm_grad": (None, [u64, C.c_int, u64, C.c_int, u64, C.c_int, u64, u64, i64, i64, u64, u64, C.c_int, u64, i64, u64]),
-    "anc_gated_ffn": (None, [u64, u64, u64, u64, u64, i64, i64, i64, i64, u64, u64, u64, u64]),
-    "anc_ffn_down": (None, [u64, u64, u64, u64, i64, i64, i64, i64, u64, u64, C.c_int, u64]),
-    "anc_gated_ffn_grad": (None, [u64, u64, u64, u64, u64, u64, i64, i64, i64, i64, u64, u64, u64, u64]),
-    "anc_gated_ffn_dx": (None, [u64, u64, u64, u64, u64, u64, i64, i64, i64, i64, u64, u64, C.c_int, u64]),
+    "anc_gated_ffn": (None, [u64, u64, u64, u64, u64, i64, i64, i64, i64, i64, u64, u64, u64, u64]),
+    "anc_ffn_down": (None, [u64, u64, u64, u64, i64, i64, i64, i64, i64, u64, u64, C.c_int, u64]),
+    "anc_gated_ffn_grad": (None, [u64, u64, u64, u64, u64, u64, i64, i64, i64, i64, i64, u64, u64, u64, u64]),
+    "anc_gated_ffn_dx": (None, [u64, u64, u64, u64, u64, u64, i64, i64, i64, i64, i64, u64, u64, C.c_int, u64]),
     "anc_gemm_dw_workspace_bytes": (i64, [i64, i64, i64]),
     "anc_gemm_dw_multi": (None, [C.POINTER(DwProblem), i32, u64]),
     "anc_expert_dw_multi": (None, [C.POINTER(ExpertDwProblem), i32, u64, u64, u64, i64, i64, u64]),

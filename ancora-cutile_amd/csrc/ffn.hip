@@ -115,30 +115,52 @@ struct Feed {
 constexpr uint32_t kNowhere = 0x80000000u;                 // an offset beyond every descriptor
 
 __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
-__device__ __forceinline__ void eight(const uint16_t *p, float (&f)[8]) {
-  const anc_u32x4 q = *(const anc_u32x4 *)p;
+__device__ __forceinline__ void eight(const anc_u32x4 &q, float (&f)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     f[2 * i] = __uint_as_float(q[i] << 16);
     f[2 * i + 1] = __uint_as_float(q[i] & 0xFFFF0000u);
   }
 }
-__device__ __forceinline__ void put_eight(uint16_t *p, const float (&f)[8]) {
-  *(anc_u32x4 *)p = anc_u32x4{anc_pk_bf16(f[0], f[1]), anc_pk_bf16(f[2], f[3]), anc_pk_bf16(f[4], f[5]), anc_pk_bf16(f[6], f[7])};
+template <bool ONCE, typename V> __device__ __forceinline__ void put(V *p, const V &v) {
+  if constexpr (ONCE) anc_st_stream(p, v);
+  else *p = v;
 }
-// Eight neighbouring values of the product (gated: of both) at element `at` of the outputs.
-template <int MODE> __device__ __forceinline__ void finish(const Ffn &p, int64_t at, float (&v)[8], const float (&w)[8]) {
+template <bool ONCE> __device__ __forceinline__ void put_eight(uint16_t *p, const float (&f)[8]) {
+  put<ONCE>((anc_u32x4 *)p, anc_u32x4{anc_pk_bf16(f[0], f[1]), anc_pk_bf16(f[2], f[3]), anc_pk_bf16(f[4], f[5]), anc_pk_bf16(f[6], f[7])});
+}
+// What eight values of the outputs take besides the product: gate and up, or the residual (fp32: both halves).
+struct Side { anc_u32x4 a, b; };
+template <int MODE> __device__ __forceinline__ Side side_of(const Ffn &p, int64_t at) {
+  Side s{};
+  if constexpr (MODE == kGrad) {
+    s.a = *(const anc_u32x4 *)(p.gate + at);
+    s.b = *(const anc_u32x4 *)(p.up + at);
+  } else if constexpr (MODE != kGated) {
+    if (p.residual != nullptr) {
+      if (p.y_f32) {
+        s.a = *(const anc_u32x4 *)((const float *)p.residual + at);
+        s.b = *(const anc_u32x4 *)((const float *)p.residual + at + 4);
+      } else {
+        s.a = *(const anc_u32x4 *)((const uint16_t *)p.residual + at);
+      }
+    }
+  }
+  return s;
+}
+// Eight neighbouring values of the product (gated: of both) at element `at` of the outputs. ONCE: past the caches.
+template <int MODE, bool ONCE> __device__ __forceinline__ void finish(const Ffn &p, int64_t at, float (&v)[8], const float (&w)[8], const Side &side) {
   if constexpr (MODE == kGated) {
     float h[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) h[k] = v[k] * sigmoid(v[k]) * w[k];
-    put_eight((uint16_t *)p.y + at, h);
-    if (p.dgate != nullptr) put_eight(p.dgate + at, v);
-    if (p.dup != nullptr) put_eight(p.dup + at, w);
+    put_eight<ONCE>((uint16_t *)p.y + at, h);
+    if (p.dgate != nullptr) put_eight<ONCE>(p.dgate + at, v);
+    if (p.dup != nullptr) put_eight<ONCE>(p.dup + at, w);
   } else if constexpr (MODE == kGrad) {
     float g[8], u[8], dg[8], du[8], h[8];
-    eight(p.gate + at, g);
-    eight(p.up + at, u);
+    eight(side.a, g);
+    eight(side.b, u);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const float s = sigmoid(g[k]), a = g[k] * s;
@@ -146,59 +168,66 @@ template <int MODE> __device__ __forceinline__ void finish(const Ffn &p, int64_t
       du[k] = v[k] * a;
       h[k] = a * u[k];
     }
-    put_eight(p.dgate + at, dg);
-    put_eight(p.dup + at, du);
-    if (p.y != nullptr) put_eight((uint16_t *)p.y + at, h);
+    put_eight<ONCE>(p.dgate + at, dg);
+    put_eight<ONCE>(p.dup + at, du);
+    if (p.y != nullptr) put_eight<ONCE>((uint16_t *)p.y + at, h);
   } else if (p.y_f32) {
     anc_f32x4 a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
     if (p.residual != nullptr) {
-      const anc_f32x4 r = *(const anc_f32x4 *)((const float *)p.residual + at), s = *(const anc_f32x4 *)((const float *)p.residual + at + 4);
-      a = anc_f32x4{a.x + r.x, a.y + r.y, a.z + r.z, a.w + r.w};
-      b = anc_f32x4{b.x + s.x, b.y + s.y, b.z + s.z, b.w + s.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        a[k] += __uint_as_float(side.a[k]);
+        b[k] += __uint_as_float(side.b[k]);
+      }
     }
-    *(anc_f32x4 *)((float *)p.y + at) = a;
-    *(anc_f32x4 *)((float *)p.y + at + 4) = b;
+    put<ONCE>((anc_f32x4 *)((float *)p.y + at), a);
+    put<ONCE>((anc_f32x4 *)((float *)p.y + at + 4), b);
   } else {
     if (p.residual != nullptr) {
       float r[8];
-      eight((const uint16_t *)p.residual + at, r);
+      eight(side.a, r);
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] += r[k];
     }
-    put_eight((uint16_t *)p.y + at, v);
+    put_eight<ONCE>((uint16_t *)p.y + at, v);
   }
 }
 
 // ---------------------------------------------------------------- many rows
-template <int MODE, int TM> __global__ void __launch_bounds__(TM * 2, 2) k_ffn_tiles(Ffn p) {
+// TM x TN values to a workgroup, WM x 64 to a wavefront, `waves` wavefronts to a SIMD.
+template <int MODE, int TM, int TN, int WM, int WAVES> __global__ void __launch_bounds__(TM / WM * TN, WAVES) k_ffn_tiles(Ffn p) {
   constexpr bool kForward = MODE == kGated || MODE == kDown;
-  constexpr int kWaves = TM / 32, kBytesA = TM * 64, kBytesB = 256 * 64, kStage = kBytesA + kBytesB, kStages = 3;
+  constexpr int kWide = TN / 64, kWaves = TM / WM * kWide, kHigh = WM / 32;       // wavefronts side by side, in all; fragments of A
+  constexpr int kBytesA = TM * 64, kBytesB = TN * 64, kStage = kBytesA + kBytesB, kStages = 3;
   constexpr int kPiecesA = kBytesA / 1024 / kWaves, kPiecesB = kBytesB / 1024 / kWaves, kPieces = kPiecesA + kPiecesB;
-  constexpr int kCols = MODE == kGated ? 128 : 256;         // columns of the outputs
-  static_assert(kWaves * 8192 <= kStages * kStage && kPieces <= 8, "room for the way out; pieces to a half step");
+  constexpr int kCols = MODE == kGated ? TN / 2 : TN;       // columns of the outputs
+  // Forwards the B tile is [32 k][kSub columns] once or twice: of either weight, or side by side.
+  constexpr int kSub = MODE == kGated ? TN / 2 : 128, kRowB = kSub * 2, kRows = 1024 / kRowB;
+  static_assert(kWaves * 8192 <= kStages * kStage && kPieces <= 2 * kHigh && kPiecesA * kWaves * 1024 == kBytesA && kPiecesB * kWaves * 1024 == kBytesB,
+                "room for the way out; pieces to a half step; whole pieces");
   __shared__ __attribute__((aligned(1024))) unsigned char ring[kStages * kStage];
   Place at;
   if (!place_of(p, TM, at)) return;
   const int K = p.K, N = p.N, lane = (int)(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int wm = wave >> 2, wn = wave & 3, n0 = at.n * kCols;
+  const int wm = wave / kWide, wn = wave % kWide, n0 = at.n * kCols;
   const int rows = at.left < TM ? at.left : TM, steps = (K + TK - 1) / TK, all = MODE == kDx ? 2 * steps : steps;
 
-  // Which of the B tile's two halves this wavefront fetches: forwards [32 k][128 columns] each (of either weight, or side by side), backwards rows.
-  const int half = wave * kPiecesB / 8;
+  const int half = wave * kPiecesB / (kSub / 16);           // the part of the B tile that this wavefront fetches
   Feed fa, fb;
   auto term = [&](int t) {
     fa = Feed{(const char *)(p.A[t] + at.row * K), (int64_t)rows * K * 2, TK * 2};
     if constexpr (kForward) {
-      const int col = MODE == kGated ? n0 : n0 + half * 128;
+      const int col = MODE == kGated ? n0 : n0 + half * kSub;
       fb = Feed{(const char *)(p.B[MODE == kGated ? half : 0] + (int64_t)at.e * K * N + col), ((int64_t)K * N - col) * 2, (int64_t)TK * N * 2};
     } else {
-      const int high = N - n0 < 256 ? N - n0 : 256;
+      const int high = N - n0 < TN ? N - n0 : TN;
       fb = Feed{(const char *)(p.B[t] + ((int64_t)at.e * N + n0) * K), (int64_t)high * K * 2, TK * 2};
     }
   };
   term(0);
-  // Offsets of the pieces, 1 KiB of LDS each. Rows of 64 bytes: 16 to a piece, their four 16-byte chunks XORed with (row >> 2) & 3; rows of 256 bytes: 4 to a
-  // piece, chunks XORed with 4 * (row & 3). Of a row's last 32 k the chunks beyond K are sent nowhere, which reads zeros.
+  // Offsets of the pieces, 1 KiB of LDS each. Rows of 64 bytes: 16 to a piece, their four 16-byte chunks XORed with (row >> 2) & 3; rows of
+  // 256 bytes: 4 to a piece, chunks XORed with 4 * (row & 3); of 128: 8, with 4 * ((row >> 1) & 1): the rows that a read touches fall into
+  // different banks. Of a row's last 32 k the chunks beyond K are sent nowhere, which reads zeros.
   const int chunk = (lane & 3) ^ (lane >> 4);
   const uint32_t beyond = chunk * 8 >= K - (steps - 1) * TK ? kNowhere : 0u;
   uint32_t va[kPiecesA], vb[kPiecesB];
@@ -207,8 +236,12 @@ template <int MODE, int TM> __global__ void __launch_bounds__(TM * 2, 2) k_ffn_t
 #pragma unroll
   for (int i = 0; i < kPiecesB; ++i) {
     const int piece = wave * kPiecesB + i;
-    if constexpr (kForward) vb[i] = (uint32_t)(((piece & 7) * 4 + (lane >> 4)) * N * 2 + (((lane & 15) ^ ((lane >> 4) << 2)) * 16));
-    else vb[i] = (uint32_t)((piece * 16 + (lane >> 2)) * K * 2 + chunk * 16);
+    if constexpr (kForward) {
+      const int row = lane / (kRowB / 16), key = kSub == 128 ? (row & 3) << 2 : (row >> 1 & 1) << 2;
+      vb[i] = (uint32_t)((piece % (kSub / 16) * kRows + row) * N * 2 + ((lane % (kRowB / 16)) ^ key) * 16);
+    } else {
+      vb[i] = (uint32_t)((piece * 16 + (lane >> 2)) * K * 2 + chunk * 16);
+    }
   }
   int fetched = 0;
   uint32_t mask = steps == 1 ? beyond : 0u;
@@ -226,32 +259,32 @@ template <int MODE, int TM> __global__ void __launch_bounds__(TM * 2, 2) k_ffn_t
   };
 
   int ta, tb[2];
-  ta = (wm * 128 + (lane & 31)) * 64;
+  ta = (wm * WM + (lane & 31)) * 64;
   if constexpr (kForward) {
-    const int s16 = lane & 15, g16 = lane >> 4, row = 8 * (g16 >> 1) + (s16 >> 2), sw = (s16 >> 2) << 2;
+    const int s16 = lane & 15, g16 = lane >> 4, row = 8 * (g16 >> 1) + (s16 >> 2), key = kSub == 128 ? (row & 3) << 2 : (row >> 1 & 1) << 2;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int sub = MODE == kGated ? j : wn >> 1, col = MODE == kGated ? wn * 4 : (wn & 1) * 8 + j * 4;     // (in chunks)
-      tb[j] = kBytesA + sub * 8192 + row * 256 + (((col + 2 * (g16 & 1) + ((s16 & 3) >> 1)) ^ sw) * 16) + (s16 & 1) * 8;
+      const int sub = MODE == kGated ? j : wn * 64 / kSub, col = MODE == kGated ? wn * 4 : wn * 64 % kSub / 8 + j * 4;     // (in chunks)
+      tb[j] = kBytesA + sub * (32 * kRowB) + row * kRowB + (((col + 2 * (g16 & 1) + ((s16 & 3) >> 1)) ^ key) * 16) + (s16 & 1) * 8;
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 2; ++j) tb[j] = kBytesA + (wn * 64 + j * 32 + (lane & 31)) * 64;
   }
-  f32x16 acc[4][2];
+  f32x16 acc[kHigh][2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < kHigh; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
-  bf16x8 a[2][4], c[2][2];
-  // fragment i (0 .. 5: b0 b1 a0 a1 a2 a3) of k 16 kk .. 16 kk + 15 of a stage
+  bf16x8 a[2][kHigh], c[2][2];
+  // fragment i (b0 b1 a0 a1 ..) of k 16 kk .. 16 kk + 15 of a stage
   auto load = [&](int set, int i, const unsigned char *stage, int kk) {
     const int sw = ((kk * 2 + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16;
     if (i >= 2) a[set][i - 2] = *(const bf16x8 *)(stage + ta + (i - 2) * (32 * 64) + sw);
-    else if constexpr (kForward) c[set][i] = anc_lds_tr_frag(stage + tb[i] + kk * (16 * 256), stage + tb[i] + kk * (16 * 256) + 4 * 256);
+    else if constexpr (kForward) c[set][i] = anc_lds_tr_frag(stage + tb[i] + kk * (16 * kRowB), stage + tb[i] + kk * (16 * kRowB) + 4 * kRowB);
     else c[set][i] = *(const bf16x8 *)(stage + tb[i] + sw);
   };
   auto multiply = [&](int set, int idx) {        // operands exchanged: a lane holds runs of 4 columns of one row
@@ -266,25 +299,25 @@ template <int MODE, int TM> __global__ void __launch_bounds__(TM * 2, 2) k_ffn_t
   wait_vm<(kStages - 1) * kPieces>();
   lds_barrier();
 #pragma unroll
-  for (int i = 0; i < 6; ++i) load(0, i, ring, 0);
+  for (int i = 0; i < kHigh + 2; ++i) load(0, i, ring, 0);
   // One step: the first half's products over the reads of the second half; then every wavefront has read the stage and the next
   // one has landed for all; then the second half's products over the next stage's first reads and the fetches into the place just read.
   auto step = [&](unsigned char *here, unsigned char *next) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 2 * kHigh; ++i) {
       multiply(0, i);
       __builtin_amdgcn_sched_barrier(0);
-      if (i < 6) load(1, i, here, 1);
+      if (i < kHigh + 2) load(1, i, here, 1);
       __builtin_amdgcn_sched_barrier(0);
     }
     wait_vm<(kStages - 2) * kPieces>();
     lds_barrier();
     const anc_i32x4 da = fa.desc(), db = fb.desc();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 2 * kHigh; ++i) {
       multiply(1, i);
       __builtin_amdgcn_sched_barrier(0);
-      if (i < 6) load(0, i, next, 0);
+      if (i < kHigh + 2) load(0, i, next, 0);
       if (i < kPieces) issue(i, da, db, here);
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -299,12 +332,31 @@ template <int MODE, int TM> __global__ void __launch_bounds__(TM * 2, 2) k_ffn_t
   wait_vm<0>();                                  // (zeros still on their way into the stages)
   lds_barrier();
 
-  // Out through LDS, 32 rows of 64 values at a time: a lane then holds 8 neighbouring columns of a row.
+  // Out through LDS, 32 rows of 64 values at a time: a lane then holds 8 neighbouring columns of a row. What the outputs take besides the
+  // product is fetched one such block ahead; results leave past the caches, which keep the operands of the tiles still to come.
   unsigned char *r = ring + wave * 8192;
-  constexpr int kOcts = MODE == kGated ? 4 : 8;
+  constexpr int kOcts = MODE == kGated ? 4 : 8, kRounds = kOcts / 2;
   const int col0 = n0 + wn * (MODE == kGated ? 32 : 64);
+  constexpr bool kAhead = WAVES < 4;                        // (128 registers hold one block's only)
+  Side side[kAhead ? 2 : 1][kRounds];
+  auto where = [&](int i, int z, int64_t &e) {
+    const int idx = z * 64 + lane, in = wm * WM + i * 32 + idx / kOcts, col = col0 + idx % kOcts * 8;
+    e = (at.row + in) * N + col;
+    return in < rows && col < N;
+  };
+  auto fetch = [&](int i) {
+    if constexpr (MODE != kGated) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+      for (int z = 0; z < kRounds; ++z) {
+        int64_t e;
+        if (where(i, z, e)) side[kAhead ? i & 1 : 0][z] = side_of<MODE>(p, e);
+      }
+    }
+  };
+  if (kAhead) fetch(0);
+#pragma unroll
+  for (int i = 0; i < kHigh; ++i) {
+    if (!kAhead) fetch(i);
     const int rr = lane & 31, hh = lane >> 5;
 #pragma unroll
     for (int j = 0; j < 2; ++j)
@@ -313,9 +365,10 @@ template <int MODE, int TM> __global__ void __launch_bounds__(TM * 2, 2) k_ffn_t
         *(anc_f32x4 *)(r + rr * 256 + (((j * 8 + 2 * g + hh) ^ (rr & 15)) * 16)) =
             anc_f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
     lds_wave_sync();
+    if (kAhead && i + 1 < kHigh) fetch(i + 1);
 #pragma unroll
-    for (int z = 0; z < kOcts / 2; ++z) {
-      const int idx = z * 64 + lane, row = idx / kOcts, oct = idx % kOcts, in = wm * 128 + i * 32 + row, col = col0 + oct * 8;
+    for (int z = 0; z < kRounds; ++z) {
+      const int idx = z * 64 + lane, row = idx / kOcts, oct = idx % kOcts;
       auto values = [&](int ch, float (&f)[8]) {
         const anc_f32x4 lo = *(const anc_f32x4 *)(r + row * 256 + ((ch ^ (row & 15)) * 16)), hi = *(const anc_f32x4 *)(r + row * 256 + (((ch + 1) ^ (row & 15)) * 16));
 #pragma unroll
@@ -324,22 +377,24 @@ template <int MODE, int TM> __global__ void __launch_bounds__(TM * 2, 2) k_ffn_t
       float v[8], w[8];
       values(2 * oct, v);
       if constexpr (MODE == kGated) values(8 + 2 * oct, w);
-      if (in < rows && col < N) finish<MODE>(p, (at.row + in) * N + col, v, w);
+      int64_t e;
+      if (where(i, z, e)) finish<MODE, true>(p, e, v, w, side[kAhead ? i & 1 : 0][z]);
     }
     lds_wave_sync();
   }
 }
 
 // ---------------------------------------------------------------- few rows
-// C blocks of 16 columns (gated: half of them of either weight).
-template <int MODE, int C> __global__ void __launch_bounds__(512, 2) k_ffn_few(Ffn p) {
+// R blocks of 16 rows by C blocks of 16 columns (gated: half of them of either weight), as many stages as LDS holds: what bounds a short
+// product is how many of its weights' bytes are under way at a time.
+template <int MODE, int R, int C> __global__ void __launch_bounds__(512, 2) k_ffn_few(Ffn p) {
   constexpr bool kForward = MODE == kGated || MODE == kDown;
-  constexpr int TM = 32, kWaves = 8, kStages = C == 4 ? 2 : 3, kStage = 2048 + C * 1024, kPieces = 2 + C;
+  constexpr int TM = 16 * R, kWaves = 8, kPieces = R + C, kStage = kPieces * 1024, kStages = 18 / kPieces;
   constexpr int kSub = MODE == kGated ? C / 2 : C;          // blocks of a row of one weight
   constexpr int kRowB = kSub * 32, kPer = 1024 / kRowB;     // bytes of it, rows to a piece
   constexpr int kCols = kSub * 16;
   __shared__ __attribute__((aligned(1024))) unsigned char ring[kWaves * kStages * kStage];
-  static_assert(kWaves * 32 * C * 64 <= sizeof(ring), "room for the partial sums");
+  static_assert(kWaves * R * C * 1024 <= (int)sizeof(ring) && kStages >= 2 && sizeof(ring) <= 147456, "room for the partial sums");
   Place at;
   if (!place_of(p, TM, at)) return;
   const int K = p.K, N = p.N, lane = (int)(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -356,24 +411,24 @@ template <int MODE, int C> __global__ void __launch_bounds__(512, 2) k_ffn_few(F
     const int64_t lefta = ((int64_t)rows * K - k0) * 2;
     const anc_i32x4 da = buffer_of((const char *)(p.A[second] + at.row * K + (there ? k0 : 0)), there ? (uint32_t)lefta : 0u);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) dma16_bounded(da, (va + (uint32_t)(i * 16 * K * 2)) | mask, lds_addr(stage + i * 1024));
+    for (int i = 0; i < R; ++i) dma16_bounded(da, (va + (uint32_t)(i * 16 * K * 2)) | mask, lds_addr(stage + i * 1024));
     if constexpr (kForward) {
 #pragma unroll
       for (int i = 0; i < C; ++i) {
         const int w = MODE == kGated ? i / (C / 2 > 0 ? C / 2 : 1) : 0, piece = MODE == kGated ? i % (C / 2 > 0 ? C / 2 : 1) : i;
         const Feed f{(const char *)(p.B[w] + (int64_t)at.e * K * N + (there ? (int64_t)k0 * N : 0) + n0), there ? ((int64_t)(K - k0) * N - n0) * 2 : 0, 0};
-        dma16_bounded(f.desc(), vb + (uint32_t)(piece * kPer * N * 2), lds_addr(stage + 2048 + i * 1024));
+        dma16_bounded(f.desc(), vb + (uint32_t)(piece * kPer * N * 2), lds_addr(stage + (R + i) * 1024));
       }
     } else {
       const int high = N - n0 < kCols ? N - n0 : kCols;
       const anc_i32x4 db = buffer_of((const char *)(p.B[second] + ((int64_t)at.e * N + n0) * K + (there ? k0 : 0)), there ? (uint32_t)(((int64_t)high * K - k0) * 2) : 0u);
 #pragma unroll
-      for (int i = 0; i < C; ++i) dma16_bounded(db, (vb + (uint32_t)(i * 16 * K * 2)) | mask, lds_addr(stage + 2048 + i * 1024));
+      for (int i = 0; i < C; ++i) dma16_bounded(db, (vb + (uint32_t)(i * 16 * K * 2)) | mask, lds_addr(stage + (R + i) * 1024));
     }
   };
-  f32x4v acc[2][C];
+  f32x4v acc[R][C];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < R; ++i)
 #pragma unroll
     for (int j = 0; j < C; ++j) acc[i][j] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
   const int s16 = lane & 15, g16 = lane >> 4;
@@ -383,16 +438,16 @@ template <int MODE, int C> __global__ void __launch_bounds__(512, 2) k_ffn_few(F
   for (int t = wave; t < all; t += kWaves) {
     const unsigned char *stage = mine + here;
     wait_vm<(kStages - 1) * kPieces>();
-    bf16x8 a[2], b[C];
+    bf16x8 a[R], b[C];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) a[i] = *(const bf16x8 *)(stage + i * 1024 + ta);
+    for (int i = 0; i < R; ++i) a[i] = *(const bf16x8 *)(stage + i * 1024 + ta);
 #pragma unroll
     for (int j = 0; j < C; ++j) {
       if constexpr (kForward) {
-        const unsigned char *q = stage + 2048 + j / kSub * (kSub * 1024) + (8 * g16 + (s16 >> 2)) * kRowB + j % kSub * 32 + (s16 & 3) * 8;
+        const unsigned char *q = stage + R * 1024 + j / kSub * (kSub * 1024) + (8 * g16 + (s16 >> 2)) * kRowB + j % kSub * 32 + (s16 & 3) * 8;
         b[j] = anc_lds_tr_frag(q, q + 4 * kRowB);
       } else {
-        b[j] = *(const bf16x8 *)(stage + 2048 + j * 1024 + ta);
+        b[j] = *(const bf16x8 *)(stage + (R + j) * 1024 + ta);
       }
     }
     lds_wave_sync();                             // (read before the stage is fetched into again)
@@ -400,7 +455,7 @@ template <int MODE, int C> __global__ void __launch_bounds__(512, 2) k_ffn_few(F
 #pragma unroll
     for (int j = 0; j < C; ++j)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
+      for (int i = 0; i < R; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
     here = here + kStage < kStages * kStage ? here + kStage : 0;
   }
   wait_vm<0>();
@@ -408,66 +463,109 @@ template <int MODE, int C> __global__ void __launch_bounds__(512, 2) k_ffn_few(F
   // The wavefronts' sums, in ascending order: [wavefront][row][column] fp32.
   float *sums = (float *)ring;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int j = 0; j < C; ++j) *(f32x4v *)(sums + (wave * 32 + i * 16 + s16) * (C * 16) + j * 16 + g16 * 4) = acc[i][j];
+    for (int j = 0; j < C; ++j) *(f32x4v *)(sums + (wave * TM + i * 16 + s16) * (C * 16) + j * 16 + g16 * 4) = acc[i][j];
   lds_barrier();
   constexpr int kOcts = kCols / 8;
-  for (int idx = (int)threadIdx.x; idx < 32 * kOcts; idx += kWaves * 64) {
+  for (int idx = (int)threadIdx.x; idx < TM * kOcts; idx += kWaves * 64) {
     const int row = idx / kOcts, oct = idx % kOcts, col = n0 + oct * 8;
     if (row >= rows || col >= N) continue;
+    const int64_t e = (at.row + row) * N + col;
+    const Side side = side_of<MODE>(p, e);
     auto total = [&](int first, float (&f)[8]) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) f[k] = sums[row * (C * 16) + first + k];
 #pragma unroll
       for (int w = 1; w < kWaves; ++w)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] += sums[(w * 32 + row) * (C * 16) + first + k];
+        for (int k = 0; k < 8; ++k) f[k] += sums[(w * TM + row) * (C * 16) + first + k];
     };
     float v[8], w[8];
     total(oct * 8, v);
     if constexpr (MODE == kGated) total(kCols + oct * 8, w);
-    finish<MODE>(p, (at.row + row) * N + col, v, w);
+    finish<MODE, false>(p, e, v, w, side);
   }
 }
 
 // ---------------------------------------------------------------- launch
-template <int MODE> int launch(Ffn p, const char *who, hipStream_t s) {
-  const int64_t E = p.experts > 0 ? p.experts : 1, mean = (p.rows + E - 1) / E;
-  const int64_t some = p.rows < E ? p.rows : E;              // segments that can hold a row
-  const int wide = MODE == kGated ? 128 : 256;
-  auto row_tiles = [&](int64_t TM) { return p.counts == nullptr ? (p.rows + TM - 1) / TM : p.rows / TM + some; };
-  auto grid_of = [&](int64_t TM) { return (row_tiles(TM) * p.tn + kXcds - 1) / kXcds * kXcds; };
+template <int V> struct IC { static constexpr int value = V; };
+// Which kernel takes a call: the one whose rounds take least by what a step of 32 k and a round cost, in us. `most`: rows that all
+// segments hold together at most. Measured on whole calls (1 to 8192 rows, 1024 x 2816, 2048 x 2048, 1024 x 4096, dense; 64 and 128 experts of
+// 1024 x 768): a step of k_ffn_tiles where up to 128, 256, .. workgroups are at work, and a round's start and end; of k_ffn_few, one workgroup
+// to a CU, a wavefront's step (of eight). Both sides of some lines, us: gated, 64 rows, 1024 -> 2816: 32x32 by eight wavefronts 10.1, 128x64
+// tiles 13.7; 256 rows 25.7 and 14.2. Down, 1024 rows, 2816 -> 1024: 64x64 by eight wavefronts 17.9, 128x128 tiles 30.4, 128x256 40; 2048 rows 32.1, 31.8,
+// 41; 4096 rows (4096 -> 1024) 47 and 59 for the tiles. Backwards, 8192 rows of 2048 x 2048 in whole rounds: 256x256 134, 128x256 150; 8192 of 1024 x
+// 2816 in half a round of 256x256: 160 and 113. 64 experts of 1024 x 768 with 4 rows each: few rows 66, 128x128 tiles 39.
+template <int MODE> int launch(Ffn p, int64_t most, const char *who, hipStream_t s) {
+  constexpr int per = MODE == kGated ? 2 : 1;                 // values of the product to one of the outputs
+  const int64_t some = p.counts == nullptr ? 1 : most < p.experts ? most : p.experts;              // segments that can hold a row
+  const float steps = (float)((p.K + TK - 1) / TK * (MODE == kDx ? 2 : 1));
+  auto columns = [&](int64_t TN) { return (p.N + TN / per - 1) / (TN / per); };
+  // workgroups that find work, about (an even routing leaves E e^(-most / E) experts without a row); and at most
+  const int64_t used = p.counts == nullptr ? 1 : (int64_t)ceilf((float)p.experts * -expm1f(-(float)most / (float)p.experts));
+  auto live = [&](int64_t TM, int64_t TN) {
+    const int64_t m = p.counts == nullptr ? (most + TM - 1) / TM : most / TM + (used + 1) / 2;
+    return (m < used ? used : m) * columns(TN);
+  };
+  auto grid_of = [&](int64_t TM) {
+    const int64_t m = p.counts == nullptr ? (most + TM - 1) / TM : most / TM + some;
+    return (m * p.tn + kXcds - 1) / kXcds * kXcds;
+  };
+  auto rounds = [&](int64_t n, int64_t slots, auto cost) { return (float)(n / slots) * cost(slots) + (n % slots ? cost(n % slots) : 0.0f); };
+  const float cold = p.counts == nullptr ? 1.0f : 1.4f;      // every expert's weights come from memory, in short rows
+  const float time[] = {
+      rounds(live(256, 256), 256, [&](int64_t r) { return steps * (r <= 128 ? 0.80f : 0.92f) + 8.0f; }),
+      rounds(live(128, 256), 512, [&](int64_t r) { return steps * (r <= 128 ? 0.46f : r <= 256 ? 0.60f : 0.98f) + 4.0f; }),
+      rounds(live(128, 128), 768, [&](int64_t r) { return steps * (r <= 128 ? 0.33f : r <= 256 ? 0.38f : r <= 512 ? 0.63f : 0.90f) + 3.5f; }),
+      rounds(live(64, 64), 256, [&](int64_t) { return cold * (steps / 8 * 0.92f + 5.7f); }),
+      rounds(live(32, 64), 256, [&](int64_t) { return cold * (steps / 8 * 0.72f + 4.6f); }),
+      rounds(live(32, 32), 256, [&](int64_t) { return cold * (steps / 8 * 0.47f + 4.2f); }),
+      MODE == kGated ? 1e30f : rounds(live(16, 16), 256, [&](int64_t) { return cold * (steps / 8 * 0.25f + 4.0f); }),
+  };
+  int best = 0;
+  for (int i = 1; i < 7; ++i)
+    if (time[i] < time[best]) best = i;
+#ifdef FFN_PICK
+  best = FFN_PICK;
+#endif
   AncProfScope prof(ANC_PROF_DW_GEMM, s);
-  if (mean <= 48) {
-    constexpr int kLeast = MODE == kGated ? 2 : 1;
-    int C = 4;
-    while (C > kLeast && row_tiles(32) * ((p.N + 16 * C / kLeast - 1) / (16 * C / kLeast)) < 256) C /= 2;
-    p.tn = (p.N + 16 * C / kLeast - 1) / (16 * C / kLeast);
-    ANC_REQUIRE(grid_of(32) < (1ll << 31) / 512, "%s: too large for one call", who);
-    const dim3 grid((unsigned)grid_of(32));
-    if (C == 4) hipLaunchKernelGGL((k_ffn_few<MODE, 4>), grid, dim3(512), 0, s, p);
-    else if (C == 2) hipLaunchKernelGGL((k_ffn_few<MODE, 2>), grid, dim3(512), 0, s, p);
-    else if constexpr (MODE != kGated) hipLaunchKernelGGL((k_ffn_few<MODE, 1>), grid, dim3(512), 0, s, p);
-  } else {
-    p.tn = (p.N + wide - 1) / wide;
-    const bool high = ((p.rows + 255) / 256) * p.tn >= 256;
-    const int TM = high ? 256 : 128;
-    ANC_REQUIRE(grid_of(TM) < (1ll << 31) / 512, "%s: too large for one call", who);
-    const dim3 grid((unsigned)grid_of(TM));
-    if (high) hipLaunchKernelGGL((k_ffn_tiles<MODE, 256>), grid, dim3(512), 0, s, p);
-    else hipLaunchKernelGGL((k_ffn_tiles<MODE, 128>), grid, dim3(256), 0, s, p);
+  auto few = [&](auto R, auto C) {
+    constexpr int r = decltype(R)::value, c = decltype(C)::value;
+    p.tn = (int)columns(16 * c);
+    ANC_REQUIRE(grid_of(16 * r) < (1ll << 31) / 512, "%s: too large for one call", who);
+    hipLaunchKernelGGL((k_ffn_few<MODE, r, c>), dim3((unsigned)grid_of(16 * r)), dim3(512), 0, s, p);
+    return ANC_OK;
+  };
+  auto tiles = [&](auto TM, auto TN, auto WM, auto W) {
+    constexpr int tm = decltype(TM)::value, tn = decltype(TN)::value, wm = decltype(WM)::value, w = decltype(W)::value;
+    p.tn = (int)columns(tn);
+    ANC_REQUIRE(grid_of(tm) < (1ll << 31) / 512, "%s: too large for one call", who);
+    hipLaunchKernelGGL((k_ffn_tiles<MODE, tm, tn, wm, w>), dim3((unsigned)grid_of(tm)), dim3(tm / wm * tn), 0, s, p);
+    return ANC_OK;
+  };
+  int rc = ANC_OK;
+  switch (best) {
+    case 0: rc = tiles(IC<256>{}, IC<256>{}, IC<128>{}, IC<2>{}); break;
+    case 1: rc = tiles(IC<128>{}, IC<256>{}, IC<128>{}, IC<2>{}); break;
+    case 2: rc = tiles(IC<128>{}, IC<128>{}, IC<64>{}, IC<3>{}); break;
+    case 3: rc = few(IC<4>{}, IC<4>{}); break;
+    case 4: rc = few(IC<2>{}, IC<4>{}); break;
+    case 5: rc = few(IC<2>{}, IC<2>{}); break;
+    default: if constexpr (per == 1) rc = few(IC<1>{}, IC<1>{}); break;
   }
+  if (rc != ANC_OK) return rc;
   ANC_LAUNCH_CHECK();
   return ANC_OK;
 }
 
-int check(const char *who, uint64_t counts, uint64_t offsets, int64_t experts, int64_t rows, int64_t H, int64_t I) {
+int check(const char *who, uint64_t counts, uint64_t offsets, int64_t experts, int64_t rows, int64_t tokens, int64_t H, int64_t I) {
   ANC_REQUIRE(H > 0 && I > 0 && H % 8 == 0 && I % 8 == 0 && H <= (1 << 17) && I <= (1 << 17),
               "%s: needs H %% 8 == 0 and I %% 8 == 0 (H=%lld I=%lld)", who, (long long)H, (long long)I);
   ANC_REQUIRE(rows >= 0 && rows < (1ll << 31), "%s: %lld rows", who, (long long)rows);
   ANC_REQUIRE((counts != 0) == (experts > 0) && (offsets != 0) == (experts > 0) && ((counts | offsets) & 3) == 0 && experts >= 0 && experts <= 512,
               "%s: bad segments (%lld experts)", who, (long long)experts);
+  ANC_REQUIRE(tokens >= 0 && tokens <= rows && (experts > 0 || tokens == rows), "%s: %lld of %lld rows in segments", who, (long long)tokens, (long long)rows);
   return ANC_OK;
 }
 // Outputs meet no other buffer of the call, but for the pairs that are one buffer on purpose (the same elements, read before they are written).
@@ -483,11 +581,11 @@ AncSpan span(uint64_t at, int64_t bytes) { return AncSpan{at, at != 0 ? bytes : 
 
 }  // namespace
 
-extern "C" int anc_gated_ffn(uint64_t x, uint64_t Wg, uint64_t Wu, uint64_t counts, uint64_t offsets, int64_t experts, int64_t rows,
+extern "C" int anc_gated_ffn(uint64_t x, uint64_t Wg, uint64_t Wu, uint64_t counts, uint64_t offsets, int64_t experts, int64_t rows, int64_t tokens,
                              int64_t H, int64_t I, uint64_t h, uint64_t gate, uint64_t up, uint64_t stream) {
   const char *who = "anc_gated_ffn";
-  if (int rc = check(who, counts, offsets, experts, rows, H, I)) return rc;
-  if (rows == 0) return ANC_OK;
+  if (int rc = check(who, counts, offsets, experts, rows, tokens, H, I)) return rc;
+  if (tokens == 0) return ANC_OK;
   ANC_REQUIRE(x && Wg && Wu && h && ((x | Wg | Wu | h | gate | up) & 15) == 0, "%s: null or misaligned pointer", who);
   const int64_t E = experts > 0 ? experts : 1, w = E * H * I * 2, n = rows * I * 2;
   if (int rc = apart<3, 5>(who, {span(h, n), span(gate, n), span(up, n)},
@@ -505,15 +603,15 @@ extern "C" int anc_gated_ffn(uint64_t x, uint64_t Wg, uint64_t Wu, uint64_t coun
   p.y = (void *)h;
   p.dgate = (uint16_t *)gate;
   p.dup = (uint16_t *)up;
-  return launch<kGated>(p, who, anc_stream(stream));
+  return launch<kGated>(p, tokens, who, anc_stream(stream));
 }
 
-extern "C" int anc_ffn_down(uint64_t h, uint64_t Wd, uint64_t counts, uint64_t offsets, int64_t experts, int64_t rows, int64_t I,
+extern "C" int anc_ffn_down(uint64_t h, uint64_t Wd, uint64_t counts, uint64_t offsets, int64_t experts, int64_t rows, int64_t tokens, int64_t I,
                             int64_t H, uint64_t residual, uint64_t y, int y_type, uint64_t stream) {
   const char *who = "anc_ffn_down";
-  if (int rc = check(who, counts, offsets, experts, rows, H, I)) return rc;
+  if (int rc = check(who, counts, offsets, experts, rows, tokens, H, I)) return rc;
   ANC_REQUIRE(y_type == ANC_F32 || y_type == ANC_BF16, "%s: bad y_type %d", who, y_type);
-  if (rows == 0) return ANC_OK;
+  if (tokens == 0) return ANC_OK;
   ANC_REQUIRE(h && Wd && y && ((h | Wd | y | residual) & 15) == 0, "%s: null or misaligned pointer", who);
   const int64_t E = experts > 0 ? experts : 1, n = rows * H * (y_type == ANC_F32 ? 4 : 2);
   if (int rc = apart<1, 5>(who, {span(y, n)}, {span(residual, n), span(h, rows * I * 2), span(Wd, E * H * I * 2), span(counts, 4 * experts), span(offsets, 4 * experts + 4)}, {0})) return rc;
@@ -529,14 +627,14 @@ extern "C" int anc_ffn_down(uint64_t h, uint64_t Wd, uint64_t counts, uint64_t o
   p.residual = (const void *)residual;
   p.y = (void *)y;
   p.y_f32 = y_type == ANC_F32;
-  return launch<kDown>(p, who, anc_stream(stream));
+  return launch<kDown>(p, tokens, who, anc_stream(stream));
 }
 
 extern "C" int anc_gated_ffn_grad(uint64_t dy, uint64_t Wd, uint64_t gate, uint64_t up, uint64_t counts, uint64_t offsets, int64_t experts,
-                                  int64_t rows, int64_t H, int64_t I, uint64_t dgate, uint64_t dup, uint64_t h, uint64_t stream) {
+                                  int64_t rows, int64_t tokens, int64_t H, int64_t I, uint64_t dgate, uint64_t dup, uint64_t h, uint64_t stream) {
   const char *who = "anc_gated_ffn_grad";
-  if (int rc = check(who, counts, offsets, experts, rows, H, I)) return rc;
-  if (rows == 0) return ANC_OK;
+  if (int rc = check(who, counts, offsets, experts, rows, tokens, H, I)) return rc;
+  if (tokens == 0) return ANC_OK;
   ANC_REQUIRE(dy && Wd && gate && up && dgate && dup && ((dy | Wd | gate | up | dgate | dup | h) & 15) == 0, "%s: null or misaligned pointer", who);
   const int64_t E = experts > 0 ? experts : 1, n = rows * I * 2;
   if (int rc = apart<3, 6>(who, {span(dgate, n), span(dup, n), span(h, n)},
@@ -555,15 +653,15 @@ extern "C" int anc_gated_ffn_grad(uint64_t dy, uint64_t Wd, uint64_t gate, uint6
   p.dgate = (uint16_t *)dgate;
   p.dup = (uint16_t *)dup;
   p.y = (void *)h;
-  return launch<kGrad>(p, who, anc_stream(stream));
+  return launch<kGrad>(p, tokens, who, anc_stream(stream));
 }
 
 extern "C" int anc_gated_ffn_dx(uint64_t dgate, uint64_t dup, uint64_t Wg, uint64_t Wu, uint64_t counts, uint64_t offsets, int64_t experts,
-                                int64_t rows, int64_t H, int64_t I, uint64_t residual, uint64_t dx, int dx_type, uint64_t stream) {
+                                int64_t rows, int64_t tokens, int64_t H, int64_t I, uint64_t residual, uint64_t dx, int dx_type, uint64_t stream) {
   const char *who = "anc_gated_ffn_dx";
-  if (int rc = check(who, counts, offsets, experts, rows, H, I)) return rc;
+  if (int rc = check(who, counts, offsets, experts, rows, tokens, H, I)) return rc;
   ANC_REQUIRE(dx_type == ANC_F32 || dx_type == ANC_BF16, "%s: bad dx_type %d", who, dx_type);
-  if (rows == 0) return ANC_OK;
+  if (tokens == 0) return ANC_OK;
   ANC_REQUIRE(dgate && dup && Wg && Wu && dx && ((dgate | dup | Wg | Wu | dx | residual) & 15) == 0, "%s: null or misaligned pointer", who);
   const int64_t E = experts > 0 ? experts : 1, w = E * H * I * 2, n = rows * H * (dx_type == ANC_F32 ? 4 : 2);
   if (int rc = apart<1, 7>(who, {span(dx, n)}, {span(residual, n), span(dgate, rows * I * 2), span(dup, rows * I * 2), span(Wg, w), span(Wu, w), span(counts, 4 * experts), span(offsets, 4 * experts + 4)}, {0})) return rc;
@@ -581,5 +679,5 @@ extern "C" int anc_gated_ffn_dx(uint64_t dgate, uint64_t dup, uint64_t Wg, uint6
   p.residual = (const void *)residual;
   p.y = (void *)dx;
   p.y_f32 = dx_type == ANC_F32;
-  return launch<kDx>(p, who, anc_stream(stream));
+  return launch<kDx>(p, tokens, who, anc_stream(stream));
 }

@@ -20,14 +20,14 @@ from .embed import _type
 
 
 def _call(who, rows_name, rows_buf, plan):
-    """(rows, experts, counts, offsets) of a call whose first operand is rows_buf (rows, K)."""
+    """(rows, rows that are tokens' at most, experts, counts, offsets) of a call whose first operand is rows_buf (rows, K)."""
     if len(rows_buf.shape) != 2 or rows_buf.dtype != np.uint16:
         raise ValueError(f"{who}: {rows_name} is {rows_buf.shape} {rows_buf.dtype}, rows of bf16 bits expected")
     if plan is None:
-        return rows_buf.shape[0], 0, 0, 0
+        return rows_buf.shape[0], rows_buf.shape[0], 0, 0, 0
     plan._used(who)
     counts, offsets = plan._at[:2]
-    return plan.capacity, plan.E, counts, offsets
+    return plan.capacity, plan.active * plan.k, plan.E, counts, offsets
 
 
 def _rows(who, name, b, rows, width, dtype=np.uint16):
@@ -63,22 +63,22 @@ def gated_ffn(x, Wg, Wu, si, h, gate=None, up=None, plan=None):
     """h = silu(x Wg) * (x Wu): x (rows, H), Wg and Wu (H, I) or (E, H, I), h (rows, I), all bf16 bits; gate and up (rows, I)
     receive x Wg and x Wu where a backward pass will want them. With a plan rows is its capacity. Asynchronous on `si`."""
     who = "gated_ffn"
-    rows, E, counts, offsets = _call(who, "x", x, plan)
+    rows, tokens, E, counts, offsets = _call(who, "x", x, plan)
     H, I = x.shape[1], h.shape[-1]
     _dims(who, H, I)
     api.anc_gated_ffn(_rows(who, "x", x, rows, H), _weight(who, "Wg", Wg, E, H, I), _weight(who, "Wu", Wu, E, H, I), counts, offsets, E,
-                      rows, H, I, _rows(who, "h", h, rows, I), _rows(who, "gate", gate, rows, I), _rows(who, "up", up, rows, I), int(si))
+                      rows, tokens, H, I, _rows(who, "h", h, rows, I), _rows(who, "gate", gate, rows, I), _rows(who, "up", up, rows, I), int(si))
 
 
 def ffn_down(h, Wd, si, y, residual=None, plan=None):
     """y = h Wd + residual: h (rows, I) and Wd (I, H) or (E, I, H) bf16 bits; y (rows, H) and residual (or None) of one type, float32 or
     bf16 bits. residual may be y itself. Asynchronous on `si`."""
     who = "ffn_down"
-    rows, E, counts, offsets = _call(who, "h", h, plan)
+    rows, tokens, E, counts, offsets = _call(who, "h", h, plan)
     I, H = h.shape[1], y.shape[-1]
     _dims(who, H, I)
     res, kind = _residual(who, residual, y, rows, H)
-    api.anc_ffn_down(_rows(who, "h", h, rows, I), _weight(who, "Wd", Wd, E, I, H), counts, offsets, E, rows, I, H, res, y.ptr, kind, int(si))
+    api.anc_ffn_down(_rows(who, "h", h, rows, I), _weight(who, "Wd", Wd, E, I, H), counts, offsets, E, rows, tokens, I, H, res, y.ptr, kind, int(si))
 
 
 def gated_ffn_grad(dy, gate, up, Wd, si, dgate, dup, h=None, plan=None):
@@ -86,11 +86,11 @@ def gated_ffn_grad(dy, gate, up, Wd, si, dgate, dup, h=None, plan=None):
     s = sigmoid(gate), dgate = dh up s (1 + gate (1 - s)), dup = dh gate s, and h = gate s up where asked for (dWd = h^T dy). gate, up, dgate,
     dup, h (rows, I) bf16 bits; dgate may be gate and dup up. Asynchronous on `si`."""
     who = "gated_ffn_grad"
-    rows, E, counts, offsets = _call(who, "dy", dy, plan)
+    rows, tokens, E, counts, offsets = _call(who, "dy", dy, plan)
     H, I = dy.shape[1], gate.shape[-1]
     _dims(who, H, I)
     api.anc_gated_ffn_grad(_rows(who, "dy", dy, rows, H), _weight(who, "Wd", Wd, E, I, H), _rows(who, "gate", gate, rows, I),
-                           _rows(who, "up", up, rows, I), counts, offsets, E, rows, H, I, _rows(who, "dgate", dgate, rows, I),
+                           _rows(who, "up", up, rows, I), counts, offsets, E, rows, tokens, H, I, _rows(who, "dgate", dgate, rows, I),
                            _rows(who, "dup", dup, rows, I), _rows(who, "h", h, rows, I), int(si))
 
 
@@ -98,9 +98,9 @@ def gated_ffn_dx(dgate, dup, Wg, Wu, si, dx, residual=None, plan=None):
     """dx = dgate Wg^T + dup Wu^T + residual: dgate and dup (rows, I), Wg and Wu (H, I) or (E, H, I) bf16 bits; dx (rows, H) and residual (the
     gradient along the residual stream, or None) of one type, float32 or bf16 bits. residual may be dx itself. Asynchronous on `si`."""
     who = "gated_ffn_dx"
-    rows, E, counts, offsets = _call(who, "dgate", dgate, plan)
+    rows, tokens, E, counts, offsets = _call(who, "dgate", dgate, plan)
     I, H = dgate.shape[1], dx.shape[-1]
     _dims(who, H, I)
     res, kind = _residual(who, residual, dx, rows, H)
     api.anc_gated_ffn_dx(_rows(who, "dgate", dgate, rows, I), _rows(who, "dup", dup, rows, I), _weight(who, "Wg", Wg, E, H, I),
-                         _weight(who, "Wu", Wu, E, H, I), counts, offsets, E, rows, H, I, res, dx.ptr, kind, int(si))
+                         _weight(who, "Wu", Wu, E, H, I), counts, offsets, E, rows, tokens, H, I, res, dx.ptr, kind, int(si))

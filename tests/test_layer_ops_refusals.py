@@ -61,20 +61,20 @@ def test_ffn_entries():
     rows, H, I, E = 1000, 64, 128, 3
     hi, ii, w = rows * H * 2, rows * I * 2, E * H * I * 2
     calls = {
-        # x, Wg, Wu, counts, offsets, experts, rows, H, I, h, gate, up, stream
-        "anc_gated_ffn": ((a[0], a[1], a[2], a[3], a[4], E, rows, H, I, a[5], a[6], a[7], 0), (0, 1, 2, 9), (10, 11), (3, 4, 5), (6, 7, 8),
-                          ((9, a[0]), (9, a[0] + hi - 16), (10, a[1] + w - 16), (11, a[4]), (10, a[5]), (11, a[6] + ii - 16), (9, a[3] - ii + 16))),
-        # h, Wd, counts, offsets, experts, rows, I, H, residual, y, y_type, stream
-        "anc_ffn_down": ((a[0], a[1], a[2], a[3], E, rows, I, H, a[4], a[5], 0, 0), (0, 1, 9), (8,), (2, 3, 4), (5, 6, 7),
-                         ((9, a[0]), (9, a[1] + w - 16), (9, a[2]), (9, a[4] + 16), (8, a[5] + 2 * hi - 16))),
-        # dy, Wd, gate, up, counts, offsets, experts, rows, H, I, dgate, dup, h, stream
-        "anc_gated_ffn_grad": ((a[0], a[1], a[2], a[3], a[4], a[5], E, rows, H, I, a[6], a[7], a[8], 0), (0, 1, 2, 3, 10, 11), (12,), (4, 5, 6), (7, 8, 9),
-                               ((10, a[3]), (11, a[2]), (12, a[2]), (12, a[3]), (10, a[0]), (11, a[1] + w - 16), (10, a[7] + 16), (12, a[6]), (10, a[2] + 16), (12, a[4] - ii + 16))),
-        # dgate, dup, Wg, Wu, counts, offsets, experts, rows, H, I, residual, dx, dx_type, stream
-        "anc_gated_ffn_dx": ((a[0], a[1], a[2], a[3], a[4], a[5], E, rows, H, I, a[6], a[7], 1, 0), (0, 1, 2, 3, 11), (10,), (4, 5, 6), (7, 8, 9),
-                             ((11, a[0]), (11, a[1] + ii - 16), (11, a[3]), (11, a[5] - hi + 16), (11, a[6] + 16))),
+        # x, Wg, Wu, counts, offsets, experts, rows, tokens, H, I, h, gate, up, stream
+        "anc_gated_ffn": ((a[0], a[1], a[2], a[3], a[4], E, rows, rows, H, I, a[5], a[6], a[7], 0), (0, 1, 2, 10), (11, 12), (3, 4, 5), (6, 7, 8, 9),
+                          ((10, a[0]), (10, a[0] + hi - 16), (11, a[1] + w - 16), (12, a[4]), (11, a[5]), (12, a[6] + ii - 16), (10, a[3] - ii + 16))),
+        # h, Wd, counts, offsets, experts, rows, tokens, I, H, residual, y, y_type, stream
+        "anc_ffn_down": ((a[0], a[1], a[2], a[3], E, rows, rows, I, H, a[4], a[5], 0, 0), (0, 1, 10), (9,), (2, 3, 4), (5, 6, 7, 8),
+                         ((10, a[0]), (10, a[1] + w - 16), (10, a[2]), (10, a[4] + 16), (9, a[5] + 2 * hi - 16))),
+        # dy, Wd, gate, up, counts, offsets, experts, rows, tokens, H, I, dgate, dup, h, stream
+        "anc_gated_ffn_grad": ((a[0], a[1], a[2], a[3], a[4], a[5], E, rows, rows, H, I, a[6], a[7], a[8], 0), (0, 1, 2, 3, 11, 12), (13,), (4, 5, 6), (7, 8, 9, 10),
+                               ((11, a[3]), (12, a[2]), (13, a[2]), (13, a[3]), (11, a[0]), (12, a[1] + w - 16), (11, a[7] + 16), (13, a[6]), (11, a[2] + 16), (13, a[4] - ii + 16))),
+        # dgate, dup, Wg, Wu, counts, offsets, experts, rows, tokens, H, I, residual, dx, dx_type, stream
+        "anc_gated_ffn_dx": ((a[0], a[1], a[2], a[3], a[4], a[5], E, rows, rows, H, I, a[6], a[7], 1, 0), (0, 1, 2, 3, 12), (11,), (4, 5, 6), (7, 8, 9, 10),
+                             ((12, a[0]), (12, a[1] + ii - 16), (12, a[3]), (12, a[5] - hi + 16), (12, a[6] + 16))),
     }
-    for name, (ok, needed, optional, (counts, offsets, experts), (nrows, d1, d2), overlaps) in calls.items():
+    for name, (ok, needed, optional, (counts, offsets, experts), (nrows, ntok, d1, d2), overlaps) in calls.items():
         for at in needed:
             _refused(lib, name, _but(ok, at, 0), "null")
         for at in needed + optional:
@@ -88,9 +88,12 @@ def test_ffn_entries():
             _refused(lib, name, _but(ok, nrows, value), "rows")
         for at, other in overlaps:
             _refused(lib, name, _but(ok, at, other), "overlap")
-        assert getattr(lib, name)(*_but(ok, nrows, 0)) == 0
-    _refused(lib, "anc_ffn_down", _but(calls["anc_ffn_down"][0], 10, 2), "y_type")
-    _refused(lib, "anc_gated_ffn_dx", _but(calls["anc_gated_ffn_dx"][0], 12, 2), "dx_type")
+        for value in (-1, rows + 1):
+            _refused(lib, name, _but(ok, ntok, value), "rows")
+        _refused(lib, name, _but(_but(_but(_but(ok, ntok, rows - 1), experts, 0), counts, 0), offsets, 0), "rows")
+        assert getattr(lib, name)(*_but(ok, ntok, 0)) == 0
+    _refused(lib, "anc_ffn_down", _but(calls["anc_ffn_down"][0], 11, 2), "y_type")
+    _refused(lib, "anc_gated_ffn_dx", _but(calls["anc_gated_ffn_dx"][0], 13, 2), "dx_type")
 
 
 def test_adamw8_entry():
@@ -219,4 +222,4 @@ def test_ffn_arguments(fake_device):
         with pytest.raises(ValueError):
             ffn_down(h, Wd, 0, f, residual=y, plan=p)
     c = fake_device.calls("anc_gated_ffn")
-    assert c[0][3:9] == (0, 0, 0, T, H, I) and c[1][5:9] == (E, plan.capacity, H, I) and c[1][3].value == plan.counts.ptr and c[1][4].value == plan.offsets.ptr
+    assert c[0][3:10] == (0, 0, 0, T, T, H, I) and c[1][5:10] == (E, plan.capacity, 2 * T, H, I) and c[1][3].value == plan.counts.ptr and c[1][4].value == plan.offsets.ptr
