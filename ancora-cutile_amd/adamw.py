@@ -183,7 +183,7 @@ class AdamW:
 
     # -- descriptor table: one row per tensor, rebuilt only when a gradient pointer changes
     def _build_table(self, gbufs):
-        key = tuple((g.ptr, g.dtype.str) for g in gbufs)
+        key = ([g.ptr for g in gbufs], [g.dtype for g in gbufs])
         if key == self._table_key:
             return
         if self._table is not None:

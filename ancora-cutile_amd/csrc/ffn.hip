@@ -40,41 +40,44 @@ typedef float f32x4v __attribute__((ext_vector_type(4)));
 // Where a workgroup's tile lies: the expert, its first row in the buffers and how many of the segment's rows are left from there.
 struct Place { int e, n; int64_t row; int left; };
 
-// Workgroup id -> tile. The tiles of all segments, TM rows each, are counted on the device; ids go round the XCDs in equal runs, a run in
-// blocks of 8 row tiles by all columns, so that what an XCD works on at a time shares its L2.
+// Sums over lanes 0 .. lane of a wavefront.
+__device__ __forceinline__ int sums_up_to(int v) {
+  const int lane = (int)(threadIdx.x & 63);
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int o = __shfl_up(v, off, 64);
+    v += lane >= off ? o : 0;
+  }
+  return v;
+}
+
+// Workgroup id -> tile. The tiles of all segments, TM rows each, are counted on the device, 64 experts at a time (the first 64 stay in registers);
+// ids go round the XCDs in equal runs, a run in blocks of 8 row tiles by all columns, so that what an XCD works on at a time shares its L2.
 __device__ __forceinline__ bool place_of(const Ffn &p, int TM, Place &at) {
   const int lane = (int)(threadIdx.x & 63);
-  int total = 0;
-  int tiles[8], upto[8], count[8], first[8];               // experts lane, lane + 64, ...: their tiles, and those up to and with them
+  // (a segment stays inside its buffers, whatever the arrays hold)
+  auto segment = [&](int e, int &first, int &count) {
+    first = count = 0;
+    if (e >= p.experts) return;
+    const int64_t o = p.offsets[e], f = o < 0 ? 0 : o < p.rows ? o : p.rows, room = p.rows - f;
+    const int n = p.counts[e];
+    first = (int)f;
+    count = n < 0 ? 0 : n < room ? n : (int)room;
+  };
+  int total, first = 0, count = 0, tiles = 0, upto = 0;
   if (p.counts == nullptr) {
     total = (int)((p.rows + TM - 1) / TM);
   } else {
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      count[c] = first[c] = 0;
-      if (c * 64 < p.experts && c * 64 + lane < p.experts) {
-        count[c] = p.counts[c * 64 + lane];
-        first[c] = p.offsets[c * 64 + lane];
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      if (c * 64 >= p.experts) { tiles[c] = 0; upto[c] = total; continue; }
-      const int64_t f = first[c] < 0 ? 0 : first[c] < p.rows ? first[c] : p.rows, room = p.rows - f;      // (a segment stays inside its buffers, whatever the arrays hold)
-      first[c] = (int)f;
-      count[c] = count[c] < 0 ? 0 : count[c] < room ? count[c] : (int)room;
-      tiles[c] = (count[c] + TM - 1) / TM;
-      int v = tiles[c];
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const int o = __shfl_up(v, off, 64);
-        v += lane >= off ? o : 0;
-      }
-      upto[c] = total + v;
-      total += __shfl(v, 63, 64);
+    segment(lane, first, count);
+    tiles = (count + TM - 1) / TM;
+    upto = sums_up_to(tiles);
+    total = __builtin_amdgcn_readlane(upto, 63);
+    for (int c = 64; c < p.experts; c += 64) {
+      int f, n;
+      segment(c + lane, f, n);
+      total += __builtin_amdgcn_readlane(sums_up_to((n + TM - 1) / TM), 63);
     }
   }
-  total = __builtin_amdgcn_readfirstlane(total);
   const int all = total * p.tn, share = (all + kXcds - 1) / kXcds, b = (int)blockIdx.x, q = b / kXcds;
   const int id = b % kXcds * share + q;
   if (q >= share || id >= all) return false;
@@ -87,19 +90,20 @@ __device__ __forceinline__ bool place_of(const Ffn &p, int TM, Place &at) {
     at.left = (int)(p.rows - at.row < 0x7FFFFFFF ? p.rows - at.row : 0x7FFFFFFF);
     return true;
   }
-  at.e = 0; at.row = 0; at.left = 0;
-#pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    const uint64_t hit = __ballot(c * 64 < p.experts && upto[c] > m && upto[c] - tiles[c] <= m);
-    if (hit == 0) continue;
-    const int l = __builtin_ctzll(hit);
-    const int mine = m - __builtin_amdgcn_readlane(upto[c] - tiles[c], l);
-    at.e = c * 64 + l;
-    at.row = (int64_t)__builtin_amdgcn_readlane(first[c], l) + (int64_t)mine * TM;
-    at.left = __builtin_amdgcn_readlane(count[c], l) - mine * TM;
+  int before = 0, c = 0;
+  uint64_t hit;
+  while ((hit = __ballot(upto > m - before && upto - tiles <= m - before)) == 0) {
+    before += __builtin_amdgcn_readlane(upto, 63);
+    c += 64;
+    if (c >= p.experts) return false;
+    segment(c + lane, first, count);
+    tiles = (count + TM - 1) / TM;
+    upto = sums_up_to(tiles);
   }
-  at.e = __builtin_amdgcn_readfirstlane(at.e);
-  at.left = __builtin_amdgcn_readfirstlane(at.left);
+  const int l = __builtin_ctzll(hit), mine = m - before - __builtin_amdgcn_readlane(upto - tiles, l);
+  at.e = c + l;
+  at.row = (int64_t)__builtin_amdgcn_readlane(first, l) + (int64_t)mine * TM;
+  at.left = __builtin_amdgcn_readlane(count, l) - mine * TM;
   return at.left > 0;
 }
 
@@ -433,6 +437,7 @@ template <int MODE, int R, int C> __global__ void __launch_bounds__(512, 2) k_ff
     for (int j = 0; j < C; ++j) acc[i][j] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
   const int s16 = lane & 15, g16 = lane >> 4;
   const int ta = s16 * 64 + ((g16 ^ ((s16 >> 2) & 3)) * 16);
+#pragma unroll 1
   for (int i = 0; i < kStages; ++i) fetch(wave + i * kWaves, mine + i * kStage);
   int here = 0;
   for (int t = wave; t < all; t += kWaves) {

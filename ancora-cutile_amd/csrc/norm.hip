@@ -333,6 +333,7 @@ extern "C" int anc_rms_norm(uint64_t x, int x_type, uint64_t residual, int strea
               "anc_rms_norm: bad types (x %d, stream %d, gain %d, y %d)", x_type, stream_type, gain_type, y_type);
   ANC_REQUIRE(width_ok(H), "anc_rms_norm: rows of %lld: a multiple of 8 up to %d", (long long)H, kWidest);
   ANC_REQUIRE(T >= 0 && T < (1ll << 31), "anc_rms_norm: %lld rows", (long long)T);
+  ANC_REQUIRE(T * lanes_of(H) <= (1ll << 32) - kThreads, "anc_rms_norm: %lld rows of %lld: too large for one call", (long long)T, (long long)H);
   if (T == 0) return ANC_OK;
   const bool mx8 = y_type == ANC_MXFP8;
   ANC_REQUIRE(x && gain && y && (scale != 0) == mx8 && (residual != 0) == (total != 0),
@@ -376,7 +377,9 @@ extern "C" int64_t anc_rms_norm_grad_workspace_bytes(int64_t T, int64_t H) {
     anc_set_error("anc_rms_norm_grad_workspace_bytes: %lld rows of %lld", (long long)T, (long long)H);
     return -1;
   }
-  return parts_of(T, H) * H * 4;
+  // (fewer rows than T may want more partial rows than T does, never more than at two rows each)
+  const int64_t per = 2 * (kGradThreads / lanes_of(H)), n = (T + per - 1) / per;
+  return (n < 1 ? 1 : n > kMostRows ? kMostRows : n) * H * 4;
 }
 
 extern "C" int anc_rms_norm_grad(uint64_t dy, int dy_type, uint64_t x, int stream_type, uint64_t gain, int gain_type, uint64_t rstd,

@@ -556,13 +556,14 @@ int anc_gated_ffn_dx(uint64_t dgate, uint64_t dup, uint64_t Wg, uint64_t Wu, uin
  * per output. x ANC_F32 or ANC_BF16; residual and total (s, written where residual is given) of stream_type; gain of gain_type; rstd
  * fp32[T] or 0. y of y_type, or ANC_MXFP8: E4M3 codes (T, H) with scale (T, H/32), one E8M0 byte per 32 elements of a row by
  * the rule of anc_quant_mxfp8_w (elements that are not finite become NaN codes).
- * H a multiple of 8 (MXFP8: 32) up to 16384; rows contiguous, 16-byte aligned. y or total may be x or residual itself (same address, same
+ * H a multiple of 8 (MXFP8: 32) up to 16384, T below 2^28 (2^26 beyond H = 256, 2^24 beyond 2048); rows contiguous, 16-byte aligned. Squares are fp32's:
+ * rows that hold values beyond 2^63 come out as zeros. y or total may be x or residual itself (same address, same
  * type); no other overlap. T = 0 does nothing. */
 int anc_rms_norm(uint64_t x, int x_type, uint64_t residual, int stream_type, uint64_t gain, int gain_type, int64_t T, int64_t H,
                  float eps, uint64_t y, int y_type, uint64_t scale, uint64_t total, uint64_t rstd, uint64_t stream);
 /* Its backward pass: x is what was normed (total, or x) of stream_type, a = dy gain, dx = r (a - x r^2 mean(a x)) + carry in stream_type (carry
  * 0: none: the gradient that comes along the residual stream), dgain fp32[H] = (or +=, `accumulate`) the sum over rows of dy x r,
- * rows added in fp32 in a fixed order that hangs on T and H alone. dx may be dy, x or carry itself where the types agree. */
+ * rows added in fp32 in a fixed order that hangs on T and H alone. A workspace for T rows serves fewer too. dx may be dy, x or carry itself where the types agree. */
 int64_t anc_rms_norm_grad_workspace_bytes(int64_t T, int64_t H);
 int anc_rms_norm_grad(uint64_t dy, int dy_type, uint64_t x, int stream_type, uint64_t gain, int gain_type, uint64_t rstd,
                       uint64_t carry, int64_t T, int64_t H, uint64_t dx, uint64_t dgain, int accumulate, uint64_t workspace,

@@ -175,6 +175,50 @@ def test_the_largest_tiles(gpu, H, I):
     c.free()
 
 
+@pytest.mark.parametrize("H,I,rows", [(520, 2816, 700), (520, 4104, 70), (4104, 264, 70), (72, 520, 4100), (520, 72, 4100), (2056, 520, 2050), (520, 2056, 2050), (2200, 2040, 8100),
+                                      (2040, 2200, 8100)])
+def test_every_size_of_tile(gpu, H, I, rows):
+    """Sizes at which each kernel that a call can take is the cheapest for one of the four calls (the last two: whole rounds of the largest tiles, with ragged
+    edges): some rows, the first and the last among them, against 64 bits."""
+    from ancora_cutile_amd import DevBuf, ffn_down, gated_ffn, gated_ffn_dx, gated_ffn_grad
+    rng = np.random.default_rng(H + I + rows)
+    pick = np.unique(np.concatenate([[0, 31, 32, 127, 128, 255, 256, rows - 1], rng.integers(0, rows, 60)]) % rows)
+    host, dev = {}, {}
+    for n, shape, std in (("Wg", (H, I), H ** -0.5), ("Wu", (H, I), H ** -0.5), ("Wd", (I, H), I ** -0.5), ("x", (rows, H), 1.0), ("h", (rows, I), 1.0),
+                          ("gate", (rows, I), 1.0), ("up", (rows, I), 1.0), ("dy", (rows, H), 1.0)):
+        b = bf16_rne_bits((std * rng.standard_normal(shape, dtype=F32))).reshape(shape)
+        dev[n], host[n] = DevBuf(b), _wide(b if n[0] == "W" else b[pick])
+    out = {n: DevBuf(np.full((rows, w), np.nan, t) if t == F32 else np.full((rows, w), 0x7FC1, t)) for n, w, t in
+           (("h", I, U16), ("y", H, F32), ("dgate", I, U16), ("dup", I, U16), ("dx", H, U16))}
+
+    def product(a, w):
+        return a @ w, (a.shape[1] + 8) * UNIT * (np.abs(a) @ np.abs(w))
+
+    def near(name, want, err):
+        got = _val(out[name])
+        assert np.isfinite(got).all(), name
+        assert np.all(np.abs(got[pick] - want) <= err + _half(out[name]) * (np.abs(want) + err) + 1e-30), name
+    gated_ffn(dev["x"], dev["Wg"], dev["Wu"], 0, out["h"])
+    (g, ge), (u, ue) = product(host["x"], host["Wg"]), product(host["x"], host["Wu"])
+    a = np.abs(g) * ref.sigmoid(g)
+    near("h", ref.gated(g, u), 1.1 * ge * (np.abs(u) + ue) + a * ue + a * np.abs(u) * (np.abs(g) + 10) * UNIT)
+    ffn_down(dev["h"], dev["Wd"], 0, out["y"])
+    near("y", *product(host["h"], host["Wd"]))
+    gated_ffn_grad(dev["dy"], dev["gate"], dev["up"], dev["Wd"], 0, out["dgate"], out["dup"])
+    dh, de = product(host["dy"], host["Wd"].T)
+    g, u = host["gate"], host["up"]
+    s = ref.sigmoid(g)
+    wg, wu, _ = ref.gated_grad(dh, g, u)
+    es, slope = (np.abs(g) + 10) * UNIT, s * (1 + np.abs(g))
+    near("dgate", wg, (1.1 * de + 2 * np.abs(dh) * es) * np.abs(u) * slope)
+    near("dup", wu, (1.1 * de + np.abs(dh) * es) * np.abs(g) * s)
+    gated_ffn_dx(dev["gate"], dev["up"], dev["Wg"], dev["Wu"], 0, out["dx"])
+    (v1, e1), (v2, e2) = product(g, host["Wg"].T), product(u, host["Wu"].T)
+    near("dx", v1 + v2, 2 * (e1 + e2))
+    for b in (*dev.values(), *out.values()):
+        b.free()
+
+
 @pytest.mark.parametrize("E", [65, 130, 512])
 def test_many_experts(gpu, E):
     rng = np.random.default_rng(E)

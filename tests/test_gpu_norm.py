@@ -135,6 +135,21 @@ def test_backward(gpu, H, dy, stream, gain, carry):
             b.free()
 
 
+@pytest.mark.parametrize("H", [64, 1024, 4096])
+def test_one_workspace_for_batches_of_any_length(gpu, H):
+    """Around the lengths where the number of partial sums changes, all with the workspace of the longest: a row of ones times ones counts the rows."""
+    from ancora_cutile_amd import DevBuf, NormWorkspace, rms_norm_grad
+    most = 8200 if H <= 1024 else 2060
+    one = np.full((most, H), 0x3F80, U16)
+    bufs = dy, x, g, r, dx, dg = DevBuf(one), DevBuf(one), DevBuf(np.ones(H, F32)), DevBuf(np.ones(most, F32)), DevBuf(one), DevBuf(np.zeros(H, F32))
+    ws = NormWorkspace(most, H)
+    for T in (most, most - 7, most - 8, most - 9, most // 2 + 1, most // 2, 1025, 1024, 1023, 17, 1):
+        rms_norm_grad(dy.view((T, H)), x, g, r, 0, dx, dg, ws)
+        assert (dg.to_numpy() == T).all(), T
+    for b in (*bufs, ws):
+        b.free()
+
+
 def test_gradient_against_differences(gpu):
     """loss = sum(y w) in fp32. The device's central difference is within its own rounding (the bound of y, twice, over the step) of the formula's difference
     in 64 bits, and that is the gradient to the third order of the step, which is computed from two steps."""

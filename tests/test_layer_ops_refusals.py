@@ -39,6 +39,15 @@ def test_norm_entry():
     for at, other in ((9, a[0]), (11, a[0] + 2 * n - 4), (11, a[3] + n - 4)):           # 8-bit rows on top of the input
         _refused(lib, "anc_rms_norm", _but(mx, at, other), "overlap")
     assert lib.anc_rms_norm(*_but(ok, 6, 0)) == 0                                       # no rows: nothing to do
+    for rows, width in ((1 << 28, 8), (1 << 26, 264), (1 << 24, 2056)):                  # more lanes than one launch has
+        _refused(lib, "anc_rms_norm", _but(_but(ok, 6, rows), 7, width), "too large")
+
+
+def test_a_workspace_for_many_rows_serves_fewer():
+    lib = _lib()
+    for H in (64, 512, 4096):
+        sizes = [lib.anc_rms_norm_grad_workspace_bytes(T, H) for T in (0, 1, 7, 100, 1000, 4095, 4096, 4097, 8191, 8192, 8193, 8194, 65536, 65537, 1 << 20)]
+        assert sizes == sorted(sizes) and sizes[0] == 4 * H
 
 
 def test_norm_gradient_entry():
