@@ -9,8 +9,8 @@
 // columns, whose fragments come from transposing LDS reads, backwards along their rows, so no transposed copy exists. Products of bf16
 // accumulate in fp32 over ascending k (dx: all of dg, then all of du); each output is rounded once.
 //
-// k_ffn_tiles: a workgroup owns TM x 256 values of the product (gated: 128 columns of either weight, so that a lane holds g and u of the
-// same element) and runs k in steps of 32 through three LDS stages; wavefronts of 128 x 64. Operands go straight to LDS through descriptors
+// k_ffn_tiles: a workgroup owns TM x TN values of the product (gated: half of the columns of either weight, so that a lane holds g and u of
+// the same element) and runs k in steps of 32 through three LDS stages; wavefronts of 128 x 64, 64 x 128 or 64 x 64. Operands go straight to LDS through descriptors
 // that end with the segment or the matrix: rows and columns beyond read zeros and are not stored.
 // k_ffn_few: up to 32 rows of a segment by 16 to 64 columns, the eight wavefronts of a workgroup taking every eighth step of k, each
 // with stages of its own and no barrier, and adding up at the end in a fixed order: with few rows the weights' bytes are the work, and
@@ -198,16 +198,16 @@ template <int MODE, bool ONCE> __device__ __forceinline__ void finish(const Ffn 
 }
 
 // ---------------------------------------------------------------- many rows
-// TM x TN values to a workgroup, WM x 64 to a wavefront, `waves` wavefronts to a SIMD.
-template <int MODE, int TM, int TN, int WM, int WAVES> __global__ void __launch_bounds__(TM / WM * TN, WAVES) k_ffn_tiles(Ffn p) {
+// TM x TN values to a workgroup, WM x WN to a wavefront, WAVES wavefronts to a SIMD.
+template <int MODE, int TM, int TN, int WM, int WN, int WAVES> __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, WAVES) k_ffn_tiles(Ffn p) {
   constexpr bool kForward = MODE == kGated || MODE == kDown;
-  constexpr int kWide = TN / 64, kWaves = TM / WM * kWide, kHigh = WM / 32;       // wavefronts side by side, in all; fragments of A
+  constexpr int kWide = TN / WN, kWaves = TM / WM * kWide, kHigh = WM / 32, kAcross = WN / 32;       // wavefronts side by side, in all; fragments of A, of B
   constexpr int kBytesA = TM * 64, kBytesB = TN * 64, kStage = kBytesA + kBytesB, kStages = 3;
   constexpr int kPiecesA = kBytesA / 1024 / kWaves, kPiecesB = kBytesB / 1024 / kWaves, kPieces = kPiecesA + kPiecesB;
   constexpr int kCols = MODE == kGated ? TN / 2 : TN;       // columns of the outputs
   // Forwards the B tile is [32 k][kSub columns] once or twice: of either weight, or side by side.
   constexpr int kSub = MODE == kGated ? TN / 2 : 128, kRowB = kSub * 2, kRows = 1024 / kRowB;
-  static_assert(kWaves * 8192 <= kStages * kStage && kPieces <= 2 * kHigh && kPiecesA * kWaves * 1024 == kBytesA && kPiecesB * kWaves * 1024 == kBytesB,
+  static_assert((MODE == kGated || WN == 64) && kWaves * 8192 <= kStages * kStage && kPieces <= kHigh * kAcross && kHigh + kAcross <= kHigh * kAcross + 1 && kPiecesA * kWaves * 1024 == kBytesA && kPiecesB * kWaves * 1024 == kBytesB,
                 "room for the way out; pieces to a half step; whole pieces");
   __shared__ __attribute__((aligned(1024))) unsigned char ring[kStages * kStage];
   Place at;
@@ -262,37 +262,41 @@ template <int MODE, int TM, int TN, int WM, int WAVES> __global__ void __launch_
     mask = k == steps - 1 ? beyond : 0u;
   };
 
-  int ta, tb[2];
+  // Columns of fragment j: gated, the first half are of Wg, the others the same ones of Wu, so that a lane holds g and u of one element.
+  int ta, tb[kAcross];
   ta = (wm * WM + (lane & 31)) * 64;
   if constexpr (kForward) {
     const int s16 = lane & 15, g16 = lane >> 4, row = 8 * (g16 >> 1) + (s16 >> 2), key = kSub == 128 ? (row & 3) << 2 : (row >> 1 & 1) << 2;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int sub = MODE == kGated ? j : wn * 64 / kSub, col = MODE == kGated ? wn * 4 : wn * 64 % kSub / 8 + j * 4;     // (in chunks)
+    for (int j = 0; j < kAcross; ++j) {
+      const int sub = MODE == kGated ? j / (kAcross / 2) : wn * WN / kSub;
+      const int col = MODE == kGated ? wn * (WN / 16) + j % (kAcross / 2) * 4 : wn * WN % kSub / 8 + j * 4;     // (in chunks)
       tb[j] = kBytesA + sub * (32 * kRowB) + row * kRowB + (((col + 2 * (g16 & 1) + ((s16 & 3) >> 1)) ^ key) * 16) + (s16 & 1) * 8;
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) tb[j] = kBytesA + (wn * 64 + j * 32 + (lane & 31)) * 64;
+    for (int j = 0; j < kAcross; ++j) tb[j] = kBytesA + (wn * WN + j * 32 + (lane & 31)) * 64;
   }
-  f32x16 acc[kHigh][2];
+  f32x16 acc[kHigh][kAcross];
 #pragma unroll
   for (int i = 0; i < kHigh; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < kAcross; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
-  bf16x8 a[2][kHigh], c[2][2];
-  // fragment i (b0 b1 a0 a1 ..) of k 16 kk .. 16 kk + 15 of a stage
+  constexpr int kLoads = kHigh + kAcross, kProducts = kHigh * kAcross;
+  bf16x8 a[2][kHigh], c[2][kAcross];
+  // fragment i (b0 b1 .. a0 a1 ..) of k 16 kk .. 16 kk + 15 of a stage
   auto load = [&](int set, int i, const unsigned char *stage, int kk) {
     const int sw = ((kk * 2 + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16;
-    if (i >= 2) a[set][i - 2] = *(const bf16x8 *)(stage + ta + (i - 2) * (32 * 64) + sw);
+    if (i >= kAcross) a[set][i - kAcross] = *(const bf16x8 *)(stage + ta + (i - kAcross) * (32 * 64) + sw);
     else if constexpr (kForward) c[set][i] = anc_lds_tr_frag(stage + tb[i] + kk * (16 * kRowB), stage + tb[i] + kk * (16 * kRowB) + 4 * kRowB);
     else c[set][i] = *(const bf16x8 *)(stage + tb[i] + sw);
   };
   auto multiply = [&](int set, int idx) {        // operands exchanged: a lane holds runs of 4 columns of one row
-    acc[idx >> 1][idx & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c[set][idx & 1], a[set][idx >> 1], acc[idx >> 1][idx & 1], 0, 0, 0);
+    f32x16 &to = acc[idx / kAcross][idx % kAcross];
+    to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(c[set][idx % kAcross], a[set][idx / kAcross], to, 0, 0, 0);
   };
   for (int i = 0; i < kStages; ++i) {
     const anc_i32x4 da = fa.desc(), db = fb.desc();
@@ -303,25 +307,25 @@ template <int MODE, int TM, int TN, int WM, int WAVES> __global__ void __launch_
   wait_vm<(kStages - 1) * kPieces>();
   lds_barrier();
 #pragma unroll
-  for (int i = 0; i < kHigh + 2; ++i) load(0, i, ring, 0);
+  for (int i = 0; i < kLoads; ++i) load(0, i, ring, 0);
   // One step: the first half's products over the reads of the second half; then every wavefront has read the stage and the next
   // one has landed for all; then the second half's products over the next stage's first reads and the fetches into the place just read.
   auto step = [&](unsigned char *here, unsigned char *next) {
 #pragma unroll
-    for (int i = 0; i < 2 * kHigh; ++i) {
+    for (int i = 0; i < kProducts; ++i) {
       multiply(0, i);
       __builtin_amdgcn_sched_barrier(0);
-      if (i < kHigh + 2) load(1, i, here, 1);
+      if (i < kLoads) load(1, i, here, 1);
       __builtin_amdgcn_sched_barrier(0);
     }
     wait_vm<(kStages - 2) * kPieces>();
     lds_barrier();
     const anc_i32x4 da = fa.desc(), db = fb.desc();
 #pragma unroll
-    for (int i = 0; i < 2 * kHigh; ++i) {
+    for (int i = 0; i < kProducts; ++i) {
       multiply(1, i);
       __builtin_amdgcn_sched_barrier(0);
-      if (i < kHigh + 2) load(0, i, next, 0);
+      if (i < kLoads) load(0, i, next, 0);
       if (i < kPieces) issue(i, da, db, here);
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -336,55 +340,76 @@ template <int MODE, int TM, int TN, int WM, int WAVES> __global__ void __launch_
   wait_vm<0>();                                  // (zeros still on their way into the stages)
   lds_barrier();
 
-  // Out through LDS, 32 rows of 64 values at a time: a lane then holds 8 neighbouring columns of a row. What the outputs take besides the
-  // product is fetched one such block ahead; results leave past the caches, which keep the operands of the tiles still to come.
   unsigned char *r = ring + wave * 8192;
-  constexpr int kOcts = MODE == kGated ? 4 : 8, kRounds = kOcts / 2;
-  const int col0 = n0 + wn * (MODE == kGated ? 32 : 64);
-  constexpr bool kAhead = WAVES < 4;                        // (128 registers hold one block's only)
-  Side side[kAhead ? 2 : 1][kRounds];
-  auto where = [&](int i, int z, int64_t &e) {
-    const int idx = z * 64 + lane, in = wm * WM + i * 32 + idx / kOcts, col = col0 + idx % kOcts * 8;
-    e = (at.row + in) * N + col;
-    return in < rows && col < N;
-  };
-  auto fetch = [&](int i) {
-    if constexpr (MODE != kGated) {
+  const int rr = lane & 31, hh = lane >> 5;
+  if constexpr (MODE == kGated) {
+    // A lane holds g and u of the same elements: h, g and u leave it as bf16, 32 rows at a time through LDS, so that a wavefront of 64 columns stores
+    // whole lines of 128 bytes, past the caches, which keep the operands of the tiles still to come. (Half lines past the caches: 3.6 TB/s, whole ones
+    // 5.4; through them 5.7 both. 32 columns to a wavefront go through them.)
+    constexpr int kReal = WN / 2, kChunks = kReal / 8, kLine = kReal * 2;
+    auto out = [&](int i, uint16_t *to, auto value) {
 #pragma unroll
-      for (int z = 0; z < kRounds; ++z) {
-        int64_t e;
-        if (where(i, z, e)) side[kAhead ? i & 1 : 0][z] = side_of<MODE>(p, e);
+      for (int j = 0; j < kAcross / 2; ++j)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          float v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = value(acc[i][j][4 * g + k], acc[i][j + kAcross / 2][4 * g + k]);
+          *(anc_u32x2 *)(r + rr * kLine + (((j * 4 + g) ^ (rr & (kChunks - 1))) * 16) + hh * 8) = anc_u32x2{anc_pk_bf16(v[0], v[1]), anc_pk_bf16(v[2], v[3])};
+        }
+      lds_wave_sync();
+#pragma unroll
+      for (int z = 0; z < kChunks / 2; ++z) {
+        const int idx = z * 64 + lane, row = idx / kChunks, ch = idx % kChunks, in = wm * WM + i * 32 + row, col = n0 + wn * kReal + ch * 8;
+        const anc_u32x4 v = *(const anc_u32x4 *)(r + row * kLine + ((ch ^ (row & (kChunks - 1))) * 16));
+        if (in < rows && col < N) put<kLine == 128>((anc_u32x4 *)(to + (at.row + in) * N + col), v);
       }
+      lds_wave_sync();
+    };
+#pragma unroll
+    for (int i = 0; i < kHigh; ++i) {
+      out(i, (uint16_t *)p.y, [](float g, float u) { return g * sigmoid(g) * u; });
+      if (p.dgate != nullptr) out(i, p.dgate, [](float g, float) { return g; });
+      if (p.dup != nullptr) out(i, p.dup, [](float, float u) { return u; });
     }
-  };
-  if (kAhead) fetch(0);
+  } else {
+    // Out through LDS, 32 rows of 64 values at a time: a lane then holds 8 neighbouring columns of a row. What the outputs take besides the
+    // product is fetched one such block ahead; results leave past the caches.
+    const int col0 = n0 + wn * 64;
+    Side side[2][4];
+    auto where = [&](int i, int z, int64_t &e) {
+      const int idx = z * 64 + lane, in = wm * WM + i * 32 + idx / 8, col = col0 + idx % 8 * 8;
+      e = (at.row + in) * N + col;
+      return in < rows && col < N;
+    };
+    auto fetch = [&](int i) {
 #pragma unroll
-  for (int i = 0; i < kHigh; ++i) {
-    if (!kAhead) fetch(i);
-    const int rr = lane & 31, hh = lane >> 5;
+      for (int z = 0; z < 4; ++z) {
+        int64_t e;
+        if (where(i, z, e)) side[i & 1][z] = side_of<MODE>(p, e);
+      }
+    };
+    fetch(0);
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int i = 0; i < kHigh; ++i) {
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *(anc_f32x4 *)(r + rr * 256 + (((j * 8 + 2 * g + hh) ^ (rr & 15)) * 16)) =
-            anc_f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-    lds_wave_sync();
-    if (kAhead && i + 1 < kHigh) fetch(i + 1);
+      for (int j = 0; j < kAcross; ++j)
 #pragma unroll
-    for (int z = 0; z < kRounds; ++z) {
-      const int idx = z * 64 + lane, row = idx / kOcts, oct = idx % kOcts;
-      auto values = [&](int ch, float (&f)[8]) {
+        for (int g = 0; g < 4; ++g)
+          *(anc_f32x4 *)(r + rr * 256 + (((j * 8 + 2 * g + hh) ^ (rr & 15)) * 16)) =
+              anc_f32x4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+      lds_wave_sync();
+      if (i + 1 < kHigh) fetch(i + 1);
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        const int idx = z * 64 + lane, row = idx / 8, ch = idx % 8 * 2;
         const anc_f32x4 lo = *(const anc_f32x4 *)(r + row * 256 + ((ch ^ (row & 15)) * 16)), hi = *(const anc_f32x4 *)(r + row * 256 + (((ch + 1) ^ (row & 15)) * 16));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) { f[k] = lo[k]; f[4 + k] = hi[k]; }
-      };
-      float v[8], w[8];
-      values(2 * oct, v);
-      if constexpr (MODE == kGated) values(8 + 2 * oct, w);
-      int64_t e;
-      if (where(i, z, e)) finish<MODE, true>(p, e, v, w, side[kAhead ? i & 1 : 0][z]);
+        float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        int64_t e;
+        if (where(i, z, e)) finish<MODE, true>(p, e, v, v, side[i & 1][z]);
+      }
+      lds_wave_sync();
     }
-    lds_wave_sync();
   }
 }
 
@@ -542,18 +567,19 @@ template <int MODE> int launch(Ffn p, int64_t most, const char *who, hipStream_t
     hipLaunchKernelGGL((k_ffn_few<MODE, r, c>), dim3((unsigned)grid_of(16 * r)), dim3(512), 0, s, p);
     return ANC_OK;
   };
-  auto tiles = [&](auto TM, auto TN, auto WM, auto W) {
-    constexpr int tm = decltype(TM)::value, tn = decltype(TN)::value, wm = decltype(WM)::value, w = decltype(W)::value;
+  auto tiles = [&](auto TM, auto TN, auto WM, auto WN, auto W) {
+    constexpr int tm = decltype(TM)::value, tn = decltype(TN)::value, wm = decltype(WM)::value, wn = decltype(WN)::value, w = decltype(W)::value;
     p.tn = (int)columns(tn);
     ANC_REQUIRE(grid_of(tm) < (1ll << 31) / 512, "%s: too large for one call", who);
-    hipLaunchKernelGGL((k_ffn_tiles<MODE, tm, tn, wm, w>), dim3((unsigned)grid_of(tm)), dim3(tm / wm * tn), 0, s, p);
+    hipLaunchKernelGGL((k_ffn_tiles<MODE, tm, tn, wm, wn, w>), dim3((unsigned)grid_of(tm)), dim3(tm / wm * (tn / wn) * 64), 0, s, p);
     return ANC_OK;
   };
+  constexpr int kTall = MODE == kGated ? 64 : 128;            // a wavefront's rows; gated: 64 columns of either weight
   int rc = ANC_OK;
   switch (best) {
-    case 0: rc = tiles(IC<256>{}, IC<256>{}, IC<128>{}, IC<2>{}); break;
-    case 1: rc = tiles(IC<128>{}, IC<256>{}, IC<128>{}, IC<2>{}); break;
-    case 2: rc = tiles(IC<128>{}, IC<128>{}, IC<64>{}, IC<3>{}); break;
+    case 0: rc = tiles(IC<256>{}, IC<256>{}, IC<kTall>{}, IC<8192 / kTall>{}, IC<2>{}); break;
+    case 1: rc = tiles(IC<128>{}, IC<256>{}, IC<kTall>{}, IC<8192 / kTall>{}, IC<2>{}); break;
+    case 2: rc = tiles(IC<128>{}, IC<128>{}, IC<64>{}, IC<64>{}, IC<3>{}); break;
     case 3: rc = few(IC<4>{}, IC<4>{}); break;
     case 4: rc = few(IC<2>{}, IC<4>{}); break;
     case 5: rc = few(IC<2>{}, IC<2>{}); break;
