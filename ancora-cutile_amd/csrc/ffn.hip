@@ -10,9 +10,13 @@
 // accumulate in fp32 over ascending k (dx: all of dg, then all of du); each output is rounded once.
 //
 // k_ffn_tiles: a workgroup owns TM x TN values of the product (gated: half of the columns of either weight, so that a lane holds g and u of
-// the same element) and runs k in steps of 32 through three LDS stages; wavefronts of 128 x 64, 64 x 128 or 64 x 64. Operands go straight to LDS through descriptors
-// that end with the segment or the matrix: rows and columns beyond read zeros and are not stored.
-// k_ffn_few: up to 32 rows of a segment by 16 to 64 columns, the eight wavefronts of a workgroup taking every eighth step of k, each
+// the same element) and runs k through LDS in two stages of 64 or three of 32; wavefronts of 128 x 64, 64 x 128 or 64 x 64. Operands go straight
+// to LDS through descriptors that end with the segment or the matrix: rows and columns beyond read zeros and are not stored. What bounds
+// its loop is the operands' way into LDS: a CU has some 64 lines under way at a time, so a line of 128 bytes asked for in halves, a step of 32 k
+// apart, counts twice. Steps of 64 ask for whole lines of what lies along k (8192 rows, dx, 1024 x 2816, 128x128 tiles: 129 us in steps of 32,
+// 100 in steps of 64; 2048 x 2048, 256x256: 130 and 120, 1.15 PFLOP/s; gated, 256x256: 131 and 116 to 125); 128x256 keeps steps of 32, of which two
+// workgroups fit a CU and hide each other's ends. What is left then is the outputs' bytes, which overlap little with the loops.
+// k_ffn_few: 16 to 64 rows of a segment by 16 to 64 columns, the eight wavefronts of a workgroup taking every eighth step of k, each
 // with stages of its own and no barrier, and adding up at the end in a fixed order: with few rows the weights' bytes are the work, and
 // this way they are spread over as many CUs as there are.
 #include "lds_dma.h"
@@ -199,52 +203,54 @@ template <int MODE, bool ONCE> __device__ __forceinline__ void finish(const Ffn 
 
 // ---------------------------------------------------------------- many rows
 // TM x TN values to a workgroup, WM x WN to a wavefront, WAVES wavefronts to a SIMD.
-template <int MODE, int TM, int TN, int WM, int WN, int WAVES> __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, WAVES) k_ffn_tiles(Ffn p) {
+template <int MODE, int TM, int TN, int WM, int WN, int STEP, int STAGES, int WAVES>
+__global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, WAVES) k_ffn_tiles(Ffn p) {
   constexpr bool kForward = MODE == kGated || MODE == kDown;
   constexpr int kWide = TN / WN, kWaves = TM / WM * kWide, kHigh = WM / 32, kAcross = WN / 32;       // wavefronts side by side, in all; fragments of A, of B
-  constexpr int kBytesA = TM * 64, kBytesB = TN * 64, kStage = kBytesA + kBytesB, kStages = 3;
+  constexpr int kRowA = STEP * 2, kBytesA = TM * kRowA, kBytesB = TN * kRowA, kStage = kBytesA + kBytesB, kStages = STAGES, kSlices = STEP / 16;
   constexpr int kPiecesA = kBytesA / 1024 / kWaves, kPiecesB = kBytesB / 1024 / kWaves, kPieces = kPiecesA + kPiecesB;
   constexpr int kCols = MODE == kGated ? TN / 2 : TN;       // columns of the outputs
-  // Forwards the B tile is [32 k][kSub columns] once or twice: of either weight, or side by side.
-  constexpr int kSub = MODE == kGated ? TN / 2 : 128, kRowB = kSub * 2, kRows = 1024 / kRowB;
-  static_assert((MODE == kGated || WN == 64) && kWaves * 8192 <= kStages * kStage && kPieces <= kHigh * kAcross && kHigh + kAcross <= kHigh * kAcross + 1 && kPiecesA * kWaves * 1024 == kBytesA && kPiecesB * kWaves * 1024 == kBytesB,
+  // Forwards the B tile is [STEP][kSub columns] once or twice: of either weight, or side by side.
+  constexpr int kSub = MODE == kGated ? TN / 2 : 128, kRowB = kSub * 2, kRows = 1024 / kRowB, kSubPieces = STEP / kRows;
+  static_assert((MODE == kGated || WN == 64) && kWaves * 8192 <= kStages * kStage && kPieces <= 2 * kHigh * kAcross && kHigh + kAcross <= kHigh * kAcross + 1 && kPiecesA * kWaves * 1024 == kBytesA && kPiecesB * kWaves * 1024 == kBytesB,
                 "room for the way out; pieces to a half step; whole pieces");
   __shared__ __attribute__((aligned(1024))) unsigned char ring[kStages * kStage];
   Place at;
   if (!place_of(p, TM, at)) return;
   const int K = p.K, N = p.N, lane = (int)(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int wm = wave / kWide, wn = wave % kWide, n0 = at.n * kCols;
-  const int rows = at.left < TM ? at.left : TM, steps = (K + TK - 1) / TK, all = MODE == kDx ? 2 * steps : steps;
+  const int rows = at.left < TM ? at.left : TM, steps = (K + STEP - 1) / STEP, all = MODE == kDx ? 2 * steps : steps;
 
-  const int half = wave * kPiecesB / (kSub / 16);           // the part of the B tile that this wavefront fetches
+  const int half = wave * kPiecesB / kSubPieces;           // the part of the B tile that this wavefront fetches
   Feed fa, fb;
   auto term = [&](int t) {
-    fa = Feed{(const char *)(p.A[t] + at.row * K), (int64_t)rows * K * 2, TK * 2};
+    fa = Feed{(const char *)(p.A[t] + at.row * K), (int64_t)rows * K * 2, kRowA};
     if constexpr (kForward) {
       const int col = MODE == kGated ? n0 : n0 + half * kSub;
-      fb = Feed{(const char *)(p.B[MODE == kGated ? half : 0] + (int64_t)at.e * K * N + col), ((int64_t)K * N - col) * 2, (int64_t)TK * N * 2};
+      fb = Feed{(const char *)(p.B[MODE == kGated ? half : 0] + (int64_t)at.e * K * N + col), ((int64_t)K * N - col) * 2, (int64_t)STEP * N * 2};
     } else {
       const int high = N - n0 < TN ? N - n0 : TN;
-      fb = Feed{(const char *)(p.B[t] + ((int64_t)at.e * N + n0) * K), (int64_t)high * K * 2, TK * 2};
+      fb = Feed{(const char *)(p.B[t] + ((int64_t)at.e * N + n0) * K), (int64_t)high * K * 2, kRowA};
     }
   };
   term(0);
-  // Offsets of the pieces, 1 KiB of LDS each. Rows of 64 bytes: 16 to a piece, their four 16-byte chunks XORed with (row >> 2) & 3; rows of
-  // 256 bytes: 4 to a piece, chunks XORed with 4 * (row & 3); of 128: 8, with 4 * ((row >> 1) & 1): the rows that a read touches fall into
-  // different banks. Of a row's last 32 k the chunks beyond K are sent nowhere, which reads zeros.
-  const int chunk = (lane & 3) ^ (lane >> 4);
-  const uint32_t beyond = chunk * 8 >= K - (steps - 1) * TK ? kNowhere : 0u;
+  // Offsets of the pieces, 1 KiB of LDS each. Rows of 64 bytes: 16 to a piece, their four 16-byte chunks XORed with (row >> 2) & 3; of 128
+  // 8, with row & 7. Forwards, B's rows of 256 bytes: 4 to a piece, with 4 * (row & 3); of 128: 8, with 4 * ((row >> 1) & 1). So the rows that a
+  // read touches fall into different banks. Of a row's last step the chunks beyond K are sent nowhere, which reads zeros.
+  constexpr int kLanes = kRowA / 16;                        // of a row
+  const int chunk = STEP == 32 ? (lane & 3) ^ (lane >> 4) : (lane & 7) ^ (lane >> 3);
+  const uint32_t beyond = chunk * 8 >= K - (steps - 1) * STEP ? kNowhere : 0u;
   uint32_t va[kPiecesA], vb[kPiecesB];
 #pragma unroll
-  for (int i = 0; i < kPiecesA; ++i) va[i] = (uint32_t)(((wave * kPiecesA + i) * 16 + (lane >> 2)) * K * 2 + chunk * 16);
+  for (int i = 0; i < kPiecesA; ++i) va[i] = (uint32_t)(((wave * kPiecesA + i) * (64 / kLanes) + lane / kLanes) * K * 2 + chunk * 16);
 #pragma unroll
   for (int i = 0; i < kPiecesB; ++i) {
     const int piece = wave * kPiecesB + i;
     if constexpr (kForward) {
       const int row = lane / (kRowB / 16), key = kSub == 128 ? (row & 3) << 2 : (row >> 1 & 1) << 2;
-      vb[i] = (uint32_t)((piece % (kSub / 16) * kRows + row) * N * 2 + ((lane % (kRowB / 16)) ^ key) * 16);
+      vb[i] = (uint32_t)((piece % kSubPieces * kRows + row) * N * 2 + ((lane % (kRowB / 16)) ^ key) * 16);
     } else {
-      vb[i] = (uint32_t)((piece * 16 + (lane >> 2)) * K * 2 + chunk * 16);
+      vb[i] = (uint32_t)((piece * (64 / kLanes) + lane / kLanes) * K * 2 + chunk * 16);
     }
   }
   int fetched = 0;
@@ -264,18 +270,18 @@ template <int MODE, int TM, int TN, int WM, int WN, int WAVES> __global__ void _
 
   // Columns of fragment j: gated, the first half are of Wg, the others the same ones of Wu, so that a lane holds g and u of one element.
   int ta, tb[kAcross];
-  ta = (wm * WM + (lane & 31)) * 64;
+  ta = (wm * WM + (lane & 31)) * kRowA;
   if constexpr (kForward) {
     const int s16 = lane & 15, g16 = lane >> 4, row = 8 * (g16 >> 1) + (s16 >> 2), key = kSub == 128 ? (row & 3) << 2 : (row >> 1 & 1) << 2;
 #pragma unroll
     for (int j = 0; j < kAcross; ++j) {
       const int sub = MODE == kGated ? j / (kAcross / 2) : wn * WN / kSub;
       const int col = MODE == kGated ? wn * (WN / 16) + j % (kAcross / 2) * 4 : wn * WN % kSub / 8 + j * 4;     // (in chunks)
-      tb[j] = kBytesA + sub * (32 * kRowB) + row * kRowB + (((col + 2 * (g16 & 1) + ((s16 & 3) >> 1)) ^ key) * 16) + (s16 & 1) * 8;
+      tb[j] = kBytesA + sub * (STEP * kRowB) + row * kRowB + (((col + 2 * (g16 & 1) + ((s16 & 3) >> 1)) ^ key) * 16) + (s16 & 1) * 8;
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < kAcross; ++j) tb[j] = kBytesA + (wn * WN + j * 32 + (lane & 31)) * 64;
+    for (int j = 0; j < kAcross; ++j) tb[j] = kBytesA + (wn * WN + j * 32 + (lane & 31)) * kRowA;
   }
   f32x16 acc[kHigh][kAcross];
 #pragma unroll
@@ -289,8 +295,8 @@ template <int MODE, int TM, int TN, int WM, int WN, int WAVES> __global__ void _
   bf16x8 a[2][kHigh], c[2][kAcross];
   // fragment i (b0 b1 .. a0 a1 ..) of k 16 kk .. 16 kk + 15 of a stage
   auto load = [&](int set, int i, const unsigned char *stage, int kk) {
-    const int sw = ((kk * 2 + (lane >> 5)) ^ ((lane >> 2) & 3)) * 16;
-    if (i >= kAcross) a[set][i - kAcross] = *(const bf16x8 *)(stage + ta + (i - kAcross) * (32 * 64) + sw);
+    const int sw = ((kk * 2 + (lane >> 5)) ^ (STEP == 32 ? (lane >> 2) & 3 : lane & 7)) * 16;
+    if (i >= kAcross) a[set][i - kAcross] = *(const bf16x8 *)(stage + ta + (i - kAcross) * (32 * kRowA) + sw);
     else if constexpr (kForward) c[set][i] = anc_lds_tr_frag(stage + tb[i] + kk * (16 * kRowB), stage + tb[i] + kk * (16 * kRowB) + 4 * kRowB);
     else c[set][i] = *(const bf16x8 *)(stage + tb[i] + sw);
   };
@@ -308,15 +314,18 @@ template <int MODE, int TM, int TN, int WM, int WN, int WAVES> __global__ void _
   lds_barrier();
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) load(0, i, ring, 0);
-  // One step: the first half's products over the reads of the second half; then every wavefront has read the stage and the next
-  // one has landed for all; then the second half's products over the next stage's first reads and the fetches into the place just read.
+  // One step, 16 k at a time: the products of one slice over the reads of the next. Before the last slice every wavefront has read the stage and
+  // the next one has landed for all; the last slice's products go over the next stage's first reads and the fetches into the place just read.
   auto step = [&](unsigned char *here, unsigned char *next) {
 #pragma unroll
-    for (int i = 0; i < kProducts; ++i) {
-      multiply(0, i);
-      __builtin_amdgcn_sched_barrier(0);
-      if (i < kLoads) load(1, i, here, 1);
-      __builtin_amdgcn_sched_barrier(0);
+    for (int kk = 0; kk + 1 < kSlices; ++kk) {
+#pragma unroll
+      for (int i = 0; i < kProducts; ++i) {
+        multiply(kk & 1, i);
+        __builtin_amdgcn_sched_barrier(0);
+        if (i < kLoads) load((kk + 1) & 1, i, here, kk + 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     wait_vm<(kStages - 2) * kPieces>();
     lds_barrier();
@@ -327,6 +336,7 @@ template <int MODE, int TM, int TN, int WM, int WN, int WAVES> __global__ void _
       __builtin_amdgcn_sched_barrier(0);
       if (i < kLoads) load(0, i, next, 0);
       if (i < kPieces) issue(i, da, db, here);
+      if (kProducts + i < kPieces) issue(kProducts + i, da, db, here);
       __builtin_amdgcn_sched_barrier(0);
     }
     advance();
@@ -523,19 +533,22 @@ template <int V> struct IC { static constexpr int value = V; };
 // Which kernel takes a call: the one whose rounds take least by what a step of 32 k and a round cost, in us. `most`: rows that all
 // segments hold together at most. Measured on whole calls (1 to 8192 rows, 1024 x 2816, 2048 x 2048, 1024 x 4096, dense; 64 and 128 experts of
 // 1024 x 768): a step of k_ffn_tiles where up to 128, 256, .. workgroups are at work, and a round's start and end; of k_ffn_few, one workgroup
-// to a CU, a wavefront's step (of eight). Both sides of some lines, us: gated, 64 rows, 1024 -> 2816: 32x32 by eight wavefronts 10.1, 128x64
-// tiles 13.7; 256 rows 25.7 and 14.2. Down, 1024 rows, 2816 -> 1024: 64x64 by eight wavefronts 17.9, 128x128 tiles 30.4, 128x256 40; 2048 rows 32.1, 31.8,
-// 41; 4096 rows (4096 -> 1024) 47 and 59 for the tiles. Backwards, 8192 rows of 2048 x 2048 in whole rounds: 256x256 134, 128x256 150; 8192 of 1024 x
-// 2816 in half a round of 256x256: 160 and 113. 64 experts of 1024 x 768 with 4 rows each: few rows 66, 128x128 tiles 39.
+// to a CU, a wavefront's step (of eight). Both sides of some lines, us:
+//   gated, 1024 -> 2816: 64 rows: 32x32 by eight wavefronts 10.1, 128x128 tiles 13.8; 256 rows: 64x64 23.4, 128x128 15.0; 1024 rows: 128x128 22.7, 128x256
+//   20.9; 2048 x 2048, 8192 rows: 128x256 125, 256x256 116
+//   down, 2816 -> 1024: 1024 rows: 64x64 17.8, 128x128 32.7; 2048 rows 32.4 and 32.9; 8192 rows: 128x128 48.0, 128x256 52.3, 256x256 67.8
+//   dx, 2048 x 2048, 8192 rows, whole rounds: 256x256 121, 128x128 142; 1024 x 2816, half a round of 256x256: 141 and 99
+//   64 experts of 1024 x 768, 4 rows each, gated: 64x64 74, 128x128 40; 128 rows each, down: 128x256 37, 256x256, which just miss one round, 50
 template <int MODE> int launch(Ffn p, int64_t most, const char *who, hipStream_t s) {
+  constexpr bool kBack = MODE == kGrad || MODE == kDx;
   constexpr int per = MODE == kGated ? 2 : 1;                 // values of the product to one of the outputs
   const int64_t some = p.counts == nullptr ? 1 : most < p.experts ? most : p.experts;              // segments that can hold a row
   const float steps = (float)((p.K + TK - 1) / TK * (MODE == kDx ? 2 : 1));
   auto columns = [&](int64_t TN) { return (p.N + TN / per - 1) / (TN / per); };
-  // workgroups that find work, about (an even routing leaves E e^(-most / E) experts without a row); and at most
+  // workgroups that find work, about (an even routing leaves E e^(-most / E) experts without a row, an uneven one some above their share); and at most
   const int64_t used = p.counts == nullptr ? 1 : (int64_t)ceilf((float)p.experts * -expm1f(-(float)most / (float)p.experts));
   auto live = [&](int64_t TM, int64_t TN) {
-    const int64_t m = p.counts == nullptr ? (most + TM - 1) / TM : most / TM + (used + 1) / 2;
+    const int64_t m = p.counts == nullptr ? (most + TM - 1) / TM : most / TM + (used * 3 + 4) / 5;
     return (m < used ? used : m) * columns(TN);
   };
   auto grid_of = [&](int64_t TM) {
@@ -545,9 +558,10 @@ template <int MODE> int launch(Ffn p, int64_t most, const char *who, hipStream_t
   auto rounds = [&](int64_t n, int64_t slots, auto cost) { return (float)(n / slots) * cost(slots) + (n % slots ? cost(n % slots) : 0.0f); };
   const float cold = p.counts == nullptr ? 1.0f : 1.4f;      // every expert's weights come from memory, in short rows
   const float time[] = {
-      rounds(live(256, 256), 256, [&](int64_t r) { return steps * (r <= 128 ? 0.80f : 0.92f) + 8.0f; }),
-      rounds(live(128, 256), 512, [&](int64_t r) { return steps * (r <= 128 ? 0.46f : r <= 256 ? 0.60f : 0.98f) + 4.0f; }),
-      rounds(live(128, 128), 768, [&](int64_t r) { return steps * (r <= 128 ? 0.33f : r <= 256 ? 0.38f : r <= 512 ? 0.63f : 0.90f) + 3.5f; }),
+      rounds(live(256, 256), 256, [&](int64_t r) { return steps * (r <= 128 ? 0.75f : 0.92f) + (MODE == kGated ? 7.0f : 5.0f); }),
+      rounds(live(128, 256), 512, [&](int64_t r) { return steps * (r <= 128 ? 0.46f : r <= 256 ? 0.60f : kBack ? 1.08f : 0.98f) + 4.0f; }),
+      MODE == kGated ? rounds(live(128, 128), 768, [&](int64_t r) { return steps * (r <= 128 ? 0.33f : r <= 256 ? 0.38f : r <= 512 ? 0.63f : 0.90f) + 3.5f; })
+                     : rounds(live(128, 128), 512, [&](int64_t r) { return steps * (r <= 128 ? 0.33f : r <= 256 ? 0.37f : 0.57f) + 4.5f; }),
       rounds(live(64, 64), 256, [&](int64_t) { return cold * (steps / 8 * 0.92f + 5.7f); }),
       rounds(live(32, 64), 256, [&](int64_t) { return cold * (steps / 8 * 0.72f + 4.6f); }),
       rounds(live(32, 32), 256, [&](int64_t) { return cold * (steps / 8 * 0.47f + 4.2f); }),
@@ -556,9 +570,6 @@ template <int MODE> int launch(Ffn p, int64_t most, const char *who, hipStream_t
   int best = 0;
   for (int i = 1; i < 7; ++i)
     if (time[i] < time[best]) best = i;
-#ifdef FFN_PICK
-  best = FFN_PICK;
-#endif
   AncProfScope prof(ANC_PROF_DW_GEMM, s);
   auto few = [&](auto R, auto C) {
     constexpr int r = decltype(R)::value, c = decltype(C)::value;
@@ -567,19 +578,22 @@ template <int MODE> int launch(Ffn p, int64_t most, const char *who, hipStream_t
     hipLaunchKernelGGL((k_ffn_few<MODE, r, c>), dim3((unsigned)grid_of(16 * r)), dim3(512), 0, s, p);
     return ANC_OK;
   };
-  auto tiles = [&](auto TM, auto TN, auto WM, auto WN, auto W) {
-    constexpr int tm = decltype(TM)::value, tn = decltype(TN)::value, wm = decltype(WM)::value, wn = decltype(WN)::value, w = decltype(W)::value;
+  auto tiles = [&](auto TM, auto TN, auto WM, auto WN, auto ST, auto SG, auto W) {
+    constexpr int tm = decltype(TM)::value, tn = decltype(TN)::value, wm = decltype(WM)::value, wn = decltype(WN)::value, st = decltype(ST)::value, sg = decltype(SG)::value, w = decltype(W)::value;
     p.tn = (int)columns(tn);
     ANC_REQUIRE(grid_of(tm) < (1ll << 31) / 512, "%s: too large for one call", who);
-    hipLaunchKernelGGL((k_ffn_tiles<MODE, tm, tn, wm, wn, w>), dim3((unsigned)grid_of(tm)), dim3(tm / wm * (tn / wn) * 64), 0, s, p);
+    hipLaunchKernelGGL((k_ffn_tiles<MODE, tm, tn, wm, wn, st, sg, w>), dim3((unsigned)grid_of(tm)), dim3(tm / wm * (tn / wn) * 64), 0, s, p);
     return ANC_OK;
   };
   constexpr int kTall = MODE == kGated ? 64 : 128;            // a wavefront's rows; gated: 64 columns of either weight
   int rc = ANC_OK;
   switch (best) {
-    case 0: rc = tiles(IC<256>{}, IC<256>{}, IC<kTall>{}, IC<8192 / kTall>{}, IC<2>{}); break;
-    case 1: rc = tiles(IC<128>{}, IC<256>{}, IC<kTall>{}, IC<8192 / kTall>{}, IC<2>{}); break;
-    case 2: rc = tiles(IC<128>{}, IC<128>{}, IC<64>{}, IC<64>{}, IC<3>{}); break;
+    case 0: rc = tiles(IC<256>{}, IC<256>{}, IC<kTall>{}, IC<8192 / kTall>{}, IC<64>{}, IC<2>{}, IC<2>{}); break;
+    case 1: rc = tiles(IC<128>{}, IC<256>{}, IC<kTall>{}, IC<8192 / kTall>{}, IC<32>{}, IC<3>{}, IC<2>{}); break;
+    case 2:
+      if constexpr (MODE == kGated) rc = tiles(IC<128>{}, IC<128>{}, IC<64>{}, IC<64>{}, IC<32>{}, IC<3>{}, IC<3>{});
+      else rc = tiles(IC<128>{}, IC<128>{}, IC<64>{}, IC<64>{}, IC<64>{}, IC<2>{}, IC<2>{});
+      break;
     case 3: rc = few(IC<4>{}, IC<4>{}); break;
     case 4: rc = few(IC<2>{}, IC<4>{}); break;
     case 5: rc = few(IC<2>{}, IC<2>{}); break;
