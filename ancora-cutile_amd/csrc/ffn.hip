@@ -10,12 +10,13 @@
 // accumulate in fp32 over ascending k (dx: all of dg, then all of du); each output is rounded once.
 //
 // k_ffn_tiles: a workgroup owns TM x TN values of the product (gated: half of the columns of either weight, so that a lane holds g and u of
-// the same element) and runs k through LDS in two stages of 64 or three of 32; wavefronts of 128 x 64, 64 x 128 or 64 x 64. Operands go straight
+// the same element) and runs k through LDS in stages of 64 or 32; wavefronts of 128 x 64, 64 x 128, 64 x 64 or 32 x 64. Operands go straight
 // to LDS through descriptors that end with the segment or the matrix: rows and columns beyond read zeros and are not stored. What bounds
 // its loop is the operands' way into LDS: a CU has some 64 lines under way at a time, so a line of 128 bytes asked for in halves, a step of 32 k
 // apart, counts twice. Steps of 64 ask for whole lines of what lies along k (8192 rows, dx, 1024 x 2816, 128x128 tiles: 129 us in steps of 32,
 // 100 in steps of 64; 2048 x 2048, 256x256: 130 and 120, 1.15 PFLOP/s; gated, 256x256: 131 and 116 to 125); 128x256 keeps steps of 32, of which two
-// workgroups fit a CU and hide each other's ends. What is left then is the outputs' bytes, which overlap little with the loops.
+// workgroups fit a CU and hide each other's ends. A CU takes in some 60 bytes a nanosecond so, which is why few tiles are small ones. What is left then is the
+// outputs' bytes, which overlap little with the loops.
 // k_ffn_few: 16 to 64 rows of a segment by 16 to 64 columns, the eight wavefronts of a workgroup taking every eighth step of k, each
 // with stages of its own and no barrier, and adding up at the end in a fixed order: with few rows the weights' bytes are the work, and
 // this way they are spread over as many CUs as there are.
@@ -202,8 +203,9 @@ template <int MODE, bool ONCE> __device__ __forceinline__ void finish(const Ffn 
 }
 
 // ---------------------------------------------------------------- many rows
-// TM x TN values to a workgroup, WM x WN to a wavefront, WAVES wavefronts to a SIMD.
-template <int MODE, int TM, int TN, int WM, int WN, int STEP, int STAGES, int WAVES>
+// TM x TN values to a workgroup, WM x WN to a wavefront, WAVES wavefronts to a SIMD; fragments are read AHEAD slices of 16 k before their products:
+// two where a wavefront has only two products to a slice, which do not cover a read (dx, 2048 rows of 1024 x 2816: 40.6 -> 37.2 us).
+template <int MODE, int TM, int TN, int WM, int WN, int STEP, int STAGES, int WAVES, int AHEAD>
 __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, WAVES) k_ffn_tiles(Ffn p) {
   constexpr bool kForward = MODE == kGated || MODE == kDown;
   constexpr int kWide = TN / WN, kWaves = TM / WM * kWide, kHigh = WM / 32, kAcross = WN / 32;       // wavefronts side by side, in all; fragments of A, of B
@@ -212,8 +214,8 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, WAVES) k_ffn_tiles(F
   constexpr int kCols = MODE == kGated ? TN / 2 : TN;       // columns of the outputs
   // Forwards the B tile is [STEP][kSub columns] once or twice: of either weight, or side by side.
   constexpr int kSub = MODE == kGated ? TN / 2 : 128, kRowB = kSub * 2, kRows = 1024 / kRowB, kSubPieces = STEP / kRows;
-  static_assert((MODE == kGated || WN == 64) && kWaves * 8192 <= kStages * kStage && kPieces <= 2 * kHigh * kAcross && kHigh + kAcross <= kHigh * kAcross + 1 && kPiecesA * kWaves * 1024 == kBytesA && kPiecesB * kWaves * 1024 == kBytesB,
-                "room for the way out; pieces to a half step; whole pieces");
+  static_assert((MODE == kGated || WN == 64) && kWaves * 8192 <= kStages * kStage && kPiecesA * kWaves * 1024 == kBytesA && kPiecesB * kWaves * 1024 == kBytesB,
+                "room for the way out; whole pieces");
   __shared__ __attribute__((aligned(1024))) unsigned char ring[kStages * kStage];
   Place at;
   if (!place_of(p, TM, at)) return;
@@ -292,7 +294,8 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, WAVES) k_ffn_tiles(F
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
   constexpr int kLoads = kHigh + kAcross, kProducts = kHigh * kAcross;
-  bf16x8 a[2][kHigh], c[2][kAcross];
+  constexpr int kSets = AHEAD == 1 ? 2 : 4;
+  bf16x8 a[kSets][kHigh], c[kSets][kAcross];
   // fragment i (b0 b1 .. a0 a1 ..) of k 16 kk .. 16 kk + 15 of a stage
   auto load = [&](int set, int i, const unsigned char *stage, int kk) {
     const int sw = ((kk * 2 + (lane >> 5)) ^ (STEP == 32 ? (lane >> 2) & 3 : lane & 7)) * 16;
@@ -313,31 +316,37 @@ __global__ void __launch_bounds__(TM / WM * (TN / WN) * 64, WAVES) k_ffn_tiles(F
   wait_vm<(kStages - 1) * kPieces>();
   lds_barrier();
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) load(0, i, ring, 0);
-  // One step, 16 k at a time: the products of one slice over the reads of the next. Before the last slice every wavefront has read the stage and
-  // the next one has landed for all; the last slice's products go over the next stage's first reads and the fetches into the place just read.
-  auto step = [&](unsigned char *here, unsigned char *next) {
+  for (int kk = 0; kk < AHEAD; ++kk)
 #pragma unroll
-    for (int kk = 0; kk + 1 < kSlices; ++kk) {
+    for (int i = 0; i < kLoads; ++i) load(kk, i, ring, kk);
+  // One step, a slice at a time: its products over the reads of a later one. Before the first reads of the next stage every wavefront has read this
+  // one and the next has landed for all; the products from there on also go over the fetches into the place just read.
+  auto step = [&](unsigned char *here, unsigned char *next) {
+    static_assert(kSlices % kSets == 0 && AHEAD < kSets, "a slice's fragments have one place");
+    anc_i32x4 da, db;
+#pragma unroll
+    for (int kk = 0; kk < kSlices; ++kk) {
+      if (kk == kSlices - AHEAD) {
+        wait_vm<(kStages - 2) * kPieces>();
+        lds_barrier();
+        da = fa.desc();
+        db = fb.desc();
+      }
 #pragma unroll
       for (int i = 0; i < kProducts; ++i) {
-        multiply(kk & 1, i);
+        multiply(kk % kSets, i);
         __builtin_amdgcn_sched_barrier(0);
-        if (i < kLoads) load((kk + 1) & 1, i, here, kk + 1);
+#pragma unroll
+        for (int q = i; q < kLoads; q += kProducts) {
+          if (kk + AHEAD < kSlices) load((kk + AHEAD) % kSets, q, here, kk + AHEAD);
+          else load((kk + AHEAD) % kSets, q, next, kk + AHEAD - kSlices);
+        }
+        if (kk >= kSlices - AHEAD) {
+#pragma unroll
+          for (int q = (kk - (kSlices - AHEAD)) * kProducts + i; q < kPieces; q += AHEAD * kProducts) issue(q, da, db, here);
+        }
         __builtin_amdgcn_sched_barrier(0);
       }
-    }
-    wait_vm<(kStages - 2) * kPieces>();
-    lds_barrier();
-    const anc_i32x4 da = fa.desc(), db = fb.desc();
-#pragma unroll
-    for (int i = 0; i < kProducts; ++i) {
-      multiply(1, i);
-      __builtin_amdgcn_sched_barrier(0);
-      if (i < kLoads) load(0, i, next, 0);
-      if (i < kPieces) issue(i, da, db, here);
-      if (kProducts + i < kPieces) issue(kProducts + i, da, db, here);
-      __builtin_amdgcn_sched_barrier(0);
     }
     advance();
   };
@@ -534,10 +543,12 @@ template <int V> struct IC { static constexpr int value = V; };
 // segments hold together at most. Measured on whole calls (1 to 8192 rows, 1024 x 2816, 2048 x 2048, 1024 x 4096, dense; 64 and 128 experts of
 // 1024 x 768): a step of k_ffn_tiles where up to 128, 256, .. workgroups are at work, and a round's start and end; of k_ffn_few, one workgroup
 // to a CU, a wavefront's step (of eight). Both sides of some lines, us:
-//   gated, 1024 -> 2816: 64 rows: 32x32 by eight wavefronts 10.1, 128x128 tiles 13.8; 256 rows: 64x64 23.4, 128x128 15.0; 1024 rows: 128x128 22.7, 128x256
-//   20.9; 2048 x 2048, 8192 rows: 128x256 125, 256x256 116
-//   down, 2816 -> 1024: 1024 rows: 64x64 17.8, 128x128 32.7; 2048 rows 32.4 and 32.9; 8192 rows: 128x128 48.0, 128x256 52.3, 256x256 67.8
-//   dx, 2048 x 2048, 8192 rows, whole rounds: 256x256 121, 128x128 142; 1024 x 2816, half a round of 256x256: 141 and 99
+//   gated, 1024 -> 2816: 64 rows: 32x32 by eight wavefronts 10.1, 128x128 tiles 13.8; 256 rows: 64x64 by eight wavefronts 23.4, 64x128 tiles 10.3, 128x128
+//   15.0; 1024 rows: 128x128 22.7, 128x256 20.9; 2048 x 2048, 8192 rows: 128x256 125, 256x256 116
+//   down, 2816 -> 1024: 1024 rows: 64x64 by eight wavefronts 17.8, 64x128 19.8, 128x128 32.7; 2048 rows 32.4, 20.1, 32.9; 8192 rows: 64x128 64, 128x128
+//   49, 128x256 52, 256x256 68
+//   grad, 512 rows of 1024 x 2816: 64x128 11.2, 128x128 17.0; dx, 2048 x 2048, 8192 rows, whole rounds: 256x256 121, 128x128 142; 1024 x 2816, half a round
+//   of 256x256: 141, and 128x128 100 to 114
 //   64 experts of 1024 x 768, 4 rows each, gated: 64x64 74, 128x128 40; 128 rows each, down: 128x256 37, 256x256, which just miss one round, 50
 template <int MODE> int launch(Ffn p, int64_t most, const char *who, hipStream_t s) {
   constexpr bool kBack = MODE == kGrad || MODE == kDx;
@@ -562,13 +573,14 @@ template <int MODE> int launch(Ffn p, int64_t most, const char *who, hipStream_t
       rounds(live(128, 256), 512, [&](int64_t r) { return steps * (r <= 128 ? 0.46f : r <= 256 ? 0.60f : kBack ? 1.08f : 0.98f) + 4.0f; }),
       MODE == kGated ? rounds(live(128, 128), 768, [&](int64_t r) { return steps * (r <= 128 ? 0.33f : r <= 256 ? 0.38f : r <= 512 ? 0.63f : 0.90f) + 3.5f; })
                      : rounds(live(128, 128), 512, [&](int64_t r) { return steps * (r <= 128 ? 0.33f : r <= 256 ? 0.37f : 0.57f) + 4.5f; }),
+      rounds(live(64, 128), 512, [&](int64_t r) { return steps * (r <= 256 ? 0.19f : 0.35f) + 4.5f; }),
       rounds(live(64, 64), 256, [&](int64_t) { return cold * (steps / 8 * 0.92f + 5.7f); }),
       rounds(live(32, 64), 256, [&](int64_t) { return cold * (steps / 8 * 0.72f + 4.6f); }),
       rounds(live(32, 32), 256, [&](int64_t) { return cold * (steps / 8 * 0.47f + 4.2f); }),
       MODE == kGated ? 1e30f : rounds(live(16, 16), 256, [&](int64_t) { return cold * (steps / 8 * 0.25f + 4.0f); }),
   };
   int best = 0;
-  for (int i = 1; i < 7; ++i)
+  for (int i = 1; i < 8; ++i)
     if (time[i] < time[best]) best = i;
   AncProfScope prof(ANC_PROF_DW_GEMM, s);
   auto few = [&](auto R, auto C) {
@@ -578,25 +590,26 @@ template <int MODE> int launch(Ffn p, int64_t most, const char *who, hipStream_t
     hipLaunchKernelGGL((k_ffn_few<MODE, r, c>), dim3((unsigned)grid_of(16 * r)), dim3(512), 0, s, p);
     return ANC_OK;
   };
-  auto tiles = [&](auto TM, auto TN, auto WM, auto WN, auto ST, auto SG, auto W) {
-    constexpr int tm = decltype(TM)::value, tn = decltype(TN)::value, wm = decltype(WM)::value, wn = decltype(WN)::value, st = decltype(ST)::value, sg = decltype(SG)::value, w = decltype(W)::value;
+  auto tiles = [&](auto TM, auto TN, auto WM, auto WN, auto ST, auto SG, auto W, auto AH) {
+    constexpr int tm = decltype(TM)::value, tn = decltype(TN)::value, wm = decltype(WM)::value, wn = decltype(WN)::value, st = decltype(ST)::value, sg = decltype(SG)::value, w = decltype(W)::value, ah = decltype(AH)::value;
     p.tn = (int)columns(tn);
     ANC_REQUIRE(grid_of(tm) < (1ll << 31) / 512, "%s: too large for one call", who);
-    hipLaunchKernelGGL((k_ffn_tiles<MODE, tm, tn, wm, wn, st, sg, w>), dim3((unsigned)grid_of(tm)), dim3(tm / wm * (tn / wn) * 64), 0, s, p);
+    hipLaunchKernelGGL((k_ffn_tiles<MODE, tm, tn, wm, wn, st, sg, w, ah>), dim3((unsigned)grid_of(tm)), dim3(tm / wm * (tn / wn) * 64), 0, s, p);
     return ANC_OK;
   };
   constexpr int kTall = MODE == kGated ? 64 : 128;            // a wavefront's rows; gated: 64 columns of either weight
   int rc = ANC_OK;
   switch (best) {
-    case 0: rc = tiles(IC<256>{}, IC<256>{}, IC<kTall>{}, IC<8192 / kTall>{}, IC<64>{}, IC<2>{}, IC<2>{}); break;
-    case 1: rc = tiles(IC<128>{}, IC<256>{}, IC<kTall>{}, IC<8192 / kTall>{}, IC<32>{}, IC<3>{}, IC<2>{}); break;
+    case 0: rc = tiles(IC<256>{}, IC<256>{}, IC<kTall>{}, IC<8192 / kTall>{}, IC<64>{}, IC<2>{}, IC<2>{}, IC<1>{}); break;
+    case 1: rc = tiles(IC<128>{}, IC<256>{}, IC<kTall>{}, IC<8192 / kTall>{}, IC<32>{}, IC<3>{}, IC<2>{}, IC<1>{}); break;
     case 2:
-      if constexpr (MODE == kGated) rc = tiles(IC<128>{}, IC<128>{}, IC<64>{}, IC<64>{}, IC<32>{}, IC<3>{}, IC<3>{});
-      else rc = tiles(IC<128>{}, IC<128>{}, IC<64>{}, IC<64>{}, IC<64>{}, IC<2>{}, IC<2>{});
+      if constexpr (MODE == kGated) rc = tiles(IC<128>{}, IC<128>{}, IC<64>{}, IC<64>{}, IC<32>{}, IC<3>{}, IC<3>{}, IC<1>{});
+      else rc = tiles(IC<128>{}, IC<128>{}, IC<64>{}, IC<64>{}, IC<64>{}, IC<2>{}, IC<2>{}, IC<1>{});
       break;
-    case 3: rc = few(IC<4>{}, IC<4>{}); break;
-    case 4: rc = few(IC<2>{}, IC<4>{}); break;
-    case 5: rc = few(IC<2>{}, IC<2>{}); break;
+    case 3: rc = tiles(IC<64>{}, IC<128>{}, IC<32>{}, IC<64>{}, IC<64>{}, IC<3>{}, IC<2>{}, IC<2>{}); break;
+    case 4: rc = few(IC<4>{}, IC<4>{}); break;
+    case 5: rc = few(IC<2>{}, IC<4>{}); break;
+    case 6: rc = few(IC<2>{}, IC<2>{}); break;
     default: if constexpr (per == 1) rc = few(IC<1>{}, IC<1>{}); break;
   }
   if (rc != ANC_OK) return rc;
