@@ -474,6 +474,12 @@ template <int MODE, int R, int C> __global__ void __launch_bounds__(512, 2) k_ff
       for (int i = 0; i < C; ++i) dma16_bounded(db, (vb + (uint32_t)(i * 16 * K * 2)) | mask, lds_addr(stage + (R + i) * 1024));
     }
   };
+  // A lane's eight values of the outputs.
+  constexpr int kOcts = kCols / 8;
+  static_assert(TM * kOcts <= kWaves * 64, "one each");
+  const int row = (int)threadIdx.x / kOcts, oct = (int)threadIdx.x % kOcts, col = n0 + oct * 8;
+  const bool ours = row < rows && col < N;
+  const int64_t e = (at.row + row) * N + col;
   f32x4v acc[R][C];
 #pragma unroll
   for (int i = 0; i < R; ++i)
@@ -507,34 +513,40 @@ template <int MODE, int R, int C> __global__ void __launch_bounds__(512, 2) k_ff
       for (int i = 0; i < R; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
     here = here + kStage < kStages * kStage ? here + kStage : 0;
   }
+  const Side side = ours ? side_of<MODE>(p, e) : Side{};     // (on its way over the sums)
   wait_vm<0>();
   lds_barrier();
-  // The wavefronts' sums, in ascending order: [wavefront][row][column] fp32.
+  // The wavefronts' sums, in ascending order: [wavefront][row][column] fp32. Where eight values to a lane leave lanes idle, all add up over the first
+  // one's first (1 to 32 rows, 1024 -> 2816: gated 0.5 us less; 1024 rows, 64x64, where none are: down 0.6 more, so not there).
   float *sums = (float *)ring;
+  constexpr int kSums = TM * C * 16, kParts = TM * kOcts < kWaves * 64 ? 1 : kWaves;
 #pragma unroll
   for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int j = 0; j < C; ++j) *(f32x4v *)(sums + (wave * TM + i * 16 + s16) * (C * 16) + j * 16 + g16 * 4) = acc[i][j];
+    for (int j = 0; j < C; ++j) *(f32x4v *)(sums + wave * kSums + (i * 16 + s16) * (C * 16) + j * 16 + g16 * 4) = acc[i][j];
   lds_barrier();
-  constexpr int kOcts = kCols / 8;
-  for (int idx = (int)threadIdx.x; idx < TM * kOcts; idx += kWaves * 64) {
-    const int row = idx / kOcts, oct = idx % kOcts, col = n0 + oct * 8;
-    if (row >= rows || col >= N) continue;
-    const int64_t e = (at.row + row) * N + col;
-    const Side side = side_of<MODE>(p, e);
-    auto total = [&](int first, float (&f)[8]) {
+  if constexpr (kParts == 1) {
+    for (int idx = (int)threadIdx.x * 4; idx < rows * (C * 16); idx += kWaves * 256) {
+      f32x4v v = *(const f32x4v *)(sums + idx);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = sums[row * (C * 16) + first + k];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] += sums[(w * TM + row) * (C * 16) + first + k];
-    };
-    float v[8], w[8];
-    total(oct * 8, v);
-    if constexpr (MODE == kGated) total(kCols + oct * 8, w);
-    finish<MODE, false>(p, e, v, w, side);
+      for (int w = 1; w < kWaves; ++w) v += *(const f32x4v *)(sums + w * kSums + idx);
+      *(f32x4v *)(sums + idx) = v;
+    }
+    lds_barrier();
   }
+  if (!ours) return;
+  auto total = [&](int first, float (&f)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = sums[row * (C * 16) + first + k];
+#pragma unroll
+    for (int w = 1; w < kParts; ++w)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] += sums[w * kSums + row * (C * 16) + first + k];
+  };
+  float v[8], w[8];
+  total(oct * 8, v);
+  if constexpr (MODE == kGated) total(kCols + oct * 8, w);
+  finish<MODE, false>(p, e, v, w, side);
 }
 
 // ---------------------------------------------------------------- launch
