@@ -18,10 +18,12 @@ from . import _lib
 from ._lib import api
 from .embed import _type
 
+_BITS = np.dtype(np.uint16)          # bf16 (buffers hold dtypes: comparing with a type costs each check 0.1 us)
+
 
 def _call(who, rows_name, rows_buf, plan):
     """(rows, rows that are tokens' at most, experts, counts, offsets) of a call whose first operand is rows_buf (rows, K)."""
-    if len(rows_buf.shape) != 2 or rows_buf.dtype != np.uint16:
+    if len(rows_buf.shape) != 2 or rows_buf.dtype != _BITS:
         raise ValueError(f"{who}: {rows_name} is {rows_buf.shape} {rows_buf.dtype}, rows of bf16 bits expected")
     if plan is None:
         return rows_buf.shape[0], rows_buf.shape[0], 0, 0, 0
@@ -30,18 +32,19 @@ def _call(who, rows_name, rows_buf, plan):
     return plan.capacity, plan.active * plan.k, plan.E, counts, offsets
 
 
-def _rows(who, name, b, rows, width, dtype=np.uint16):
+def _rows(who, name, b, rows, width, dtype=_BITS):
     if b is None:
         return 0
-    if len(b.shape) != 2 or b.shape[0] < rows or b.shape[1] != width or (dtype is not None and b.dtype != dtype):
+    shape = b.shape
+    if len(shape) != 2 or shape[0] < rows or shape[1] != width or (dtype is not None and b.dtype != dtype):
         raise ValueError(f"{who}: {name} is {b.shape} {b.dtype}, ({rows}, {width}) "
-                         f"{'of bf16 bits' if dtype == np.uint16 else '' if dtype is None else np.dtype(dtype)} expected")
+                         f"{'of bf16 bits' if dtype == _BITS else '' if dtype is None else dtype} expected")
     return b.ptr
 
 
 def _weight(who, name, w, E, K, N):
-    if w.dtype != np.uint16 or w.shape[-1] != N or w.size != max(E, 1) * K * N or len(w.shape) not in (2, 3) \
-            or (len(w.shape) == 3 and w.shape[1] != K):
+    shape, n = w.shape, E or 1
+    if w.dtype != _BITS or (shape != (n * K, N) and shape != (n, K, N)):
         raise ValueError(f"{who}: {name} is {w.shape} {w.dtype}, {(E, K, N) if E else (K, N)} of bf16 bits expected")
     return w.ptr
 
