@@ -35,6 +35,10 @@ How each function is pinned (see tests/test_oracle_*.py):
   id_groups / embed_dw_rows /       (embed_ref.py) defining properties of the group arrays (permutation,
   embed_dw_scatter                  stability, counts), an exact integer case, the reference-held gate
                                     against an fp64 scatter-add (tests/kernels/test_embed_dw_scatter.py:55-61,91)
+  rms_norm(_grad), gated(_grad),    (layer_ref.py) the formulas in fp64: gradients against differences, segments against products of
+  by_segment, mx8_rows              their own rows, MXFP8 rows against quant_mxfp8_w of the transposed matrix
+  decode, encode, the 8-bit step    (adamw8_ref.py) codes against their formats' definition by value, neighbours and unbiasedness of the
+                                    stored moments, a decaying moment that keeps moving, values that are not finite
 ns_chain_model.py and ns_inputs.py are not restatements of the reference: the first models the
 arithmetic of this library's bf16 chain (rounding points, plan, gate statistics, the 8-bit low
 half), the second holds input families for walking its thresholds. The model is pinned to the GPU
