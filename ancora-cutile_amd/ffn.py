@@ -10,7 +10,8 @@ between `dispatch` and `combine`, and the operands of the weight gradients (`gra
 Weights are the bf16 copies that the optimizer refreshes, as they lie: (H, I) and (I, H), stacked per expert (E, H, I) or (E*H, I) with a
 plan; no transposed copies are read. Mirrors SwiGLU and the grouped products of the reference's layers (ancora/kernels/activation.py,
 ancora/kernels/moe.py). Products accumulate in fp32, each output is rounded once. Without a plan every row of x is a row of the product; with
-one, rows that fill up a segment or lie behind the last are neither read nor written. Each call may be captured into a graph.
+one, rows that fill up a segment or lie behind the last are neither read nor written. Each call may be captured into a graph, whose replays then
+work on no more tokens than the plan held at the capture (`plan.active`), as its routing and dispatch do.
 """
 import numpy as np
 

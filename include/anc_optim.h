@@ -288,7 +288,7 @@ int anc_adamw_multi(uint64_t desc_table, int32_t n_tensors, int64_t total_blocks
  * 0x3C6EF372), a code is the lower neighbour, plus one where the dropped part of the magnitude and 16 bits of h (m: low half, v: high half), as
  * a fraction of the codes' distance, add up to one or more. A v above zero is stored as no less than the least code, so that the update's
  * divisor does not vanish. A moment that is not finite gets the NaN code 0x7F (m: with its sign) and does not count in its block's
- * largest. sr and seeds as in anc_adamw_multi, but seed_base always counts (it is the moments' too), and sr may be ANC_SR_STEP_SEED
+ * largest; one within an eighth (v: a quarter) of the largest fp32 may round up to a value that is not finite. sr and seeds as in anc_adamw_multi, but seed_base always counts (it is the moments' too), and sr may be ANC_SR_STEP_SEED
  * alone. Elements are independent of how tensors share a launch. blk0 and total_blocks count anc_adamw_num_blocks(n).
  * Alignment: g, p32 16 bytes (bf16 g: 8), p16 8, m and v 4. */
 typedef struct {
@@ -531,7 +531,8 @@ int anc_expert_dw_multi(const anc_expert_dw_problem_t *problems, int32_t n_probl
  * ancora/kernels/moe.py around the weights the step updates), over all `rows` rows (counts = offsets = 0, experts = 0) or over tokens
  * sorted by expert (anc_route's counts and offsets on the device, `rows` slots, of which the segments hold `tokens` at most, all together: what
  * anc_route was given; dense: tokens = rows): rows that fill up a segment, or lie behind the last, are neither read nor written. Where the
- * segments hold more than `tokens`, rows may be left out, none is touched outside the buffers. Weights are bf16 as the step keeps them, (in, out) row-major, one after the other per expert: Wg, Wu (H, I), Wd (I, H).
+ * segments hold more than `tokens`, rows may be left out, none is touched outside the buffers. Weights are bf16 as the step keeps them,
+ * (in, out) row-major, one after the other per expert: Wg, Wu (H, I), Wd (I, H).
  *   anc_gated_ffn:       h = silu(x Wg) * (x Wu); gate, up (0: not kept) receive x Wg and x Wu for the backward pass. All bf16.
  *   anc_ffn_down:        y = h Wd + residual (0: none), y and residual of y_type (ANC_F32 or ANC_BF16)
  *   anc_gated_ffn_grad:  with dh = dy Wd^T and s = sigmoid(gate): dgate = dh up s (1 + gate (1 - s)), dup = dh gate s, h = gate s up (0: not

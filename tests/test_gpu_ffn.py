@@ -372,3 +372,67 @@ def test_no_tokens_at_all(gpu):
     assert (h.to_numpy() == 7).all() and (y.to_numpy() == 7).all()
     for b in (*bufs, plan, ids):
         b.free()
+
+
+@pytest.mark.parametrize("H,I,E,tokens", [(72, 2056, 2, 3000), (2056, 40, 2, 3000), (264, 264, 6, 16000), (520, 520, 2, 16000), (2056, 520, 2, 700),
+                                          (520, 4104, 2, 1500), (1544, 1032, 2, 5000)])
+def test_every_size_of_tile_over_segments(gpu, H, I, E, tokens):
+    """Uneven segments at sizes where each of the kernels is the cheapest for one of the four calls: rows at the tiles' edges and some others of every segment
+    against 64 bits, nothing else written."""
+    from ancora_cutile_amd import DevBuf, ffn_down, gated_ffn, gated_ffn_dx, gated_ffn_grad
+    rng = np.random.default_rng(H + I + tokens)
+    counts = rng.multinomial(tokens, np.linspace(0.6, 1.4, E) / E)
+    plan, counts, offsets = _plan_of(counts, 8, 5)
+    rows, mine = plan.capacity, np.zeros(plan.capacity, bool)
+    pick, of = [], []
+    for e, (n, o) in enumerate(zip(counts, offsets)):
+        mine[o:o + n] = True
+        p = np.unique(np.concatenate([[0, 31, 63, 64, 127, 128, 255, 256, n - 1], rng.integers(0, n, 25)]) % n)
+        pick.append(o + p)
+        of.append(np.full(p.size, e))
+    pick, of = np.concatenate(pick), np.concatenate(of)
+    host, dev = {}, {}
+    for n, shape, std in (("Wg", (E, H, I), H ** -0.5), ("Wu", (E, H, I), H ** -0.5), ("Wd", (E, I, H), I ** -0.5), ("x", (rows, H), 1.0), ("h", (rows, I), 1.0),
+                          ("gate", (rows, I), 1.0), ("up", (rows, I), 1.0), ("dy", (rows, H), 1.0), ("res", (rows, H), 1.0)):
+        b = bf16_rne_bits((std * rng.standard_normal(shape, dtype=F32))).reshape(shape)
+        if n[0] != "W":
+            b[~mine] = 0x7FFF
+        dev[n], host[n] = DevBuf(b), _wide(b if n[0] == "W" else b[pick])
+    out = {n: DevBuf(np.full((rows, w), np.nan, t) if t == F32 else np.full((rows, w), 0x7FC1, t)) for n, w, t in
+           (("h", I, U16), ("g", I, U16), ("u", I, U16), ("y", H, F32), ("dgate", I, U16), ("dup", I, U16), ("h2", I, U16), ("dx", H, U16))}
+
+    def product(a, w):
+        v, m = np.empty((a.shape[0], w.shape[2])), np.empty((a.shape[0], w.shape[2]))
+        for e in range(E):
+            v[of == e], m[of == e] = a[of == e] @ w[e], np.abs(a[of == e]) @ np.abs(w[e])
+        return v, (a.shape[1] + 8) * UNIT * m
+
+    def near(name, want, err):
+        got = _val(out[name])
+        assert np.isfinite(got[mine]).all(), name
+        assert np.all(np.abs(got[pick] - want) <= err + _half(out[name]) * (np.abs(want) + err) + 1e-30), name
+        _untouched(out[name], mine)
+    gated_ffn(dev["x"], dev["Wg"], dev["Wu"], 0, out["h"], gate=out["g"], up=out["u"], plan=plan)
+    (g, ge), (u, ue) = product(host["x"], host["Wg"]), product(host["x"], host["Wu"])
+    a = np.abs(g) * ref.sigmoid(g)
+    near("h", ref.gated(g, u), 1.1 * ge * (np.abs(u) + ue) + a * ue + a * np.abs(u) * (np.abs(g) + 10) * UNIT)
+    near("g", g, ge)
+    near("u", u, ue)
+    ffn_down(dev["h"], dev["Wd"], 0, out["y"], plan=plan)
+    near("y", *product(host["h"], host["Wd"]))
+    gated_ffn_grad(dev["dy"], dev["gate"], dev["up"], dev["Wd"], 0, out["dgate"], out["dup"], h=out["h2"], plan=plan)
+    flip = lambda w: np.swapaxes(w, 1, 2)  # noqa: E731
+    dh, de = product(host["dy"], flip(host["Wd"]))
+    g, u = host["gate"], host["up"]
+    s = ref.sigmoid(g)
+    wg, wu, wh = ref.gated_grad(dh, g, u)
+    es, slope = (np.abs(g) + 10) * UNIT, s * (1 + np.abs(g))
+    near("dgate", wg, (1.1 * de + 2 * np.abs(dh) * es) * np.abs(u) * slope)
+    near("dup", wu, (1.1 * de + np.abs(dh) * es) * np.abs(g) * s)
+    near("h2", wh, np.abs(wh) * es)
+    gated_ffn_dx(dev["gate"], dev["up"], dev["Wg"], dev["Wu"], 0, out["dx"], residual=dev["res"], plan=plan)
+    (v1, e1), (v2, e2) = product(g, flip(host["Wg"])), product(u, flip(host["Wu"]))
+    want = v1 + v2 + host["res"]
+    near("dx", want, 2 * (e1 + e2) + 2.0 ** -24 * (np.abs(want) + 2 * (e1 + e2)))
+    for b in (*dev.values(), *out.values(), plan):
+        b.free()
