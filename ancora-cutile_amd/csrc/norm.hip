@@ -6,7 +6,7 @@
 //   format of quant.hip with the blocks along the row, which is the axis that a product with the weights runs over
 //   a = dy gain,  dx = r (a - s r^2 mean(a s)) + carry,  dgain = sum over rows of dy s r
 //
-// HBM-bound. A row is held in registers by 16, 64 or 256 lanes, 8 elements (16 bytes of bf16) to a piece, so that it is read once.
+// HBM-bound. A row is held in registers by 16, 64 or 256 lanes (backwards up to 512), 8 elements (16 bytes of bf16) to a piece, so that it is read once.
 // The gain's gradient: workgroups add up their rows in registers, then their groups of lanes through LDS, and leave one fp32 row each; a
 // second launch adds those in a fixed order. The bits are a function of the inputs and the shape.
 #include "rows.h"
@@ -50,16 +50,19 @@ template <int T> __device__ __forceinline__ void store8(uint64_t p, int64_t e, c
   }
 }
 
-// Sum over the LPR lanes of a row, in all of them, in a fixed order. LPR = 256: every lane of the workgroup calls it.
-template <int LPR> __device__ __forceinline__ float row_sum(float v, float *lds) {
+// Sum over the LPR lanes of a row, in all of them, in a fixed order. LPR > 64: every lane of the workgroup calls it; lds: a float per wavefront, two
+// sets in turn (`odd`), so that one barrier parts a call from the one before it.
+template <int LPR> __device__ __forceinline__ float row_sum(float v, float *lds, int odd = 0) {
 #pragma unroll
   for (int off = LPR == 16 ? 8 : 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-  if constexpr (LPR == 256) {
-    __syncthreads();                                  // (the last call's values have been read)
+  if constexpr (LPR > 64) {
+    lds += odd * (kGradThreads / 64);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
-    const float *w = lds + (threadIdx.x >> 8) * 4;
-    v = (w[0] + w[1]) + (w[2] + w[3]);
+    const float *w = lds + threadIdx.x / LPR * (LPR / 64);
+    if constexpr (LPR == 128) v = w[0] + w[1];
+    else if constexpr (LPR == 256) v = (w[0] + w[1]) + (w[2] + w[3]);
+    else v = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
   }
   return v;
 }
@@ -161,18 +164,18 @@ struct GradArgs {
 // One row's pieces in registers, as they lie in memory.
 template <int DT, int ST, bool CARRY, int CH> struct GradRow {
   Eight<DT> d[CH];
-  Eight<ST> s[CH], c[CARRY && CH < 8 ? CH : 1];
+  Eight<ST> s[CH], c[CARRY ? CH : 1];
   float r;
 };
 
 // Group g of workgroup b takes rows b * groups + g, then every rows * groups further. The gain is kept, or read again where four or more
-// pieces leave no room for it. (8192 rows of 1024 in bf16 with carry, both launches: 256 lanes and 512 partial rows 16.2 us, 512 lanes 15.2, 256 partial
-// rows 16.1; the next row's loads ahead of this row's sums 16.7: the wavefronts that their registers displace were worth more.)
+// pieces leave no room for it. (8192 rows of 1024 in bf16 with carry, both launches, 64 lanes to a row: workgroups of 256 lanes 16.2 us, of 512 15.2; 256
+// partial rows 16.1; the next row's loads ahead of this row's sums 16.7: the wavefronts that their registers displace were worth more.)
 template <int DT, int ST, int WT, bool CARRY, int LPR, int CH>
 __global__ void __launch_bounds__(kGradThreads, 1) k_rms_norm_grad(GradArgs a) {
   constexpr int kGroups = kGradThreads / LPR;
   constexpr bool kKeep = CH < 4;
-  __shared__ float lds[kGradThreads / 64];
+  __shared__ float lds[2 * kGradThreads / 64];
   __shared__ float sums[kGroups > 1 ? kGroups * LPR * CH * 8 : 1];
   const int sub = (int)threadIdx.x % LPR, group = (int)threadIdx.x / LPR;
   Eight<WT> kept[kKeep ? CH : 1];
@@ -191,10 +194,11 @@ __global__ void __launch_bounds__(kGradThreads, 1) k_rms_norm_grad(GradArgs a) {
       if (col >= a.H) continue;
       v.d[j] = load8<DT>(a.dy, row * a.H + col);
       v.s[j] = load8<ST>(a.x, row * a.H + col);
-      if constexpr (CARRY && CH < 8) v.c[j] = load8<ST>(a.carry, row * a.H + col);      // (eight pieces: no room, fetched where it is added)
+      if constexpr (CARRY) v.c[j] = load8<ST>(a.carry, row * a.H + col);
     }
   };
   Row now;
+  int odd = 0;
 #pragma unroll
   for (int j = 0; j < CH; ++j) {
     const int col = (sub + j * LPR) * 8;
@@ -224,7 +228,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) k_rms_norm_grad(GradArgs a) {
         sum = __builtin_fmaf(d[k] * g[k], xh, sum);
       }
     }
-    const float c = row_sum<LPR>(sum, lds) / (float)a.H;
+    const float c = row_sum<LPR>(sum, lds, odd) / (float)a.H;
+    odd ^= 1;
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
       if (!live || (sub + j * LPR) * 8 >= a.H) continue;
@@ -236,8 +241,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) k_rms_norm_grad(GradArgs a) {
       for (int k = 0; k < 8; ++k) o[k] = r * (d[k] * g[k] - s[k] * r * c);
       if constexpr (CARRY) {
         float f[8];
-        if constexpr (CH < 8) widen<ST>(now.c[j], f);
-        else widen<ST>(load8<ST>(a.carry, row * a.H + (sub + j * LPR) * 8), f);
+        widen<ST>(now.c[j], f);
 #pragma unroll
         for (int k = 0; k < 8; ++k) o[k] += f[k];
       }
@@ -266,33 +270,42 @@ __global__ void __launch_bounds__(kGradThreads, 1) k_rms_norm_grad(GradArgs a) {
     for (int j = 0; j < CH; ++j) {
       const int col = (sub + j * LPR) * 8;
       if (col >= a.H) continue;
+      if (onto) {
+        float f[8];
+        widen<ANC_F32>(load8<ANC_F32>((uint64_t)out, col), f);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) out[col + k] = onto ? out[col + k] + dg[j][k] : dg[j][k];
+        for (int k = 0; k < 8; ++k) dg[j][k] += f[k];
+      }
+      store8<ANC_F32>((uint64_t)out, col, dg[j]);
     }
   }
 }
 
-// dgain (+)= the sum of `rows` rows: 16 columns to a workgroup, 64 groups of 4 lanes taking every 64th row.
-__global__ void __launch_bounds__(kThreads) k_gain_sum(const float *parts, float *dgain, int rows, int H, int accumulate) {
-  __shared__ float sums[64][17];
-  const int c4 = (int)threadIdx.x & 3, q = (int)threadIdx.x >> 2, col = (int)blockIdx.x * 16 + c4 * 4;
+// dgain (+)= the sum of `rows` rows: 32 columns, a line, to a workgroup, 64 groups of 8 lanes taking every 64th row, all their loads under way
+// at once. (Both launches, us: half lines and loads as they come 15.1 at 3000 x 2048, 18.0 at 500 x 8192; lines 14.5, 17.0; at once 12.7, 16.8; the partial rows
+// stored 16 bytes a lane where a row is a workgroup's 12.7, 12.9.)
+constexpr int kSumThreads = 512;
+__global__ void __launch_bounds__(kSumThreads) k_gain_sum(const float *parts, float *dgain, int rows, int H, int accumulate) {
+  __shared__ float sums[64][33];
+  const int c8 = (int)threadIdx.x & 7, q = (int)threadIdx.x >> 3, col = (int)blockIdx.x * 32 + c8 * 4;
   anc_f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
   if (col < H) {
-#pragma unroll 8
-    for (int r = q; r < rows; r += 64) {
-      const anc_f32x4 p = *(const anc_f32x4 *)(parts + (int64_t)r * H + col);
-      v = anc_f32x4{v.x + p.x, v.y + p.y, v.z + p.z, v.w + p.w};
-    }
+    anc_f32x4 p[kMostRows / 64];                      // (all under way at once)
+#pragma unroll
+    for (int i = 0; i < kMostRows / 64; ++i)
+      p[i] = q + 64 * i < rows ? *(const anc_f32x4 *)(parts + (int64_t)(q + 64 * i) * H + col) : anc_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < kMostRows / 64; ++i) v = anc_f32x4{v.x + p[i].x, v.y + p[i].y, v.z + p[i].z, v.w + p[i].w};
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) sums[q][c4 * 4 + k] = v[k];
+  for (int k = 0; k < 4; ++k) sums[q][c8 * 4 + k] = v[k];
   __syncthreads();
   // 16 lanes to a column: four rows each, then across the lanes
   const int c = (int)threadIdx.x >> 4, part = (int)threadIdx.x & 15;
   float t = ((sums[part][c] + sums[part + 16][c]) + sums[part + 32][c]) + sums[part + 48][c];
 #pragma unroll
   for (int off = 8; off >= 1; off >>= 1) t += __shfl_xor(t, off, 64);
-  const int out = (int)blockIdx.x * 16 + c;
+  const int out = (int)blockIdx.x * 32 + c;
   if (part == 0 && out < H) dgain[out] = accumulate ? dgain[out] + t : t;
 }
 
@@ -313,6 +326,21 @@ template <typename F> void with_layout(int H, F &&f) {
   else if (pieces <= 1024) f(IC<256>{}, IC<4>{});
   else f(IC<256>{}, IC<8>{});
 }
+// The same for the backward pass, whose lanes hold three rows' pieces and dgain's sums: fewer of them to a lane, so that two workgroups or more fit a
+// CU. (Both launches, us, half as many lanes or less and these: 8192 x 1024 15.4, 15.1; 3000 x 2048 17.1, 15.1; 8000 x 16384 260, 242; but 4096
+// x 4096 with twice these 34.2, 33.2.)
+template <typename F> void with_grad_layout(int H, F &&f) {
+  const int pieces = H / 8;
+  if (pieces <= 16) f(IC<16>{}, IC<1>{});
+  else if (pieces <= 32) f(IC<16>{}, IC<2>{});
+  else if (pieces <= 64) f(IC<64>{}, IC<1>{});
+  else if (pieces <= 128) f(IC<128>{}, IC<1>{});
+  else if (pieces <= 256) f(IC<256>{}, IC<1>{});
+  else if (pieces <= 512) f(IC<256>{}, IC<2>{});
+  else if (pieces <= 1024) f(IC<512>{}, IC<2>{});
+  else f(IC<512>{}, IC<4>{});
+}
+int grad_lanes(int64_t H) { return H <= 256 ? 16 : H <= 512 ? 64 : H <= 1024 ? 128 : H <= 4096 ? 256 : 512; }
 int lanes_of(int64_t H) { return H <= 256 ? 16 : H <= 2048 ? 64 : 256; }
 bool width_ok(int64_t H) { return H > 0 && H % 8 == 0 && H <= kWidest; }
 bool type_ok(int t) { return t == ANC_F32 || t == ANC_BF16; }
@@ -320,7 +348,7 @@ int64_t elem(int t) { return t == ANC_BF16 ? 2 : 4; }
 // Partial rows of dgain: two rows of the batch per group of lanes at least, as many workgroups as keep the memory busy at most, all with
 // as many rows as the fullest.
 int64_t parts_of(int64_t T, int64_t H) {
-  const int64_t groups = kGradThreads / lanes_of(H), most = kMostRows * groups;
+  const int64_t groups = kGradThreads / grad_lanes(H), most = kMostRows * groups;
   const int64_t each = T <= 2 * most ? 2 : (T + most - 1) / most, n = (T + each * groups - 1) / (each * groups);
   return n < 1 ? 1 : n;
 }
@@ -378,7 +406,7 @@ extern "C" int64_t anc_rms_norm_grad_workspace_bytes(int64_t T, int64_t H) {
     return -1;
   }
   // (fewer rows than T may want more partial rows than T does, never more than at two rows each)
-  const int64_t per = 2 * (kGradThreads / lanes_of(H)), n = (T + per - 1) / per;
+  const int64_t per = 2 * (kGradThreads / grad_lanes(H)), n = (T + per - 1) / per;
   return (n < 1 ? 1 : n > kMostRows ? kMostRows : n) * H * 4;
 }
 
@@ -405,7 +433,7 @@ extern "C" int anc_rms_norm_grad(uint64_t dy, int dy_type, uint64_t x, int strea
   GradArgs a{dy, x, gain, rstd, carry, dx, dgain, workspace, T, (int)H, (int)parts_of(T, H), accumulate != 0};
   hipStream_t s = anc_stream(stream);
   AncProfScope prof(ANC_PROF_MISC, s);
-  with_layout((int)H, [&](auto L, auto C) {
+  with_grad_layout((int)H, [&](auto L, auto C) {
     constexpr int lpr = decltype(L)::value, ch = decltype(C)::value;
     with_type(dy_type, [&](auto D) { with_type(stream_type, [&](auto S) { with_type(gain_type, [&](auto G) {
       constexpr int dt = decltype(D)::value, st = decltype(S)::value, gt = decltype(G)::value;
@@ -414,7 +442,7 @@ extern "C" int anc_rms_norm_grad(uint64_t dy, int dy_type, uint64_t x, int strea
     }); }); });
   });
   ANC_LAUNCH_CHECK();
-  if (a.rows > 1) hipLaunchKernelGGL(k_gain_sum, dim3((unsigned)((H + 15) / 16)), dim3(kThreads), 0, s, (const float *)workspace, (float *)dgain, a.rows, (int)H, a.accumulate);
+  if (a.rows > 1) hipLaunchKernelGGL(k_gain_sum, dim3((unsigned)((H + 31) / 32)), dim3(kSumThreads), 0, s, (const float *)workspace, (float *)dgain, a.rows, (int)H, a.accumulate);
   ANC_LAUNCH_CHECK();
   return ANC_OK;
 }
