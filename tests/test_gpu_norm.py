@@ -220,3 +220,27 @@ def test_captured_and_replayed(gpu):
     for b in (x, g, dy, *(v for q in sets for v in q.values())):
         b.free()
     gpu.api.anc_stream_destroy(s)
+
+
+@pytest.mark.parametrize("T,H", [(4500, 200), (9000, 520), (4200, 1000), (2100, 1544), (2300, 4096), (1300, 5000), (1100, 16384)])
+def test_backward_of_many_rows(gpu, T, H):
+    """Three rows and more to every group of lanes, at each number of lanes: the bounds of `test_backward`."""
+    from ancora_cutile_amd import DevBuf, NormWorkspace, rms_norm_grad
+    rng = np.random.default_rng(T)
+    (db, dv), (sb, sv), (gb, gv), (cb, cv) = _make(rng, (T, H), U16, 0.1), _make(rng, (T, H), U16), _make(rng, (H,), F32), _make(rng, (T, H), U16, 0.1)
+    r32 = ref.rms_norm(sv, gv, EPS)[1].astype(F32)
+    bufs = d, s, g, c, r, dx, dg = (DevBuf(db), DevBuf(sb), DevBuf(gb), DevBuf(cb), DevBuf(r32), DevBuf.empty((T, H), U16), DevBuf.empty((H,), F32))
+    ws, u = NormWorkspace(T, H), 2.0 ** -24
+    rms_norm_grad(d, s, g, r, 0, dx, dg, ws, carry=c)
+    first = dx.to_numpy(), dg.to_numpy()
+    want, wdg = ref.rms_norm_grad(dv, sv, gv, r32)
+    a, xh = np.abs(dv * gv), np.abs(sv * r32[:, None].astype(np.float64))
+    err = r32[:, None] * (4 * u * a + xh * (a * xh).mean(1, keepdims=True) * (H + 10) * u)
+    want = want + cv
+    err = err + u * (np.abs(want) + err)
+    assert np.all(np.abs(_val(dx) - want) <= err + _half(U16) * (np.abs(want) + err) + 1e-38)
+    assert np.all(np.abs(_val(dg) - wdg) <= (T + 3) * u * (np.abs(dv) * xh).sum(0))
+    rms_norm_grad(d, s, g, r, 0, dx, dg, ws, carry=c)
+    assert bits_equal(dx.to_numpy(), first[0]) and bits_equal(dg.to_numpy(), first[1])
+    for b in (*bufs, ws):
+        b.free()
