@@ -551,16 +551,17 @@ template <int MODE, int R, int C> __global__ void __launch_bounds__(512, 2) k_ff
 
 // ---------------------------------------------------------------- launch
 template <int V> struct IC { static constexpr int value = V; };
-// Which kernel takes a call: the one whose rounds take least by what a step of 32 k and a round cost, in us. `most`: rows that all
-// segments hold together at most. Measured on whole calls (1 to 8192 rows, 1024 x 2816, 2048 x 2048, 1024 x 4096, dense; 64 and 128 experts of
-// 1024 x 768): a step of k_ffn_tiles where up to 128, 256, .. workgroups are at work, and a round's start and end; of k_ffn_few, one workgroup
-// to a CU, a wavefront's step (of eight). Both sides of some lines, us:
+// Which kernel takes a call: the one whose rounds take least by what a step of 32 k and a round cost, in us: of k_ffn_tiles where up to 128, 256,
+// .. workgroups are at work; of k_ffn_few, one workgroup to a CU, for a wavefront's step (of eight). `most`: rows that all segments hold together at
+// most. Fitted to whole calls (1 to 8192 rows, up to 2272 x 4096, dense; 3 to 128 experts of up to 1128 x 2128): over 36 calls of each kind the choice is
+// 0.5 to 1.5 % off the best of the eight on average. Both sides of some lines, us:
 //   gated, 1024 -> 2816: 64 rows: 32x32 by eight wavefronts 10.1, 128x128 tiles 13.8; 256 rows: 64x64 by eight wavefronts 23.4, 64x128 tiles 10.3, 128x128
 //   15.0; 1024 rows: 128x128 22.7, 128x256 20.9; 2048 x 2048, 8192 rows: 128x256 125, 256x256 116
 //   down, 2816 -> 1024: 1024 rows: 64x64 by eight wavefronts 17.8, 64x128 19.8, 128x128 32.7; 2048 rows 32.4, 20.1, 32.9; 8192 rows: 64x128 64, 128x128
 //   49, 128x256 52, 256x256 68
 //   grad, 512 rows of 1024 x 2816: 64x128 11.2, 128x128 17.0; dx, 2048 x 2048, 8192 rows, whole rounds: 256x256 121, 128x128 142; 1024 x 2816, half a round
 //   of 256x256: 141, and 128x128 100 to 114
+//   grad of a short k, 57 experts of 104 x 2032, 87 rows each, where the outputs' bytes are the work: 64x128 35, 128x256 44
 //   64 experts of 1024 x 768, 4 rows each, gated: 64x64 74, 128x128 40; 128 rows each, down: 128x256 37, 256x256, which just miss one round, 50
 template <int MODE> int launch(Ffn p, int64_t most, const char *who, hipStream_t s) {
   constexpr bool kBack = MODE == kGrad || MODE == kDx;
@@ -580,13 +581,15 @@ template <int MODE> int launch(Ffn p, int64_t most, const char *who, hipStream_t
   };
   auto rounds = [&](int64_t n, int64_t slots, auto cost) { return (float)(n / slots) * cost(slots) + (n % slots ? cost(n % slots) : 0.0f); };
   const float cold = p.counts == nullptr ? 1.0f : 1.4f;      // every expert's weights come from memory, in short rows
+  // The backward epilogue's ten bytes an element at 5.5 TB/s, and how much of them the other workgroups' loops leave uncovered.
+  auto outputs = [&](int64_t r, int tile, float share) { return MODE == kGrad ? (float)r * (float)tile * 10.0f / 5.5e6f * share : 0.0f; };
   const float time[] = {
-      rounds(live(256, 256), 256, [&](int64_t r) { return steps * (r <= 128 ? 0.75f : 0.92f) + (MODE == kGated ? 7.0f : 5.0f); }),
-      rounds(live(128, 256), 512, [&](int64_t r) { return steps * (r <= 128 ? 0.46f : r <= 256 ? 0.60f : kBack ? 1.08f : 0.98f) + 4.0f; }),
+      rounds(live(256, 256), 256, [&](int64_t r) { return steps * (r <= 128 ? 0.75f : 0.92f) + (MODE == kGated ? 7.0f : 5.0f) + outputs(r, 256 * 256, 0.7f); }),
+      rounds(live(128, 256), 512, [&](int64_t r) { return steps * (r <= 128 ? 0.46f : r <= 256 ? 0.60f : kBack ? 1.08f : 0.98f) + 4.0f + outputs(r, 128 * 256, 0.6f); }),
       MODE == kGated ? rounds(live(128, 128), 768, [&](int64_t r) { return steps * (r <= 128 ? 0.33f : r <= 256 ? 0.38f : r <= 512 ? 0.63f : 0.90f) + 3.5f; })
-                     : rounds(live(128, 128), 512, [&](int64_t r) { return steps * (r <= 128 ? 0.33f : r <= 256 ? 0.37f : 0.57f) + 4.5f; }),
-      rounds(live(64, 128), 512, [&](int64_t r) { return steps * (r <= 256 ? 0.19f : 0.35f) + 4.5f; }),
-      rounds(live(64, 64), 256, [&](int64_t) { return cold * (steps / 8 * 0.92f + 5.7f); }),
+                     : rounds(live(128, 128), 512, [&](int64_t r) { return steps * (r <= 128 ? 0.33f : r <= 256 ? 0.37f : 0.57f) + 4.5f + outputs(r, 128 * 128, 0.4f); }),
+      rounds(live(64, 128), 512, [&](int64_t r) { return steps * (r <= 256 ? 0.19f : 0.35f) + 4.5f + outputs(r, 64 * 128, 0.2f); }),
+      rounds(live(64, 64), 256, [&](int64_t) { return cold * (steps / 8 * 0.90f + 7.7f); }),
       rounds(live(32, 64), 256, [&](int64_t) { return cold * (steps / 8 * 0.72f + 4.6f); }),
       rounds(live(32, 32), 256, [&](int64_t) { return cold * (steps / 8 * 0.47f + 4.2f); }),
       MODE == kGated ? 1e30f : rounds(live(16, 16), 256, [&](int64_t) { return cold * (steps / 8 * 0.25f + 4.0f); }),

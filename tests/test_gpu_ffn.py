@@ -176,9 +176,9 @@ def test_the_largest_tiles(gpu, H, I):
 
 
 @pytest.mark.parametrize("H,I,rows", [(520, 2816, 700), (520, 4104, 70), (4104, 264, 70), (72, 520, 4100), (520, 72, 4100), (2056, 520, 2050), (520, 2056, 2050), (2200, 2040, 8100),
-                                      (2040, 2200, 8100)])
+                                      (2040, 2200, 8100), (4104, 2040, 200), (4088, 4088, 200), (136, 2816, 8100)])
 def test_every_size_of_tile(gpu, H, I, rows):
-    """Sizes at which each kernel that a call can take is the cheapest for one of the four calls (the last two: whole rounds of the largest tiles, with ragged
+    """Sizes at which each kernel that a call can take is the cheapest for one of the four calls (2200 and 2040: whole rounds of the largest tiles, with ragged
     edges): some rows, the first and the last among them, against 64 bits."""
     from ancora_cutile_amd import DevBuf, ffn_down, gated_ffn, gated_ffn_dx, gated_ffn_grad
     rng = np.random.default_rng(H + I + rows)
