@@ -553,7 +553,7 @@ template <int MODE, int R, int C> __global__ void __launch_bounds__(512, 2) k_ff
 template <int V> struct IC { static constexpr int value = V; };
 // Which kernel takes a call: the one whose rounds take least by what a step of 32 k and a round cost, in us: of k_ffn_tiles where up to 128, 256,
 // .. workgroups are at work; of k_ffn_few, one workgroup to a CU, for a wavefront's step (of eight). `most`: rows that all segments hold together at
-// most. Fitted to whole calls (1 to 8192 rows, up to 2272 x 4096, dense; 3 to 128 experts of up to 1128 x 2128): over 36 calls of each kind the choice is
+// most. Fitted to whole calls (1 to 8192 rows, up to 2272 x 4096, dense; 3 to 128 experts of up to 1128 x 2128): over 35 calls of each kind the choice is
 // 0.5 to 1.5 % off the best of the eight on average. Both sides of some lines, us:
 //   gated, 1024 -> 2816: 64 rows: 32x32 by eight wavefronts 10.1, 128x128 tiles 13.8; 256 rows: 64x64 by eight wavefronts 23.4, 64x128 tiles 10.3, 128x128
 //   15.0; 1024 rows: 128x128 22.7, 128x256 20.9; 2048 x 2048, 8192 rows: 128x256 125, 256x256 116
