@@ -492,7 +492,9 @@ template <int MODE, int R, int C> __global__ void __launch_bounds__(512, 2) k_ff
   int here = 0;
   for (int t = wave; t < all; t += kWaves) {
     const unsigned char *stage = mine + here;
-    wait_vm<(kStages - 1) * kPieces>();
+    // (behind the last step nothing is fetched, and the last stages wait for one another: 1 to 64 rows 0.4 us less than fetching zeros)
+    if (t + (kStages - 1) * kWaves < all) wait_vm<(kStages - 1) * kPieces>();
+    else wait_vm<0>();
     bf16x8 a[R], b[C];
 #pragma unroll
     for (int i = 0; i < R; ++i) a[i] = *(const bf16x8 *)(stage + i * 1024 + ta);
@@ -506,7 +508,7 @@ template <int MODE, int R, int C> __global__ void __launch_bounds__(512, 2) k_ff
       }
     }
     lds_wave_sync();                             // (read before the stage is fetched into again)
-    fetch(t + kStages * kWaves, mine + here);
+    if (t + kStages * kWaves < all) fetch(t + kStages * kWaves, mine + here);
 #pragma unroll
     for (int j = 0; j < C; ++j)
 #pragma unroll
