@@ -14,9 +14,10 @@
 // to LDS through descriptors that end with the segment or the matrix: rows and columns beyond read zeros and are not stored. What bounds
 // its loop is the operands' way into LDS: a CU has some 64 lines under way at a time, so a line of 128 bytes asked for in halves, a step of 32 k
 // apart, counts twice. Steps of 64 ask for whole lines of what lies along k (8192 rows, dx, 1024 x 2816, 128x128 tiles: 129 us in steps of 32,
-// 100 in steps of 64; 2048 x 2048, 256x256: 130 and 120, 1.15 PFLOP/s; gated, 256x256: 131 and 116 to 125); 128x256 keeps steps of 32, of which two
-// workgroups fit a CU and hide each other's ends. A CU takes in some 60 bytes a nanosecond so, which is why few tiles are small ones. What is left then is the
-// outputs' bytes, which overlap little with the loops.
+// 100 in steps of 64; 2048 x 2048, 256x256: 130 and 120, 1.15 PFLOP/s; gated, 256x256: 131 and 116 to 125). Forwards 128x256 keeps steps of 32, of
+// which two workgroups fit a CU and hide each other's ends (8192 rows, 1024 x 2816, gated: 107 us, one workgroup in steps of 64 143); backwards
+// one of eight wavefronts in three stages of 64 beats them (64 experts of 1024 x 768, 16384 rows: dx 101 and 93). A CU takes in some 60 bytes a
+// nanosecond so, which is why few tiles are small ones. What is left then is the outputs' bytes, which overlap little with the loops.
 // k_ffn_few: 16 to 64 rows of a segment by 16 to 64 columns, the eight wavefronts of a workgroup taking every eighth step of k, each
 // with stages of its own and no barrier, and adding up at the end in a fixed order: with few rows the weights' bytes are the work, and
 // this way they are spread over as many CUs as there are.
@@ -573,7 +574,7 @@ template <int MODE, int R, int C> __global__ void __launch_bounds__(512, 2) k_ff
 //   49, 128x256 52, 256x256 68
 //   grad, 512 rows of 1024 x 2816: 64x128 11.2, 128x128 17.0; dx, 2048 x 2048, 8192 rows, whole rounds: 256x256 121, 128x128 142; 1024 x 2816, half a round
 //   of 256x256: 141, and 128x128 100 to 114
-//   grad of a short k, 57 experts of 104 x 2032, 87 rows each, where the outputs' bytes are the work: 64x128 35, 128x256 44
+//   grad of a short k, 57 experts of 104 x 2032, 87 rows each, where the outputs' bytes are the work: 64x128 35, 128x256 43
 //   64 experts of 1024 x 768, 4 rows each, gated: 64x64 74, 128x128 40; 128 rows each, down: 128x256 37, 256x256, which just miss one round, 50
 template <int MODE> int launch(Ffn p, int64_t most, const char *who, hipStream_t s) {
   constexpr bool kBack = MODE == kGrad || MODE == kDx;
@@ -597,7 +598,8 @@ template <int MODE> int launch(Ffn p, int64_t most, const char *who, hipStream_t
   auto outputs = [&](int64_t r, int tile, float share) { return MODE == kGrad ? (float)r * (float)tile * 10.0f / 5.5e6f * share : 0.0f; };
   const float time[] = {
       rounds(live(256, 256), 256, [&](int64_t r) { return steps * (r <= 128 ? 0.75f : 0.92f) + (MODE == kGated ? 7.0f : 5.0f) + outputs(r, 256 * 256, 0.7f); }),
-      rounds(live(128, 256), 512, [&](int64_t r) { return steps * (r <= 128 ? 0.46f : r <= 256 ? 0.60f : kBack ? 1.08f : 0.98f) + 4.0f + outputs(r, 128 * 256, 0.6f); }),
+      kBack ? rounds(live(128, 256), 256, [&](int64_t r) { return steps * (r <= 128 ? 0.37f : 0.52f) + 4.0f + outputs(r, 128 * 256, 0.5f); })
+            : rounds(live(128, 256), 512, [&](int64_t r) { return steps * (r <= 128 ? 0.46f : r <= 256 ? 0.60f : 0.98f) + 4.0f; }),
       MODE == kGated ? rounds(live(128, 128), 768, [&](int64_t r) { return steps * (r <= 128 ? 0.33f : r <= 256 ? 0.38f : r <= 512 ? 0.63f : 0.90f) + 3.5f; })
                      : rounds(live(128, 128), 512, [&](int64_t r) { return steps * (r <= 128 ? 0.33f : r <= 256 ? 0.37f : 0.57f) + 4.5f + outputs(r, 128 * 128, 0.4f); }),
       rounds(live(64, 128), 512, [&](int64_t r) { return steps * (r <= 256 ? 0.19f : 0.35f) + 4.5f + outputs(r, 64 * 128, 0.2f); }),
@@ -628,7 +630,10 @@ template <int MODE> int launch(Ffn p, int64_t most, const char *who, hipStream_t
   int rc = ANC_OK;
   switch (best) {
     case 0: rc = tiles(IC<256>{}, IC<256>{}, IC<kTall>{}, IC<8192 / kTall>{}, IC<64>{}, IC<2>{}, IC<2>{}, IC<1>{}); break;
-    case 1: rc = tiles(IC<128>{}, IC<256>{}, IC<kTall>{}, IC<8192 / kTall>{}, IC<32>{}, IC<3>{}, IC<2>{}, IC<1>{}); break;
+    case 1:
+      if constexpr (kBack) rc = tiles(IC<128>{}, IC<256>{}, IC<64>{}, IC<64>{}, IC<64>{}, IC<3>{}, IC<2>{}, IC<1>{});
+      else rc = tiles(IC<128>{}, IC<256>{}, IC<kTall>{}, IC<8192 / kTall>{}, IC<32>{}, IC<3>{}, IC<2>{}, IC<1>{});
+      break;
     case 2:
       if constexpr (MODE == kGated) rc = tiles(IC<128>{}, IC<128>{}, IC<64>{}, IC<64>{}, IC<32>{}, IC<3>{}, IC<3>{}, IC<1>{});
       else rc = tiles(IC<128>{}, IC<128>{}, IC<64>{}, IC<64>{}, IC<64>{}, IC<2>{}, IC<2>{}, IC<1>{});
