@@ -573,7 +573,7 @@ template <int MODE, int R, int C> __global__ void __launch_bounds__(512, 2) k_ff
 //   down, 2816 -> 1024: 1024 rows: 64x64 by eight wavefronts 17.8, 64x128 19.8, 128x128 32.7; 2048 rows 32.4, 20.1, 32.9; 8192 rows: 64x128 64, 128x128
 //   49, 128x256 52, 256x256 68
 //   grad, 512 rows of 1024 x 2816: 64x128 11.2, 128x128 17.0; dx, 2048 x 2048, 8192 rows, whole rounds: 256x256 121, 128x128 142; 1024 x 2816, half a round
-//   of 256x256: 141, and 128x128 100 to 114
+//   of 256x256: 141, 128x128 100 to 114, 128x256 97 to 101
 //   grad of a short k, 57 experts of 104 x 2032, 87 rows each, where the outputs' bytes are the work: 64x128 35, 128x256 43
 //   64 experts of 1024 x 768, 4 rows each, gated: 64x64 74, 128x128 40; 128 rows each, down: 128x256 37, 256x256, which just miss one round, 50
 template <int MODE> int launch(Ffn p, int64_t most, const char *who, hipStream_t s) {
