@@ -27,7 +27,7 @@ from . import _lib
 from ._lib import (api, AdamWHyper, AdamWDesc, AdamW8Desc, AdamWStepEntry, F32, BF16, FORM_DIV, FORM_IBC, SR_ON,
                    SR_STEP_SEED)
 from .bf16 import bf16_bits as _bf16_bits, bits_f32 as _bits_f32  # noqa: F401  (re-exported)
-from .devbuf import DevBuf, upload_table
+from .devbuf import DevBuf, checked_state, upload_table
 from .gradnorm import ctl_ptr
 
 C = 64   # every tensor is a flat (numel // 64, 64) view (ancora/optim/adamw.py:20)
@@ -285,17 +285,16 @@ class AdamW:
                 out[f"{n}/{k}"] = s[k].to_numpy()
         return out
 
+    def checked_state(self, sd):
+        """What `load_state_dict` uploads, and the step count; ValueError where the checkpoint is another optimizer's (moments of other bits included)."""
+        return checked_state(sd, self.st, self._kept, f"AdamW.load_state_dict (moments of {self.state_bits} bits)")
+
     def load_state_dict(self, sd, stream_int=0):
-        for n, s in self.st.items():
-            for k in self._kept:
-                if f"{n}/{k}" not in sd:
-                    raise ValueError(f"AdamW.load_state_dict: '{n}/{k}' is missing (moments of {self.state_bits} bits are held here)")
-                a = np.asarray(sd[f"{n}/{k}"])
-                if a.size != s[k].size or a.dtype != s[k].dtype:
-                    raise ValueError(f"AdamW.load_state_dict: '{n}/{k}' is {a.dtype}[{a.size}], "
-                                     f"expected {s[k].dtype}[{s[k].size}]")
-                s[k].upload(a.reshape(s[k].shape), stream_int)
-        self.t = int(sd["t"])
+        """Take over what `state_dict` gave. A checkpoint that does not fit is refused before anything is changed."""
+        uploads, t = self.checked_state(sd)
+        for buf, a in uploads:
+            buf.upload(a, stream_int)
+        self.t = t
 
     def master(self):
         return {n: s["p32"].numpy().reshape(s["shape"]) for n, s in self.st.items()}

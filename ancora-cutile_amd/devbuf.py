@@ -124,3 +124,20 @@ def upload_table(structs):
     if pad:
         raw = np.concatenate([raw, np.zeros(pad, np.uint8)])
     return DevBuf(raw)
+
+
+def checked_state(sd, st, keys, who, step_count=True):
+    """The uploads of a checkpoint, [(buffer, array)], and its step count (None where `step_count` is false): every entry f"{name}/{key}" of the named
+    buffers `st` is looked at before the caller changes anything. ValueError names the first that is missing or of another kind or size."""
+    uploads = []
+    for n, s in st.items():
+        for k in keys:
+            if f"{n}/{k}" not in sd:
+                raise ValueError(f"{who}: '{n}/{k}' is missing")
+            a = np.asarray(sd[f"{n}/{k}"])
+            if a.size != s[k].size or a.dtype != s[k].dtype:
+                raise ValueError(f"{who}: '{n}/{k}' is {a.dtype}[{a.size}], expected {s[k].dtype}[{s[k].size}]")
+            uploads.append((s[k], a.reshape(s[k].shape)))
+    if step_count and "t" not in sd:
+        raise ValueError(f"{who}: 't' is missing")
+    return uploads, int(sd["t"]) if step_count else None

@@ -216,8 +216,11 @@ class HybridOptimizer:
         return out
 
     def load_state_dict(self, sd, stream_int=0):
-        self.muon.load_state_dict({k[5:]: v for k, v in sd.items() if k.startswith("muon/")}, stream_int)
-        self.adamw.load_state_dict({k[6:]: v for k, v in sd.items() if k.startswith("adamw/")}, stream_int)
+        """Take over what `state_dict` gave. A checkpoint that does not fit either group is refused before anything is changed."""
+        muon, adamw = ({k[len(of):]: v for k, v in sd.items() if k.startswith(of)} for of in ("muon/", "adamw/"))
+        self.adamw.checked_state(adamw)
+        self.muon.load_state_dict(muon, stream_int)
+        self.adamw.load_state_dict(adamw, stream_int)
         self._pending = None
         if self.guard is not None:
             self.guard.set_t(self.adamw.t, stream_int)

@@ -23,7 +23,7 @@ import numpy as np
 from . import _lib
 from ._lib import api, MuonDesc, F32, BF16, MUON_MAX_SCALES, MUON_P16T, SR_ON, SR_STEP_SEED
 from .bf16 import bf16_bits, bits_f32, bf16_round as _bf        # noqa: F401
-from .devbuf import DevBuf, upload_table
+from .devbuf import DevBuf, checked_state, upload_table
 from .gradnorm import ctl_ptr
 from . import muon_ns
 from .muon_ns import NTM, _KELLER, NsWorkspace
@@ -664,16 +664,17 @@ class Muon:
                 out[f"{n}/{k}"] = s[k].to_numpy()
         return out
 
+    def checked_state(self, sd):
+        """What `load_state_dict` uploads, and the step count; ValueError where the checkpoint is another optimizer's."""
+        return checked_state(sd, self.st, ("p32", "buf", "p16"), "Muon.load_state_dict", self.engine is not None)
+
     def load_state_dict(self, sd, stream_int=0):
-        for n, s in self.st.items():
-            for k in ("p32", "buf", "p16"):
-                a = np.asarray(sd[f"{n}/{k}"])
-                if a.size != s[k].size or a.dtype != s[k].dtype:
-                    raise ValueError(f"Muon.load_state_dict: '{n}/{k}' is {a.dtype}[{a.size}], "
-                                     f"expected {s[k].dtype}[{s[k].size}]")
-                s[k].upload(a.reshape(s[k].shape), stream_int)
+        """Take over what `state_dict` gave. A checkpoint that does not fit is refused before anything is changed."""
+        uploads, t = self.checked_state(sd)
+        for buf, a in uploads:
+            buf.upload(a, stream_int)
         if self.engine is not None:
-            self.engine.t = int(sd["t"])
+            self.engine.t = t
 
     def weights(self):
         """bf16-valued fp32 weights for the forward (ancora/optim/muon.py:311-312)."""
