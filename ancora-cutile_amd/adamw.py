@@ -186,8 +186,6 @@ class AdamW:
         key = ([g.ptr for g in gbufs], [g.dtype for g in gbufs])
         if key == self._table_key:
             return
-        if self._table is not None:
-            self._table.free()
         descs, blk0 = [], 0
         for seed, ((name, s), g) in enumerate(zip(self.st.items(), gbufs)):
             n = s["R"] * C
@@ -203,22 +201,23 @@ class AdamW:
                 descs.append(AdamWDesc(g.ptr, s["m"].ptr, s["v"].ptr, s["p32"].ptr, s["p16"].ptr, n,
                                        blk0, s["wd"], seed, _g_code(g.dtype), 0))
             blk0 += api.anc_adamw_num_blocks(n)
-        self._total_blocks = blk0
-        self._table = upload_table(descs)
-        self._table_key = key
+        table = upload_table(descs)
+        if self._table is not None:
+            self._table.free()
+        self._table, self._total_blocks, self._table_key = table, blk0, key
 
-    def _hyper(self):
-        sb = sr_seed_base(self.seed, self.t) if self.sr or self.state_bits == 8 else 0
+    def _hyper(self, t):
+        sb = sr_seed_base(self.seed, t) if self.sr or self.state_bits == 8 else 0
         if self.form == "div":
-            return hyper_div(self.lr, self.b1, self.b2, self.eps, self.t, self.sr, sb)
-        ibc1 = 1.0 / (1.0 - self.b1 ** self.t)
-        ibc2 = 1.0 / (1.0 - self.b2 ** self.t)
+            return hyper_div(self.lr, self.b1, self.b2, self.eps, t, self.sr, sb)
+        ibc1 = 1.0 / (1.0 - self.b1 ** t)
+        ibc2 = 1.0 / (1.0 - self.b2 ** t)
         return hyper_ibc(self.lr, self.b1, self.b2, self.eps, ibc1, ibc2, self.sr, sb)
 
     def launch(self, grads, stream_int, guard=None, device_steps=False, t_upper=None, uploader=None):
         """Asynchronous part of the step: upload host gradients (DevBuf gradients are used in
-        place; `uploader`, if given, puts the uploads on a stream beside `stream_int`) and launch the fused kernel once over all tensors. `t` is advanced first, as in
-        ancora/optim/adamw.py:89-91; a caller that later finds the step skipped calls `unstep()`.
+        place; `uploader`, if given, puts the uploads on a stream beside `stream_int`) and launch the fused kernel once over all tensors. `t` is advanced, as in
+        ancora/optim/adamw.py:89-91, unless the call raises; a caller that later finds the step skipped calls `unstep()`.
         With `device_steps` the step count lives in the guard's control block (advanced by
         `guard.compute(..., count_step=True)` unless the step is skipped): the kernel takes the
         bias corrections of that step from a table and forms the rounding seed from the count, `t`
@@ -227,8 +226,6 @@ class AdamW:
             if guard is None:
                 raise ValueError("AdamW.launch: device_steps needs the guard whose block counts the steps")
             self._ensure_step_table(self.t + 1 if t_upper is None else t_upper)
-        else:
-            self.t += 1
         gbufs = []
         for name, s in self.st.items():
             g = grads[name]
@@ -254,9 +251,11 @@ class AdamW:
             h.sr = (SR_ON | SR_STEP_SEED) if self.sr else SR_STEP_SEED if self.state_bits == 8 else 0
             h.step_table, h.step_cap = self._steps.ptr, self._steps_cap
         else:
-            h = self._hyper()
+            h = self._hyper(self.t + 1)
         step = api.anc_adamw8_multi if self.state_bits == 8 else api.anc_adamw_multi
         step(self._table.ptr, len(self.st), self._total_blocks, ctypes.byref(h), ctl_ptr(guard), int(stream_int))
+        if not device_steps:
+            self.t += 1
 
     def unstep(self):
         """Undo the counter advance of a step the guard skipped (state was left untouched)."""
