@@ -111,7 +111,8 @@ class AdamW:
     """fp32-master AdamW. params: {name: fp32 ndarray}. no_decay: names with wd=0 (norm gains /
     biases). step(grads, stream) updates in place; .weights() returns the bf16-valued fp32
     weights for the forward (ancora/optim/adamw.py:69-109). state_bits=8 holds m and v as 8-bit codes `st[name]["m"]`, `["v"]`
-    (R, 64) with scale bytes `["ms"]`, `["vs"]` (R,); `seed` then decides their rounding too."""
+    (R, 64) with scale bytes `["ms"]`, `["vs"]` (R,); `seed` then decides their rounding too, and a launch under graph capture is refused unless
+    its steps are counted on the device (`launch(device_steps=True)`, HybridOptimizer's guarded step): replays would repeat one step's rounding."""
 
     def __init__(self, params, lr=3e-4, betas=(0.9, 0.95), eps=1e-8, wd=0.01, no_decay=(),
                  form="div", sr=False, seed=0, grad_dtype=np.float32, state_bits=32):

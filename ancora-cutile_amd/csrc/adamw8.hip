@@ -9,7 +9,8 @@
 // Both are stored by stochastic rounding, the code's lower neighbour plus one where the dropped bits and 16 bits of a hash
 // of (row, column, seed) carry (v_cvt_sr_fp8_f32 / v_cvt_sr_bf8_f32 with the 16 bits in the upper half of their operand): rounded to nearest, a
 // moment that moves by a thousandth a step would stay where it is for ever, since a code's step is an eighth (m) or a quarter (v); this
-// way its expectation is the exact moment's.
+// way its expectation is the exact moment's. That takes a dither of each step's own: a launch whose seed does not move with the steps counted on the
+// device is not captured into a graph (300 replays with one dither leave v at 0.12 of what it should be on average, m at 0.72).
 //
 // Bound: 16 1/16 bytes per element (bf16 gradients; read g 2, m 1, v 1, p32 4, write m 1, v 1, p32 4, p16 2, scales) against the 28 of 32-bit
 // moments, so little that the arithmetic counts as much: the first form took 173 instructions per element and 179 us for 51.5 M elements (4.6
@@ -230,6 +231,11 @@ extern "C" int anc_adamw8_multi(uint64_t desc_table, int32_t n_tensors, int64_t 
               "anc_adamw8_multi: steps counted on the device need the control block");
   ANC_REQUIRE(desc_table != 0 && (desc_table & 7) == 0 && n_tensors > 0, "anc_adamw8_multi: empty descriptor table");
   ANC_REQUIRE(total_blocks > 0 && total_blocks < (1ll << 31), "anc_adamw8_multi: total_blocks=%lld out of range", (long long)total_blocks);
+  if (!(h->sr & ANC_SR_STEP_SEED)) {       // replays would round every moment by one and the same dither, which stops them where they are
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    ANC_HIP(hipStreamIsCapturing(anc_stream(stream), &st));
+    ANC_REQUIRE(st == hipStreamCaptureStatusNone, "anc_adamw8_multi: a launch that carries its step's seed cannot be captured into a graph (ANC_SR_STEP_SEED can)");
+  }
   const anc_adamw_hyper_t hh = *h;
   AncProfScope prof(ANC_PROF_ADAMW, anc_stream(stream));
   dispatch_form_sr(hh.form, hh.sr & ANC_SR_ON, [&](auto F, auto S) {

@@ -289,7 +289,8 @@ int anc_adamw_multi(uint64_t desc_table, int32_t n_tensors, int64_t total_blocks
  * a fraction of the codes' distance, add up to one or more. A v above zero is stored as no less than the least code, so that the update's
  * divisor does not vanish. A moment that is not finite gets the NaN code 0x7F (m: with its sign) and does not count in its block's
  * largest; one within an eighth (v: a quarter) of the largest fp32 may round up to a value that is not finite. sr and seeds as in anc_adamw_multi, but seed_base always counts (it is the moments' too), and sr may be ANC_SR_STEP_SEED
- * alone. Elements are independent of how tensors share a launch. blk0 and total_blocks count anc_adamw_num_blocks(n).
+ * alone. Under graph capture ANC_SR_STEP_SEED is asked for: replays with one seed would round every moment alike, which stops them where they are.
+ * Elements are independent of how tensors share a launch. blk0 and total_blocks count anc_adamw_num_blocks(n).
  * Alignment: g, p32 16 bytes (bf16 g: 8), p16 8, m and v 4. */
 typedef struct {
   uint64_t g, m, v, ms, vs, p32, p16;   /* ms, vs: the scale bytes, n / 64 each           */

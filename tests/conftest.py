@@ -12,6 +12,21 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu)")
 
 
+# Tests that ask for what was shown to be wrong since, with the tests that took their place.
+SUPERSEDED = {
+    "test_gpu_adamw8.py::test_captured_and_replayed":
+        "asks that every replay of an 8-bit AdamW launch round its moments by one and the same dither, which stops them (test_adamw8_state.py); such a capture "
+        "is refused now, and the refusal would leave this test's capture open: test_gpu_adamw8_capture.py",
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        for name, why in SUPERSEDED.items():
+            if item.nodeid.endswith(name):
+                item.add_marker(pytest.mark.skip(reason=why))
+
+
 @pytest.fixture(scope="session")
 def gpu():
     """Initialise the library on device 0; a missing library or GPU is an error, not a skip."""
