@@ -611,7 +611,7 @@ template <int MODE> int launch(Ffn p, int64_t most, const char *who, hipStream_t
   int best = 0;
   for (int i = 1; i < 8; ++i)
     if (time[i] < time[best]) best = i;
-  AncProfScope prof(ANC_PROF_DW_GEMM, s);
+  AncProfScope prof(ANC_PROF_MISC, s);
   auto few = [&](auto R, auto C) {
     constexpr int r = decltype(R)::value, c = decltype(C)::value;
     p.tn = (int)columns(16 * c);

@@ -120,7 +120,7 @@ int anc_copy_kernel(uint64_t dst, uint64_t src, int64_t n_bytes, uint64_t stream
 #define ANC_PROF_NS_BMAT      8   /* B = b A + c A A     (bf16 matrix-core GEMM) */
 #define ANC_PROF_NS_BX        9   /* X = a X + B X       (bf16 matrix-core GEMM) */
 #define ANC_PROF_NS_GEMM_F32 10   /* any GEMM of the fp32 validation chain        */
-#define ANC_PROF_MISC        11   /* casts, conversions, transposes, fill         */
+#define ANC_PROF_MISC        11   /* the rest: casts, fills, token-indexed operators, norm, feed-forward block */
 #define ANC_PROF_COPY        12
 #define ANC_PROF_NS_BX_UPD   13   /* X = a X + B X whose epilogue applies the weight update */
 #define ANC_PROF_DW_GEMM     14   /* weight-gradient product, partial tiles (bf16 matrix-core GEMM) */
