@@ -33,7 +33,7 @@ def rms_norm(x, gain, si, y=None, residual=None, total=None, fp8=None, scale=Non
     """s = x + residual (or x), r = 1 / sqrt(mean(s^2) + eps) per row, result s * r * gain. x (T, H), gain (H,): float32 or bf16 bits;
     residual and total (s itself, rounded to their type; given together): float32 or bf16 bits, of one type. The result goes to y
     (T, H), float32 or bf16 bits, or to fp8 (T, H) and scale (T, H / 32) uint8. rstd (T,) float32 receives r for `rms_norm_grad`. H is
-    a multiple of 8 (32 with fp8) up to 16384. y or total may be x or residual itself; other overlaps are refused. Asynchronous on `si`."""
+    a multiple of 8 (32 with fp8) up to 16384; a row whose squares add up beyond fp32 (values of 2^64 / sqrt(H)) becomes zeros. y or total may be x or residual itself; other overlaps are refused. Asynchronous on `si`."""
     T, H = x.shape if len(x.shape) == 2 else (-1, -1)
     if T < 0:
         raise ValueError(f"rms_norm: x is {x.shape}, (T, H) expected")

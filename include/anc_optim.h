@@ -559,7 +559,7 @@ int anc_gated_ffn_dx(uint64_t dgate, uint64_t dup, uint64_t Wg, uint64_t Wu, uin
  * fp32[T] or 0. y of y_type, or ANC_MXFP8: E4M3 codes (T, H) with scale (T, H/32), one E8M0 byte per 32 elements of a row by
  * the rule of anc_quant_mxfp8_w (elements that are not finite become NaN codes).
  * H a multiple of 8 (MXFP8: 32) up to 16384, T below 2^28 (2^26 beyond H = 256, 2^24 beyond 2048); rows contiguous, 16-byte aligned. Squares are fp32's:
- * rows that hold values beyond 2^63 come out as zeros. y or total may be x or residual itself (same address, same
+ * a row whose squares add up to 2^128 or more (values of 2^64 / sqrt(H): 2^62.5 at H = 8, 2^57 at 16384) comes out as zeros, with r = 0. y or total may be x or residual itself (same address, same
  * type); no other overlap. T = 0 does nothing. */
 int anc_rms_norm(uint64_t x, int x_type, uint64_t residual, int stream_type, uint64_t gain, int gain_type, int64_t T, int64_t H,
                  float eps, uint64_t y, int y_type, uint64_t scale, uint64_t total, uint64_t rstd, uint64_t stream);
