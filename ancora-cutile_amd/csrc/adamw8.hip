@@ -3,14 +3,17 @@
 // step of adamw.hip operation by operation, and go back as codes of the new block's scale.
 //
 // byte = (biased fp32 exponent of the block's largest magnitude) - 7 for m, - 14 for v (at least 1), so that the largest lands in
-// [128, 256) of E4M3's 448, in [2^14, 2^15) of E5M2's 57344. v takes the wider range because the update divides by its root: 2^31 between
-// a block's largest v and its least normal one is 2^15 between gradients, and a v that is not zero never becomes zero.
+// [128, 256) of E4M3's 448, in [2^14, 2^15) of E5M2's 57344. v takes the wider range because the update divides by its root: 2^30 and more between
+// a block's largest v and its least code is 2^15 between gradients, and a v that is not zero never becomes zero.
 //
 // Both are stored by stochastic rounding, the code's lower neighbour plus one where the dropped bits and 16 bits of a hash
 // of (row, column, seed) carry (v_cvt_sr_fp8_f32 / v_cvt_sr_bf8_f32 with the 16 bits in the upper half of their operand): rounded to nearest, a
 // moment that moves by a thousandth a step would stay where it is for ever, since a code's step is an eighth (m) or a quarter (v); this
-// way its expectation is the exact moment's. That takes a dither of each step's own: a launch whose seed does not move with the steps counted on the
-// device is not captured into a graph (300 replays with one dither leave v at 0.12 of what it should be on average, m at 0.72).
+// way its expectation is the exact moment's. For v that ends at the least code, 2^-31 to 2^-30 of the block's largest: one whose gradients have ended
+// stays there while the block's largest does. It also takes a dither of each step's own: a launch whose seed does not move with the steps
+// counted on the device is not captured into a graph (300 replays with one dither leave v at 0.12 of what it should be on average, m at 0.72).
+// Single elements stray: random gradients of one size, 400 steps: v 23 % rms off the one of 32 bits at beta2 0.95, 29 % at 0.999, m 9 %, the
+// update 15 to 18 %.
 //
 // Bound: 16 1/16 bytes per element (bf16 gradients; read g 2, m 1, v 1, p32 4, write m 1, v 1, p32 4, p16 2, scales) against the 28 of 32-bit
 // moments, so little that the arithmetic counts as much: the first form took 173 instructions per element and 179 us for 51.5 M elements (4.6
