@@ -26,7 +26,7 @@ constexpr int kThreads = 256, kVec = 4, kSlabs = 4;
 constexpr int kSlab = kThreads * kVec, kBlockElems = kSlab * kSlabs;      // as adamw.hip: anc_adamw_num_blocks
 constexpr uint32_t kStateSeed = 0x3C6EF372u;                              // apart from the weights' dither
 constexpr uint32_t kInf = 0x7F800000u;
-constexpr int64_t kFewBlocks = 512;
+constexpr int64_t kFewBlocks = 2048;                                     // see k_adamw8_multi
 
 __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
 // The largest of 16 neighbouring lanes, in all of them: rotations within a row of the data-parallel moves.
@@ -206,8 +206,9 @@ __device__ __forceinline__ void adamw8_slabs(const anc_adamw8_desc_t &t, int64_t
   }
 }
 
-// SLABS = 4: a workgroup takes a whole block of 4096 elements, all of a lane's loads before its arithmetic; 1: a quarter of one, for
-// launches of few blocks.
+// SLABS = 4: a workgroup takes a whole block of 4096 elements, all of a lane's loads before its arithmetic; 1: a quarter of one, for launches of fewer
+// than kFewBlocks blocks, whose last round leaves fewer CUs idle that way. One card, whole blocks and quarters, us: 64 blocks 7.0 and 5.7, 300 10.3 and 7.0,
+// 600 13.5 and 10.3 (3.8 TB/s), 1200 21.3 and 17.0, 1600 27.6 and 22.7, 2500 40.5 and 40.0, 5000 73.2 and 74.2, 12576 167 and 166.
 template <int FORM, int SR, int SLABS>
 __global__ void __launch_bounds__(kThreads)
 k_adamw8_multi(const anc_adamw8_desc_t *__restrict__ table, int n_tensors, anc_adamw_hyper_t h, const anc_step_ctl_t *__restrict__ ctl) {
