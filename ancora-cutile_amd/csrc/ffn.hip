@@ -566,14 +566,15 @@ template <int MODE, int R, int C> __global__ void __launch_bounds__(512, 2) k_ff
 // ---------------------------------------------------------------- launch
 // Which kernel takes a call: the one whose rounds take least by what a step of 32 k and a round cost, in us: of k_ffn_tiles where up to 128, 256,
 // .. workgroups are at work; of k_ffn_few, one workgroup to a CU, for a wavefront's step (of eight). `most`: rows that all segments hold together at
-// most. Fitted to whole calls (1 to 8192 rows, up to 2272 x 4096, dense; 3 to 128 experts of up to 1128 x 2128): over 35 calls of each kind the choice is
-// 0.5 to 1.5 % off the best of the eight on average. Both sides of some lines, us:
+// most. Fitted to whole calls (1 to 8192 rows, up to 2272 x 4096, dense; 3 to 128 experts of up to 1128 x 2128): over 35 calls of each kind the choice was
+// 0.5 to 1.5 % off the best of the eight on average, before the backward pass's 128x256 tiles took their present form (its line was fitted again by
+// itself). The tiles' side knows no weights' bytes: for larger experts with few rows each its ranking is a guess. Both sides of some lines, us:
 //   gated, 1024 -> 2816: 64 rows: 32x32 by eight wavefronts 10.1, 128x128 tiles 13.8; 256 rows: 64x64 by eight wavefronts 23.4, 64x128 tiles 10.3, 128x128
 //   15.0; 1024 rows: 128x128 22.7, 128x256 20.9; 2048 x 2048, 8192 rows: 128x256 125, 256x256 116
 //   down, 2816 -> 1024: 1024 rows: 64x64 by eight wavefronts 17.8, 64x128 19.8, 128x128 32.7; 2048 rows 32.4, 20.1, 32.9; 8192 rows: 64x128 64, 128x128
 //   49, 128x256 52, 256x256 68
 //   grad, 512 rows of 1024 x 2816: 64x128 11.2, 128x128 17.0; dx, 2048 x 2048, 8192 rows, whole rounds: 256x256 121, 128x128 142; 1024 x 2816, half a round
-//   of 256x256: 141, 128x128 100 to 114, 128x256 97 to 101
+//   of 256x256: 141, 128x128 100 or 114 by the buffers' places (no reason found), 128x256 92 to 102
 //   grad of a short k, 57 experts of 104 x 2032, 87 rows each, where the outputs' bytes are the work: 64x128 35, 128x256 43
 //   64 experts of 1024 x 768, 4 rows each, gated: 64x64 74, 128x128 40; 128 rows each, down: 128x256 37, 256x256, which just miss one round, 50
 template <int MODE> int launch(Ffn p, int64_t most, const char *who, hipStream_t s) {

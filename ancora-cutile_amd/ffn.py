@@ -9,7 +9,8 @@ between `dispatch` and `combine`, and the operands of the weight gradients (`gra
 
 Weights are the bf16 copies that the optimizer refreshes, as they lie: (H, I) and (I, H), stacked per expert (E, H, I) or (E*H, I) with a
 plan; no transposed copies are read. Mirrors SwiGLU and the grouped products of the reference's layers (ancora/kernels/activation.py,
-ancora/kernels/moe.py). Products accumulate in fp32, each output is rounded once. Without a plan every row of x is a row of the product; with
+ancora/kernels/moe.py). Products accumulate in fp32, each output is rounded once (h, dgate and dup in between too: they are
+the caller's bf16 buffers). Without a plan every row of x is a row of the product; with
 one, rows that fill up a segment or lie behind the last are neither read nor written. Each call may be captured into a graph, whose replays then
 work on no more tokens than the plan held at the capture (`plan.active`), as its routing and dispatch do.
 """
@@ -87,7 +88,8 @@ def ffn_down(h, Wd, si, y, residual=None, plan=None):
 
 def gated_ffn_grad(dy, gate, up, Wd, si, dgate, dup, h=None, plan=None):
     """From the gradient dy (rows, H) of the block's result to those of the pre-activations: with dh = dy Wd^T and
-    s = sigmoid(gate), dgate = dh up s (1 + gate (1 - s)), dup = dh gate s, and h = gate s up where asked for (dWd = h^T dy). gate, up, dgate,
+    s = sigmoid(gate), dgate = dh up s (1 + gate (1 - s)), dup = dh gate s, and h = gate s up where asked for (dWd = h^T dy): of gate and up as they were
+    kept, rounded, so not the bits of the h that `gated_ffn` made before it rounded them; a caller who wants those in dWd keeps that h. gate, up, dgate,
     dup, h (rows, I) bf16 bits; dgate may be gate and dup up. Asynchronous on `si`."""
     who = "gated_ffn_grad"
     rows, tokens, E, counts, offsets = _call(who, "dy", dy, plan)

@@ -4,8 +4,8 @@ front of the products whose weights the step updates (RMSNorm, ancora/kernels/no
     rms_norm(x, gain, si, y=y, residual=res, total=res2, rstd=r)        # res2 = x + res, y = res2 * r * gain
     rms_norm_grad(dy, res2, gain, r, si, dx, dgain, workspace, carry=dres)   # dx = gradient of res2 through the norm, + dres
 
-8-bit rows (`fp8=`, `scale=` instead of `y=`) are MXFP8 as `Mxfp8WeightCache` holds the weights, blocks of 32 along the row: both
-operands of a product that runs over it. Arithmetic is fp32 with one rounding per output.
+8-bit rows (`fp8=`, `scale=` instead of `y=`) are MXFP8 as `Mxfp8WeightCache` holds the weights, blocks of 32 along the row, for a product over it that the
+caller brings: the products here take bf16. Arithmetic is fp32 with one rounding per output.
 """
 from . import _lib
 from ._lib import api

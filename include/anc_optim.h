@@ -537,12 +537,13 @@ int anc_expert_dw_multi(const anc_expert_dw_problem_t *problems, int32_t n_probl
  *   anc_gated_ffn:       h = silu(x Wg) * (x Wu); gate, up (0: not kept) receive x Wg and x Wu for the backward pass. All bf16.
  *   anc_ffn_down:        y = h Wd + residual (0: none), y and residual of y_type (ANC_F32 or ANC_BF16)
  *   anc_gated_ffn_grad:  with dh = dy Wd^T and s = sigmoid(gate): dgate = dh up s (1 + gate (1 - s)), dup = dh gate s, h = gate s up (0: not
- *                        wanted): what the weight gradients (x^T dgate, x^T dup, h^T dy) and anc_gated_ffn_dx read
+ *                        wanted; of the rounded gate and up: not the bits of the forward pass's): what the weight gradients (x^T dgate, x^T dup, h^T dy)
+ *                        and anc_gated_ffn_dx read
  *   anc_gated_ffn_dx:    dx = dgate Wg^T + dup Wu^T + residual (0: none), dx and residual of dx_type
  * Products of bf16 accumulate in fp32, each output is rounded once. The order of a sum hangs on the sizes of the call (tokens, experts, H, I)
  * alone: ascending k, or eight interleaved runs of it where there are few rows; the same bits on every run.
  * H, I multiples of 8 up to 2^17, at most 512 experts, pointers 16-byte aligned. residual may be the output itself, dgate may be gate and dup
- * up; no other overlap. tokens = 0 does nothing. */
+ * up; no other overlap. tokens = 0 does nothing; more than 2^22 tiles of the product are refused (rows of narrow outputs beyond some 2^28). */
 int anc_gated_ffn(uint64_t x, uint64_t Wg, uint64_t Wu, uint64_t counts, uint64_t offsets, int64_t experts, int64_t rows, int64_t tokens,
                   int64_t H, int64_t I, uint64_t h, uint64_t gate, uint64_t up, uint64_t stream);
 int anc_ffn_down(uint64_t h, uint64_t Wd, uint64_t counts, uint64_t offsets, int64_t experts, int64_t rows, int64_t tokens, int64_t I,
