@@ -145,6 +145,7 @@ class AdamW:
                 half = (R + 3) // 4 * 4
                 block = DevBuf.zeros((2 * half,), np.uint8)
                 self.st[name].update(scales=block, ms=block.view((R,)), vs=DevBuf(shape=(R,), dtype=np.uint8, ptr=block.ptr + half))
+        _lib.stream_sync(0)                    # (streams that do not wait for the null stream may use all of this at once)
         self._table = None
         self._table_key = None
         self.last_skipped = False

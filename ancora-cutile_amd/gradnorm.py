@@ -73,6 +73,7 @@ class StepGuard:
         self.max_norm = 0.0 if max_norm is None else float(max_norm)
         self.eps = float(eps)
         self._ctl = DevBuf.zeros((8,), np.uint32)
+        _lib.stream_sync(0)                    # (streams that do not wait for the null stream may use it at once)
         self._partials = None
         self._tables = {}
         self._part0 = []

@@ -583,6 +583,7 @@ class Muon:
         self._gptr = {}                       # name -> pointer of the resident gradient last bound
         self.engine = MuonEngine(recs, momentum, ns_steps, nesterov, chunk, None, mode, sr, seed) \
             if recs else None
+        _lib.stream_sync(0)                    # (streams that do not wait for the null stream may use all of this at once)
         self.last_skipped = False
 
     @staticmethod

@@ -72,3 +72,18 @@ def test_hybrid(fake_device):
     assert opt.adamw.t == 7 and opt.muon.engine.t == 9
     s = opt.muon.st["o_proj"]["buf"]
     assert bytes(fake_device.at(s.ptr, s.nbytes)) == good["muon/o_proj/buf"].tobytes()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_fresh_state_is_in_place_for_every_stream(fake_device, bits):
+    """The zeros of a new optimizer are filled in on the null stream; a checkpoint may be loaded on one that does not wait for it. Every constructor ends with the
+    wait, behind its last fill."""
+    from ancora_cutile_amd import AdamW, HybridOptimizer, Muon
+    for make in (lambda: AdamW(PARAMS, state_bits=bits), lambda: Muon({"q": np.zeros((128, 256), F32)}),
+                 lambda: HybridOptimizer({"q": np.zeros((128, 256), F32), "w_norm": np.zeros(64, F32)}, adamw_kw=dict(state_bits=bits))):
+        before = len(fake_device.log)
+        make()
+        log = fake_device.log[before:]
+        fills = [i for i, (n, _) in enumerate(log) if n == "anc_fill_u32"]
+        waits = [i for i, (n, a) in enumerate(log) if n == "anc_stream_sync" and a == (0,)]
+        assert fills and waits and waits[-1] > fills[-1]
